@@ -446,6 +446,72 @@ int nnh_embedding_add_forward(const float* weight, size_t V, size_t D, const int
 int nnh_embedding_backward(const float* g, const int* rows, size_t count, size_t V, size_t D, float* dweight, int first,
                            void* stream);
 
+/*
+ * Operators of language models. They have no counterpart in the reference (its attention, src/autograd/ops.cpp:1226-1296, is
+ * nnh_attention_forward above) and no bits of its to keep: results are those of the formulas in fp32 (or better, where
+ * said), repeat bit for bit, and never depend on atomics. Operands are fp32 or bf16 (nnh types below); sums and statistics
+ * are fp32 in both. Captured into a graph, a call that needs scratch takes the buffer registered for its stream
+ * (nnh_set_workspace) and is refused with NNH_ERR_WORKSPACE without one; graphs that may run at once need one each.
+ */
+#define NNH_F32 0
+#define NNH_BF16 1
+
+/* Heads in place: element (n, t, h, d) is data[n * sample + t * row + h * head + d]. Strides are in elements; an input may
+ * have strides of 0 (shared), an output's elements must not overlap. Any strides are taken; rows whose starts and lengths
+ * are multiples of 16 bytes are faster. */
+typedef struct nnh_head_tensor {
+	void* data;
+	size_t sample, row, head;
+} nnh_head_tensor;
+
+/*
+ * What scores become and which keys a query sees. With s = scale q.k for query i of sample n at position pos = q_start[n] +
+ * i and key j at position j:
+ *   c = cap tanh(s / cap), or s when cap is 0;   z = c - slopes[h] |pos - j|, or c without slopes
+ * and the query sees key j when j < k_lens[n], and both belong to one document (q_docs[n, i] == k_docs[n, j], not negative),
+ * and either j < prefix[n], or (causal: j <= pos) and (window > 0: |pos - j| < window).
+ * Arrays are device memory, int32 (slopes: float); null ones mean: no slopes, q_start 0, k_lens Tk, prefix 0, one document.
+ * Values out of range are clamped: k_lens and prefix to the keys there are, q_start to +-2^30.
+ */
+typedef struct nnh_attention_rule {
+	float scale; /* 0: 1 / sqrt(Dh) */
+	float cap;   /* 0: none */
+	const float* slopes; /* {H} */
+	int causal;
+	size_t window; /* 0: none */
+	const int* q_start; /* {N} */
+	const int* k_lens;  /* {N} */
+	const int* prefix;  /* {N} */
+	const int* q_docs;  /* {N, Tq}, together with k_docs */
+	const int* k_docs;  /* {N, Tk} */
+} nnh_attention_rule;
+
+/*
+ * out = softmax(z over the keys seen) v, for H query heads over Hkv key heads (query head h reads key head h / (H / Hkv)), of
+ * Dh <= 128 elements. lse {N, H, Tq} receives log(sum exp z). A query that sees no key gets zeros and an lse of -infinity.
+ * Keys past k_lens are never read; what a query does not see never reaches its result, infinities and NaN included.
+ * For a training batch, q_start is null and k_lens the sequences' lengths; serving one token (or a few) against a cache,
+ * q_start is what the cache held before them and k_lens that plus Tq. Up to 32 query rows take a form that divides the
+ * keys over the GPU (its scratch: nnh_masked_attention_workspace_size).
+ */
+int nnh_masked_attention_forward(int type, size_t N, size_t Tq, size_t Tk, size_t H, size_t Hkv, size_t Dh,
+                                 const nnh_head_tensor* q, const nnh_head_tensor* k, const nnh_head_tensor* v,
+                                 const nnh_attention_rule* rule, const nnh_head_tensor* out, float* lse, void* stream);
+
+/* Its backward rule, from the forward's out and lse: gradients of q, k and v (null: not wanted) given g, out's. *_first
+ * stores, otherwise the gradient is added to what is there. The gradients may lie beside each other in one buffer of
+ * the same rows; they may not overlap. */
+int nnh_masked_attention_backward(int type, size_t N, size_t Tq, size_t Tk, size_t H, size_t Hkv, size_t Dh,
+                                  const nnh_head_tensor* g, const nnh_head_tensor* q, const nnh_head_tensor* k,
+                                  const nnh_head_tensor* v, const nnh_head_tensor* out, const float* lse,
+                                  const nnh_attention_rule* rule, const nnh_head_tensor* dq, int dq_first,
+                                  const nnh_head_tensor* dk, int dk_first, const nnh_head_tensor* dv, int dv_first,
+                                  void* stream);
+
+/* Scratch of the forward (backward 0) or the backward call; documents: whether the rule has them. */
+int nnh_masked_attention_workspace_size(size_t N, size_t Tq, size_t Tk, size_t H, size_t Hkv, size_t Dh, int documents,
+                                        int backward, size_t* bytes);
+
 #ifdef __cplusplus
 }
 #endif

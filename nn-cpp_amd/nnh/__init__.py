@@ -125,6 +125,9 @@ _EXTRA_DECLS = {
     "nnh_gelu_backward": [_vp, _vp, _vp, _sz, _vp, C.c_int, _vp],
     "nnh_embedding_forward": [_vp, _sz, _sz, _vp, _sz, _vp, _vp],
     "nnh_embedding_backward": [_vp, _vp, _sz, _sz, _sz, _vp, C.c_int, _vp],
+    "nnh_masked_attention_forward": [C.c_int] + [_sz] * 6 + [_vp] * 7,
+    "nnh_masked_attention_backward": [C.c_int] + [_sz] * 6 + [_vp] * 8 + [C.c_int, _vp, C.c_int, _vp, C.c_int, _vp],
+    "nnh_masked_attention_workspace_size": [_sz] * 6 + [C.c_int, C.c_int, _szp],
     "nnh_set_stream_numerics": [_vp, C.c_int],
     "nnh_get_stream_numerics": [_vp],
 }
@@ -596,6 +599,128 @@ def layernorm_backward(g, x, gamma, mean, inv_std, dx=None, dx_first=True, dgamm
     check(lib().nnh_layernorm_backward(_p(g), _p(x), _p(gamma), _p(mean), _p(inv_std), R, D, _p(dx),
                                        int(dx_first), _p(dgamma), int(dgamma_first), _p(dbeta), int(dbeta_first),
                                        _stream(stream)))
+
+
+# ---- operators of language models ----
+
+F32, BF16 = 0, 1
+
+
+class HeadTensor(C.Structure):
+    _fields_ = [("data", _vp), ("sample", _sz), ("row", _sz), ("head", _sz)]
+
+
+class _Rule(C.Structure):
+    _fields_ = [("scale", C.c_float), ("cap", C.c_float), ("slopes", _vp), ("causal", C.c_int), ("window", _sz),
+                ("q_start", _vp), ("k_lens", _vp), ("prefix", _vp), ("q_docs", _vp), ("k_docs", _vp)]
+
+
+def _type(t):
+    torch = _torch or _load_torch()
+    if t.dtype == torch.bfloat16:
+        return BF16
+    if t.dtype == torch.float32:
+        return F32
+    raise NnhError(ERR_INVALID, f"fp32 or bf16 is needed, not {t.dtype}")
+
+
+def _on(t, device, dtype=None, shape=None, what="tensor"):
+    """The address of a tensor that has to be on the calls' device, of a type and shape and contiguous where these are given."""
+    if t is None:
+        return None
+    if t.get_device() != device:
+        raise NnhError(ERR_INVALID, f"{what} is not on the current device")
+    if dtype is not None and t.dtype != dtype:
+        raise NnhError(ERR_INVALID, f"{what} must be {dtype}, not {t.dtype}")
+    if shape is not None:
+        if tuple(t.shape) != shape:
+            raise ShapeError(ERR_SHAPE, f"{what} must be {shape}, not {tuple(t.shape)}")
+        if not t.is_contiguous():
+            raise NnhError(ERR_INVALID, f"{what} must be contiguous")
+    return t.data_ptr()
+
+
+def _heads(t, like, device, shape, what):
+    """A {N, T, H, Dh} tensor in place."""
+    if t is None:
+        return None
+    if t.dtype != like.dtype:
+        raise NnhError(ERR_INVALID, f"{what} must be {like.dtype}, not {t.dtype}")
+    if tuple(t.shape) != shape:
+        raise ShapeError(ERR_SHAPE, f"{what} must be {shape}, not {tuple(t.shape)}")
+    n, r, h, d = t.stride()
+    if d != 1 and shape[3] > 1:
+        raise NnhError(ERR_INVALID, f"{what}: the elements of a head must be consecutive")
+    return HeadTensor(_on(t, device, what=what), n, r, h)
+
+
+class AttentionRule:
+    """What masked attention does with scores and which keys a query sees (nnh_attention_rule in nnh.h): cap, slopes {H},
+    causal, window, and per sample q_start, k_lens and prefix {N}, per token q_docs {N, Tq} and k_docs {N, Tk} (int32)."""
+
+    def __init__(self, scale=0.0, cap=0.0, slopes=None, causal=False, window=0, q_start=None, k_lens=None, prefix=None,
+                 q_docs=None, k_docs=None):
+        self.scale, self.cap, self.causal, self.window = float(scale), float(cap), bool(causal), int(window)
+        self.slopes, self.q_start, self.k_lens, self.prefix = slopes, q_start, k_lens, prefix
+        self.q_docs, self.k_docs = q_docs, k_docs
+
+    def _struct(self, N, Tq, Tk, H, device):
+        torch = _torch or _load_torch()
+        i32 = torch.int32
+        if self.window < 0:
+            raise NnhError(ERR_INVALID, "window must not be negative")
+        return _Rule(self.scale, self.cap, _on(self.slopes, device, torch.float32, (H,), "slopes"), self.causal, self.window,
+                     _on(self.q_start, device, i32, (N,), "q_start"), _on(self.k_lens, device, i32, (N,), "k_lens"),
+                     _on(self.prefix, device, i32, (N,), "prefix"), _on(self.q_docs, device, i32, (N, Tq), "q_docs"),
+                     _on(self.k_docs, device, i32, (N, Tk), "k_docs"))
+
+
+def _attention_sizes(q, k, v):
+    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
+        raise ShapeError(ERR_SHAPE, "q, k and v are {N, T, H, Dh}")
+    N, Tq, H, Dh = q.shape
+    return N, Tq, k.shape[1], H, k.shape[2], Dh
+
+
+def masked_attention_forward(q, k, v, rule, out=None, lse=None, stream=None):
+    """nnh_masked_attention_forward on {N, T, heads, Dh} tensors of fp32 or bf16 in place (any strides, the elements of a head
+    consecutive); returns (out, lse)."""
+    torch = _torch or _load_torch()
+    N, Tq, Tk, H, Hkv, Dh = _attention_sizes(q, k, v)
+    device = torch.cuda.current_device()
+    if out is None:
+        out = torch.empty((N, Tq, H, Dh), dtype=q.dtype, device=q.device)
+    if lse is None:
+        lse = torch.empty((N, H, Tq), dtype=torch.float32, device=q.device)
+    qs, ks = (N, Tq, H, Dh), (N, Tk, Hkv, Dh)
+    t = [_heads(x, q, device, s, w) for x, s, w in ((q, qs, "q"), (k, ks, "k"), (v, ks, "v"), (out, qs, "out"))]
+    r = rule._struct(N, Tq, Tk, H, device)
+    check(lib().nnh_masked_attention_forward(_type(q), N, Tq, Tk, H, Hkv, Dh, C.byref(t[0]), C.byref(t[1]), C.byref(t[2]),
+                                             C.byref(r), C.byref(t[3]), _on(lse, device, torch.float32, (N, H, Tq), "lse"),
+                                             _stream(stream)))
+    return out, lse
+
+
+def masked_attention_backward(g, q, k, v, out, lse, rule, dq=None, dq_first=True, dk=None, dk_first=True, dv=None,
+                              dv_first=True, stream=None):
+    """nnh_masked_attention_backward; gradients that are not given are made (and returned with the others)."""
+    torch = _torch or _load_torch()
+    N, Tq, Tk, H, Hkv, Dh = _attention_sizes(q, k, v)
+    device = torch.cuda.current_device()
+    qs, ks = (N, Tq, H, Dh), (N, Tk, Hkv, Dh)
+    grads = []
+    for t, shape, first in ((dq, qs, dq_first), (dk, ks, dk_first), (dv, ks, dv_first)):
+        if t is None and not first:
+            raise NnhError(ERR_INVALID, "a gradient to add to has to be given")
+        grads.append(torch.empty(shape, dtype=q.dtype, device=q.device) if t is None else t)
+    named = ((g, qs, "g"), (q, qs, "q"), (k, ks, "k"), (v, ks, "v"), (out, qs, "out"), (grads[0], qs, "dq"),
+             (grads[1], ks, "dk"), (grads[2], ks, "dv"))
+    t = [C.byref(_heads(x, q, device, s, w)) for x, s, w in named]
+    r = rule._struct(N, Tq, Tk, H, device)
+    check(lib().nnh_masked_attention_backward(_type(q), N, Tq, Tk, H, Hkv, Dh, *t[:5],
+                                              _on(lse, device, torch.float32, (N, H, Tq), "lse"), C.byref(r), t[5],
+                                              int(dq_first), t[6], int(dk_first), t[7], int(dv_first), _stream(stream)))
+    return tuple(grads)
 
 
 _bench_lib = None

@@ -1,0 +1,60 @@
+// masked_attention.hpp - attention over heads that may share keys and values, with capped scores, a distance bias and
+// causal, window, prefix, document and length masks; probabilities are never stored (internal to libnnh).
+//
+//   s = scale q.k,  c = cap tanh(s / cap) (cap > 0),  z = c - slope_h |pos - j|,  out = softmax(z over visible j) v
+//   pos = q_start + i;  visible(i, j): j < k_len and the documents agree, and (causal: j <= pos; window: |pos - j| <
+//   window) or j < prefix
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace nnh {
+
+enum ElemType : int { kF32 = 0, kBf16 = 1 };
+
+// An operand's element strides: sample, row (token) and head; the elements of a head are consecutive.
+struct HeadStrides {
+	int64_t sample, row, head;
+};
+
+// What one block of 64 tokens holds: the least and largest document number (negative ones left out; lo > hi: none) and
+// whether a token belongs to none.
+struct DocRange {
+	int lo, hi, none;
+};
+
+struct MaskedAttentionArgs {
+	const void *q, *k, *v;
+	HeadStrides qs, ks, vs;
+	void* out;  // forward: written; backward: the forward's
+	HeadStrides os;
+	float* lse;  // {N, H, Tq}, natural logarithm
+	int N, Tq, Tk, H, Hkv, G, dh;  // G = H / Hkv query heads to a key head
+	float scale, cap;
+	const float* slopes;  // {H} or null
+	int causal, window;   // window 0: none
+	const int *q_start, *k_lens, *prefix, *q_docs, *k_docs;  // null: 0, Tk, 0, one document
+	const DocRange *q_ranges, *k_ranges;                     // {N, ceil(T / 64)}, set where documents are
+	// backward
+	const void* g;
+	HeadStrides gs;
+	float* delta;  // {N, H, Tq}: g.out per row
+	void *dq, *dk, *dv;
+	HeadStrides dqs, dks, dvs;
+	int dq_first, dk_first, dv_first;
+	// the split form
+	float* partial;  // {splits, N, H, Tq}: maximum, sum and dh sums of p v each
+	int splits;
+};
+
+// Whether the split form (few query rows, the keys divided over the grid) takes a call, and into how many parts.
+int masked_attention_splits(int N, int Tq, int Tk, int H, int Hkv);
+size_t masked_attention_partial_floats(const MaskedAttentionArgs& a);
+
+hipError_t document_ranges(const int* docs, int N, int T, DocRange* out, hipStream_t s);
+hipError_t masked_attention_forward(const MaskedAttentionArgs& a, int type, bool vec, hipStream_t s);
+hipError_t masked_attention_split(const MaskedAttentionArgs& a, int type, bool vec, hipStream_t s);
+hipError_t masked_attention_backward(const MaskedAttentionArgs& a, int type, bool vec, hipStream_t s);
+
+}  // namespace nnh

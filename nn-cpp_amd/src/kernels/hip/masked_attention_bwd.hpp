@@ -1,0 +1,544 @@
+// masked_attention_bwd.hpp - the backward kernels of masked attention (masked_attention.hpp), instantiated per element type
+// by masked_attention_bwd_*.hip.
+//
+//   p = exp(z - lse),  dz = p (g.v - delta),  delta = g.out,  ds = dz (1 - (c / cap)^2)
+//   dq = scale ds k,   dk = scale ds^T q,     dv = p^T g
+//
+// Two kernels, each recomputing the scores of its own products: dq by query rows (which also leaves delta), then dk and dv
+// by key rows, where the queries of all heads that share the key head are added in their order. No gradient is added by
+// atomics, so the results repeat bit for bit; the price is seven products of a pair of rows where five would do.
+#pragma once
+
+#include "masked_attention_tile.hpp"
+
+namespace nnh {
+namespace attn {
+
+constexpr int kBwdWaves = 4, kBwdRows = 32 * kBwdWaves;
+
+// Stores a column of a gradient, or adds it to what the row holds.
+template <typename T, int DH, bool VEC>
+__device__ __forceinline__ void store_gradient(T* o, const f32x16* x, float f, int dh, int half, bool first) {
+#pragma unroll
+	for (int b = 0; b < DH / 32; ++b)
+#pragma unroll
+		for (int g = 0; g < 4; ++g) {
+			const int d = 32 * b + 8 * g + 4 * half;
+			union {
+				T e[4];
+				uint64_t w8;
+				u32x4 w16;
+			} y;
+			if (VEC) {
+				if (d >= dh) continue;
+				if (!first) {
+					if constexpr (sizeof(T) == 2) y.w8 = *(const uint64_t*)(o + d);
+					else y.w16 = *(const u32x4*)(o + d);
+				}
+#pragma unroll
+				for (int i = 0; i < 4; ++i) y.e[i] = (T)(first ? x[b][4 * g + i] * f : to_float(y.e[i]) + x[b][4 * g + i] * f);
+				if constexpr (sizeof(T) == 2) *(uint64_t*)(o + d) = y.w8;
+				else *(u32x4*)(o + d) = y.w16;
+			} else {
+#pragma unroll
+				for (int i = 0; i < 4; ++i)
+					if (d + i < dh) o[d + i] = (T)(first ? x[b][4 * g + i] * f : to_float(o[d + i]) + x[b][4 * g + i] * f);
+			}
+		}
+}
+
+// Turns a block of raw scores into p (before masking) and, where scores are capped, leaves 1 - (c / cap)^2 in slope.
+// far: the distance of register i's pair; lse2: its row's lse in units of log 2.
+template <typename T, typename Far, typename Lse>
+__device__ __forceinline__ void weights(f32x16& s, f32x16& slope, const MaskedAttentionArgs& a, float slope2, Far far, Lse lse2) {
+	if (a.cap > 0.0f) {
+		const float in = a.scale / a.cap, out = a.cap * kLog2e;
+#pragma unroll
+		for (int i = 0; i < 16; ++i) {
+			const float t = tanh_of<T>(s[i] * in);
+			slope[i] = 1.0f - t * t;
+			s[i] = t * out;
+		}
+	} else {
+		const float c = a.scale * kLog2e;
+#pragma unroll
+		for (int i = 0; i < 16; ++i) s[i] *= c;
+	}
+	if (a.slopes) {
+#pragma unroll
+		for (int i = 0; i < 16; ++i) s[i] -= slope2 * far(i);
+	}
+#pragma unroll
+	for (int i = 0; i < 16; ++i) s[i] = exp2_of(s[i] - lse2(i));
+}
+
+// dq: a workgroup's 128 queries of one head against the keys they see, as in the forward kernel: transposed scores, a query
+// a lane, dQ^T += K^T dS^T. Without a.dq it only leaves delta. The second pass is the forward's (values that are not finite
+// in a partly seen tile).
+template <typename T, int DH, bool VEC>
+__global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void masked_attention_dq_kernel(MaskedAttentionArgs a) {
+	constexpr int RB = row_bytes<T, DH>(), KT = RB >= 512 ? 32 : 64, kTile = KT * RB;
+	__shared__ __attribute__((aligned(1024))) char lds[4 * kTile];
+	__shared__ __attribute__((aligned(16))) int docs_of[kBwdWaves][KT];
+	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+	const int col = lane & 31, half = lane >> 5;
+	int* const docs = docs_of[wave];
+	const int tiles = (a.Tq + kBwdRows - 1) / kBwdRows, pairs = a.N * a.Hkv;
+	int tile, h, n;
+	{
+		const unsigned block = blockIdx.x;
+		unsigned pair, rest;
+		if (pairs % 8 == 0) {
+			const unsigned per = pairs / 8, in = block / 8;
+			pair = block % 8 * per + in % per;
+			rest = in / per;
+		} else {
+			pair = block % pairs;
+			rest = block / pairs;
+		}
+		n = pair / a.Hkv;
+		h = pair % a.Hkv * a.G + rest % a.G;
+		tile = tiles - 1 - (int)(rest / a.G);
+	}
+	const int q0 = tile * kBwdRows, i = q0 + wave * 32 + col, hk = h / a.G;
+	const int live = live_keys(a, n), pos0 = first_position(a, n);
+	const T* const kbase = (const T*)a.k + n * a.ks.sample + hk * a.ks.head;
+	const T* const vbase = (const T*)a.v + n * a.vs.sample + hk * a.vs.head;
+	const bool live_row = i < a.Tq;
+	const int64_t row = ((int64_t)n * a.H + h) * a.Tq + min(i, a.Tq - 1);
+
+	Frag<T> q[DH / 16], g[DH / 16];
+	float delta = 0.0f;
+	{
+		const int64_t r = min(i, a.Tq - 1);
+		const T* qr = (const T*)a.q + n * a.qs.sample + r * a.qs.row + h * a.qs.head;
+		const T* gr = (const T*)a.g + n * a.gs.sample + r * a.gs.row + h * a.gs.head;
+		const T* orow = (const T*)a.out + n * a.os.sample + r * a.os.row + h * a.os.head;
+#pragma unroll
+		for (int t = 0; t < DH / 16; ++t) {
+			row_from<T, VEC>(q[t], qr, a.dh, half, t, live_row);
+			row_from<T, VEC>(g[t], gr, a.dh, half, t, live_row);
+			Frag<T> o;
+			row_from<T, VEC>(o, orow, a.dh, half, t, live_row);
+#pragma unroll
+			for (int j = 0; j < 8; ++j) delta += to_float(g[t].e[j]) * to_float(o.e[j]);
+		}
+		delta = add_halves(delta);
+		if (live_row && half == 0) a.delta[row] = delta;
+	}
+	if (!a.dq) return;
+	const Sight see = sight_of(a, n, i, live, pos0);
+	const int pos = pos0 + i;
+	const float slope2 = a.slopes ? a.slopes[h] * kLog2e : 0.0f, lse2 = a.lse[row] * kLog2e;
+	int lo = 0, hi = live, pre = a.prefix ? clamped(a.prefix[n], 0, live) : 0;
+	{
+		const int64_t first = (int64_t)pos0 + q0, last = (int64_t)pos0 + min(q0 + kBwdRows, a.Tq) - 1;
+		if (a.causal) hi = clamped(last + 1, 0, live);
+		if (a.window) {
+			lo = clamped(first - a.window + 1, 0, live);
+			hi = min(hi, clamped(last + a.window, 0, live));
+		}
+	}
+	const int kb = (a.Tk + 63) / 64;
+	DocRange mine{0, 0, 0};
+	if (a.q_docs) {
+		const int nb = (a.Tq + 63) / 64, b0 = q0 / 64;
+		mine = a.q_ranges[(int64_t)n * nb + b0];
+		if (b0 + 1 < nb) {
+			const DocRange o = a.q_ranges[(int64_t)n * nb + b0 + 1];
+			mine.lo = min(mine.lo, o.lo);
+			mine.hi = max(mine.hi, o.hi);
+		}
+	}
+	const int nt = (max(hi, pre) + KT - 1) / KT;
+	f32x16 d[DH / 32];
+
+	for (int pass = 0; pass < 2; ++pass) {
+#pragma unroll
+		for (int b = 0; b < DH / 32; ++b)
+#pragma unroll
+			for (int x = 0; x < 16; ++x) d[b][x] = 0.0f;
+		int base = -64;
+		uint64_t on = 0;
+		auto next = [&]() -> int {
+			while (on == 0) {
+				base += 64;
+				if (base >= nt) return -1;
+				const int x = base + lane, k0 = x * KT;
+				bool s = x < nt && ((k0 < hi && k0 + KT > lo) || k0 < pre);
+				if (s && a.k_docs) {
+					const DocRange r = a.k_ranges[(int64_t)n * kb + k0 / 64];
+					s = r.lo <= mine.hi && r.hi >= mine.lo;
+				}
+				on = __ballot(s);
+			}
+			const int x = __builtin_ctzll(on);
+			on &= on - 1;
+			return base + x;
+		};
+		auto load = [&](int x, int buf) {
+			load_tile<T, DH, KT, kBwdWaves, VEC>(lds + buf * 2 * kTile, kbase + (int64_t)x * KT * a.ks.row, a.ks.row, live - x * KT, a.dh, wave, lane);
+			load_tile<T, DH, KT, kBwdWaves, VEC>(lds + (buf * 2 + 1) * kTile, vbase + (int64_t)x * KT * a.vs.row, a.vs.row, live - x * KT, a.dh, wave, lane);
+		};
+		auto take = [&](const char* kt, const char* vt, int k0) {
+			bool some = (k0 < see.hi && k0 + KT > see.lo) || k0 < see.pre;
+			bool all = (k0 >= see.lo && k0 + KT <= see.hi) || k0 + KT <= see.pre;
+			if (a.k_docs) {
+				const DocRange r = a.k_ranges[(int64_t)n * kb + k0 / 64];
+				some = some && see.doc >= r.lo && see.doc <= r.hi;
+				all = all && see.doc == r.lo && see.doc == r.hi && !r.none;
+			}
+			if (!__any(some)) return;
+			const bool partial = !__all(all);
+			if (partial && a.k_docs && lane < KT) docs[lane] = a.k_docs[(int64_t)n * a.Tk + min(k0 + lane, a.Tk - 1)];
+#pragma unroll
+			for (int x = 0; x < KT / 32; ++x) {
+				f32x16 s, dp, slope;
+#pragma unroll
+				for (int j = 0; j < 16; ++j) s[j] = dp[j] = 0.0f;
+#pragma unroll
+				for (int t = 0; t < DH / 16; ++t) {
+					Frag<T> f;
+					rows_of<T, DH>(f, kt, 32 * x + col, half, t);
+					mma(s, f, q[t]);
+					rows_of<T, DH>(f, vt, 32 * x + col, half, t);
+					mma(dp, f, g[t]);
+				}
+				const int j0 = k0 + 32 * x + 4 * half;
+				weights<T>(s, slope, a, slope2, [&](int j) { const int y = pos - (j0 + 8 * (j / 4) + j % 4); return (float)(y < 0 ? -y : y); },
+				           [&](int) { return lse2; });
+#pragma unroll
+				for (int j = 0; j < 16; ++j) s[j] *= dp[j] - delta;
+				if (a.cap > 0.0f) {
+#pragma unroll
+					for (int j = 0; j < 16; ++j) s[j] *= slope[j];
+				}
+				unsigned seen = 0xffff;
+				if (partial) {
+					seen = 0;
+#pragma unroll
+					for (int j = 0; j < 16; ++j) seen |= see.sees(j0 + 8 * (j / 4) + j % 4) ? 1u << j : 0u;
+					if (a.k_docs) {
+#pragma unroll
+						for (int y = 0; y < 4; ++y) {
+							const i32x4 e = *(const i32x4*)(docs + 32 * x + 8 * y + 4 * half);
+#pragma unroll
+							for (int j = 0; j < 4; ++j) seen &= e[j] == see.doc ? ~0u : ~(1u << (4 * y + j));
+						}
+					}
+#pragma unroll
+					for (int j = 0; j < 16; ++j) s[j] = seen >> j & 1 ? s[j] : 0.0f;
+				}
+				const bool clean = pass != 0 && partial;
+#pragma unroll
+				for (int t = 0; t < 2; ++t) {
+					Frag<T> ds;
+					operand_of(ds, s, t);
+#pragma unroll
+					for (int b = 0; b < DH / 32; ++b) {
+						Frag<T> f;
+						columns_of<T, DH>(f, kt, 32 * x + 16 * t, lane, b);
+						if (clean) only_finite(f);
+						mma(d[b], f, ds);
+					}
+				}
+				if (clean) {  // a key that is not finite makes the queries that see it NaN
+#pragma clang loop unroll(disable)
+					for (int j = 0; j < 32; ++j) {
+						const int bit = (j >> 3) * 4 + (j & 3), owner = col + 32 * ((j >> 2) & 1);
+						const bool sees = (unsigned)__shfl((int)seen, owner) >> bit & 1;
+#pragma unroll
+						for (int b = 0; b < DH / 32; ++b)
+#pragma unroll
+							for (int y = 0; y < 16; ++y) {
+								const float v = element_of<T, DH>(kt, 32 * x + j, 32 * b + 8 * (y / 4) + 4 * half + y % 4);
+								d[b][y] += sees && not_finite(v) ? v - v : 0.0f;
+							}
+					}
+				}
+			}
+		};
+		int cur = next(), buf = 0;
+		if (cur >= 0) load(cur, 0);
+		while (cur >= 0) {
+			wait_loads();
+			__builtin_amdgcn_s_barrier();
+			asm volatile("" ::: "memory");
+			const int then = next();
+			if (then >= 0) load(then, buf ^ 1);
+			take(lds + buf * 2 * kTile, lds + (buf * 2 + 1) * kTile, cur * KT);
+			cur = then;
+			buf ^= 1;
+		}
+		bool bad = false;
+#pragma unroll
+		for (int b = 0; b < DH / 32; ++b)
+#pragma unroll
+			for (int x = 0; x < 16; ++x) bad |= not_finite(d[b][x]);
+		if (!__syncthreads_or(bad)) break;
+	}
+	if (live_row)
+		store_gradient<T, DH, VEC>((T*)a.dq + n * a.dqs.sample + (int64_t)i * a.dqs.row + h * a.dqs.head, d, a.scale, a.dh, half,
+		                           a.dq_first != 0);
+}
+
+// dk and dv: a workgroup's 128 keys of one key head against the queries, of all its heads in turn, that see them. Scores
+// as they are (S = Q K^T), a key a lane: dV^T += G^T P, dK^T += Q^T dS. The workgroup's K and V stay in registers, the tiles
+// of Q and G come through LDS with their rows' lse, delta and documents.
+template <typename T, int DH, bool VEC>
+__global__ __launch_bounds__(256, 1) void masked_attention_dkv_kernel(MaskedAttentionArgs a) {
+	constexpr int RB = row_bytes<T, DH>(), QT = RB >= 512 ? 32 : 64, kTile = QT * RB;
+	__shared__ __attribute__((aligned(1024))) char lds[4 * kTile];
+	__shared__ __attribute__((aligned(16))) float lse_of[2][64], delta_of[2][64];
+	__shared__ __attribute__((aligned(16))) int docs_of[2][64];
+	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+	const int col = lane & 31, half = lane >> 5;
+	const int pairs = a.N * a.Hkv;
+	int tile, pair;
+	{
+		const unsigned block = blockIdx.x;
+		if (pairs % 8 == 0) {
+			const unsigned per = pairs / 8, in = block / 8;
+			pair = block % 8 * per + in % per;
+			tile = in / per;
+		} else {
+			pair = block % pairs;
+			tile = block / pairs;
+		}
+	}
+	const int n = pair / a.Hkv, hk = pair % a.Hkv, k0 = tile * kBwdRows, j = k0 + wave * 32 + col;
+	const int live = live_keys(a, n), pos0 = first_position(a, n), pre = a.prefix ? clamped(a.prefix[n], 0, live) : 0;
+	// The queries that see key j: lo <= i < hi (all of them for a key of the prefix).
+	Sight see{0, 0, 0, 0};
+	if (j < live) {
+		see.doc = a.k_docs ? a.k_docs[(int64_t)n * a.Tk + j] : 0;
+		if (see.doc >= 0) {
+			see.hi = a.Tq;
+			if (j >= pre) {
+				const int64_t at = (int64_t)j - pos0;  // the query at key j's own position
+				if (a.causal) see.lo = clamped(at, 0, a.Tq);
+				if (a.window) {
+					see.lo = max(see.lo, clamped(at - a.window + 1, 0, a.Tq));
+					see.hi = clamped(at + a.window, 0, a.Tq);
+				}
+			}
+		}
+	}
+	// and those that may see any of the workgroup's
+	int lo = 0, hi = k0 < live ? a.Tq : 0;
+	if (k0 >= pre) {
+		const int64_t first = (int64_t)k0 - pos0, last = (int64_t)min(k0 + kBwdRows, live) - 1 - pos0;
+		if (a.causal) lo = clamped(first, 0, a.Tq);
+		if (a.window) {
+			lo = max(lo, clamped(first - a.window + 1, 0, a.Tq));
+			hi = min(hi, clamped(last + a.window, 0, a.Tq));
+		}
+	}
+	const int qb = (a.Tq + 63) / 64;
+	DocRange mine{0, 0, 0};
+	if (a.k_docs && k0 < live) {
+		const int nb = (a.Tk + 63) / 64, b0 = k0 / 64;
+		mine = a.k_ranges[(int64_t)n * nb + b0];
+		if (b0 + 1 < nb) {
+			const DocRange o = a.k_ranges[(int64_t)n * nb + b0 + 1];
+			mine.lo = min(mine.lo, o.lo);
+			mine.hi = max(mine.hi, o.hi);
+		}
+	}
+	const int nt = (hi + QT - 1) / QT;
+
+	Frag<T> kf[DH / 16], vf[DH / 16];
+	{
+		const int64_t r = min(j, a.Tk - 1);
+		const T* kr = (const T*)a.k + n * a.ks.sample + r * a.ks.row + hk * a.ks.head;
+		const T* vr = (const T*)a.v + n * a.vs.sample + r * a.vs.row + hk * a.vs.head;
+#pragma unroll
+		for (int t = 0; t < DH / 16; ++t) {
+			row_from<T, VEC>(kf[t], kr, a.dh, half, t, j < live);
+			row_from<T, VEC>(vf[t], vr, a.dh, half, t, j < live);
+		}
+	}
+	f32x16 dk[DH / 32], dv[DH / 32];
+
+	for (int pass = 0; pass < 2; ++pass) {
+#pragma unroll
+		for (int b = 0; b < DH / 32; ++b)
+#pragma unroll
+			for (int x = 0; x < 16; ++x) dk[b][x] = dv[b][x] = 0.0f;
+		// the tiles of each head's queries in turn
+		int head = -1, base = nt;
+		uint64_t on = 0;
+		auto next = [&]() -> int {
+			while (on == 0) {
+				base += 64;
+				if (base >= nt) {
+					if (nt == 0 || ++head >= a.G) return -1;
+					base = lo / QT / 64 * 64;
+				}
+				const int x = base + lane, q0 = x * QT;
+				bool s = x < nt && q0 + QT > lo;
+				if (s && a.q_docs) {
+					const DocRange r = a.q_ranges[(int64_t)n * qb + q0 / 64];
+					s = r.lo <= mine.hi && r.hi >= mine.lo;
+				}
+				on = __ballot(s);
+			}
+			const int x = __builtin_ctzll(on);
+			on &= on - 1;
+			return base + x;
+		};
+		auto load = [&](int x, int buf) {
+			const int h = hk * a.G + head, q0 = x * QT;
+			load_tile<T, DH, QT, kBwdWaves, VEC>(lds + buf * 2 * kTile, (const T*)a.q + n * a.qs.sample + (int64_t)q0 * a.qs.row + h * a.qs.head, a.qs.row, a.Tq - q0, a.dh, wave, lane);
+			load_tile<T, DH, QT, kBwdWaves, VEC>(lds + (buf * 2 + 1) * kTile, (const T*)a.g + n * a.gs.sample + (int64_t)q0 * a.gs.row + h * a.gs.head, a.gs.row, a.Tq - q0, a.dh, wave, lane);
+			const int64_t r = min(q0 + lane, a.Tq - 1), row = ((int64_t)n * a.H + h) * a.Tq + r;
+			if (wave == 0) __builtin_amdgcn_global_load_lds((global_void*)(a.lse + row), (lds_void*)lse_of[buf], 4, 0, 0);
+			if (wave == 1) __builtin_amdgcn_global_load_lds((global_void*)(a.delta + row), (lds_void*)delta_of[buf], 4, 0, 0);
+			if (wave == 2 && a.q_docs) __builtin_amdgcn_global_load_lds((global_void*)(a.q_docs + (int64_t)n * a.Tq + r), (lds_void*)docs_of[buf], 4, 0, 0);
+		};
+		auto take = [&](const char* qt, const char* gt, const float* lse, const float* delta, const int* docs, int q0, int h) {
+			bool some = q0 < see.hi && q0 + QT > see.lo, all = q0 >= see.lo && q0 + QT <= see.hi;
+			if (a.q_docs) {
+				const DocRange r = a.q_ranges[(int64_t)n * qb + q0 / 64];
+				some = some && see.doc >= r.lo && see.doc <= r.hi;
+				all = all && see.doc == r.lo && see.doc == r.hi && !r.none;
+			}
+			if (!__any(some)) return;
+			const bool partial = !__all(all);
+			const float slope2 = a.slopes ? a.slopes[h] * kLog2e : 0.0f;
+#pragma unroll
+			for (int x = 0; x < QT / 32; ++x) {
+				f32x16 s, dp, slope;
+#pragma unroll
+				for (int y = 0; y < 16; ++y) s[y] = dp[y] = 0.0f;
+#pragma unroll
+				for (int t = 0; t < DH / 16; ++t) {
+					Frag<T> f;
+					rows_of<T, DH>(f, qt, 32 * x + col, half, t);
+					mma(s, f, kf[t]);
+					rows_of<T, DH>(f, gt, 32 * x + col, half, t);
+					mma(dp, f, vf[t]);
+				}
+				const int i0 = 32 * x + 4 * half;  // the tile's row of register y: i0 + 8 (y / 4) + y % 4
+				f32x4 l[4], e[4];
+#pragma unroll
+				for (int y = 0; y < 4; ++y) {
+					l[y] = *(const f32x4*)(lse + i0 + 8 * y);
+					e[y] = *(const f32x4*)(delta + i0 + 8 * y);
+				}
+				weights<T>(s, slope, a, slope2,
+				           [&](int y) { const int z = pos0 + q0 + i0 + 8 * (y / 4) + y % 4 - j; return (float)(z < 0 ? -z : z); },
+				           [&](int y) { return l[y / 4][y % 4] * kLog2e; });
+#pragma unroll
+				for (int y = 0; y < 16; ++y) dp[y] = s[y] * (dp[y] - e[y / 4][y % 4]);
+				if (a.cap > 0.0f) {
+#pragma unroll
+					for (int y = 0; y < 16; ++y) dp[y] *= slope[y];
+				}
+				unsigned seen = 0xffff;
+				if (partial) {
+					seen = 0;
+#pragma unroll
+					for (int y = 0; y < 16; ++y) seen |= see.sees(q0 + i0 + 8 * (y / 4) + y % 4) ? 1u << y : 0u;
+					if (a.q_docs) {
+#pragma unroll
+						for (int z = 0; z < 4; ++z) {
+							const i32x4 o = *(const i32x4*)(docs + i0 + 8 * z);
+#pragma unroll
+							for (int y = 0; y < 4; ++y) seen &= o[y] == see.doc ? ~0u : ~(1u << (4 * z + y));
+						}
+					}
+#pragma unroll
+					for (int y = 0; y < 16; ++y) {
+						s[y] = seen >> y & 1 ? s[y] : 0.0f;
+						dp[y] = seen >> y & 1 ? dp[y] : 0.0f;
+					}
+				}
+				const bool clean = pass != 0 && partial;
+#pragma unroll
+				for (int t = 0; t < 2; ++t) {
+					Frag<T> p, ds;
+					operand_of(p, s, t);
+					operand_of(ds, dp, t);
+#pragma unroll
+					for (int b = 0; b < DH / 32; ++b) {
+						Frag<T> f;
+						columns_of<T, DH>(f, gt, 32 * x + 16 * t, lane, b);
+						if (clean) only_finite(f);
+						mma(dv[b], f, p);
+						columns_of<T, DH>(f, qt, 32 * x + 16 * t, lane, b);
+						if (clean) only_finite(f);
+						mma(dk[b], f, ds);
+					}
+				}
+				if (clean) {  // rows that are not finite, to the keys that they see
+#pragma clang loop unroll(disable)
+					for (int i = 0; i < 32; ++i) {
+						const int bit = (i >> 3) * 4 + (i & 3), owner = col + 32 * ((i >> 2) & 1);
+						const bool sees = (unsigned)__shfl((int)seen, owner) >> bit & 1;
+#pragma unroll
+						for (int b = 0; b < DH / 32; ++b)
+#pragma unroll
+							for (int y = 0; y < 16; ++y) {
+								const int d = 32 * b + 8 * (y / 4) + 4 * half + y % 4;
+								const float gv = element_of<T, DH>(gt, 32 * x + i, d), qv = element_of<T, DH>(qt, 32 * x + i, d);
+								dv[b][y] += sees && not_finite(gv) ? gv : 0.0f;
+								dk[b][y] += sees && not_finite(qv) ? qv - qv : 0.0f;
+							}
+					}
+				}
+			}
+		};
+		int cur = next(), buf = 0;
+		if (cur >= 0) load(cur, 0);
+		while (cur >= 0) {
+			wait_loads();
+			__builtin_amdgcn_s_barrier();
+			asm volatile("" ::: "memory");
+			const int h = hk * a.G + head, then = next();
+			if (then >= 0) load(then, buf ^ 1);
+			take(lds + buf * 2 * kTile, lds + (buf * 2 + 1) * kTile, lse_of[buf], delta_of[buf], docs_of[buf], cur * QT, h);
+			cur = then;
+			buf ^= 1;
+		}
+		bool bad = false;
+#pragma unroll
+		for (int b = 0; b < DH / 32; ++b)
+#pragma unroll
+			for (int x = 0; x < 16; ++x) bad |= not_finite(dk[b][x]) || not_finite(dv[b][x]);
+		if (!__syncthreads_or(bad)) break;
+	}
+	if (j < a.Tk) {
+		if (a.dk)
+			store_gradient<T, DH, VEC>((T*)a.dk + n * a.dks.sample + (int64_t)j * a.dks.row + hk * a.dks.head, dk, a.scale, a.dh, half,
+			                           a.dk_first != 0);
+		if (a.dv)
+			store_gradient<T, DH, VEC>((T*)a.dv + n * a.dvs.sample + (int64_t)j * a.dvs.row + hk * a.dvs.head, dv, 1.0f, a.dh, half,
+			                           a.dv_first != 0);
+	}
+}
+
+template <typename T, int DH, bool VEC>
+hipError_t launch_backward(const MaskedAttentionArgs& a, hipStream_t s) {
+	if (a.Tq > 0) {
+		const int64_t blocks = (int64_t)a.N * a.H * ((a.Tq + kBwdRows - 1) / kBwdRows);
+		masked_attention_dq_kernel<T, DH, VEC><<<(unsigned)blocks, 256, 0, s>>>(a);
+		const hipError_t e = hipGetLastError();
+		if (e != hipSuccess) return e;
+	}
+	if (!(a.dk || a.dv) || a.Tk == 0) return hipSuccess;
+	const int64_t blocks = (int64_t)a.N * a.Hkv * ((a.Tk + kBwdRows - 1) / kBwdRows);
+	masked_attention_dkv_kernel<T, DH, VEC><<<(unsigned)blocks, 256, 0, s>>>(a);
+	return hipGetLastError();
+}
+
+template <typename T>
+hipError_t backward_of(const MaskedAttentionArgs& a, bool vec, hipStream_t s) {
+	if (!vec) return launch_backward<T, 128, false>(a, s);
+	if (a.dh <= 64) return launch_backward<T, 64, true>(a, s);
+	if (a.dh <= 96) return launch_backward<T, 96, true>(a, s);
+	return launch_backward<T, 128, true>(a, s);
+}
+
+}  // namespace attn
+}  // namespace nnh

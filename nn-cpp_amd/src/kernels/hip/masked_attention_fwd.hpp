@@ -1,0 +1,520 @@
+// masked_attention_fwd.hpp - the forward kernels of masked attention (masked_attention.hpp), instantiated per element type
+// by masked_attention_fwd_*.hip.
+//
+// One pass over the keys with the running maximum and sum of the softmax. Scores are computed transposed, S^T = K Q^T, so a
+// lane holds one query's column: its maximum, sum and rescaling are one number a lane, and P^T goes into O^T += V^T P^T from
+// the registers it was computed in (masked_attention_tile.hpp).
+#pragma once
+
+#include "masked_attention_tile.hpp"
+
+namespace nnh {
+namespace attn {
+
+// A wave's 32 query columns.
+template <typename T, int DH>
+struct Rows {
+	Frag<T> q[DH / 16];
+	f32x16 o[DH / 32];
+	float m, l;  // maximum in units of log 2, and this half's part of the sum
+	Sight s;
+	int pos;
+	float slope2;
+
+	__device__ __forceinline__ void clear() {
+		m = -kInf;
+		l = 0.0f;
+#pragma unroll
+		for (int b = 0; b < DH / 32; ++b)
+#pragma unroll
+			for (int i = 0; i < 16; ++i) o[b][i] = 0.0f;
+	}
+	__device__ __forceinline__ bool bad() const {
+		bool r = false;
+#pragma unroll
+		for (int b = 0; b < DH / 32; ++b)
+#pragma unroll
+			for (int i = 0; i < 16; ++i) r |= not_finite(o[b][i]);
+		return r;
+	}
+};
+
+// Takes the KT keys from k0 on, whose rows are in kt and vt, into the wave's columns. docs: the wave's own room for KT ints.
+template <typename T, int DH, int KT>
+__device__ __forceinline__ void take_keys(Rows<T, DH>& r, const MaskedAttentionArgs& a, int n, const char* kt,
+                                          const char* vt, int* docs, int k0, int lane, bool safe) {
+	const int col = lane & 31, half = lane >> 5;
+	// whether some of the wave's queries see some of the tile, and whether all of them all of it
+	bool some = (k0 < r.s.hi && k0 + KT > r.s.lo) || k0 < r.s.pre;
+	bool all = (k0 >= r.s.lo && k0 + KT <= r.s.hi) || k0 + KT <= r.s.pre;
+	if (a.k_docs) {
+		const DocRange d = a.k_ranges[(int64_t)n * ((a.Tk + 63) / 64) + k0 / 64];
+		some = some && r.s.doc >= d.lo && r.s.doc <= d.hi;
+		all = all && r.s.doc == d.lo && r.s.doc == d.hi && !d.none;
+	}
+	if (!__any(some)) return;
+	const bool partial = !__all(all);
+
+	f32x16 s[KT / 32];
+#pragma unroll
+	for (int x = 0; x < KT / 32; ++x)
+#pragma unroll
+		for (int i = 0; i < 16; ++i) s[x][i] = 0.0f;
+#pragma unroll
+	for (int t = 0; t < DH / 16; ++t)
+#pragma unroll
+		for (int x = 0; x < KT / 32; ++x) {
+			Frag<T> k;
+			rows_of<T, DH>(k, kt, 32 * x + col, half, t);
+			mma(s[x], k, r.q[t]);
+		}
+
+	if (a.cap > 0.0f) {
+		const float in = a.scale / a.cap, out = a.cap * kLog2e;
+#pragma unroll
+		for (int x = 0; x < KT / 32; ++x)
+#pragma unroll
+			for (int i = 0; i < 16; ++i) s[x][i] = out * tanh_of<T>(s[x][i] * in);
+	} else {
+		const float c = a.scale * kLog2e;
+#pragma unroll
+		for (int x = 0; x < KT / 32; ++x)
+#pragma unroll
+			for (int i = 0; i < 16; ++i) s[x][i] *= c;
+	}
+	if (a.slopes) {
+#pragma unroll
+		for (int x = 0; x < KT / 32; ++x)
+#pragma unroll
+			for (int i = 0; i < 16; ++i) {
+				const int d = r.pos - (k0 + 32 * x + 8 * (i / 4) + 4 * half + i % 4);
+				s[x][i] -= r.slope2 * (float)(d < 0 ? -d : d);
+			}
+	}
+	unsigned seen[KT / 32];  // bit i: the lane's query sees the key of register i
+	if (partial) {
+		if (a.k_docs && lane < KT) docs[lane] = a.k_docs[(int64_t)n * a.Tk + min(k0 + lane, a.Tk - 1)];
+#pragma unroll
+		for (int x = 0; x < KT / 32; ++x) {
+			seen[x] = 0;
+#pragma unroll
+			for (int i = 0; i < 16; ++i) seen[x] |= r.s.sees(k0 + 32 * x + 8 * (i / 4) + 4 * half + i % 4) ? 1u << i : 0u;
+			if (a.k_docs) {
+#pragma unroll
+				for (int g = 0; g < 4; ++g) {
+					const i32x4 d = *(const i32x4*)(docs + 32 * x + 8 * g + 4 * half);
+#pragma unroll
+					for (int i = 0; i < 4; ++i) seen[x] &= d[i] == r.s.doc ? ~0u : ~(1u << (4 * g + i));
+				}
+			}
+#pragma unroll
+			for (int i = 0; i < 16; ++i) s[x][i] = seen[x] >> i & 1 ? s[x][i] : -kInf;
+		}
+	}
+
+	float top = -kInf;
+#pragma unroll
+	for (int x = 0; x < KT / 32; ++x)
+#pragma unroll
+		for (int i = 0; i < 16; ++i) top = fmaxf(top, s[x][i]);
+	top = max_halves(top);
+	if (__any(top > r.m)) {  // seldom after a row's first tiles
+		const float m = fmaxf(r.m, top), f = m == -kInf ? 1.0f : exp2_of(r.m - m);
+		r.m = m;
+		r.l *= f;
+#pragma unroll
+		for (int b = 0; b < DH / 32; ++b)
+#pragma unroll
+			for (int i = 0; i < 16; ++i) r.o[b][i] *= f;
+	}
+	const float base = r.m == -kInf ? 0.0f : r.m;
+#pragma unroll
+	for (int x = 0; x < KT / 32; ++x)
+#pragma unroll
+		for (int i = 0; i < 16; ++i) {
+			s[x][i] = exp2_of(s[x][i] - base);
+			r.l += s[x][i];
+		}
+
+	const bool clean = safe && partial;
+#pragma unroll
+	for (int x = 0; x < KT / 32; ++x)
+#pragma unroll
+		for (int t = 0; t < 2; ++t) {
+			Frag<T> p;
+			operand_of(p, s[x], t);
+#pragma unroll
+			for (int b = 0; b < DH / 32; ++b) {
+				Frag<T> v;
+				columns_of<T, DH>(v, vt, 32 * x + 16 * t, lane, b);
+				if (clean) only_finite(v);
+				mma(r.o[b], v, p);
+			}
+		}
+	if (clean) {  // what the product left out, to the queries that see it
+#pragma clang loop unroll(disable)
+		for (int j = 0; j < KT; ++j) {
+			const unsigned word = j < 32 ? seen[0] : seen[KT / 32 - 1];
+			const int i = ((j & 31) >> 3) * 4 + (j & 3), owner = col + 32 * ((j >> 2) & 1);
+			const bool on = (unsigned)__shfl((int)word, owner) >> i & 1;
+#pragma unroll
+			for (int b = 0; b < DH / 32; ++b)
+#pragma unroll
+				for (int x = 0; x < 16; ++x) {
+					const float v = element_of<T, DH>(vt, j, 32 * b + 8 * (x / 4) + 4 * half + x % 4);
+					r.o[b][x] += on && not_finite(v) ? v : 0.0f;
+				}
+		}
+	}
+}
+
+// Stores a column: head row `o` takes the dh sums times f.
+template <typename T, int DH, bool VEC>
+__device__ __forceinline__ void store_column(T* o, const f32x16* x, float f, int dh, int half) {
+#pragma unroll
+	for (int b = 0; b < DH / 32; ++b)
+#pragma unroll
+		for (int g = 0; g < 4; ++g) {
+			const int d = 32 * b + 8 * g + 4 * half;
+			union {
+				T e[4];
+				uint64_t w8;
+				u32x4 w16;
+			} y;
+#pragma unroll
+			for (int i = 0; i < 4; ++i) y.e[i] = (T)(x[b][4 * g + i] * f);
+			if (VEC) {
+				if (d < dh) {
+					if constexpr (sizeof(T) == 2) *(uint64_t*)(o + d) = y.w8;
+					else *(u32x4*)(o + d) = y.w16;
+				}
+			} else {
+#pragma unroll
+				for (int i = 0; i < 4; ++i)
+					if (d + i < dh) o[d + i] = y.e[i];
+			}
+		}
+}
+
+constexpr int kWaves = 4, kQueries = 32 * kWaves;
+
+// Keys to a tile: what two buffers of K and V leave two workgroups a CU for (one where a row is 512 bytes or more).
+template <typename T, int DH>
+constexpr int keys_per_tile() {
+	return row_bytes<T, DH>() >= 512 ? 32 : 64;
+}
+
+// A workgroup's 128 queries of one head against all keys they see, the tiles read by all four waves.
+//
+// A masked score is taken out before the maximum, so a masked key's weight is exactly zero; the product with V still
+// multiplies it, and zero times an infinity or NaN would reach queries that do not see the key. That shows in the result,
+// so where a workgroup ends with one it starts over with such values out of the partly seen tiles' V, adding them to the
+// queries that do see them.
+template <typename T, int DH, bool VEC>
+__global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void masked_attention_forward_kernel(MaskedAttentionArgs a) {
+	constexpr int KT = keys_per_tile<T, DH>(), RB = row_bytes<T, DH>(), kTile = KT * RB;
+	__shared__ __attribute__((aligned(1024))) char lds[4 * kTile];
+	__shared__ __attribute__((aligned(16))) int docs[kWaves][KT];
+	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+	const int col = lane & 31, half = lane >> 5;
+	// Heads of one key head stay on one XCD where the pairs divide evenly (its L2 then holds their keys); the queries that
+	// see most come first.
+	const int tiles = (a.Tq + kQueries - 1) / kQueries, pairs = a.N * a.Hkv;
+	int tile, h, n;
+	{
+		const unsigned block = blockIdx.x;
+		unsigned pair, rest;
+		if (pairs % 8 == 0) {
+			const unsigned per = pairs / 8, in = block / 8;
+			pair = block % 8 * per + in % per;
+			rest = in / per;
+		} else {
+			pair = block % pairs;
+			rest = block / pairs;
+		}
+		n = pair / a.Hkv;
+		h = pair % a.Hkv * a.G + rest % a.G;
+		tile = tiles - 1 - (int)(rest / a.G);
+	}
+	const int q0 = tile * kQueries, i = q0 + wave * 32 + col, hk = h / a.G;
+	const int live = live_keys(a, n), pos0 = first_position(a, n);
+	const T* const kbase = (const T*)a.k + n * a.ks.sample + hk * a.ks.head;
+	const T* const vbase = (const T*)a.v + n * a.vs.sample + hk * a.vs.head;
+
+	Rows<T, DH> r;
+	r.s = sight_of(a, n, i, live, pos0);
+	r.pos = pos0 + i;
+	r.slope2 = a.slopes ? a.slopes[h] * kLog2e : 0.0f;
+	{
+		const T* row = (const T*)a.q + n * a.qs.sample + (int64_t)min(i, a.Tq - 1) * a.qs.row + h * a.qs.head;
+#pragma unroll
+		for (int t = 0; t < DH / 16; ++t) row_from<T, VEC>(r.q[t], row, a.dh, half, t, i < a.Tq);
+	}
+	// what the workgroup's queries can see at most (positions, then documents)
+	int lo = 0, hi = live, pre = a.prefix ? clamped(a.prefix[n], 0, live) : 0;
+	{
+		const int64_t first = (int64_t)pos0 + q0, last = (int64_t)pos0 + min(q0 + kQueries, a.Tq) - 1;
+		if (a.causal) hi = clamped(last + 1, 0, live);
+		if (a.window) {
+			lo = clamped(first - a.window + 1, 0, live);
+			hi = min(hi, clamped(last + a.window, 0, live));
+		}
+	}
+	DocRange mine{0, 0, 0};
+	if (a.q_docs) {
+		const int nb = (a.Tq + 63) / 64, b0 = q0 / 64;
+		mine = a.q_ranges[(int64_t)n * nb + b0];
+		if (b0 + 1 < nb) {
+			const DocRange o = a.q_ranges[(int64_t)n * nb + b0 + 1];
+			mine.lo = min(mine.lo, o.lo);
+			mine.hi = max(mine.hi, o.hi);
+		}
+	}
+	const int nt = (max(hi, pre) + KT - 1) / KT;
+
+	for (int pass = 0; pass < 2; ++pass) {
+		r.clear();
+		// the tiles that some query may see, 64 at a time
+		int base = -64;
+		uint64_t on = 0;
+		auto next = [&]() -> int {
+			while (on == 0) {
+				base += 64;
+				if (base >= nt) return -1;
+				const int x = base + lane, k0 = x * KT;
+				bool see = x < nt && ((k0 < hi && k0 + KT > lo) || k0 < pre);
+				if (see && a.k_docs) {
+					const DocRange d = a.k_ranges[(int64_t)n * ((a.Tk + 63) / 64) + k0 / 64];
+					see = d.lo <= mine.hi && d.hi >= mine.lo;
+				}
+				on = __ballot(see);
+			}
+			const int x = __builtin_ctzll(on);
+			on &= on - 1;
+			return base + x;
+		};
+		auto load = [&](int x, int buf) {
+			load_tile<T, DH, KT, kWaves, VEC>(lds + buf * 2 * kTile, kbase + (int64_t)x * KT * a.ks.row, a.ks.row, live - x * KT, a.dh, wave, lane);
+			load_tile<T, DH, KT, kWaves, VEC>(lds + (buf * 2 + 1) * kTile, vbase + (int64_t)x * KT * a.vs.row, a.vs.row, live - x * KT, a.dh, wave, lane);
+		};
+		int cur = next(), buf = 0;
+		if (cur >= 0) load(cur, 0);
+		while (cur >= 0) {
+			wait_loads();
+			__builtin_amdgcn_s_barrier();  // this tile has arrived for all waves, and all are done with the last one
+			asm volatile("" ::: "memory");
+			const int then = next();
+			if (then >= 0) load(then, buf ^ 1);
+			take_keys<T, DH, KT>(r, a, n, lds + buf * 2 * kTile, lds + (buf * 2 + 1) * kTile, docs[wave], cur * KT, lane, pass != 0);
+			cur = then;
+			buf ^= 1;
+		}
+		if (!__syncthreads_or(r.bad())) break;
+	}
+
+	const float l = add_halves(r.l);
+	if (i < a.Tq) {
+		T* o = (T*)a.out + n * a.os.sample + (int64_t)i * a.os.row + h * a.os.head;
+		store_column<T, DH, VEC>(o, r.o, l == 0.0f ? 0.0f : 1.0f / l, a.dh, half);
+		if (half == 0) a.lse[((int64_t)n * a.H + h) * a.Tq + i] = l == 0.0f ? -kInf : r.m * kLn2 + logf(l);
+	}
+}
+
+// The split form, for few query rows: the G heads of a key head and the Tq queries together are the columns (32 to a
+// workgroup), and the keys are divided over the grid and over a workgroup's waves, each with a ring of tiles of its own.
+template <typename T, int DH>
+struct SplitShape {
+	static constexpr int KT = 32, RB = row_bytes<T, DH>(), kTile = KT * RB, kStage = 2 * kTile;
+	static constexpr int NW = kStage * 4 <= 128 * 1024 ? 4 : 2;
+	static constexpr int ST = kStage * NW * 4 <= 128 * 1024 ? 4 : kStage * NW * 2 <= 128 * 1024 ? 2 : 1;
+	static constexpr int kLoads = 2 * kTile / 1024;  // a wave's load instructions for a stage
+	static constexpr int kMerge = NW * 32 * (DH + 4) * 4;
+	static constexpr int kLds = NW * ST * kStage > kMerge ? NW * ST * kStage : kMerge;
+	static_assert(kLds <= 160 * 1024 && (ST - 1) * kLoads <= 63, "LDS, and loads that a wave may have outstanding");
+};
+
+template <typename T, int DH, bool VEC>
+__global__ __launch_bounds__((64 * SplitShape<T, DH>::NW), 1) void masked_attention_split_kernel(MaskedAttentionArgs a) {
+	using S = SplitShape<T, DH>;
+	constexpr int KT = S::KT, NW = S::NW, ST = S::ST;
+	__shared__ __attribute__((aligned(1024))) char lds[S::kLds];
+	__shared__ __attribute__((aligned(16))) int docs[NW][KT];
+	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+	const int col = lane & 31, half = lane >> 5;
+	const int columns = a.Tq * a.G, pairs = a.N * a.Hkv;
+	const int split = blockIdx.x % a.splits, pair = blockIdx.x / a.splits % pairs, group = blockIdx.x / a.splits / pairs;
+	const int n = pair / a.Hkv, hk = pair % a.Hkv, c = group * 32 + col;
+	const bool on_col = c < columns;
+	const int i = on_col ? c / a.G : a.Tq, h = hk * a.G + (on_col ? c % a.G : 0);
+	const int live = live_keys(a, n), pos0 = first_position(a, n);
+	const T* const kbase = (const T*)a.k + n * a.ks.sample + hk * a.ks.head;
+	const T* const vbase = (const T*)a.v + n * a.vs.sample + hk * a.vs.head;
+
+	Rows<T, DH> r;
+	r.s = sight_of(a, n, i, live, pos0);
+	r.pos = pos0 + i;
+	r.slope2 = a.slopes ? a.slopes[h] * kLog2e : 0.0f;
+	{
+		const T* row = (const T*)a.q + n * a.qs.sample + (int64_t)min(i, a.Tq - 1) * a.qs.row + h * a.qs.head;
+#pragma unroll
+		for (int t = 0; t < DH / 16; ++t) row_from<T, VEC>(r.q[t], row, a.dh, half, t, on_col);
+	}
+	// the keys that some query of the sample may see, divided into splits * NW runs of whole tiles
+	int lo = 0, hi = live;
+	const int pre = a.prefix ? clamped(a.prefix[n], 0, live) : 0;
+	{
+		const int64_t last = (int64_t)pos0 + a.Tq - 1;
+		if (a.causal) hi = clamped(last + 1, 0, live);
+		if (a.window) {
+			lo = clamped((int64_t)pos0 - a.window + 1, 0, live);
+			hi = min(hi, clamped(last + a.window, 0, live));
+		}
+		if (pre) lo = 0;
+		hi = max(hi, pre);
+	}
+	const int t0 = lo / KT, t1 = (hi + KT - 1) / KT, per = (max(t1 - t0, 0) + a.splits * NW - 1) / (a.splits * NW);
+	const int begin = min(t0 + (split * NW + wave) * per, t1), end = min(begin + per, t1);
+	char* const ring = lds + wave * ST * S::kStage;
+
+	for (int pass = 0; pass < 2; ++pass) {
+		r.clear();
+		auto load = [&](int x, int stage) {
+			char* at = ring + stage * S::kStage;
+			load_tile<T, DH, KT, 1, VEC>(at, kbase + (int64_t)x * KT * a.ks.row, a.ks.row, live - x * KT, a.dh, 0, lane);
+			load_tile<T, DH, KT, 1, VEC>(at + S::kTile, vbase + (int64_t)x * KT * a.vs.row, a.vs.row, live - x * KT, a.dh, 0, lane);
+		};
+#pragma unroll
+		for (int x = 0; x < ST - 1; ++x)
+			if (begin + x < end) load(begin + x, x);
+		int stage = 0;
+		for (int x = begin; x < end; ++x) {
+			if (ST > 1) {
+				if (x + ST - 1 < end) {
+					load(x + ST - 1, (stage + ST - 1) % ST);
+					asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((ST - 1) * S::kLoads) : "memory");
+				} else {
+					wait_loads();
+				}
+			} else {
+				load(x, 0);
+				wait_loads();
+			}
+			char* at = ring + stage * S::kStage;
+			take_keys<T, DH, KT>(r, a, n, at, at + S::kTile, docs[wave], x * KT, lane, pass != 0);
+			// the stage is loaded over next: its reads are done
+			asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+			stage = (stage + 1) % ST;
+		}
+		if (!__syncthreads_or(r.bad())) break;
+	}
+
+	// the waves' parts, merged in their order
+	float* const part = (float*)lds;  // {NW, 32, DH + 4}
+	r.l = add_halves(r.l);
+	{
+		float* at = part + (wave * 32 + col) * (DH + 4);
+#pragma unroll
+		for (int b = 0; b < DH / 32; ++b)
+#pragma unroll
+			for (int g = 0; g < 4; ++g)
+				*(f32x4*)(at + 32 * b + 8 * g + 4 * half) = f32x4{r.o[b][4 * g], r.o[b][4 * g + 1], r.o[b][4 * g + 2], r.o[b][4 * g + 3]};
+		if (half == 0) {
+			at[DH] = r.m;
+			at[DH + 1] = r.l;
+		}
+	}
+	__syncthreads();
+	for (int x = wave; x < 32 && group * 32 + x < columns; x += NW) {
+		const int cc = group * 32 + x, ii = cc / a.G, hh = hk * a.G + cc % a.G;
+		float m = -kInf, l = 0.0f, f[NW];
+#pragma unroll
+		for (int w = 0; w < NW; ++w) m = fmaxf(m, part[(w * 32 + x) * (DH + 4) + DH]);
+		const float base = m == -kInf ? 0.0f : m;
+#pragma unroll
+		for (int w = 0; w < NW; ++w) {
+			f[w] = exp2_of(part[(w * 32 + x) * (DH + 4) + DH] - base);
+			l += f[w] * part[(w * 32 + x) * (DH + 4) + DH + 1];
+		}
+		const int64_t row = ((int64_t)n * a.H + hh) * a.Tq + ii;
+		float* const to = a.partial + ((int64_t)split * a.N * a.H * a.Tq + row) * (a.dh + 2);
+		T* const o = (T*)a.out + n * a.os.sample + (int64_t)ii * a.os.row + hh * a.os.head;
+		const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+		for (int d = lane; d < a.dh; d += 64) {
+			float y = 0.0f;
+#pragma unroll
+			for (int w = 0; w < NW; ++w) y += f[w] * part[(w * 32 + x) * (DH + 4) + d];
+			if (a.splits == 1) o[d] = (T)(y * inv);
+			else to[2 + d] = y;
+		}
+		if (lane == 0) {
+			if (a.splits == 1) {
+				a.lse[row] = l == 0.0f ? -kInf : m * kLn2 + logf(l);
+			} else {
+				to[0] = m;
+				to[1] = l;
+			}
+		}
+	}
+}
+
+// Joins the split form's parts, one wave to a row, in their order.
+template <typename T>
+__global__ __launch_bounds__(256) void masked_attention_join_kernel(MaskedAttentionArgs a) {
+	const int lane = threadIdx.x & 63;
+	const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), rows = (int64_t)a.N * a.H * a.Tq;
+	if (row >= rows) return;
+	const int i = (int)(row % a.Tq), h = (int)(row / a.Tq % a.H), n = (int)(row / a.Tq / a.H);
+	const int64_t step = rows * (a.dh + 2);
+	const float* const from = a.partial + row * (a.dh + 2);
+	float m = -kInf;
+	for (int s = lane; s < a.splits; s += 64) m = fmaxf(m, from[s * step]);
+	for (int x = 32; x; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
+	const float base = m == -kInf ? 0.0f : m;
+	float l = 0.0f, y[2] = {0.0f, 0.0f};
+	for (int s = 0; s < a.splits; ++s) {
+		const float* p = from + s * step;
+		const float f = exp2_of(p[0] - base);
+		l += f * p[1];
+#pragma unroll
+		for (int x = 0; x < 2; ++x)
+			if (lane + 64 * x < a.dh) y[x] += f * p[2 + lane + 64 * x];
+	}
+	T* const o = (T*)a.out + n * a.os.sample + (int64_t)i * a.os.row + h * a.os.head;
+	const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+	for (int x = 0; x < 2; ++x)
+		if (lane + 64 * x < a.dh) o[lane + 64 * x] = (T)(y[x] * inv);
+	if (lane == 0) a.lse[row] = l == 0.0f ? -kInf : m * kLn2 + logf(l);
+}
+
+template <typename T, int DH, bool VEC>
+hipError_t launch_forward(const MaskedAttentionArgs& a, hipStream_t s) {
+	const int64_t blocks = (int64_t)a.N * a.H * ((a.Tq + kQueries - 1) / kQueries);
+	masked_attention_forward_kernel<T, DH, VEC><<<(unsigned)blocks, 256, 0, s>>>(a);
+	return hipGetLastError();
+}
+
+template <typename T, int DH, bool VEC>
+hipError_t launch_split(const MaskedAttentionArgs& a, hipStream_t s) {
+	const int64_t groups = ((int64_t)a.Tq * a.G + 31) / 32, blocks = groups * a.N * a.Hkv * a.splits;
+	masked_attention_split_kernel<T, DH, VEC><<<(unsigned)blocks, 64 * SplitShape<T, DH>::NW, 0, s>>>(a);
+	hipError_t e = hipGetLastError();
+	if (e != hipSuccess || a.splits == 1) return e;
+	const int64_t rows = (int64_t)a.N * a.H * a.Tq;
+	masked_attention_join_kernel<T><<<(unsigned)((rows + 3) / 4), 256, 0, s>>>(a);
+	return hipGetLastError();
+}
+
+// The head width that a kernel is built for; rows that are not 16-byte aligned take the widest.
+template <typename T>
+hipError_t forward_of(const MaskedAttentionArgs& a, bool vec, bool split, hipStream_t s) {
+#define NNH_ATTN(DH, VEC) (split ? launch_split<T, DH, VEC>(a, s) : launch_forward<T, DH, VEC>(a, s))
+	if (!vec) return NNH_ATTN(128, false);
+	if (a.dh <= 64) return NNH_ATTN(64, true);
+	if (a.dh <= 96) return NNH_ATTN(96, true);
+	return NNH_ATTN(128, true);
+#undef NNH_ATTN
+}
+
+}  // namespace attn
+}  // namespace nnh

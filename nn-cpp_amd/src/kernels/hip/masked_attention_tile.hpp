@@ -1,0 +1,273 @@
+// masked_attention_tile.hpp - the pieces that the masked attention kernels share: tiles in LDS, their matrix operands,
+// and what a query sees.
+//
+// Products are 32 x 32 blocks of MFMA. The accumulator of a block has, in lane l, column l % 32 and rows
+// 8 (i / 4) + 4 (l / 32) + i % 4 in register i; an operand of 16 depths has, in lane l, row (or column) l % 32 and the
+// eight depths 8 (l / 32) + 0..7. A block's scores therefore go into the next product as they are, as the operand whose
+// depth is the accumulator's row axis, when the other operand takes its depths in the same order: depth block t of lane
+// half h is 16 t + 4 h + {0..3} and 16 t + 8 + 4 h + {0..3}. No probability moves between lanes.
+//
+// A tile is [row][RB bytes] in LDS, its 16-byte words permuted within a row so that both reads of it are free of bank
+// conflicts: 16-byte words of 8 consecutive rows (an operand with the tile's rows as rows) and the transposed reads of 4
+// rows by 64 bytes (an operand with the tile's rows as depth). Words move from memory into LDS without passing through
+// registers, so the permutation is in what each lane loads.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "masked_attention.hpp"
+
+namespace nnh {
+namespace attn {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) void lds_void;
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+typedef const __attribute__((address_space(1))) void global_void;
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kInf = __builtin_huge_valf();
+
+// 16 zero bytes that lanes without a word of their own load.
+static __device__ const u32x4 kZeroWord = {0, 0, 0, 0};
+
+__device__ __forceinline__ float to_float(float x) { return x; }
+__device__ __forceinline__ float to_float(__bf16 x) { return (float)x; }
+
+// Eight consecutive depths of one operand row.
+template <typename T>
+struct Frag;
+template <>
+struct Frag<__bf16> {
+	union {
+		bf16x8 v;
+		u32x4 w;
+		s16x4 h[2];
+		bf16x2 p[4];
+		__bf16 e[8];
+	};
+};
+template <>
+struct Frag<float> {
+	union {
+		f32x4 h[2];
+		u32x4 w2[2];
+		float e[8];
+	};
+};
+
+// acc += A B over 16 depths.
+__device__ __forceinline__ void mma(f32x16& acc, const Frag<__bf16>& a, const Frag<__bf16>& b) {
+	acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.v, b.v, acc, 0, 0, 0);
+}
+__device__ __forceinline__ void mma(f32x16& acc, const Frag<float>& a, const Frag<float>& b) {
+#pragma unroll
+	for (int j = 0; j < 8; ++j) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a.e[j], b.e[j], acc, 0, 0, 0);
+}
+
+// Registers 8 t .. 8 t + 7 of a block as an operand; in bf16 each value is rounded to the nearest once (the operand's
+// type: its sum, and the statistics beside it, stay in fp32).
+__device__ __forceinline__ void operand_of(Frag<__bf16>& f, const f32x16& x, int t) {
+#pragma unroll
+	for (int j = 0; j < 4; ++j) f.p[j] = __builtin_convertvector(f32x2{x[8 * t + 2 * j], x[8 * t + 2 * j + 1]}, bf16x2);
+}
+__device__ __forceinline__ void operand_of(Frag<float>& f, const f32x16& x, int t) {
+#pragma unroll
+	for (int j = 0; j < 8; ++j) f.e[j] = x[8 * t + j];
+}
+
+// Bytes of a tile's row: the power of two that holds DH elements.
+template <typename T, int DH>
+constexpr int row_bytes() {
+	int b = 64;
+	while (b < DH * (int)sizeof(T)) b *= 2;
+	return b;
+}
+
+// Where the 16-byte word c of a row lives: c ^ swizzle(row).
+template <int RB>
+__device__ __forceinline__ int swizzle(int row) {
+	if (RB == 64) return (row >> 2) & 3;
+	if (RB == 128) return ((row >> 1) & 1) << 2 | ((row >> 2) & 3);
+	return (row & 3) << 2 | ((row >> 2) & 3);
+}
+
+// Loads `live` rows (of R; the others are zeros) of `dh` elements into a tile, from base + row * stride. VEC: every row is
+// 16-byte aligned and dh a whole number of words; then nothing passes through registers, and the caller waits for the
+// loads (wait_loads). NW waves share the work.
+template <typename T, int DH, int R, int NW, bool VEC>
+__device__ __forceinline__ void load_tile(char* tile, const T* base, int64_t stride, int live, int dh, int wave, int lane) {
+	constexpr int RB = row_bytes<T, DH>(), W = RB / 16, E = 16 / (int)sizeof(T), kSteps = R * RB / 1024 / NW;
+	static_assert(kSteps * NW * 1024 == R * RB, "a tile splits evenly over the waves");
+#pragma unroll
+	for (int j = 0; j < kSteps; ++j) {
+		const int first = (j * NW + wave) * 64, row = (first + lane) / W, c = ((first + lane) % W) ^ swizzle<RB>(row);
+		if (VEC) {
+			const bool on = row < live && c * E < dh;
+			const void* src = on ? (const void*)(base + row * stride + c * E) : (const void*)&kZeroWord;
+			if (DH * (int)sizeof(T) == RB || c * E < DH)
+				__builtin_amdgcn_global_load_lds((global_void*)src, (lds_void*)(tile + first * 16), 16, 0, 0);
+		} else {
+			union {
+				T e[E];
+				u32x4 w;
+			} x;
+#pragma unroll
+			for (int i = 0; i < E; ++i) x.e[i] = row < live && c * E + i < dh ? base[row * stride + c * E + i] : (T)0.0f;
+			*(u32x4*)(tile + (first + lane) * 16) = x.w;
+		}
+	}
+}
+
+// Every load into LDS that the wave has issued has arrived.
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
+
+// Operand with the tile's rows as rows: row `row`, depths 16 t + 8 half + 0..7.
+template <typename T, int DH>
+__device__ __forceinline__ void rows_of(Frag<T>& f, const char* tile, int row, int half, int t) {
+	constexpr int RB = row_bytes<T, DH>();
+	const int sw = swizzle<RB>(row);
+	if constexpr (sizeof(T) == 2) {
+		f.w = *(const u32x4*)(tile + row * RB + (((2 * t + half) ^ sw) * 16));
+	} else {
+		f.w2[0] = *(const u32x4*)(tile + row * RB + (((4 * t + 2 * half) ^ sw) * 16));
+		f.w2[1] = *(const u32x4*)(tile + row * RB + (((4 * t + 2 * half + 1) ^ sw) * 16));
+	}
+}
+
+// Operand with the tile's rows as depth, in the order of the accumulator's rows: depths row0 + 4 half + {0..3} and
+// row0 + 8 + 4 half + {0..3}, of column 32 block + lane % 32. In 16 bits one transposed read fetches, for each 16 lanes, 4
+// rows of 16 elements (each lane naming 4 consecutive ones) and hands each lane a column of them.
+template <typename T, int DH>
+__device__ __forceinline__ void columns_of(Frag<T>& f, const char* tile, int row0, int lane, int block) {
+	constexpr int RB = row_bytes<T, DH>();
+	const int half = lane >> 5;
+	if constexpr (sizeof(T) == 2) {
+		const int i = lane & 15, d = 32 * block + 16 * ((lane >> 4) & 1) + 4 * (i & 3);
+#pragma unroll
+		for (int x = 0; x < 2; ++x) {
+			const int row = row0 + 8 * x + 4 * half + (i >> 2);
+			const char* at = tile + row * RB + (((d >> 3) ^ swizzle<RB>(row)) * 16) + (d & 4) * 2;
+			f.h[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at);
+		}
+	} else {
+		const int d = 32 * block + (lane & 31);
+#pragma unroll
+		for (int j = 0; j < 8; ++j) {
+			const int row = row0 + 8 * (j >> 2) + 4 * half + (j & 3);
+			f.e[j] = *(const float*)(tile + row * RB + (((d >> 2) ^ swizzle<RB>(row)) * 16) + (d & 3) * 4);
+		}
+	}
+}
+
+// One element of a tile.
+template <typename T, int DH>
+__device__ __forceinline__ float element_of(const char* tile, int row, int d) {
+	constexpr int RB = row_bytes<T, DH>(), E = 16 / (int)sizeof(T);
+	return to_float(*(const T*)(tile + row * RB + (((d / E) ^ swizzle<RB>(row)) * 16) + (d % E) * (int)sizeof(T)));
+}
+
+// Operand straight from memory: one row's depths 16 t + 8 half + 0..7, zeros past dh and where off.
+template <typename T, bool VEC>
+__device__ __forceinline__ void row_from(Frag<T>& f, const T* row, int dh, int half, int t, bool on) {
+	const int d = 16 * t + 8 * half;
+	if (VEC) {
+		constexpr int E = 16 / (int)sizeof(T);
+#pragma unroll
+		for (int x = 0; x < 8 / E; ++x) {
+			u32x4 w = {0, 0, 0, 0};
+			if (on && d + x * E < dh) w = *(const u32x4*)(row + d + x * E);
+			if constexpr (sizeof(T) == 2) f.w = w;
+			else f.w2[x] = w;
+		}
+	} else {
+#pragma unroll
+		for (int j = 0; j < 8; ++j) f.e[j] = on && d + j < dh ? row[d + j] : (T)0.0f;
+	}
+}
+
+__device__ __forceinline__ bool not_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u; }
+// Infinities and NaN out of an operand (the safe pass: see masked_attention_forward_kernel).
+template <typename T>
+__device__ __forceinline__ void only_finite(Frag<T>& f) {
+#pragma unroll
+	for (int j = 0; j < 8; ++j)
+		if (not_finite(to_float(f.e[j]))) f.e[j] = (T)0.0f;
+}
+
+// x of the other half's lane with the same column, added to or maximised with the own.
+__device__ __forceinline__ float max_halves(float x) {
+	const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+	return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float add_halves(float x) {
+	const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+	return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+__device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// tanh(x). In 16 bits 1 - 2 / (1 + e^2x) with the hardware's reciprocal: off by about 1e-7 of 1, far below the operands'
+// own rounding. In 32 bits the sum loses the small x's last bits, so below 0.55 the odd power series (to x^15, the rest is
+// under 5e-8 of the value there), above it the quotient divided exactly.
+template <typename T>
+__device__ __forceinline__ float tanh_of(float x) {
+	const float e = exp2_of(x * (2.0f * kLog2e));
+	if constexpr (sizeof(T) == 2) {
+		return __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + e), 1.0f);
+	} else {
+		const float y = x * x;
+		float p = -929569.0f / 638512875.0f;
+		p = __builtin_fmaf(p, y, 21844.0f / 6081075.0f);
+		p = __builtin_fmaf(p, y, -1382.0f / 155925.0f);
+		p = __builtin_fmaf(p, y, 62.0f / 2835.0f);
+		p = __builtin_fmaf(p, y, -17.0f / 315.0f);
+		p = __builtin_fmaf(p, y, 2.0f / 15.0f);
+		p = __builtin_fmaf(p, y, -1.0f / 3.0f);
+		return y < 0.3025f ? __builtin_fmaf(x * y, p, x) : 1.0f - 2.0f / (1.0f + e);
+	}
+}
+
+// What one query sees of the keys: lo <= j < hi or j < pre, and its own document's. A query that is none (past the last
+// row, or of no document) sees nothing.
+struct Sight {
+	int lo, hi, pre, doc;
+	__device__ __forceinline__ bool sees(int j) const { return (j >= lo && j < hi) || j < pre; }
+};
+
+// The bounds of an int expression that may pass 2^31 (positions are at most 2^30 + 2^30).
+__device__ __forceinline__ int clamped(int64_t x, int lo, int hi) { return (int)(x < lo ? lo : x > hi ? hi : x); }
+
+__device__ __forceinline__ int live_keys(const MaskedAttentionArgs& a, int n) {
+	return a.k_lens ? clamped(a.k_lens[n], 0, a.Tk) : a.Tk;
+}
+// The position of sample n's first query.
+__device__ __forceinline__ int first_position(const MaskedAttentionArgs& a, int n) {
+	return a.q_start ? clamped(a.q_start[n], -(1 << 30), 1 << 30) : 0;
+}
+__device__ __forceinline__ Sight sight_of(const MaskedAttentionArgs& a, int n, int i, int live, int pos0) {
+	Sight s{0, 0, 0, 0};
+	if (i >= a.Tq) return s;
+	s.doc = a.q_docs ? a.q_docs[(int64_t)n * a.Tq + i] : 0;
+	if (a.q_docs && s.doc < 0) return s;
+	const int64_t pos = (int64_t)pos0 + i;
+	s.hi = live;
+	if (a.causal) s.hi = clamped(pos + 1, 0, live);
+	if (a.window) {
+		s.lo = clamped(pos - a.window + 1, 0, live);
+		s.hi = min(s.hi, clamped(pos + a.window, 0, live));
+	}
+	if (a.prefix) s.pre = clamped(a.prefix[n], 0, live);
+	return s;
+}
+
+}  // namespace attn
+}  // namespace nnh

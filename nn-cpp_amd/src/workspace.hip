@@ -45,4 +45,6 @@ hipError_t stream_workspace_external(hipStream_t s, bool& external, size_t& byte
 	return Table::instance().external(s, external, bytes);
 }
 
+hipError_t registered_workspace(hipStream_t s, void*& p, size_t& bytes) { return Table::instance().registered(s, p, bytes); }
+
 }  // namespace nnh

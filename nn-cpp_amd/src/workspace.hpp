@@ -57,4 +57,7 @@ hipError_t set_stream_workspace(hipStream_t s, void* p, size_t bytes);
 // Whether stream s has a caller-registered buffer, and its size.
 hipError_t stream_workspace_external(hipStream_t s, bool& external, size_t& bytes);
 
+// The buffer a caller registered for stream s (null, 0: none).
+hipError_t registered_workspace(hipStream_t s, void*& p, size_t& bytes);
+
 }  // namespace nnh

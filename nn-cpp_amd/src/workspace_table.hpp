@@ -113,6 +113,19 @@ public:
 		return Rt::kOk;
 	}
 
+	// The registered buffer of stream s and its size (null, 0: none).
+	Error registered(Stream s, void*& p, size_t& bytes) {
+		p = nullptr;
+		bytes = 0;
+		Slot* sl = nullptr;
+		const Error e = find(s, sl);
+		if (e != Rt::kOk) return e;
+		std::lock_guard<std::mutex> lock(sl->busy);
+		p = sl->ext;
+		bytes = sl->ext_bytes;
+		return Rt::kOk;
+	}
+
 	// The library-owned buffer of stream s and its size (null, 0 before the first take): for tests.
 	Error owned(Stream s, void*& p, size_t& bytes) {
 		p = nullptr;

@@ -1,0 +1,108 @@
+"""Plain 64-bit forms of the operators of language models, with a bound on what rounding may do to each output.
+
+A rounding to a type t is off by at most u(t) = finfo(t).eps / 2 of the value. The bounds below add up, to first order, what
+the formulas' roundings can do: products accumulated in fp32 over K terms (K u32 of the sum of absolute values), the
+exponential and the capped score's tanh (a few u32), and, for bf16 operands, the roundings that the kernels document: the
+probabilities and score gradients as operands of a product, and the stored results."""
+import math
+
+import torch
+
+U32 = torch.finfo(torch.float32).eps / 2
+
+
+def unit(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def visible(N, Tq, Tk, causal=False, window=0, q_start=None, k_lens=None, prefix=None, q_docs=None, k_docs=None):
+    i = torch.arange(Tq)[None, :, None] + (torch.zeros(N, dtype=torch.long) if q_start is None else q_start.long().cpu())[:, None, None]
+    j = torch.arange(Tk)[None, None, :]
+    see = torch.ones(N, Tq, Tk, dtype=torch.bool)
+    if causal:
+        see &= j <= i
+    if window:
+        see &= (i - j).abs() < window
+    if prefix is not None:
+        see |= j < prefix.long().cpu()[:, None, None]
+    if k_lens is not None:
+        see &= j < k_lens.long().cpu()[:, None, None]
+    if q_docs is not None:
+        qd, kd = q_docs.cpu()[:, :, None], k_docs.cpu()[:, None, :]
+        see &= (qd == kd) & (kd >= 0)
+    return see, (i - j).abs().double()
+
+
+def masked_attention(q, k, v, g=None, scale=0.0, cap=0.0, slopes=None, **mask):
+    """{name: (value, bound)} of out, lse and, with g, dq, dk, dv; q {N, Tq, H, D}, k and v {N, Tk, Hkv, D}. Values of keys
+    and queries that no pair uses do not matter, finite or not."""
+    t = q.dtype
+    u = unit(t) if t != torch.float32 else 0.0
+    q, k, v = (x.detach().cpu().double() for x in (q, k, v))
+    N, Tq, H, D = q.shape
+    Tk, grp = k.shape[1], H // k.shape[2]
+    scale = scale or 1.0 / math.sqrt(D)
+    see, far = visible(N, Tq, Tk, **mask)
+    kq = see.any(2)  # queries and keys that are in use
+    kk = see.any(1)
+    q = torch.where(kq[:, :, None, None], q, 0.0)
+    k, v = (torch.where(kk[:, :, None, None], x, 0.0) for x in (k, v))
+    Q, K, V = q.transpose(1, 2), k.transpose(1, 2).repeat_interleave(grp, 1), v.transpose(1, 2).repeat_interleave(grp, 1)
+    see, far = see[:, None], far[:, None]
+    s = scale * Q @ K.transpose(2, 3)
+    es = (D + 2) * U32 * scale * (Q.abs() @ K.abs().transpose(2, 3))
+    th = torch.tanh(s / cap) if cap else None
+    z = cap * th if cap else s
+    # the 16-bit kernels' tanh is off by up to 4 u32 of 1 (its reciprocal and exponential), the 32-bit ones' by as much of it
+    ez = es + (4 * U32 * (cap if t != torch.float32 else (cap * th).abs()) + 4 * U32 * z.abs() if cap else 2 * U32 * z.abs())
+    if slopes is not None:
+        b = slopes.double().cpu()[None, :, None, None] * far
+        z = z - b
+        ez = ez + 4 * U32 * (b + z.abs())
+    z = torch.where(see, z, -math.inf)
+    lse = torch.logsumexp(z, 3)
+    p = torch.where(see, torch.exp(z - torch.where(lse == -math.inf, 0.0, lse)[..., None]), 0.0)
+    ez = torch.where(see, ez + 4 * U32 * (1 + z.abs().nan_to_num(posinf=0.0)), 0.0)
+    worst = ez.amax(3, keepdim=True) if Tk else ez.sum(3, keepdim=True)  # of a row's scores: what its maximum and sum can be off by
+    ep = p * (ez + worst + (Tk + 8) * U32)
+    o = p @ V
+    eo = (ep + p * (u + Tk * U32)) @ V.abs()
+    back = lambda x: x.transpose(1, 2)  # noqa: E731
+    stored = lambda x, e: (back(x), back(e + (u + 2 * U32) * (x.abs() + e)))  # noqa: E731
+    res = {"out": stored(o, eo), "lse": (lse, worst[..., 0] + (Tk + 4) * U32 + 4 * U32 * lse.abs().nan_to_num(posinf=0.0))}
+    if g is None:
+        return res
+    G = torch.where(kq[:, :, None, None], g.detach().cpu().double(), 0.0).transpose(1, 2)
+    dp = G @ V.transpose(2, 3)
+    delta = (G * o).sum(3, keepdim=True)
+    # delta is taken from the stored out
+    ed = (G.abs() * (eo + (u + 2 * U32) * (o.abs() + eo))).sum(3, keepdim=True) + D * U32 * (G.abs() * o.abs()).sum(3, keepdim=True)
+    edp = (D + 2) * U32 * (G.abs() @ V.abs().transpose(2, 3))
+    ep = ep + 4 * U32 * p * (1 + lse.abs().nan_to_num(posinf=0.0))[..., None]
+    bend = 1.0 - th * th if cap else torch.ones_like(s)
+    ds = p * (dp - delta) * bend
+    eds = ep * (dp - delta).abs() * bend + p * (edp + ed) * bend + (u + 6 * U32) * ds.abs()
+    if cap:
+        eds = eds + p * (dp - delta).abs() * 12 * U32 + p * (dp - delta).abs() * 2 * th.abs() * es / cap
+    fold = lambda x: x.view(N, H // grp, grp, Tk, D).sum(2)  # noqa: E731
+    res["dq"] = stored(scale * ds @ K, scale * (eds + Tk * U32 * ds.abs()) @ K.abs())
+    st, est = ds.transpose(2, 3), (eds + Tq * grp * U32 * ds.abs()).transpose(2, 3)
+    res["dk"] = stored(fold(scale * st @ Q), fold(scale * est @ Q.abs()))
+    pt, ept = p.transpose(2, 3), (ep + p * (u + Tq * grp * U32)).transpose(2, 3)
+    res["dv"] = stored(fold(pt @ G), fold(ept @ G.abs()))
+    return res
+
+
+def assert_within(got, want, what=""):
+    """got (a tensor) against (value, bound), not finite values included."""
+    value, bound = want
+    got = got.detach().cpu().double()
+    assert got.shape == value.shape, (what, got.shape, value.shape)
+    fine = torch.isfinite(value)
+    assert torch.equal(torch.isnan(got), torch.isnan(value)), f"{what}: NaN in other places"
+    assert torch.equal(got[~fine].nan_to_num(nan=0.0), value[~fine].nan_to_num(nan=0.0)), f"{what}: infinities differ"
+    over = (got - value).abs()[fine] - bound[fine]
+    if over.numel() and over.max() > 0:
+        at = int(over.argmax())
+        raise AssertionError(f"{what}: {int((over > 0).sum())} of {over.numel()} out of bounds; worst: got "
+                             f"{got[fine][at].item()}, want {value[fine][at].item()} within {bound[fine][at].item()}")
