@@ -512,6 +512,41 @@ int nnh_masked_attention_backward(int type, size_t N, size_t Tq, size_t Tk, size
 int nnh_masked_attention_workspace_size(size_t N, size_t Tq, size_t Tk, size_t H, size_t Hkv, size_t Dh, int documents,
                                         int backward, size_t* bytes);
 
+/* One tensor of an AdamW step: count parameters, their gradients, the two moments (fp32, or 8-bit codes with a scale byte
+ * for each 64 elements, ceil(count / 64) of them) and, where wanted, a bf16 copy that the new parameters are stored to. */
+typedef struct nnh_adamw_tensor {
+	void* p;
+	const void* g;
+	void* m;
+	void* v;
+	unsigned char* m_scale; /* 8 bits only */
+	unsigned char* v_scale;
+	void* copy; /* may be NULL */
+	size_t count;
+} nnh_adamw_tensor;
+
+typedef struct nnh_adamw {
+	int p_type, g_type; /* NNH_F32 or NNH_BF16 */
+	int bits;           /* 32 or 8: how the moments are kept */
+	double lr, beta1, beta2, eps, weight_decay;
+	size_t step;             /* t, from 1 */
+	const int* step_device;  /* device memory, or NULL: t read when the step runs, in place of step */
+	const float* lr_device;  /* the same for lr */
+	const float* grad_scale; /* the same: a factor of every gradient (clipping, a loss scale's inverse) */
+} nnh_adamw;
+
+/*
+ * One AdamW step over n tensors (the reference's optimizer updates one at a time on the host, src/optim/adamw.cpp:15), a
+ * launch for each 52 of them:
+ *   g' = grad_scale g;  m = beta1 m + (1 - beta1) g';  v = beta2 v + (1 - beta2) g'^2
+ *   p = p (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * Moments in 8 bits: a block of 64 elements (from each tensor's first) has one scale 2^(byte - 127); m is an e4m3 code
+ * times it, v the square of one. Codes are the nearest to the value in 64 bits, ties to even; the scale brings the block's
+ * largest value into [128, 256); a second moment that is not zero does not become zero. All bytes 0 is a state of zeros.
+ * What the step writes overlaps nothing else it uses: a tensor given twice is refused.
+ */
+int nnh_adamw_step(const nnh_adamw* options, const nnh_adamw_tensor* tensors, size_t n, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

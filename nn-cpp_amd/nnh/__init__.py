@@ -128,6 +128,7 @@ _EXTRA_DECLS = {
     "nnh_masked_attention_forward": [C.c_int] + [_sz] * 6 + [_vp] * 7,
     "nnh_masked_attention_backward": [C.c_int] + [_sz] * 6 + [_vp] * 8 + [C.c_int, _vp, C.c_int, _vp, C.c_int, _vp],
     "nnh_masked_attention_workspace_size": [_sz] * 6 + [C.c_int, C.c_int, _szp],
+    "nnh_adamw_step": [_vp, _vp, _sz, _vp],
     "nnh_set_stream_numerics": [_vp, C.c_int],
     "nnh_get_stream_numerics": [_vp],
 }
@@ -721,6 +722,75 @@ def masked_attention_backward(g, q, k, v, out, lse, rule, dq=None, dq_first=True
                                               _on(lse, device, torch.float32, (N, H, Tq), "lse"), C.byref(r), t[5],
                                               int(dq_first), t[6], int(dk_first), t[7], int(dv_first), _stream(stream)))
     return tuple(grads)
+
+
+class AdamWTensor(C.Structure):
+    _fields_ = [("p", _vp), ("g", _vp), ("m", _vp), ("v", _vp), ("m_scale", _vp), ("v_scale", _vp), ("copy", _vp),
+                ("count", _sz)]
+
+
+class _AdamW(C.Structure):
+    _fields_ = [("p_type", C.c_int), ("g_type", C.c_int), ("bits", C.c_int), ("lr", C.c_double), ("beta1", C.c_double),
+                ("beta2", C.c_double), ("eps", C.c_double), ("weight_decay", C.c_double), ("step", _sz),
+                ("step_device", _vp), ("lr_device", _vp), ("grad_scale", _vp)]
+
+
+class AdamW:
+    """AdamW over lists of parameters and their gradient buffers (contiguous, fp32 or bf16, one type each), both kept by the
+    caller. The moments m and v are made here (zeros, kept in `bits` bits) or given: fp32 tensors, or uint8 codes with uint8
+    m_scale and v_scale of ceil(count / 64) elements. copies: bf16 tensors that the new parameters are also stored to."""
+
+    def __init__(self, params, grads, m=None, v=None, m_scale=None, v_scale=None, copies=None, bits=32, lr=1e-3, beta1=0.9,
+                 beta2=0.999, eps=1e-8, weight_decay=0.01, steps=0):
+        torch = _torch or _load_torch()
+        device = torch.cuda.current_device()
+        self.params, self.grads, self.copies, n = list(params), list(grads), copies, len(params)
+        self.lr, self.beta1, self.beta2, self.eps, self.weight_decay = lr, beta1, beta2, eps, weight_decay
+        self.steps = int(steps)
+        self.bits = bits if m is None else 8 if len(m) and m[0].dtype == torch.uint8 else 32
+        kept = torch.uint8 if self.bits == 8 else torch.float32
+        if (m is None) != (v is None) or (m is not None and self.bits == 8 and (m_scale is None or v_scale is None)):
+            raise NnhError(ERR_INVALID, "moments are given together, in 8 bits with their scales")
+
+        def zeros(per, dtype):
+            return [torch.zeros((p.numel() + per - 1) // per, dtype=dtype, device=p.device) for p in self.params]
+
+        self.m, self.v = (zeros(1, kept), zeros(1, kept)) if m is None else (list(m), list(v))
+        self.m_scale = self.v_scale = [None] * n
+        if self.bits == 8:
+            self.m_scale, self.v_scale = (zeros(64, torch.uint8), zeros(64, torch.uint8)) if m is None else (list(m_scale), list(v_scale))
+        outs = [None] * n if copies is None else list(copies)
+        lists = (self.params, self.grads, self.m, self.v, self.m_scale, self.v_scale, outs)
+        if any(len(x) != n for x in lists):
+            raise ShapeError(ERR_SHAPE, "one tensor of each kind for every parameter")
+        self._tensors = (AdamWTensor * max(1, n))()
+        for i, row in enumerate(zip(*lists)):
+            count = row[0].numel()
+            for t, what, dtype, size in zip(row, ("a parameter", "a gradient", "m", "v", "m_scale", "v_scale", "a copy"),
+                                            (self.params[0].dtype, self.grads[0].dtype, kept, kept, torch.uint8, torch.uint8, torch.bfloat16),
+                                            (count, count, count, count, (count + 63) // 64, (count + 63) // 64, count)):
+                if t is None:
+                    continue
+                if t.numel() != size:
+                    raise ShapeError(ERR_SHAPE, f"{what} has {t.numel()} elements, not {size}")
+                _on(t, device, dtype, tuple(t.shape), what)
+            self._tensors[i] = AdamWTensor(*(None if t is None else t.data_ptr() for t in row), count)
+        self._types = (_type(self.params[0]), _type(self.grads[0])) if n else (F32, F32)
+        self._n = n
+
+    def step(self, grad_scale=None, lr_device=None, step_device=None, stream=None):
+        """One step; grad_scale and lr_device: one-element fp32 tensors, step_device: an int32 one that holds this step's number
+        (for a captured step; self.steps counts calls either way)."""
+        torch = _torch or _load_torch()
+        device = torch.cuda.current_device()
+        for t, dtype, what in ((grad_scale, torch.float32, "grad_scale"), (lr_device, torch.float32, "lr_device"), (step_device, torch.int32, "step_device")):
+            if t is not None and t.numel() != 1:
+                raise ShapeError(ERR_SHAPE, f"{what} must have one element")
+            _on(t, device, dtype, None, what)
+        o = _AdamW(*self._types, self.bits, self.lr, self.beta1, self.beta2, self.eps, self.weight_decay, self.steps + 1,
+                   *(None if t is None else t.data_ptr() for t in (step_device, lr_device, grad_scale)))
+        check(lib().nnh_adamw_step(C.byref(o), self._tensors, self._n, _stream(stream)))
+        self.steps += 1
 
 
 _bench_lib = None

@@ -106,3 +106,39 @@ def assert_within(got, want, what=""):
         at = int(over.argmax())
         raise AssertionError(f"{what}: {int((over > 0).sum())} of {over.numel()} out of bounds; worst: got "
                              f"{got[fine][at].item()}, want {value[fine][at].item()} within {bound[fine][at].item()}")
+
+
+# ---- AdamW ----
+
+E4M3 = torch.arange(127, dtype=torch.uint8).view(torch.float8_e4m3fn).double()  # 0 .. 448
+
+
+def nearest_e4m3(x):
+    """The nearest e4m3 values of |x| <= 448, ties to the even code."""
+    border, a = (E4M3[1:] + E4M3[:-1]) / 2, x.abs()
+    low, high = torch.searchsorted(border, a), torch.searchsorted(border, a, right=True)
+    return torch.copysign(E4M3[torch.where(low % 2 == 0, low, high)], x)
+
+
+def block_codes(x, root):
+    """Moments as 8-bit codes and scale bytes (root: x is v, kept as its square root), and the values they stand for."""
+    n = x.numel()
+    y = torch.nn.functional.pad(x.sqrt() if root else x, (0, -n % 64)).view(-1, 64)
+    fine = torch.where(torch.isfinite(y), y, 0.0)
+    top = fine.abs().amax(1, keepdim=True)
+    e = torch.where(top > 0, (torch.frexp(top).exponent - 8 + 127).clamp(0, 254), 0)
+    unit = torch.tensor([math.ldexp(1.0, k - 127) for k in range(255)], dtype=torch.float64)[e.long()]
+    q = nearest_e4m3(fine / unit)
+    if root:
+        q = torch.where((fine > 0) & (q == 0), 2.0 ** -9, q)
+    q = torch.where(torch.isfinite(y), q, math.nan)
+    return q.view(-1)[:n], e.view(-1).to(torch.uint8), (q * unit).view(-1)[:n]
+
+
+def adamw(p, g, m, v, step, lr, beta1, beta2, eps, weight_decay, scale=1.0):
+    """One step in 64 bits: new p, m and v."""
+    p, g, m, v = p.double(), g.double() * scale, m.double(), v.double()
+    m = beta1 * m + (1 - beta1) * g
+    v = beta2 * v + (1 - beta2) * g * g
+    new = p - lr * weight_decay * p - lr * (m / (1 - beta1 ** step)) / ((v / (1 - beta2 ** step)).sqrt() + eps)
+    return new, m, v
