@@ -547,6 +547,35 @@ typedef struct nnh_adamw {
  */
 int nnh_adamw_step(const nnh_adamw* options, const nnh_adamw_tensor* tensors, size_t n, void* stream);
 
+#define NNH_REDUCE_NONE 0 /* a loss (and a gradient g) for every row */
+#define NNH_REDUCE_MEAN 1 /* one: the mean over the rows that have a target (NaN without any) */
+#define NNH_REDUCE_SUM 2
+
+/*
+ * Softmax cross entropy of a linear head: z = x w^T + bias, lse = log sum exp z over the vocabulary, loss = lse - z[target],
+ * for x {rows, D}, w {V, D}, bias {V} or NULL (all of one type, contiguous) and targets {rows} (int32, device memory). A
+ * negative target means none: loss 0, no gradient, not counted by the mean. A target of V or more gives a NaN loss and no
+ * gradient. The scores are made in pieces of the vocabulary and not kept; loss {rows} or {1} and lse {rows} are fp32.
+ * bf16 rows of a length that is no multiple of 8, or not 16-byte aligned, are first copied to scratch.
+ */
+int nnh_linear_cross_entropy_forward(int type, const void* x, size_t rows, size_t D, const void* w, size_t V, const void* bias,
+                                     const int* targets, int reduction, float* loss, float* lse, void* stream);
+
+/* Its backward rule from the forward's lse, the scores made again: gradients of x, w and bias (NULL: not wanted) given g {rows}
+ * or {1}, loss's (NULL: ones). *_first stores, otherwise the gradient is added to what is there. */
+int nnh_linear_cross_entropy_backward(int type, const float* g, const void* x, size_t rows, size_t D, const void* w, size_t V,
+                                      const void* bias, const int* targets, const float* lse, int reduction, void* dx, int dx_first,
+                                      void* dw, int dw_first, void* db, int db_first, void* stream);
+
+/* Both in one call, for a g known beforehand: the scores are made once where rows * V elements take at most 4 GiB, which
+ * they then do in scratch for the length of the call. */
+int nnh_linear_cross_entropy_train(int type, const float* g, const void* x, size_t rows, size_t D, const void* w, size_t V,
+                                   const void* bias, const int* targets, int reduction, float* loss, void* dx, int dx_first, void* dw,
+                                   int dw_first, void* db, int db_first, void* stream);
+
+/* Scratch of a call: 0 forward, 1 backward, 2 train; aligned: whether bf16 x and w are 16-byte aligned. */
+int nnh_linear_cross_entropy_workspace_size(int type, size_t rows, size_t D, size_t V, int call, int aligned, size_t* bytes);
+
 #ifdef __cplusplus
 }
 #endif

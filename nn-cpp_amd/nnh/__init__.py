@@ -129,6 +129,12 @@ _EXTRA_DECLS = {
     "nnh_masked_attention_backward": [C.c_int] + [_sz] * 6 + [_vp] * 8 + [C.c_int, _vp, C.c_int, _vp, C.c_int, _vp],
     "nnh_masked_attention_workspace_size": [_sz] * 6 + [C.c_int, C.c_int, _szp],
     "nnh_adamw_step": [_vp, _vp, _sz, _vp],
+    "nnh_linear_cross_entropy_forward": [C.c_int, _vp, _sz, _sz, _vp, _sz, _vp, _vp, C.c_int, _vp, _vp, _vp],
+    "nnh_linear_cross_entropy_backward": [C.c_int, _vp, _vp, _sz, _sz, _vp, _sz, _vp, _vp, _vp, C.c_int, _vp, C.c_int, _vp,
+                                          C.c_int, _vp, C.c_int, _vp],
+    "nnh_linear_cross_entropy_train": [C.c_int, _vp, _vp, _sz, _sz, _vp, _sz, _vp, _vp, C.c_int, _vp, _vp, C.c_int, _vp,
+                                       C.c_int, _vp, C.c_int, _vp],
+    "nnh_linear_cross_entropy_workspace_size": [C.c_int, _sz, _sz, _sz, C.c_int, C.c_int, _szp],
     "nnh_set_stream_numerics": [_vp, C.c_int],
     "nnh_get_stream_numerics": [_vp],
 }
@@ -722,6 +728,83 @@ def masked_attention_backward(g, q, k, v, out, lse, rule, dq=None, dq_first=True
                                               _on(lse, device, torch.float32, (N, H, Tq), "lse"), C.byref(r), t[5],
                                               int(dq_first), t[6], int(dk_first), t[7], int(dv_first), _stream(stream)))
     return tuple(grads)
+
+
+_REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+
+
+def _head(x, w, targets, bias, reduction):
+    """The arguments that the cross entropy calls share, checked: (type, rows, D, V, leading shape, device, reduction)."""
+    torch = _torch or _load_torch()
+    device = torch.cuda.current_device()
+    if x.dim() < 1 or w.dim() != 2 or x.shape[-1] != w.shape[1]:
+        raise ShapeError(ERR_SHAPE, "x is {..., D} and w {V, D}")
+    if reduction not in _REDUCTIONS:
+        raise NnhError(ERR_INVALID, f"reduction must be one of {sorted(_REDUCTIONS)}")
+    lead, (V, D) = tuple(x.shape[:-1]), w.shape
+    rows = targets.numel()
+    _on(x, device, None, lead + (D,), "x")
+    _on(w, device, x.dtype, (V, D), "w")
+    _on(bias, device, x.dtype, (V,), "bias")
+    _on(targets, device, torch.int32, lead, "targets")
+    return _type(x), rows, D, V, lead, device, _REDUCTIONS[reduction]
+
+
+def linear_cross_entropy_forward(x, w, targets, bias=None, reduction="mean", stream=None):
+    """nnh_linear_cross_entropy_forward on contiguous x {..., D}, w {V, D} (fp32 or bf16) and int32 targets {...}; returns
+    (loss, lse) in fp32, loss of targets' shape or, for "mean" and "sum", one number."""
+    torch = _torch or _load_torch()
+    t, rows, D, V, lead, _, red = _head(x, w, targets, bias, reduction)
+    loss = torch.empty(() if red else lead, dtype=torch.float32, device=x.device)
+    lse = torch.empty(lead, dtype=torch.float32, device=x.device)
+    check(lib().nnh_linear_cross_entropy_forward(t, x.data_ptr(), rows, D, w.data_ptr(), V, None if bias is None else bias.data_ptr(),
+                                                 targets.data_ptr(), red, loss.data_ptr(), lse.data_ptr(), _stream(stream)))
+    return loss, lse
+
+
+def _head_gradients(x, w, bias, device, dx, dw, db, firsts):
+    torch = _torch or _load_torch()
+    out = []
+    for t, like, first, what in ((dx, x, firsts[0], "dx"), (dw, w, firsts[1], "dw"), (db, bias, firsts[2], "db")):
+        if t is None and like is not None:
+            if not first:
+                raise NnhError(ERR_INVALID, "a gradient to add to has to be given")
+            t = torch.empty_like(like)
+        if t is not None:
+            _on(t, device, x.dtype, tuple(like.shape) if like is not None else (w.shape[0],), what)
+        out.append(t)
+    return out
+
+
+def linear_cross_entropy_backward(g, x, w, targets, lse, bias=None, reduction="mean", dx=None, dx_first=True, dw=None,
+                                  dw_first=True, db=None, db_first=True, stream=None):
+    """nnh_linear_cross_entropy_backward; g: the loss's gradient (fp32, of its shape) or None for ones. Gradients that are not
+    given are made (db where there is a bias); returns (dx, dw, db)."""
+    torch = _torch or _load_torch()
+    t, rows, D, V, lead, device, red = _head(x, w, targets, bias, reduction)
+    _on(lse, device, torch.float32, lead, "lse")
+    _on(g, device, torch.float32, () if red else lead, "g")
+    out = _head_gradients(x, w, bias, device, dx, dw, db, (dx_first, dw_first, db_first))
+    p = [None if o is None else o.data_ptr() for o in [g, bias] + out]
+    check(lib().nnh_linear_cross_entropy_backward(t, p[0], x.data_ptr(), rows, D, w.data_ptr(), V, p[1], targets.data_ptr(),
+                                                  lse.data_ptr(), red, p[2], int(dx_first), p[3], int(dw_first), p[4],
+                                                  int(db_first), _stream(stream)))
+    return tuple(out)
+
+
+def linear_cross_entropy_train(x, w, targets, bias=None, reduction="mean", g=None, dx=None, dx_first=True, dw=None,
+                               dw_first=True, db=None, db_first=True, stream=None):
+    """nnh_linear_cross_entropy_train: forward and backward in one call; returns (loss, dx, dw, db)."""
+    torch = _torch or _load_torch()
+    t, rows, D, V, lead, device, red = _head(x, w, targets, bias, reduction)
+    _on(g, device, torch.float32, () if red else lead, "g")
+    loss = torch.empty(() if red else lead, dtype=torch.float32, device=x.device)
+    out = _head_gradients(x, w, bias, device, dx, dw, db, (dx_first, dw_first, db_first))
+    p = [None if o is None else o.data_ptr() for o in [g, bias] + out]
+    check(lib().nnh_linear_cross_entropy_train(t, p[0], x.data_ptr(), rows, D, w.data_ptr(), V, p[1], targets.data_ptr(), red,
+                                               loss.data_ptr(), p[2], int(dx_first), p[3], int(dw_first), p[4], int(db_first),
+                                               _stream(stream)))
+    return (loss,) + tuple(out)
 
 
 class AdamWTensor(C.Structure):

@@ -1,0 +1,285 @@
+// gemm16.hpp - bf16 products on the matrix cores for the linear head's cross entropy, with its epilogues (internal to libnnh).
+//
+// out[outer][inner] = sum over depth of A[inner][depth] B[outer][depth], fp32 accumulators. The product is computed
+// transposed (A's rows are the MFMA's rows), so a lane holds, of one outer row, runs of four consecutive inner elements:
+// a softmax over the inner axis is a reduction within the lane.
+//
+// What bounds it: the matrix cores, 32 cycles a 32 x 32 x 16 MFMA and SIMD. A workgroup's waves hold 128 x 64 (64 x 64) of the
+// tile each, so a depth of 16 takes 6 KB (4 KB) of operands from LDS for 256 (128) cycles of MFMA: three quarters of (as
+// much as) LDS delivers beside. Operands go from memory into LDS without passing through registers, one 64-deep stage
+// ahead of the one in use, one barrier a stage; an operand whose depth is not the contiguous axis is read by transposed LDS
+// reads and needs no transposed copy.
+#pragma once
+
+#include "linear_cross_entropy.hpp"
+#include "masked_attention_tile.hpp"
+
+namespace nnh {
+namespace g16 {
+
+using attn::bf16x2;
+using attn::f32x16;
+using attn::f32x2;
+using attn::f32x4;
+using attn::Frag;
+using attn::global_void;
+using attn::kInf;
+using attn::kLog2e;
+using attn::lds_s16x4;
+using attn::lds_void;
+using attn::u32x4;
+
+constexpr int BK = 64;
+
+template <int BM_, int BN_, int WM_, int WN_>
+struct Tile {
+	static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;
+	static constexpr int kWaves = (BM / WM) * (BN / WN), kThreads = 64 * kWaves;
+	static constexpr int kA = BM * BK * 2, kB = BN * BK * 2, kStage = kA + kB;  // bytes
+	static constexpr int kLds = 2 * kStage > BM * BN * 2 ? 2 * kStage : BM * BN * 2;
+	static_assert(kA % (1024 * kWaves) == 0 && kB % (1024 * kWaves) == 0, "a stage splits evenly over the waves");
+	static_assert(kLds <= 160 * 1024, "LDS");
+};
+
+// What a wave loads of one operand, R rows to the tile: kSteps words a lane and stage. TR: depth is not contiguous.
+template <int R, int NW, bool TR>
+struct Loader {
+	static constexpr int kSteps = R * BK * 2 / 1024 / NW;
+	const __bf16* p[kSteps];
+	int64_t step;  // elements from one stage to the next
+
+	__device__ __forceinline__ void begin(const __bf16* base, int64_t ld, int first_row, int rows, int wave, int lane) {
+		step = TR ? BK * ld : BK;
+#pragma unroll
+		for (int j = 0; j < kSteps; ++j) {
+			const int w = (j * NW + wave) * 64 + lane;
+			if (TR) {
+				const int k = w / (R / 8), c = (w % (R / 8)) ^ attn::swizzle<R * 2>(k);
+				// words past the operand's rows come from its first ones: their outputs are not stored
+				const int r = first_row + c * 8 < rows ? first_row + c * 8 : 0;
+				p[j] = base + k * ld + r;
+			} else {
+				const int r = w / 8, c = (w % 8) ^ attn::swizzle<128>(r);
+				p[j] = base + (int64_t)min(first_row + r, rows - 1) * ld + c * 8;
+			}
+		}
+	}
+	// Loads the stage and moves on; live: depths left (what is past them is zero).
+	__device__ __forceinline__ void load(char* tile, int live, int wave, int lane) {
+#pragma unroll
+		for (int j = 0; j < kSteps; ++j) {
+			const int w = (j * NW + wave) * 64 + lane;
+			const void* src = p[j];
+			if (live < BK) {
+				const int k = TR ? w / (R / 8) : ((w % 8) ^ attn::swizzle<128>(w / 8)) * 8;
+				if (k >= live) src = &attn::kZeroWord;
+			}
+			__builtin_amdgcn_global_load_lds((global_void*)src, (lds_void*)(tile + (j * NW + wave) * 1024), 16, 0, 0);
+			p[j] += step;
+		}
+	}
+};
+
+// Operand rows row0 + lane % 32, depths 16 t + 8 (lane / 32) + 0..7.
+template <int R, bool TR>
+__device__ __forceinline__ void operand(Frag<__bf16>& f, const char* tile, int row0, int lane, int t) {
+	if (!TR) {
+		attn::rows_of<__bf16, 64>(f, tile, row0 + (lane & 31), lane >> 5, t);
+	} else {
+		const int i = lane & 15, r = row0 + 16 * ((lane >> 4) & 1) + 4 * (i & 3);
+#pragma unroll
+		for (int x = 0; x < 2; ++x) {
+			const int k = 16 * t + 8 * (lane >> 5) + 4 * x + (i >> 2);
+			const char* at = tile + k * (R * 2) + (((r >> 3) ^ attn::swizzle<R * 2>(k)) * 16) + (r & 4) * 2;
+			f.h[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at);
+		}
+	}
+}
+
+// Which tile of the grid a workgroup takes: a run of tiles to each XCD, eight outer tiles wide, so that the tiles in
+// flight on one share their operands in its L2.
+__device__ __forceinline__ void tile_of(int inner_tiles, int outer_tiles, int& inner, int& outer) {
+	const unsigned total = (unsigned)inner_tiles * outer_tiles, q = total / 8, r = total % 8, x = blockIdx.x % 8;
+	const unsigned id = x * q + min(x, r) + blockIdx.x / 8;
+	const unsigned g = id / (8u * inner_tiles), in = id % (8u * inner_tiles), width = min(8u, outer_tiles - 8 * g);
+	outer = 8 * g + in % width;
+	inner = in / width;
+}
+
+template <class T, bool ATR, bool BTR, int EPI>
+__global__ __launch_bounds__(T::kThreads, 2) void gemm16_kernel(Gemm16Args a) {
+	constexpr int BM = T::BM, BN = T::BN, WM = T::WM, WN = T::WN, I = WM / 32, J = WN / 32, NW = T::kWaves;
+	__shared__ __attribute__((aligned(1024))) char lds[T::kLds];
+	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+	const int col = lane & 31, half = lane >> 5, wm = wave % (BM / WM) * WM, wn = wave / (BM / WM) * WN;
+	int m0, n0;
+	tile_of((a.inner + BM - 1) / BM, (a.outer + BN - 1) / BN, m0, n0);
+	m0 *= BM;
+	n0 *= BN;
+	Loader<BM, NW, ATR> la;
+	Loader<BN, NW, BTR> lb;
+	la.begin((const __bf16*)a.a, a.lda, m0, a.inner, wave, lane);
+	lb.begin((const __bf16*)a.b, a.ldb, n0, a.outer, wave, lane);
+	f32x16 acc[I][J];
+#pragma unroll
+	for (int i = 0; i < I; ++i)
+#pragma unroll
+		for (int j = 0; j < J; ++j)
+#pragma unroll
+			for (int x = 0; x < 16; ++x) acc[i][j][x] = 0.0f;
+
+	const int stages = (a.depth + BK - 1) / BK;
+	la.load(lds, a.depth, wave, lane);
+	lb.load(lds + T::kA, a.depth, wave, lane);
+	for (int s = 0; s < stages; ++s) {
+		attn::wait_loads();
+		__builtin_amdgcn_s_barrier();  // the stage has arrived for all waves, and all are done with the other one
+		asm volatile("" ::: "memory");
+		const char* at = lds + (s & 1) * T::kStage;
+		if (s + 1 < stages) {
+			char* to = lds + (~s & 1) * T::kStage;
+			const int live = a.depth - (s + 1) * BK;
+			la.load(to, live, wave, lane);
+			lb.load(to + T::kA, live, wave, lane);
+		}
+#pragma unroll
+		for (int t = 0; t < BK / 16; ++t) {
+			Frag<__bf16> fa[I], fb[J];
+#pragma unroll
+			for (int i = 0; i < I; ++i) operand<BM, ATR>(fa[i], at, wm + 32 * i, lane, t);
+#pragma unroll
+			for (int j = 0; j < J; ++j) operand<BN, BTR>(fb[j], at + T::kA, wn + 32 * j, lane, t);
+#pragma unroll
+			for (int i = 0; i < I; ++i)
+#pragma unroll
+				for (int j = 0; j < J; ++j) attn::mma(acc[i][j], fa[i], fb[j]);
+		}
+	}
+	__syncthreads();  // LDS is the output tile's from here on
+
+	// register 4 g + x of block (i, j): inner m0 + wm + 32 i + 8 g + 4 half + x, outer n0 + wn + 32 j + col
+	const int mw = m0 + wm + 4 * half;
+	if constexpr (EPI == kGemm16Out) {
+		const float scale = a.scale ? *a.scale * a.factor : a.factor;
+#pragma unroll
+		for (int j = 0; j < J; ++j) {
+			const int n = n0 + wn + 32 * j + col;
+			if (n >= a.outer) continue;
+#pragma unroll
+			for (int i = 0; i < I; ++i)
+#pragma unroll
+				for (int g = 0; g < 4; ++g) {
+					const int m = mw + 32 * i + 8 * g;
+#pragma unroll
+					for (int x = 0; x < 4; ++x) {
+						if (m + x >= a.inner) continue;
+						float y = acc[i][j][4 * g + x] * scale;
+						if (a.sum_in) y += a.sum[(int64_t)n * a.inner + m + x];
+						if (a.sum_out) {
+							a.sum[(int64_t)n * a.inner + m + x] = y;
+						} else {
+							__bf16* o = (__bf16*)a.out + (int64_t)n * a.ldo + m + x;
+							if (!a.first) y += (float)*o;
+							*o = (__bf16)y;
+						}
+					}
+				}
+		}
+		return;
+	} else {
+		// a row's scores z = x w + b, in the lane: the whole softmax's statistics of this wave's WM columns, and what the
+		// tile stores
+		__bf16* const tile = (__bf16*)lds;
+		if (a.bias) {
+#pragma unroll
+			for (int i = 0; i < I; ++i)
+#pragma unroll
+				for (int x = 0; x < 16; ++x) {
+					const int m = mw + 32 * i + 8 * (x / 4) + x % 4;
+					const float b = m < a.inner ? (float)((const __bf16*)a.bias)[m] : 0.0f;
+#pragma unroll
+					for (int j = 0; j < J; ++j) acc[i][j][x] += b;
+				}
+		}
+#pragma unroll
+		for (int j = 0; j < J; ++j) {
+			const int n = n0 + wn + 32 * j + col;
+			const bool on = n < a.outer;
+			const int target = on ? a.targets[n] - a.first_inner : -1;
+			if constexpr (EPI == kGemm16Grad) {
+				const float lse2 = on ? a.lse[n] * kLog2e : 0.0f, f = on ? a.weight[n] : 0.0f;
+#pragma unroll
+				for (int i = 0; i < I; ++i)
+#pragma unroll
+					for (int x = 0; x < 16; ++x) {
+						const int m = mw + 32 * i + 8 * (x / 4) + x % 4;
+						float y = attn::exp2_of(__builtin_fmaf(acc[i][j][x], kLog2e, -lse2));
+						y = (m == target ? y - 1.0f : y) * f;
+						acc[i][j][x] = m < a.inner && f != 0.0f ? y : 0.0f;
+					}
+			} else {
+				float top = -kInf, sum = 0.0f;
+				if (m0 + wm + WM > a.inner) {
+#pragma unroll
+					for (int i = 0; i < I; ++i)
+#pragma unroll
+						for (int x = 0; x < 16; ++x)
+							if (mw + 32 * i + 8 * (x / 4) + x % 4 >= a.inner) acc[i][j][x] = -kInf;
+				}
+#pragma unroll
+				for (int i = 0; i < I; ++i)
+#pragma unroll
+					for (int x = 0; x < 16; ++x) top = fmaxf(top, acc[i][j][x]);
+				top = attn::max_halves(top);
+				const int chunk = (m0 + wm) / WM;
+				if (__any(target >= m0 + wm && target < m0 + wm + WM)) {
+#pragma unroll
+					for (int i = 0; i < I; ++i)
+#pragma unroll
+						for (int x = 0; x < 16; ++x)
+							if (mw + 32 * i + 8 * (x / 4) + x % 4 == target && target < a.inner) a.hit[n] = acc[i][j][x];
+				}
+				const float base = top == -kInf ? 0.0f : top * kLog2e;
+#pragma unroll
+				for (int i = 0; i < I; ++i)
+#pragma unroll
+					for (int x = 0; x < 16; ++x) {
+						acc[i][j][x] = attn::exp2_of(__builtin_fmaf(acc[i][j][x], kLog2e, -base));
+						sum += acc[i][j][x];
+					}
+				sum = attn::add_halves(sum);
+				if (on && half == 0 && m0 + wm < a.inner) ((f32x2*)a.stats)[(int64_t)n * a.chunks + chunk] = f32x2{top, sum};
+			}
+		}
+		if constexpr (EPI != kGemm16Stats) {
+			// the tile in 16 bits through LDS, 16-byte words permuted by row, for whole rows of stores
+			constexpr int W = BM / 8;  // words to a row
+#pragma unroll
+			for (int j = 0; j < J; ++j) {
+				const int r = wn + 32 * j + col;
+#pragma unroll
+				for (int i = 0; i < I; ++i)
+#pragma unroll
+					for (int g = 0; g < 4; ++g) {
+						union {
+							bf16x2 p[2];
+							uint64_t w;
+						} y;
+						y.p[0] = __builtin_convertvector(f32x2{acc[i][j][4 * g], acc[i][j][4 * g + 1]}, bf16x2);
+						y.p[1] = __builtin_convertvector(f32x2{acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]}, bf16x2);
+						const int m = wm + 32 * i + 8 * g;
+						*(uint64_t*)(tile + r * BM + (((m / 8) ^ (r % W)) * 8) + 4 * half) = y.w;
+					}
+			}
+			__syncthreads();
+			for (int w = threadIdx.x; w < BN * W; w += T::kThreads) {
+				const int r = w / W, c = w % W;
+				if (n0 + r < a.outer && m0 + c * 8 < a.ldo)
+					*(u32x4*)((__bf16*)a.out + (int64_t)(n0 + r) * a.ldo + m0 + c * 8) = *(const u32x4*)(tile + r * BM + ((c ^ (r % W)) * 8));
+			}
+		}
+	}
+}
+
+}  // namespace g16
+}  // namespace nnh

@@ -142,3 +142,53 @@ def adamw(p, g, m, v, step, lr, beta1, beta2, eps, weight_decay, scale=1.0):
     v = beta2 * v + (1 - beta2) * g * g
     new = p - lr * weight_decay * p - lr * (m / (1 - beta1 ** step)) / ((v / (1 - beta2 ** step)).sqrt() + eps)
     return new, m, v
+
+
+# ---- linear cross entropy ----
+
+def linear_cross_entropy(x, w, targets, bias=None, reduction="mean", g=None, kept=False):
+    """{name: (value, bound)} of loss, lse, dx, dw and, with a bias, db. kept: the call that rounds exp(z) to bf16 before dz."""
+    t = x.dtype
+    u = unit(t) if t != torch.float32 else 0.0
+    x, w, targets = x.detach().cpu().double(), w.detach().cpu().double(), targets.cpu().long()
+    b = torch.zeros(w.shape[0], dtype=torch.float64) if bias is None else bias.detach().cpu().double()
+    D, V, rows = x.shape[1], w.shape[0], x.shape[0]
+    z = x @ w.t() + b
+    ez = (D + 2) * U32 * (x.abs() @ w.abs().t() + b.abs()) + 4 * U32 * (1 + z.abs())
+    worst = ez.amax(1, keepdim=True)
+    lse = torch.logsumexp(z, 1)
+    el = worst[:, 0] + (V + 8) * U32 + 4 * U32 * lse.abs()
+    live = (targets >= 0) & (targets < V)
+    count = int((targets >= 0).sum())
+    at = targets.clamp(0, V - 1)[:, None]
+    each = torch.where(live, lse - z.gather(1, at)[:, 0], torch.where(targets < 0, 0.0, math.nan))
+    ee = (el + ez.gather(1, at)[:, 0] + 2 * U32 * (lse.abs() + each.abs().nan_to_num())) * live
+    up = torch.ones(rows if reduction == "none" else (), dtype=torch.float64) if g is None else g.detach().cpu().double()
+    # the 32-bit calls' last sums are in 64 bits
+    if reduction == "none":
+        loss, eloss, f = each, ee, up[:, None]
+    elif reduction == "sum":
+        loss, eloss, f = each.sum(), ee.sum() + 2 * U32 * each.sum().abs(), up
+    else:
+        loss = each.sum() / count if count else torch.tensor(math.nan, dtype=torch.float64)
+        eloss, f = ee.sum() / max(1, count) + 2 * U32 * loss.abs(), up / max(1, count)
+    p = torch.exp(z - lse[:, None])
+    ep = p * (ez + el[:, None] + 4 * U32 * (1 + z.abs() + lse.abs()[:, None]))
+    hot = torch.zeros_like(p)
+    hot[live, targets[live]] = 1.0
+    dz, edz = (p - hot) * live[:, None], (ep + 2 * U32 * (p + hot)) * live[:, None]
+    edz = edz + (u * p if kept else 0.0) + u * (dz.abs() + edz)
+    if reduction == "none":  # a factor for each row is part of dz
+        dz, edz, f = dz * f, (edz + 2 * U32 * dz.abs()) * f.abs(), 1.0
+    f = torch.as_tensor(f, dtype=torch.float64)
+
+    def stored(v, e):
+        v, e = f * v, f.abs() * e
+        return v, e + (u + 6 * U32) * (v.abs() + e) + 1e-45
+
+    res = {"loss": (loss, eloss), "lse": (lse, el)}
+    res["dx"] = stored(dz @ w, (edz + V * U32 * dz.abs()) @ w.abs())
+    res["dw"] = stored(dz.t() @ x, (edz + rows * U32 * dz.abs()).t() @ x.abs())
+    if bias is not None:
+        res["db"] = stored(dz.sum(0), (edz + rows * U32 * dz.abs()).sum(0))
+    return res
