@@ -80,21 +80,31 @@ struct Loader {
 	}
 };
 
-// Operand rows row0 + lane % 32, depths 16 t + 8 (lane / 32) + 0..7.
+// Where a lane reads its operands: operand rows row0 + lane % 32 (row0 a multiple of 32), depths 16 t + 8 (lane / 32) + 0..7.
+// As in attn::Reader, further depths are an XOR or a constant away.
 template <int R, bool TR>
-__device__ __forceinline__ void operand(Frag<__bf16>& f, const char* tile, int row0, int lane, int t) {
-	if (!TR) {
-		attn::rows_of<__bf16, 64>(f, tile, row0 + (lane & 31), lane >> 5, t);
-	} else {
-		const int i = lane & 15, r = row0 + 16 * ((lane >> 4) & 1) + 4 * (i & 3);
-#pragma unroll
-		for (int x = 0; x < 2; ++x) {
-			const int k = 16 * t + 8 * (lane >> 5) + 4 * x + (i >> 2);
-			const char* at = tile + k * (R * 2) + (((r >> 3) ^ attn::swizzle<R * 2>(k)) * 16) + (r & 4) * 2;
-			f.h[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at);
+struct Reader {
+	int at;
+	__device__ __forceinline__ Reader(int row0, int lane) {
+		const int half = lane >> 5, i = lane & 15;
+		if (TR) {
+			const int k = 8 * half + (i >> 2);
+			at = k * (R * 2) + (((row0 / 8 + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1)) ^ attn::swizzle<R * 2>(k)) * 16) + (i & 1) * 8;
+		} else {
+			at = (row0 + (lane & 31)) * 128 + ((half ^ attn::swizzle<128>(lane & 31)) * 16);
 		}
 	}
-}
+	// Block i of 32 rows from row0 on.
+	__device__ __forceinline__ void read(Frag<__bf16>& f, const char* tile, int i, int t) const {
+		if (TR) {
+			// four rows further the permutation's low bits differ by 1; 16 rows further it is the same
+			f.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(tile + 16 * t * (R * 2) + (at ^ (64 * i))));
+			f.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(tile + (16 * t + 4) * (R * 2) + (at ^ (64 * i) ^ 16)));
+		} else {
+			f.w = *(const u32x4*)(tile + i * 32 * 128 + (at ^ (32 * t)));
+		}
+	}
+};
 
 // Which tile of the grid a workgroup takes: a run of tiles to each XCD, eight outer tiles wide, so that the tiles in
 // flight on one share their operands in its L2.
@@ -128,16 +138,17 @@ __global__ __launch_bounds__(T::kThreads, 2) void gemm16_kernel(Gemm16Args a) {
 #pragma unroll
 			for (int x = 0; x < 16; ++x) acc[i][j][x] = 0.0f;
 
+	const Reader<BM, ATR> ra(wm, lane);
+	const Reader<BN, BTR> rb(wn, lane);
 	const int stages = (a.depth + BK - 1) / BK;
 	la.load(lds, a.depth, wave, lane);
 	lb.load(lds + T::kA, a.depth, wave, lane);
-	for (int s = 0; s < stages; ++s) {
+	// one stage from `at`, the next one on its way to `to`
+	auto step = [&](int s, const char* at, char* to) {
 		attn::wait_loads();
 		__builtin_amdgcn_s_barrier();  // the stage has arrived for all waves, and all are done with the other one
 		asm volatile("" ::: "memory");
-		const char* at = lds + (s & 1) * T::kStage;
 		if (s + 1 < stages) {
-			char* to = lds + (~s & 1) * T::kStage;
 			const int live = a.depth - (s + 1) * BK;
 			la.load(to, live, wave, lane);
 			lb.load(to + T::kA, live, wave, lane);
@@ -146,14 +157,18 @@ __global__ __launch_bounds__(T::kThreads, 2) void gemm16_kernel(Gemm16Args a) {
 		for (int t = 0; t < BK / 16; ++t) {
 			Frag<__bf16> fa[I], fb[J];
 #pragma unroll
-			for (int i = 0; i < I; ++i) operand<BM, ATR>(fa[i], at, wm + 32 * i, lane, t);
+			for (int i = 0; i < I; ++i) ra.read(fa[i], at, i, t);
 #pragma unroll
-			for (int j = 0; j < J; ++j) operand<BN, BTR>(fb[j], at + T::kA, wn + 32 * j, lane, t);
+			for (int j = 0; j < J; ++j) rb.read(fb[j], at + T::kA, j, t);
 #pragma unroll
 			for (int i = 0; i < I; ++i)
 #pragma unroll
 				for (int j = 0; j < J; ++j) attn::mma(acc[i][j], fa[i], fb[j]);
 		}
+	};
+	for (int s = 0; s < stages; s += 2) {
+		step(s, lds, lds + T::kStage);
+		if (s + 1 < stages) step(s + 1, lds + T::kStage, lds);
 	}
 	__syncthreads();  // LDS is the output tile's from here on
 

@@ -9,6 +9,8 @@
 // atomics, so the results repeat bit for bit; the price is seven products of a pair of rows where five would do.
 #pragma once
 
+#include <type_traits>
+
 #include "masked_attention_tile.hpp"
 
 namespace nnh {
@@ -73,8 +75,10 @@ __device__ __forceinline__ void weights(f32x16& s, f32x16& slope, const MaskedAt
 }
 
 // dq: a workgroup's 128 queries of one head against the keys they see, as in the forward kernel: transposed scores, a query
-// a lane, dQ^T += K^T dS^T. Without a.dq it only leaves delta. The second pass is the forward's (values that are not finite
-// in a partly seen tile).
+// a lane, dQ^T += K^T dS^T. The second pass is the forward's (values that are not finite in a partly seen tile).
+//
+// It starts from delta = g.out of the stored out, which in 16 bits is off by out's rounding. A row's p add up to 1, so its
+// sum of p (g.v - delta) is what delta was off by: the delta that is left for the other kernel has it added.
 template <typename T, int DH, bool VEC>
 __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void masked_attention_dq_kernel(MaskedAttentionArgs a) {
 	constexpr int RB = row_bytes<T, DH>(), KT = RB >= 512 ? 32 : 64, kTile = KT * RB;
@@ -124,9 +128,7 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 			for (int j = 0; j < 8; ++j) delta += to_float(g[t].e[j]) * to_float(o.e[j]);
 		}
 		delta = add_halves(delta);
-		if (live_row && half == 0) a.delta[row] = delta;
 	}
-	if (!a.dq) return;
 	const Sight see = sight_of(a, n, i, live, pos0);
 	const int pos = pos0 + i;
 	const float slope2 = a.slopes ? a.slopes[h] * kLog2e : 0.0f, lse2 = a.lse[row] * kLog2e;
@@ -152,8 +154,11 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 	}
 	const int nt = (max(hi, pre) + KT - 1) / KT;
 	f32x16 d[DH / 32];
+	float off;
 
-	for (int pass = 0; pass < 2; ++pass) {
+	const Reader<T, RB> reader(lane);
+	auto run = [&](auto safe) {
+		off = 0.0f;
 #pragma unroll
 		for (int b = 0; b < DH / 32; ++b)
 #pragma unroll
@@ -176,9 +181,9 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 			on &= on - 1;
 			return base + x;
 		};
-		auto load = [&](int x, int buf) {
-			load_tile<T, DH, KT, kBwdWaves, VEC>(lds + buf * 2 * kTile, kbase + (int64_t)x * KT * a.ks.row, a.ks.row, live - x * KT, a.dh, wave, lane);
-			load_tile<T, DH, KT, kBwdWaves, VEC>(lds + (buf * 2 + 1) * kTile, vbase + (int64_t)x * KT * a.vs.row, a.vs.row, live - x * KT, a.dh, wave, lane);
+		auto load = [&](int x, char* to) {
+			load_tile<T, DH, KT, kBwdWaves, VEC>(to, kbase + (int64_t)x * KT * a.ks.row, a.ks.row, live - x * KT, a.dh, wave, lane);
+			load_tile<T, DH, KT, kBwdWaves, VEC>(to + kTile, vbase + (int64_t)x * KT * a.vs.row, a.vs.row, live - x * KT, a.dh, wave, lane);
 		};
 		auto take = [&](const char* kt, const char* vt, int k0) {
 			bool some = (k0 < see.hi && k0 + KT > see.lo) || k0 < see.pre;
@@ -191,28 +196,25 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 			if (!__any(some)) return;
 			const bool partial = !__all(all);
 			if (partial && a.k_docs && lane < KT) docs[lane] = a.k_docs[(int64_t)n * a.Tk + min(k0 + lane, a.Tk - 1)];
-#pragma unroll
+#pragma clang loop unroll(disable)
 			for (int x = 0; x < KT / 32; ++x) {
+				const Reader<T, RB> at = reader.again();
 				f32x16 s, dp, slope;
 #pragma unroll
 				for (int j = 0; j < 16; ++j) s[j] = dp[j] = 0.0f;
 #pragma unroll
 				for (int t = 0; t < DH / 16; ++t) {
 					Frag<T> f;
-					rows_of<T, DH>(f, kt, 32 * x + col, half, t);
+					at.rows(f, kt + 32 * x * RB, t);
 					mma(s, f, q[t]);
-					rows_of<T, DH>(f, vt, 32 * x + col, half, t);
+					at.rows(f, vt + 32 * x * RB, t);
 					mma(dp, f, g[t]);
 				}
-				const int j0 = k0 + 32 * x + 4 * half;
+				const int j0 = fresh(k0 + 32 * x + 4 * half);
 				weights<T>(s, slope, a, slope2, [&](int j) { const int y = pos - (j0 + 8 * (j / 4) + j % 4); return (float)(y < 0 ? -y : y); },
 				           [&](int) { return lse2; });
 #pragma unroll
 				for (int j = 0; j < 16; ++j) s[j] *= dp[j] - delta;
-				if (a.cap > 0.0f) {
-#pragma unroll
-					for (int j = 0; j < 16; ++j) s[j] *= slope[j];
-				}
 				unsigned seen = 0xffff;
 				if (partial) {
 					seen = 0;
@@ -229,7 +231,15 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 #pragma unroll
 					for (int j = 0; j < 16; ++j) s[j] = seen >> j & 1 ? s[j] : 0.0f;
 				}
-				const bool clean = pass != 0 && partial;
+				float part[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+				for (int j = 4; j < 16; ++j) part[j % 4] += s[j];
+				off += (part[0] + part[1]) + (part[2] + part[3]);
+				if (a.cap > 0.0f) {
+#pragma unroll
+					for (int j = 0; j < 16; ++j) s[j] *= slope[j];
+				}
+				const bool clean = decltype(safe)::value && partial;
 #pragma unroll
 				for (int t = 0; t < 2; ++t) {
 					Frag<T> ds;
@@ -237,7 +247,7 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 #pragma unroll
 					for (int b = 0; b < DH / 32; ++b) {
 						Frag<T> f;
-						columns_of<T, DH>(f, kt, 32 * x + 16 * t, lane, b);
+						at.columns(f, kt + (32 * x + 16 * t) * RB, b);
 						if (clean) only_finite(f);
 						mma(d[b], f, ds);
 					}
@@ -258,39 +268,47 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 				}
 			}
 		};
-		int cur = next(), buf = 0;
-		if (cur >= 0) load(cur, 0);
-		while (cur >= 0) {
+		int cur = next();
+		auto step = [&](char* from, char* to) {
 			wait_loads();
 			__builtin_amdgcn_s_barrier();
 			asm volatile("" ::: "memory");
 			const int then = next();
-			if (then >= 0) load(then, buf ^ 1);
-			take(lds + buf * 2 * kTile, lds + (buf * 2 + 1) * kTile, cur * KT);
+			if (then >= 0) load(then, to);
+			take(from, from + kTile, cur * KT);
 			cur = then;
-			buf ^= 1;
+		};
+		if (cur >= 0) load(cur, lds);
+		while (cur >= 0) {
+			step(lds, lds + 2 * kTile);
+			if (cur >= 0) step(lds + 2 * kTile, lds);
 		}
 		bool bad = false;
 #pragma unroll
 		for (int b = 0; b < DH / 32; ++b)
 #pragma unroll
 			for (int x = 0; x < 16; ++x) bad |= not_finite(d[b][x]);
-		if (!__syncthreads_or(bad)) break;
-	}
-	if (live_row)
+		return __syncthreads_or(bad);
+	};
+	if (run(std::false_type{})) run(std::true_type{});
+	off = add_halves(off);
+	if (live_row && half == 0) a.delta[row] = delta + off;
+	if (live_row && a.dq)
 		store_gradient<T, DH, VEC>((T*)a.dq + n * a.dqs.sample + (int64_t)i * a.dqs.row + h * a.dqs.head, d, a.scale, a.dh, half,
 		                           a.dq_first != 0);
 }
 
 // dk and dv: a workgroup's 128 keys of one key head against the queries, of all its heads in turn, that see them. Scores
-// as they are (S = Q K^T), a key a lane: dV^T += G^T P, dK^T += Q^T dS. The workgroup's K and V stay in registers, the tiles
-// of Q and G come through LDS with their rows' lse, delta and documents.
+// as they are (S = Q K^T), a key a lane: dV^T += G^T P, dK^T += Q^T dS. A wave's K stays in registers and the workgroup's V in
+// LDS; the tiles of Q and G come through LDS with their rows' lse, delta and documents.
 template <typename T, int DH, bool VEC>
-__global__ __launch_bounds__(256, 1) void masked_attention_dkv_kernel(MaskedAttentionArgs a) {
-	constexpr int RB = row_bytes<T, DH>(), QT = RB >= 512 ? 32 : 64, kTile = QT * RB;
-	__shared__ __attribute__((aligned(1024))) char lds[4 * kTile];
+__global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void masked_attention_dkv_kernel(MaskedAttentionArgs a) {
+	constexpr int RB = row_bytes<T, DH>(), QT = 32, kTile = QT * RB;
+	__shared__ __attribute__((aligned(1024))) char lds[kBwdRows * RB + 4 * kTile];
 	__shared__ __attribute__((aligned(16))) float lse_of[2][64], delta_of[2][64];
 	__shared__ __attribute__((aligned(16))) int docs_of[2][64];
+	char* const vt = lds;
+	char* const ring = lds + kBwdRows * RB;
 	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 	const int col = lane & 31, half = lane >> 5;
 	const int pairs = a.N * a.Hkv;
@@ -305,6 +323,10 @@ __global__ __launch_bounds__(256, 1) void masked_attention_dkv_kernel(MaskedAtte
 			pair = block % pairs;
 			tile = block / pairs;
 		}
+		// The first keys are seen most. Where all workgroups run at once, two to a CU, the second half comes lightest first:
+		// a CU then holds a heavy and a light one.
+		const int tiles = (a.Tk + kBwdRows - 1) / kBwdRows;
+		if (a.causal && gridDim.x <= 512 && tile >= (tiles + 1) / 2) tile = tiles - 1 - (tile - (tiles + 1) / 2);
 	}
 	const int n = pair / a.Hkv, hk = pair % a.Hkv, k0 = tile * kBwdRows, j = k0 + wave * 32 + col;
 	const int live = live_keys(a, n), pos0 = first_position(a, n), pre = a.prefix ? clamped(a.prefix[n], 0, live) : 0;
@@ -347,20 +369,17 @@ __global__ __launch_bounds__(256, 1) void masked_attention_dkv_kernel(MaskedAtte
 	}
 	const int nt = (hi + QT - 1) / QT;
 
-	Frag<T> kf[DH / 16], vf[DH / 16];
+	load_tile<T, DH, kBwdRows, kBwdWaves, VEC>(vt, (const T*)a.v + n * a.vs.sample + hk * a.vs.head + (int64_t)k0 * a.vs.row, a.vs.row, live - k0, a.dh, wave, lane);
+	Frag<T> kf[DH / 16];
 	{
-		const int64_t r = min(j, a.Tk - 1);
-		const T* kr = (const T*)a.k + n * a.ks.sample + r * a.ks.row + hk * a.ks.head;
-		const T* vr = (const T*)a.v + n * a.vs.sample + r * a.vs.row + hk * a.vs.head;
+		const T* kr = (const T*)a.k + n * a.ks.sample + (int64_t)min(j, a.Tk - 1) * a.ks.row + hk * a.ks.head;
 #pragma unroll
-		for (int t = 0; t < DH / 16; ++t) {
-			row_from<T, VEC>(kf[t], kr, a.dh, half, t, j < live);
-			row_from<T, VEC>(vf[t], vr, a.dh, half, t, j < live);
-		}
+		for (int t = 0; t < DH / 16; ++t) row_from<T, VEC>(kf[t], kr, a.dh, half, t, j < live);
 	}
 	f32x16 dk[DH / 32], dv[DH / 32];
 
-	for (int pass = 0; pass < 2; ++pass) {
+	const Reader<T, RB> reader(lane);
+	auto run = [&](auto safe) {
 #pragma unroll
 		for (int b = 0; b < DH / 32; ++b)
 #pragma unroll
@@ -389,8 +408,8 @@ __global__ __launch_bounds__(256, 1) void masked_attention_dkv_kernel(MaskedAtte
 		};
 		auto load = [&](int x, int buf) {
 			const int h = hk * a.G + head, q0 = x * QT;
-			load_tile<T, DH, QT, kBwdWaves, VEC>(lds + buf * 2 * kTile, (const T*)a.q + n * a.qs.sample + (int64_t)q0 * a.qs.row + h * a.qs.head, a.qs.row, a.Tq - q0, a.dh, wave, lane);
-			load_tile<T, DH, QT, kBwdWaves, VEC>(lds + (buf * 2 + 1) * kTile, (const T*)a.g + n * a.gs.sample + (int64_t)q0 * a.gs.row + h * a.gs.head, a.gs.row, a.Tq - q0, a.dh, wave, lane);
+			load_tile<T, DH, QT, kBwdWaves, VEC>(ring + buf * 2 * kTile, (const T*)a.q + n * a.qs.sample + (int64_t)q0 * a.qs.row + h * a.qs.head, a.qs.row, a.Tq - q0, a.dh, wave, lane);
+			load_tile<T, DH, QT, kBwdWaves, VEC>(ring + (buf * 2 + 1) * kTile, (const T*)a.g + n * a.gs.sample + (int64_t)q0 * a.gs.row + h * a.gs.head, a.gs.row, a.Tq - q0, a.dh, wave, lane);
 			const int64_t r = min(q0 + lane, a.Tq - 1), row = ((int64_t)n * a.H + h) * a.Tq + r;
 			if (wave == 0) __builtin_amdgcn_global_load_lds((global_void*)(a.lse + row), (lds_void*)lse_of[buf], 4, 0, 0);
 			if (wave == 1) __builtin_amdgcn_global_load_lds((global_void*)(a.delta + row), (lds_void*)delta_of[buf], 4, 0, 0);
@@ -405,109 +424,112 @@ __global__ __launch_bounds__(256, 1) void masked_attention_dkv_kernel(MaskedAtte
 			}
 			if (!__any(some)) return;
 			const bool partial = !__all(all);
-			const float slope2 = a.slopes ? a.slopes[h] * kLog2e : 0.0f;
+			const Reader<T, RB> at = reader.again();
+			f32x16 s, dp, slope;
 #pragma unroll
-			for (int x = 0; x < QT / 32; ++x) {
-				f32x16 s, dp, slope;
+			for (int y = 0; y < 16; ++y) s[y] = dp[y] = 0.0f;
 #pragma unroll
-				for (int y = 0; y < 16; ++y) s[y] = dp[y] = 0.0f;
+			for (int t = 0; t < DH / 16; ++t) {
+				Frag<T> f, v;
+				at.rows(f, qt, t);
+				mma(s, f, kf[t]);
+				at.rows(f, gt, t);
+				at.rows(v, vt + wave * 32 * RB, t);
+				mma(dp, f, v);
+			}
+			const int i0 = fresh(4 * half);  // the tile's row of register y: i0 + 8 (y / 4) + y % 4
+			f32x4 l[4], e[4];
 #pragma unroll
-				for (int t = 0; t < DH / 16; ++t) {
+			for (int y = 0; y < 4; ++y) {
+				l[y] = *(const f32x4*)(lse + i0 + 8 * y);
+				e[y] = *(const f32x4*)(delta + i0 + 8 * y);
+			}
+			weights<T>(s, slope, a, a.slopes ? a.slopes[h] * kLog2e : 0.0f,
+			           [&](int y) { const int z = pos0 + q0 + i0 + 8 * (y / 4) + y % 4 - j; return (float)(z < 0 ? -z : z); },
+			           [&](int y) { return l[y / 4][y % 4] * kLog2e; });
+#pragma unroll
+			for (int y = 0; y < 16; ++y) dp[y] = s[y] * (dp[y] - e[y / 4][y % 4]);
+			if (a.cap > 0.0f) {
+#pragma unroll
+				for (int y = 0; y < 16; ++y) dp[y] *= slope[y];
+			}
+			unsigned seen = 0xffff;
+			if (partial) {
+				seen = 0;
+#pragma unroll
+				for (int y = 0; y < 16; ++y) seen |= see.sees(q0 + i0 + 8 * (y / 4) + y % 4) ? 1u << y : 0u;
+				if (a.q_docs) {
+#pragma unroll
+					for (int z = 0; z < 4; ++z) {
+						const i32x4 o = *(const i32x4*)(docs + i0 + 8 * z);
+#pragma unroll
+						for (int y = 0; y < 4; ++y) seen &= o[y] == see.doc ? ~0u : ~(1u << (4 * z + y));
+					}
+				}
+#pragma unroll
+				for (int y = 0; y < 16; ++y) {
+					s[y] = seen >> y & 1 ? s[y] : 0.0f;
+					dp[y] = seen >> y & 1 ? dp[y] : 0.0f;
+				}
+			}
+			const bool clean = decltype(safe)::value && partial;
+#pragma unroll
+			for (int t = 0; t < 2; ++t) {
+				Frag<T> p, ds;
+				operand_of(p, s, t);
+				operand_of(ds, dp, t);
+#pragma unroll
+				for (int b = 0; b < DH / 32; ++b) {
 					Frag<T> f;
-					rows_of<T, DH>(f, qt, 32 * x + col, half, t);
-					mma(s, f, kf[t]);
-					rows_of<T, DH>(f, gt, 32 * x + col, half, t);
-					mma(dp, f, vf[t]);
+					at.columns(f, gt + 16 * t * RB, b);
+					if (clean) only_finite(f);
+					mma(dv[b], f, p);
+					at.columns(f, qt + 16 * t * RB, b);
+					if (clean) only_finite(f);
+					mma(dk[b], f, ds);
 				}
-				const int i0 = 32 * x + 4 * half;  // the tile's row of register y: i0 + 8 (y / 4) + y % 4
-				f32x4 l[4], e[4];
-#pragma unroll
-				for (int y = 0; y < 4; ++y) {
-					l[y] = *(const f32x4*)(lse + i0 + 8 * y);
-					e[y] = *(const f32x4*)(delta + i0 + 8 * y);
-				}
-				weights<T>(s, slope, a, slope2,
-				           [&](int y) { const int z = pos0 + q0 + i0 + 8 * (y / 4) + y % 4 - j; return (float)(z < 0 ? -z : z); },
-				           [&](int y) { return l[y / 4][y % 4] * kLog2e; });
-#pragma unroll
-				for (int y = 0; y < 16; ++y) dp[y] = s[y] * (dp[y] - e[y / 4][y % 4]);
-				if (a.cap > 0.0f) {
-#pragma unroll
-					for (int y = 0; y < 16; ++y) dp[y] *= slope[y];
-				}
-				unsigned seen = 0xffff;
-				if (partial) {
-					seen = 0;
-#pragma unroll
-					for (int y = 0; y < 16; ++y) seen |= see.sees(q0 + i0 + 8 * (y / 4) + y % 4) ? 1u << y : 0u;
-					if (a.q_docs) {
-#pragma unroll
-						for (int z = 0; z < 4; ++z) {
-							const i32x4 o = *(const i32x4*)(docs + i0 + 8 * z);
-#pragma unroll
-							for (int y = 0; y < 4; ++y) seen &= o[y] == see.doc ? ~0u : ~(1u << (4 * z + y));
-						}
-					}
-#pragma unroll
-					for (int y = 0; y < 16; ++y) {
-						s[y] = seen >> y & 1 ? s[y] : 0.0f;
-						dp[y] = seen >> y & 1 ? dp[y] : 0.0f;
-					}
-				}
-				const bool clean = pass != 0 && partial;
-#pragma unroll
-				for (int t = 0; t < 2; ++t) {
-					Frag<T> p, ds;
-					operand_of(p, s, t);
-					operand_of(ds, dp, t);
-#pragma unroll
-					for (int b = 0; b < DH / 32; ++b) {
-						Frag<T> f;
-						columns_of<T, DH>(f, gt, 32 * x + 16 * t, lane, b);
-						if (clean) only_finite(f);
-						mma(dv[b], f, p);
-						columns_of<T, DH>(f, qt, 32 * x + 16 * t, lane, b);
-						if (clean) only_finite(f);
-						mma(dk[b], f, ds);
-					}
-				}
-				if (clean) {  // rows that are not finite, to the keys that they see
+			}
+			if (clean) {  // rows that are not finite, to the keys that they see
 #pragma clang loop unroll(disable)
-					for (int i = 0; i < 32; ++i) {
-						const int bit = (i >> 3) * 4 + (i & 3), owner = col + 32 * ((i >> 2) & 1);
-						const bool sees = (unsigned)__shfl((int)seen, owner) >> bit & 1;
+				for (int i = 0; i < 32; ++i) {
+					const int bit = (i >> 3) * 4 + (i & 3), owner = col + 32 * ((i >> 2) & 1);
+					const bool sees = (unsigned)__shfl((int)seen, owner) >> bit & 1;
 #pragma unroll
-						for (int b = 0; b < DH / 32; ++b)
+					for (int b = 0; b < DH / 32; ++b)
 #pragma unroll
-							for (int y = 0; y < 16; ++y) {
-								const int d = 32 * b + 8 * (y / 4) + 4 * half + y % 4;
-								const float gv = element_of<T, DH>(gt, 32 * x + i, d), qv = element_of<T, DH>(qt, 32 * x + i, d);
-								dv[b][y] += sees && not_finite(gv) ? gv : 0.0f;
-								dk[b][y] += sees && not_finite(qv) ? qv - qv : 0.0f;
-							}
-					}
+						for (int y = 0; y < 16; ++y) {
+							const int d = 32 * b + 8 * (y / 4) + 4 * half + y % 4;
+							const float gv = element_of<T, DH>(gt, i, d), qv = element_of<T, DH>(qt, i, d);
+							dv[b][y] += sees && not_finite(gv) ? gv : 0.0f;
+							dk[b][y] += sees && not_finite(qv) ? qv - qv : 0.0f;
+						}
 				}
 			}
 		};
-		int cur = next(), buf = 0;
-		if (cur >= 0) load(cur, 0);
-		while (cur >= 0) {
+		int cur = next();
+		auto step = [&](auto buf) {
+			constexpr int B = decltype(buf)::value;
 			wait_loads();
 			__builtin_amdgcn_s_barrier();
 			asm volatile("" ::: "memory");
 			const int h = hk * a.G + head, then = next();
-			if (then >= 0) load(then, buf ^ 1);
-			take(lds + buf * 2 * kTile, lds + (buf * 2 + 1) * kTile, lse_of[buf], delta_of[buf], docs_of[buf], cur * QT, h);
+			if (then >= 0) load(then, 1 - B);
+			take(ring + B * 2 * kTile, ring + (B * 2 + 1) * kTile, lse_of[B], delta_of[B], docs_of[B], cur * QT, h);
 			cur = then;
-			buf ^= 1;
+		};
+		if (cur >= 0) load(cur, 0);
+		while (cur >= 0) {
+			step(std::integral_constant<int, 0>{});
+			if (cur >= 0) step(std::integral_constant<int, 1>{});
 		}
 		bool bad = false;
 #pragma unroll
 		for (int b = 0; b < DH / 32; ++b)
 #pragma unroll
 			for (int x = 0; x < 16; ++x) bad |= not_finite(dk[b][x]) || not_finite(dv[b][x]);
-		if (!__syncthreads_or(bad)) break;
-	}
+		return __syncthreads_or(bad);
+	};
+	if (run(std::false_type{})) run(std::true_type{});
 	if (j < a.Tk) {
 		if (a.dk)
 			store_gradient<T, DH, VEC>((T*)a.dk + n * a.dks.sample + (int64_t)j * a.dks.row + hk * a.dks.head, dk, a.scale, a.dh, half,

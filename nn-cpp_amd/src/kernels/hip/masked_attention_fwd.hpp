@@ -6,6 +6,8 @@
 // the registers it was computed in (masked_attention_tile.hpp).
 #pragma once
 
+#include <type_traits>
+
 #include "masked_attention_tile.hpp"
 
 namespace nnh {
@@ -40,9 +42,10 @@ struct Rows {
 };
 
 // Takes the KT keys from k0 on, whose rows are in kt and vt, into the wave's columns. docs: the wave's own room for KT ints.
-template <typename T, int DH, int KT>
-__device__ __forceinline__ void take_keys(Rows<T, DH>& r, const MaskedAttentionArgs& a, int n, const char* kt,
-                                          const char* vt, int* docs, int k0, int lane, bool safe) {
+template <typename T, int DH, int KT, bool SAFE>
+__device__ __forceinline__ void take_keys(Rows<T, DH>& r, const Reader<T, row_bytes<T, DH>()>& reader, const MaskedAttentionArgs& a,
+                                          int n, const char* kt, const char* vt, int* docs, int k0, int lane) {
+	constexpr int RB = row_bytes<T, DH>();
 	const int col = lane & 31, half = lane >> 5;
 	// whether some of the wave's queries see some of the tile, and whether all of them all of it
 	bool some = (k0 < r.s.hi && k0 + KT > r.s.lo) || k0 < r.s.pre;
@@ -54,6 +57,8 @@ __device__ __forceinline__ void take_keys(Rows<T, DH>& r, const MaskedAttentionA
 	}
 	if (!__any(some)) return;
 	const bool partial = !__all(all);
+	const Reader<T, RB> at = reader.again();
+	const int j0 = fresh(k0 + 4 * half);  // the key of block x's register i: j0 + 32 x + 8 (i / 4) + i % 4
 
 	f32x16 s[KT / 32];
 #pragma unroll
@@ -65,7 +70,7 @@ __device__ __forceinline__ void take_keys(Rows<T, DH>& r, const MaskedAttentionA
 #pragma unroll
 		for (int x = 0; x < KT / 32; ++x) {
 			Frag<T> k;
-			rows_of<T, DH>(k, kt, 32 * x + col, half, t);
+			at.rows(k, kt + 32 * x * RB, t);
 			mma(s[x], k, r.q[t]);
 		}
 
@@ -87,7 +92,7 @@ __device__ __forceinline__ void take_keys(Rows<T, DH>& r, const MaskedAttentionA
 		for (int x = 0; x < KT / 32; ++x)
 #pragma unroll
 			for (int i = 0; i < 16; ++i) {
-				const int d = r.pos - (k0 + 32 * x + 8 * (i / 4) + 4 * half + i % 4);
+				const int d = r.pos - (j0 + 32 * x + 8 * (i / 4) + i % 4);
 				s[x][i] -= r.slope2 * (float)(d < 0 ? -d : d);
 			}
 	}
@@ -98,7 +103,7 @@ __device__ __forceinline__ void take_keys(Rows<T, DH>& r, const MaskedAttentionA
 		for (int x = 0; x < KT / 32; ++x) {
 			seen[x] = 0;
 #pragma unroll
-			for (int i = 0; i < 16; ++i) seen[x] |= r.s.sees(k0 + 32 * x + 8 * (i / 4) + 4 * half + i % 4) ? 1u << i : 0u;
+			for (int i = 0; i < 16; ++i) seen[x] |= r.s.sees(j0 + 32 * x + 8 * (i / 4) + i % 4) ? 1u << i : 0u;
 			if (a.k_docs) {
 #pragma unroll
 				for (int g = 0; g < 4; ++g) {
@@ -136,7 +141,7 @@ __device__ __forceinline__ void take_keys(Rows<T, DH>& r, const MaskedAttentionA
 			r.l += s[x][i];
 		}
 
-	const bool clean = safe && partial;
+	const bool clean = SAFE && partial;
 #pragma unroll
 	for (int x = 0; x < KT / 32; ++x)
 #pragma unroll
@@ -146,7 +151,7 @@ __device__ __forceinline__ void take_keys(Rows<T, DH>& r, const MaskedAttentionA
 #pragma unroll
 			for (int b = 0; b < DH / 32; ++b) {
 				Frag<T> v;
-				columns_of<T, DH>(v, vt, 32 * x + 16 * t, lane, b);
+				at.columns(v, vt + (32 * x + 16 * t) * RB, b);
 				if (clean) only_finite(v);
 				mma(r.o[b], v, p);
 			}
@@ -272,7 +277,8 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 	}
 	const int nt = (max(hi, pre) + KT - 1) / KT;
 
-	for (int pass = 0; pass < 2; ++pass) {
+	const Reader<T, RB> at(lane);
+	auto run = [&](auto safe) {
 		r.clear();
 		// the tiles that some query may see, 64 at a time
 		int base = -64;
@@ -293,24 +299,29 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 			on &= on - 1;
 			return base + x;
 		};
-		auto load = [&](int x, int buf) {
-			load_tile<T, DH, KT, kWaves, VEC>(lds + buf * 2 * kTile, kbase + (int64_t)x * KT * a.ks.row, a.ks.row, live - x * KT, a.dh, wave, lane);
-			load_tile<T, DH, KT, kWaves, VEC>(lds + (buf * 2 + 1) * kTile, vbase + (int64_t)x * KT * a.vs.row, a.vs.row, live - x * KT, a.dh, wave, lane);
+		auto load = [&](int x, char* to) {
+			load_tile<T, DH, KT, kWaves, VEC>(to, kbase + (int64_t)x * KT * a.ks.row, a.ks.row, live - x * KT, a.dh, wave, lane);
+			load_tile<T, DH, KT, kWaves, VEC>(to + kTile, vbase + (int64_t)x * KT * a.vs.row, a.vs.row, live - x * KT, a.dh, wave, lane);
 		};
-		int cur = next(), buf = 0;
-		if (cur >= 0) load(cur, 0);
-		while (cur >= 0) {
+		int cur = next();
+		// one tile from `from`, the next one on its way to `to`
+		auto step = [&](char* from, char* to) {
 			wait_loads();
 			__builtin_amdgcn_s_barrier();  // this tile has arrived for all waves, and all are done with the last one
 			asm volatile("" ::: "memory");
 			const int then = next();
-			if (then >= 0) load(then, buf ^ 1);
-			take_keys<T, DH, KT>(r, a, n, lds + buf * 2 * kTile, lds + (buf * 2 + 1) * kTile, docs[wave], cur * KT, lane, pass != 0);
+			if (then >= 0) load(then, to);
+			take_keys<T, DH, KT, decltype(safe)::value>(r, at, a, n, from, from + kTile, docs[wave], cur * KT, lane);
 			cur = then;
-			buf ^= 1;
+		};
+		if (cur >= 0) load(cur, lds);
+		while (cur >= 0) {
+			step(lds, lds + 2 * kTile);
+			if (cur >= 0) step(lds + 2 * kTile, lds);
 		}
-		if (!__syncthreads_or(r.bad())) break;
-	}
+		return __syncthreads_or(r.bad());
+	};
+	if (run(std::false_type{})) run(std::true_type{});
 
 	const float l = add_halves(r.l);
 	if (i < a.Tq) {
@@ -376,12 +387,13 @@ __global__ __launch_bounds__((64 * SplitShape<T, DH>::NW), 1) void masked_attent
 	const int begin = min(t0 + (split * NW + wave) * per, t1), end = min(begin + per, t1);
 	char* const ring = lds + wave * ST * S::kStage;
 
-	for (int pass = 0; pass < 2; ++pass) {
+	const Reader<T, S::RB> at(lane);
+	auto run = [&](auto safe) {
 		r.clear();
 		auto load = [&](int x, int stage) {
-			char* at = ring + stage * S::kStage;
-			load_tile<T, DH, KT, 1, VEC>(at, kbase + (int64_t)x * KT * a.ks.row, a.ks.row, live - x * KT, a.dh, 0, lane);
-			load_tile<T, DH, KT, 1, VEC>(at + S::kTile, vbase + (int64_t)x * KT * a.vs.row, a.vs.row, live - x * KT, a.dh, 0, lane);
+			char* to = ring + stage * S::kStage;
+			load_tile<T, DH, KT, 1, VEC>(to, kbase + (int64_t)x * KT * a.ks.row, a.ks.row, live - x * KT, a.dh, 0, lane);
+			load_tile<T, DH, KT, 1, VEC>(to + S::kTile, vbase + (int64_t)x * KT * a.vs.row, a.vs.row, live - x * KT, a.dh, 0, lane);
 		};
 #pragma unroll
 		for (int x = 0; x < ST - 1; ++x)
@@ -399,14 +411,15 @@ __global__ __launch_bounds__((64 * SplitShape<T, DH>::NW), 1) void masked_attent
 				load(x, 0);
 				wait_loads();
 			}
-			char* at = ring + stage * S::kStage;
-			take_keys<T, DH, KT>(r, a, n, at, at + S::kTile, docs[wave], x * KT, lane, pass != 0);
+			const char* from = ring + stage * S::kStage;
+			take_keys<T, DH, KT, decltype(safe)::value>(r, at, a, n, from, from + S::kTile, docs[wave], x * KT, lane);
 			// the stage is loaded over next: its reads are done
 			asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 			stage = (stage + 1) % ST;
 		}
-		if (!__syncthreads_or(r.bad())) break;
-	}
+		return __syncthreads_or(r.bad());
+	};
+	if (run(std::false_type{})) run(std::true_type{});
 
 	// the waves' parts, merged in their order
 	float* const part = (float*)lds;  // {NW, 32, DH + 4}

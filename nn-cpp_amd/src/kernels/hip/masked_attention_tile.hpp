@@ -130,43 +130,60 @@ __device__ __forceinline__ void load_tile(char* tile, const T* base, int64_t str
 // Every load into LDS that the wave has issued has arrived.
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
 
-// Operand with the tile's rows as rows: row `row`, depths 16 t + 8 half + 0..7.
-template <typename T, int DH>
-__device__ __forceinline__ void rows_of(Frag<T>& f, const char* tile, int row, int half, int t) {
-	constexpr int RB = row_bytes<T, DH>();
-	const int sw = swizzle<RB>(row);
-	if constexpr (sizeof(T) == 2) {
-		f.w = *(const u32x4*)(tile + row * RB + (((2 * t + half) ^ sw) * 16));
-	} else {
-		f.w2[0] = *(const u32x4*)(tile + row * RB + (((4 * t + 2 * half) ^ sw) * 16));
-		f.w2[1] = *(const u32x4*)(tile + row * RB + (((4 * t + 2 * half + 1) ^ sw) * 16));
-	}
+// A lane's value that the compiler takes as new here: what follows from it is worked out again instead of being kept in
+// registers over a whole loop, a dozen per constant added, until accumulators are spilled for them.
+__device__ __forceinline__ int fresh(int x) {
+	asm volatile("" : "+v"(x));
+	return x;
 }
 
-// Operand with the tile's rows as depth, in the order of the accumulator's rows: depths row0 + 4 half + {0..3} and
-// row0 + 8 + 4 half + {0..3}, of column 32 block + lane % 32. In 16 bits one transposed read fetches, for each 16 lanes, 4
-// rows of 16 elements (each lane naming 4 consecutive ones) and hands each lane a column of them.
-template <typename T, int DH>
-__device__ __forceinline__ void columns_of(Frag<T>& f, const char* tile, int row0, int lane, int block) {
-	constexpr int RB = row_bytes<T, DH>();
-	const int half = lane >> 5;
-	if constexpr (sizeof(T) == 2) {
-		const int i = lane & 15, d = 32 * block + 16 * ((lane >> 4) & 1) + 4 * (i & 3);
-#pragma unroll
-		for (int x = 0; x < 2; ++x) {
-			const int row = row0 + 8 * x + 4 * half + (i >> 2);
-			const char* at = tile + row * RB + (((d >> 3) ^ swizzle<RB>(row)) * 16) + (d & 4) * 2;
-			f.h[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at);
-		}
-	} else {
-		const int d = 32 * block + (lane & 31);
-#pragma unroll
-		for (int j = 0; j < 8; ++j) {
-			const int row = row0 + 8 * (j >> 2) + 4 * half + (j & 3);
-			f.e[j] = *(const float*)(tile + row * RB + (((d >> 2) ^ swizzle<RB>(row)) * 16) + (d & 3) * 4);
+// Where a lane reads its operands in a tile of RB-byte rows. The permutation XORs a row's low bits onto its words' numbers, so
+// with a lane's own part worked out once, every further step (depth, column block) is an XOR by a constant and every block of
+// 16 or 32 rows a constant to add.
+template <typename T, int RB>
+struct Reader {
+	int r, c;
+
+	__device__ __forceinline__ Reader again() const {
+		Reader x = *this;
+		x.r = fresh(r);
+		x.c = fresh(c);
+		return x;
+	}
+	__device__ __forceinline__ explicit Reader(int lane) {
+		const int col = lane & 31, half = lane >> 5, i = lane & 15;
+		if constexpr (sizeof(T) == 2) {
+			r = col * RB + ((half ^ swizzle<RB>(col)) * 16);
+			const int row = 4 * half + (i >> 2);
+			c = row * RB + (((2 * ((lane >> 4) & 1) + ((i & 3) >> 1)) ^ swizzle<RB>(row)) * 16) + (i & 1) * 8;
+		} else {
+			r = col * RB + (((2 * half) ^ swizzle<RB>(col)) * 16);
+			c = 4 * half * RB + (((col >> 2) ^ half) * 16) + (col & 3) * 4;
 		}
 	}
-}
+	// Operand with the 32 rows from `at` on as rows: row lane % 32, depths 16 t + 8 half + 0..7.
+	__device__ __forceinline__ void rows(Frag<T>& f, const char* at, int t) const {
+		if constexpr (sizeof(T) == 2) {
+			f.w = *(const u32x4*)(at + (r ^ (32 * t)));
+		} else {
+			f.w2[0] = *(const u32x4*)(at + (r ^ (64 * t)));
+			f.w2[1] = *(const u32x4*)(at + (r ^ (64 * t) ^ 16));
+		}
+	}
+	// Operand with the 16 rows from `at` on as depth, in the order of the accumulator's rows: 4 half + {0..3} and 8 + 4 half +
+	// {0..3}, of column 32 block + lane % 32. In 16 bits one transposed read fetches, for each 16 lanes, 4 rows of 16 elements
+	// (each lane naming 4 consecutive ones) and hands each lane a column of them.
+	__device__ __forceinline__ void columns(Frag<T>& f, const char* at, int block) const {
+		if constexpr (sizeof(T) == 2) {
+			f.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + (c ^ (64 * block))));
+			f.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 8 * RB + (c ^ (64 * block) ^ 32)));
+		} else {
+#pragma unroll
+			for (int j = 0; j < 8; ++j)
+				f.e[j] = *(const float*)(at + (8 * (j >> 2) + (j & 3)) * RB + (c ^ (128 * block) ^ (64 * (j & 3)) ^ (32 * (j >> 2))));
+		}
+	}
+};
 
 // One element of a tile.
 template <typename T, int DH>
