@@ -18,6 +18,9 @@ struct HeadStrides {
 	int64_t sample, row, head;
 };
 
+// Rows that a tile's loads reach with 32-bit offsets.
+inline bool wide_row(int64_t row_bytes) { return row_bytes <= (int64_t)1 << 23; }
+
 // What one block of 64 tokens holds: the least and largest document number (negative ones left out; lo > hi: none) and
 // whether a token belongs to none.
 struct DocRange {

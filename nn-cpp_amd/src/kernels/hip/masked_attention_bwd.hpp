@@ -156,7 +156,6 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 	f32x16 d[DH / 32];
 	float off;
 
-	const Reader<T, RB> reader(lane);
 	auto run = [&](auto safe) {
 		off = 0.0f;
 #pragma unroll
@@ -198,7 +197,7 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 			if (partial && a.k_docs && lane < KT) docs[lane] = a.k_docs[(int64_t)n * a.Tk + min(k0 + lane, a.Tk - 1)];
 #pragma clang loop unroll(disable)
 			for (int x = 0; x < KT / 32; ++x) {
-				const Reader<T, RB> at = reader.again();
+				const Reader<T, RB> at(fresh_lane());
 				f32x16 s, dp, slope;
 #pragma unroll
 				for (int j = 0; j < 16; ++j) s[j] = dp[j] = 0.0f;
@@ -369,7 +368,8 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 	}
 	const int nt = (hi + QT - 1) / QT;
 
-	load_tile<T, DH, kBwdRows, kBwdWaves, VEC>(vt, (const T*)a.v + n * a.vs.sample + hk * a.vs.head + (int64_t)k0 * a.vs.row, a.vs.row, live - k0, a.dh, wave, lane);
+	if (k0 < live)
+		load_tile<T, DH, kBwdRows, kBwdWaves, VEC>(vt, (const T*)a.v + n * a.vs.sample + hk * a.vs.head + (int64_t)k0 * a.vs.row, a.vs.row, live - k0, a.dh, wave, lane);
 	Frag<T> kf[DH / 16];
 	{
 		const T* kr = (const T*)a.k + n * a.ks.sample + (int64_t)min(j, a.Tk - 1) * a.ks.row + hk * a.ks.head;
@@ -378,7 +378,6 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 	}
 	f32x16 dk[DH / 32], dv[DH / 32];
 
-	const Reader<T, RB> reader(lane);
 	auto run = [&](auto safe) {
 #pragma unroll
 		for (int b = 0; b < DH / 32; ++b)
@@ -424,35 +423,22 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 			}
 			if (!__any(some)) return;
 			const bool partial = !__all(all);
-			const Reader<T, RB> at = reader.again();
+			const Reader<T, RB> at(fresh_lane());
+			// Each step's loads stay with it (sched_barrier): moved ahead they cost the registers that K is held in.
 			f32x16 s, dp, slope;
 #pragma unroll
 			for (int y = 0; y < 16; ++y) s[y] = dp[y] = 0.0f;
 #pragma unroll
 			for (int t = 0; t < DH / 16; ++t) {
-				Frag<T> f, v;
+				Frag<T> f;
 				at.rows(f, qt, t);
 				mma(s, f, kf[t]);
-				at.rows(f, gt, t);
-				at.rows(v, vt + wave * 32 * RB, t);
-				mma(dp, f, v);
 			}
+			__builtin_amdgcn_sched_barrier(0);
 			const int i0 = fresh(4 * half);  // the tile's row of register y: i0 + 8 (y / 4) + y % 4
-			f32x4 l[4], e[4];
-#pragma unroll
-			for (int y = 0; y < 4; ++y) {
-				l[y] = *(const f32x4*)(lse + i0 + 8 * y);
-				e[y] = *(const f32x4*)(delta + i0 + 8 * y);
-			}
 			weights<T>(s, slope, a, a.slopes ? a.slopes[h] * kLog2e : 0.0f,
 			           [&](int y) { const int z = pos0 + q0 + i0 + 8 * (y / 4) + y % 4 - j; return (float)(z < 0 ? -z : z); },
-			           [&](int y) { return l[y / 4][y % 4] * kLog2e; });
-#pragma unroll
-			for (int y = 0; y < 16; ++y) dp[y] = s[y] * (dp[y] - e[y / 4][y % 4]);
-			if (a.cap > 0.0f) {
-#pragma unroll
-				for (int y = 0; y < 16; ++y) dp[y] *= slope[y];
-			}
+			           [&](int y) { return lse[i0 + 8 * (y / 4) + y % 4] * kLog2e; });
 			unsigned seen = 0xffff;
 			if (partial) {
 				seen = 0;
@@ -467,23 +453,41 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 					}
 				}
 #pragma unroll
-				for (int y = 0; y < 16; ++y) {
-					s[y] = seen >> y & 1 ? s[y] : 0.0f;
-					dp[y] = seen >> y & 1 ? dp[y] : 0.0f;
-				}
+				for (int y = 0; y < 16; ++y) s[y] = seen >> y & 1 ? s[y] : 0.0f;
+			}
+			Frag<T> p[2];
+			operand_of(p[0], s, 0);
+			operand_of(p[1], s, 1);
+			if (a.cap > 0.0f) {
+#pragma unroll
+				for (int y = 0; y < 16; ++y) s[y] *= slope[y];
+			}
+			__builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+			for (int t = 0; t < DH / 16; ++t) {
+				Frag<T> f, v;
+				at.rows(f, gt, t);
+				at.rows(v, vt + wave * 32 * RB, t);
+				mma(dp, f, v);
+			}
+			__builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+			for (int y = 0; y < 16; ++y) dp[y] = s[y] * (dp[y] - delta[i0 + 8 * (y / 4) + y % 4]);
+			if (partial) {
+#pragma unroll
+				for (int y = 0; y < 16; ++y) dp[y] = seen >> y & 1 ? dp[y] : 0.0f;
 			}
 			const bool clean = decltype(safe)::value && partial;
 #pragma unroll
 			for (int t = 0; t < 2; ++t) {
-				Frag<T> p, ds;
-				operand_of(p, s, t);
+				Frag<T> ds;
 				operand_of(ds, dp, t);
 #pragma unroll
 				for (int b = 0; b < DH / 32; ++b) {
 					Frag<T> f;
 					at.columns(f, gt + 16 * t * RB, b);
 					if (clean) only_finite(f);
-					mma(dv[b], f, p);
+					mma(dv[b], f, p[t]);
 					at.columns(f, qt + 16 * t * RB, b);
 					if (clean) only_finite(f);
 					mma(dk[b], f, ds);

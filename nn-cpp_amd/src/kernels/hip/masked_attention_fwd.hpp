@@ -43,8 +43,7 @@ struct Rows {
 
 // Takes the KT keys from k0 on, whose rows are in kt and vt, into the wave's columns. docs: the wave's own room for KT ints.
 template <typename T, int DH, int KT, bool SAFE>
-__device__ __forceinline__ void take_keys(Rows<T, DH>& r, const Reader<T, row_bytes<T, DH>()>& reader, const MaskedAttentionArgs& a,
-                                          int n, const char* kt, const char* vt, int* docs, int k0, int lane) {
+__device__ __forceinline__ void take_keys(Rows<T, DH>& r, const MaskedAttentionArgs& a, int n, const char* kt, const char* vt, int* docs, int k0, int lane) {
 	constexpr int RB = row_bytes<T, DH>();
 	const int col = lane & 31, half = lane >> 5;
 	// whether some of the wave's queries see some of the tile, and whether all of them all of it
@@ -57,7 +56,7 @@ __device__ __forceinline__ void take_keys(Rows<T, DH>& r, const Reader<T, row_by
 	}
 	if (!__any(some)) return;
 	const bool partial = !__all(all);
-	const Reader<T, RB> at = reader.again();
+	const Reader<T, RB> at(fresh_lane());
 	const int j0 = fresh(k0 + 4 * half);  // the key of block x's register i: j0 + 32 x + 8 (i / 4) + i % 4
 
 	f32x16 s[KT / 32];
@@ -277,7 +276,6 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 	}
 	const int nt = (max(hi, pre) + KT - 1) / KT;
 
-	const Reader<T, RB> at(lane);
 	auto run = [&](auto safe) {
 		r.clear();
 		// the tiles that some query may see, 64 at a time
@@ -311,7 +309,7 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 			asm volatile("" ::: "memory");
 			const int then = next();
 			if (then >= 0) load(then, to);
-			take_keys<T, DH, KT, decltype(safe)::value>(r, at, a, n, from, from + kTile, docs[wave], cur * KT, lane);
+			take_keys<T, DH, KT, decltype(safe)::value>(r, a, n, from, from + kTile, docs[wave], cur * KT, lane);
 			cur = then;
 		};
 		if (cur >= 0) load(cur, lds);
@@ -387,7 +385,6 @@ __global__ __launch_bounds__((64 * SplitShape<T, DH>::NW), 1) void masked_attent
 	const int begin = min(t0 + (split * NW + wave) * per, t1), end = min(begin + per, t1);
 	char* const ring = lds + wave * ST * S::kStage;
 
-	const Reader<T, S::RB> at(lane);
 	auto run = [&](auto safe) {
 		r.clear();
 		auto load = [&](int x, int stage) {
@@ -412,7 +409,7 @@ __global__ __launch_bounds__((64 * SplitShape<T, DH>::NW), 1) void masked_attent
 				wait_loads();
 			}
 			const char* from = ring + stage * S::kStage;
-			take_keys<T, DH, KT, decltype(safe)::value>(r, at, a, n, from, from + S::kTile, docs[wave], x * KT, lane);
+			take_keys<T, DH, KT, decltype(safe)::value>(r, a, n, from, from + S::kTile, docs[wave], x * KT, lane);
 			// the stage is loaded over next: its reads are done
 			asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 			stage = (stage + 1) % ST;

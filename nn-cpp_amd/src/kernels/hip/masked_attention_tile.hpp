@@ -100,22 +100,55 @@ __device__ __forceinline__ int swizzle(int row) {
 	return (row & 3) << 2 | ((row >> 2) & 3);
 }
 
-// Loads `live` rows (of R; the others are zeros) of `dh` elements into a tile, from base + row * stride. VEC: every row is
-// 16-byte aligned and dh a whole number of words; then nothing passes through registers, and the caller waits for the
-// loads (wait_loads). NW waves share the work.
+// A lane's value that the compiler takes as new here: what follows from it is worked out again instead of being kept in
+// registers over a whole loop, a dozen per constant added, until accumulators are spilled for them.
+__device__ __forceinline__ int fresh(int x) {
+	asm volatile("" : "+v"(x));
+	return x;
+}
+
+// The lane's number, worked out anew for the same reason.
+__device__ __forceinline__ int fresh_lane() {
+	int x;
+	asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=&v"(x));
+	return x;
+}
+
+// Loads a tile of R rows of `dh` elements from base + row * stride, NW waves sharing the work. Rows past the `live` (at least one)
+// first ones, which nothing sees, are the last live one again, or zeros. VEC: every row is 16-byte aligned, dh a whole number
+// of words and a tile's extent below 2^31 bytes (wide_row); then nothing passes through registers, and the caller waits
+// for the loads (wait_loads). A load instruction fills 64 words, whole rows of them from a row that is a multiple of their number
+// on: the permutation of a word is then the lane's own part XOR the instruction's.
 template <typename T, int DH, int R, int NW, bool VEC>
 __device__ __forceinline__ void load_tile(char* tile, const T* base, int64_t stride, int live, int dh, int wave, int lane) {
 	constexpr int RB = row_bytes<T, DH>(), W = RB / 16, E = 16 / (int)sizeof(T), kSteps = R * RB / 1024 / NW;
 	static_assert(kSteps * NW * 1024 == R * RB, "a tile splits evenly over the waves");
+	if constexpr (VEC) {
+		lane = fresh_lane();
+		const int r = lane / W, w = (lane % W) ^ swizzle<RB>(r);
+		const unsigned pitch = (unsigned)(stride * (int64_t)sizeof(T));
+		const unsigned at = r * pitch;
+		if (live >= R && dh == DH) {
 #pragma unroll
-	for (int j = 0; j < kSteps; ++j) {
-		const int first = (j * NW + wave) * 64, row = (first + lane) / W, c = ((first + lane) % W) ^ swizzle<RB>(row);
-		if (VEC) {
-			const bool on = row < live && c * E < dh;
-			const void* src = on ? (const void*)(base + row * stride + c * E) : (const void*)&kZeroWord;
-			if (DH * (int)sizeof(T) == RB || c * E < DH)
-				__builtin_amdgcn_global_load_lds((global_void*)src, (lds_void*)(tile + first * 16), 16, 0, 0);
+			for (int j = 0; j < kSteps; ++j) {
+				const int first = (j * NW + wave) * 64, row0 = first / W, c = w ^ swizzle<RB>(row0);
+				if (DH * (int)sizeof(T) == RB || c * E < DH)
+					__builtin_amdgcn_global_load_lds((global_void*)((const char*)(base + row0 * stride) + (at + c * 16)), (lds_void*)(tile + first * 16), 16, 0, 0);
+			}
 		} else {
+#pragma unroll
+			for (int j = 0; j < kSteps; ++j) {
+				const int first = (j * NW + wave) * 64, row0 = first / W, c = w ^ swizzle<RB>(row0);
+				const void* src = (const char*)base + (min(row0 + r, live - 1) * pitch + c * 16);
+				if (c * E >= dh) src = &kZeroWord;  // depths past dh multiply zeros: finite ones
+				if (DH * (int)sizeof(T) == RB || c * E < DH)
+					__builtin_amdgcn_global_load_lds((global_void*)src, (lds_void*)(tile + first * 16), 16, 0, 0);
+			}
+		}
+	} else {
+#pragma unroll
+		for (int j = 0; j < kSteps; ++j) {
+			const int first = (j * NW + wave) * 64, row = (first + lane) / W, c = ((first + lane) % W) ^ swizzle<RB>(row);
 			union {
 				T e[E];
 				u32x4 w;
@@ -130,13 +163,6 @@ __device__ __forceinline__ void load_tile(char* tile, const T* base, int64_t str
 // Every load into LDS that the wave has issued has arrived.
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
 
-// A lane's value that the compiler takes as new here: what follows from it is worked out again instead of being kept in
-// registers over a whole loop, a dozen per constant added, until accumulators are spilled for them.
-__device__ __forceinline__ int fresh(int x) {
-	asm volatile("" : "+v"(x));
-	return x;
-}
-
 // Where a lane reads its operands in a tile of RB-byte rows. The permutation XORs a row's low bits onto its words' numbers, so
 // with a lane's own part worked out once, every further step (depth, column block) is an XOR by a constant and every block of
 // 16 or 32 rows a constant to add.
@@ -144,12 +170,6 @@ template <typename T, int RB>
 struct Reader {
 	int r, c;
 
-	__device__ __forceinline__ Reader again() const {
-		Reader x = *this;
-		x.r = fresh(r);
-		x.c = fresh(c);
-		return x;
-	}
 	__device__ __forceinline__ explicit Reader(int lane) {
 		const int col = lane & 31, half = lane >> 5, i = lane & 15;
 		if constexpr (sizeof(T) == 2) {

@@ -75,7 +75,8 @@ HeadStrides strides_of(const nnh_head_tensor* t) {
 bool wide(const Geom& g, const Operand& o) {
 	if (!o.t || !o.span) return true;
 	const size_t e = 16 / g.size();
-	return reinterpret_cast<uintptr_t>(o.t->data) % 16 == 0 && o.t->sample % e == 0 && o.t->row % e == 0 && o.t->head % e == 0;
+	return reinterpret_cast<uintptr_t>(o.t->data) % 16 == 0 && o.t->sample % e == 0 && o.t->row % e == 0 && o.t->head % e == 0 &&
+	       wide_row((int64_t)(o.t->row * g.size()));
 }
 
 int check_rule(const Geom& g, const nnh_attention_rule* r, MaskedAttentionArgs& a) {
