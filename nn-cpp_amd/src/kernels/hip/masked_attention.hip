@@ -46,8 +46,10 @@ int masked_attention_splits(int N, int Tq, int Tk, int H, int Hkv) {
 	return (int)std::max<int64_t>(1, std::min<int64_t>((512 + groups - 1) / groups, Tk / 256));
 }
 
-size_t masked_attention_partial_floats(const MaskedAttentionArgs& a) {
-	return a.splits > 1 ? (size_t)a.splits * a.N * a.H * a.Tq * (a.dh + 2) : 0;
+// Parts enough for 1024 workgroups (two a CU, twice), each with 16 tiles of queries at least.
+int masked_attention_parts(int N, int Tq, int Tk, int H, int Hkv) {
+	const int64_t blocks = std::max<int64_t>(1, (int64_t)N * Hkv * ((Tk + 127) / 128)), steps = (int64_t)(H / Hkv) * ((Tq + 31) / 32);
+	return (int)std::max<int64_t>(1, std::min<int64_t>({(1024 + blocks - 1) / blocks, steps / 16, (Tq + 31) / 32, 8}));
 }
 
 hipError_t masked_attention_forward(const MaskedAttentionArgs& a, int type, bool vec, hipStream_t s) {

@@ -46,14 +46,16 @@ struct MaskedAttentionArgs {
 	void *dq, *dk, *dv;
 	HeadStrides dqs, dks, dvs;
 	int dq_first, dk_first, dv_first;
-	// the split form
-	float* partial;  // {splits, N, H, Tq}: maximum, sum and dh sums of p v each
-	int splits;
+	// the split form: {splits, N, H, Tq}, maximum, sum and dh sums of p v each; dk and dv in parts: {parts, 2, N, Hkv, Tk}, dh
+	// sums each, rounded up to a multiple of 4
+	float* partial;
+	int splits, parts;
 };
 
 // Whether the split form (few query rows, the keys divided over the grid) takes a call, and into how many parts.
 int masked_attention_splits(int N, int Tq, int Tk, int H, int Hkv);
-size_t masked_attention_partial_floats(const MaskedAttentionArgs& a);
+// Workgroups that share a key tile of the backward pass.
+int masked_attention_parts(int N, int Tq, int Tk, int H, int Hkv);
 
 hipError_t document_ranges(const int* docs, int N, int T, DocRange* out, hipStream_t s);
 hipError_t masked_attention_forward(const MaskedAttentionArgs& a, int type, bool vec, hipStream_t s);

@@ -299,7 +299,10 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 
 // dk and dv: a workgroup's 128 keys of one key head against the queries, of all its heads in turn, that see them. Scores
 // as they are (S = Q K^T), a key a lane: dV^T += G^T P, dK^T += Q^T dS. A wave's K stays in registers and the workgroup's V in
-// LDS; the tiles of Q and G come through LDS with their rows' lse, delta and documents.
+// LDS; the tiles of Q and G come through LDS with their rows' lse, delta and documents. A wave's step of 32 queries is a chain of
+// products and exponentials that two waves a SIMD do not hide in full, and a causal mask gives the first keys a whole
+// sequence of them: with too few workgroups to fill the GPU, a.parts of them share a key tile, each taking every
+// a.parts-th tile of queries, and their sums are added afterwards in their order (masked_attention_dkv_join_kernel).
 template <typename T, int DH, bool VEC>
 __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void masked_attention_dkv_kernel(MaskedAttentionArgs a) {
 	constexpr int RB = row_bytes<T, DH>(), QT = 32, kTile = QT * RB;
@@ -311,21 +314,20 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 	const int col = lane & 31, half = lane >> 5;
 	const int pairs = a.N * a.Hkv;
-	int tile, pair;
+	int tile, pair, part;  // the first keys, which are seen most, come first
 	{
 		const unsigned block = blockIdx.x;
+		unsigned rest;
 		if (pairs % 8 == 0) {
 			const unsigned per = pairs / 8, in = block / 8;
 			pair = block % 8 * per + in % per;
-			tile = in / per;
+			rest = in / per;
 		} else {
 			pair = block % pairs;
-			tile = block / pairs;
+			rest = block / pairs;
 		}
-		// The first keys are seen most. Where all workgroups run at once, two to a CU, the second half comes lightest first:
-		// a CU then holds a heavy and a light one.
-		const int tiles = (a.Tk + kBwdRows - 1) / kBwdRows;
-		if (a.causal && gridDim.x <= 512 && tile >= (tiles + 1) / 2) tile = tiles - 1 - (tile - (tiles + 1) / 2);
+		part = rest % a.parts;
+		tile = rest / a.parts;
 	}
 	const int n = pair / a.Hkv, hk = pair % a.Hkv, k0 = tile * kBwdRows, j = k0 + wave * 32 + col;
 	const int live = live_keys(a, n), pos0 = first_position(a, n), pre = a.prefix ? clamped(a.prefix[n], 0, live) : 0;
@@ -383,26 +385,27 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 		for (int b = 0; b < DH / 32; ++b)
 #pragma unroll
 			for (int x = 0; x < 16; ++x) dk[b][x] = dv[b][x] = 0.0f;
-		// the tiles of each head's queries in turn
-		int head = -1, base = nt;
+		// The tiles of each head's queries in turn, the last ones first: those are seen by most keys under a causal mask, so the
+		// workgroups of one key head read the same rows at about the same time.
+		int head = -1, base = -64;
 		uint64_t on = 0;
 		auto next = [&]() -> int {
 			while (on == 0) {
-				base += 64;
-				if (base >= nt) {
+				base -= 64;
+				if (base + 64 <= lo / QT || base < -63) {
 					if (nt == 0 || ++head >= a.G) return -1;
-					base = lo / QT / 64 * 64;
+					base = (nt - 1) / 64 * 64;
 				}
 				const int x = base + lane, q0 = x * QT;
-				bool s = x < nt && q0 + QT > lo;
+				bool s = x < nt && q0 + QT > lo && x % a.parts == part;
 				if (s && a.q_docs) {
 					const DocRange r = a.q_ranges[(int64_t)n * qb + q0 / 64];
 					s = r.lo <= mine.hi && r.hi >= mine.lo;
 				}
 				on = __ballot(s);
 			}
-			const int x = __builtin_ctzll(on);
-			on &= on - 1;
+			const int x = 63 - __builtin_clzll(on);
+			on &= ~((uint64_t)1 << x);
 			return base + x;
 		};
 		auto load = [&](int x, int buf) {
@@ -534,13 +537,42 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 		return __syncthreads_or(bad);
 	};
 	if (run(std::false_type{})) run(std::true_type{});
-	if (j < a.Tk) {
+	if (j >= a.Tk) return;
+	if (a.parts > 1) {
+		const int64_t rows = (int64_t)pairs * a.Tk, row = (int64_t)pair * a.Tk + j;
+		const int width = (a.dh + 3) & ~3;
+		store_gradient<float, DH, true>(a.partial + (2 * part * rows + row) * width, dk, a.scale, width, half, true);
+		store_gradient<float, DH, true>(a.partial + ((2 * part + 1) * rows + row) * width, dv, 1.0f, width, half, true);
+	} else {
 		if (a.dk)
 			store_gradient<T, DH, VEC>((T*)a.dk + n * a.dks.sample + (int64_t)j * a.dks.row + hk * a.dks.head, dk, a.scale, a.dh, half,
 			                           a.dk_first != 0);
 		if (a.dv)
 			store_gradient<T, DH, VEC>((T*)a.dv + n * a.dvs.sample + (int64_t)j * a.dvs.row + hk * a.dvs.head, dv, 1.0f, a.dh, half,
 			                           a.dv_first != 0);
+	}
+}
+
+// Adds the parts' sums of dk and dv, a thread to four elements.
+template <typename T>
+__global__ __launch_bounds__(256) void masked_attention_dkv_join_kernel(MaskedAttentionArgs a) {
+	const int fours = (a.dh + 3) / 4, width = 4 * fours;
+	const int64_t rows = (int64_t)a.N * a.Hkv * a.Tk, at = (int64_t)blockIdx.x * 256 + threadIdx.x, row = at / fours;
+	const int d = (int)(at % fours) * 4;
+	if (row >= rows) return;
+	const int j = (int)(row % a.Tk), hk = (int)(row / a.Tk % a.Hkv), n = (int)(row / a.Tk / a.Hkv);
+#pragma unroll
+	for (int x = 0; x < 2; ++x) {
+		T* const o = x ? (T*)a.dv : (T*)a.dk;
+		if (!o) continue;
+		const HeadStrides s = x ? a.dvs : a.dks;
+		const bool first = x ? a.dv_first != 0 : a.dk_first != 0;
+		f32x4 y = *(const f32x4*)(a.partial + (x * rows + row) * width + d);
+		for (int p = 1; p < a.parts; ++p) y += *(const f32x4*)(a.partial + ((2 * p + x) * rows + row) * width + d);
+		T* const to = o + n * s.sample + (int64_t)j * s.row + hk * s.head + d;
+#pragma unroll
+		for (int i = 0; i < 4; ++i)
+			if (d + i < a.dh) to[i] = (T)(first ? y[i] : to_float(to[i]) + y[i]);
 	}
 }
 
@@ -553,8 +585,12 @@ hipError_t launch_backward(const MaskedAttentionArgs& a, hipStream_t s) {
 		if (e != hipSuccess) return e;
 	}
 	if (!(a.dk || a.dv) || a.Tk == 0) return hipSuccess;
-	const int64_t blocks = (int64_t)a.N * a.Hkv * ((a.Tk + kBwdRows - 1) / kBwdRows);
+	const int64_t blocks = (int64_t)a.N * a.Hkv * ((a.Tk + kBwdRows - 1) / kBwdRows) * a.parts;
 	masked_attention_dkv_kernel<T, DH, VEC><<<(unsigned)blocks, 256, 0, s>>>(a);
+	const hipError_t e = hipGetLastError();
+	if (e != hipSuccess || a.parts == 1) return e;
+	const int64_t fours = (int64_t)a.N * a.Hkv * a.Tk * ((a.dh + 3) / 4);
+	masked_attention_dkv_join_kernel<T><<<(unsigned)((fours + 255) / 256), 256, 0, s>>>(a);
 	return hipGetLastError();
 }
 
