@@ -122,14 +122,18 @@ __global__ __launch_bounds__(T::kThreads, 2) void gemm16_kernel(Gemm16Args a) {
 	__shared__ __attribute__((aligned(1024))) char lds[T::kLds];
 	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 	const int col = lane & 31, half = lane >> 5, wm = wave % (BM / WM) * WM, wn = wave / (BM / WM) * WN;
-	int m0, n0;
+	int m0, n0, from = 0;
 	tile_of((a.inner + BM - 1) / BM, (a.outer + BN - 1) / BN, m0, n0);
 	m0 *= BM;
 	n0 *= BN;
 	Loader<BM, NW, ATR> la;
 	Loader<BN, NW, BTR> lb;
-	la.begin((const __bf16*)a.a, a.lda, m0, a.inner, wave, lane);
-	lb.begin((const __bf16*)a.b, a.ldb, n0, a.outer, wave, lane);
+	if (EPI == kGemm16Out && a.parts) {
+		from = blockIdx.y * a.part_depth;
+		a.depth = min(a.depth - from, a.part_depth);
+	}
+	la.begin((const __bf16*)a.a + from * (ATR ? a.lda : 1), a.lda, m0, a.inner, wave, lane);
+	lb.begin((const __bf16*)a.b + from * (BTR ? a.ldb : 1), a.ldb, n0, a.outer, wave, lane);
 	f32x16 acc[I][J];
 #pragma unroll
 	for (int i = 0; i < I; ++i)
@@ -141,31 +145,61 @@ __global__ __launch_bounds__(T::kThreads, 2) void gemm16_kernel(Gemm16Args a) {
 	const Reader<BM, ATR> ra(wm, lane);
 	const Reader<BN, BTR> rb(wn, lane);
 	const int stages = (a.depth + BK - 1) / BK;
-	la.load(lds, a.depth, wave, lane);
-	lb.load(lds + T::kA, a.depth, wave, lane);
-	// one stage from `at`, the next one on its way to `to`
-	auto step = [&](int s, const char* at, char* to) {
-		attn::wait_loads();
-		__builtin_amdgcn_s_barrier();  // the stage has arrived for all waves, and all are done with the other one
-		asm volatile("" ::: "memory");
-		if (s + 1 < stages) {
-			const int live = a.depth - (s + 1) * BK;
-			la.load(to, live, wave, lane);
-			lb.load(to + T::kA, live, wave, lane);
-		}
+	Frag<__bf16> fa[2][I], fb[2][J];
+	auto read = [&](int set, const char* at, int t) {
 #pragma unroll
-		for (int t = 0; t < BK / 16; ++t) {
-			Frag<__bf16> fa[I], fb[J];
+		for (int i = 0; i < I; ++i) ra.read(fa[set][i], at, i, t);
 #pragma unroll
-			for (int i = 0; i < I; ++i) ra.read(fa[i], at, i, t);
-#pragma unroll
-			for (int j = 0; j < J; ++j) rb.read(fb[j], at + T::kA, j, t);
-#pragma unroll
-			for (int i = 0; i < I; ++i)
-#pragma unroll
-				for (int j = 0; j < J; ++j) attn::mma(acc[i][j], fa[i], fb[j]);
-		}
+		for (int j = 0; j < J; ++j) rb.read(fb[set][j], at + T::kA, j, t);
 	};
+	auto multiply = [&](int set) {
+#pragma unroll
+		for (int i = 0; i < I; ++i)
+#pragma unroll
+			for (int j = 0; j < J; ++j) attn::mma(acc[i][j], fa[set][i], fb[set][j]);
+		// a read of the next depths behind each product of these
+		constexpr int kReads = I * (ATR ? 2 : 1) + J * (BTR ? 2 : 1);
+#pragma unroll
+		for (int x = 0; x < I * J; ++x) {
+			__builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+			__builtin_amdgcn_sched_group_barrier(0x100, (kReads + I * J - 1) / (I * J), 0);
+		}
+		__builtin_amdgcn_sched_barrier(0);
+	};
+	// The stage at `at`, whose first operands are in registers. Before its last depths are multiplied every wave has read them,
+	// and the next stage (at `to`) has arrived: from there on the one after it may take this one's place, and its own
+	// first operands are read.
+	auto step = [&](int s, char* at, const char* to) {
+#pragma unroll
+		for (int t = 0; t < BK / 16 - 1; ++t) {
+			read(~t & 1, at, t + 1);
+			multiply(t & 1);
+		}
+		if (s + 1 < stages) {
+			attn::wait_loads();
+			__builtin_amdgcn_s_barrier();
+			asm volatile("" ::: "memory");
+			if (s + 2 < stages) {
+				const int live = a.depth - (s + 2) * BK;
+				la.load(at, live, wave, lane);
+				lb.load(at + T::kA, live, wave, lane);
+			}
+			read(0, to, 0);
+		}
+		multiply(1);
+	};
+	if (stages > 0) {
+		la.load(lds, a.depth, wave, lane);
+		lb.load(lds + T::kA, a.depth, wave, lane);
+		if (stages > 1) {
+			la.load(lds + T::kStage, a.depth - BK, wave, lane);
+			lb.load(lds + T::kStage + T::kA, a.depth - BK, wave, lane);
+		}
+		attn::wait_loads();
+		__builtin_amdgcn_s_barrier();
+		asm volatile("" ::: "memory");
+		read(0, lds, 0);
+	}
 	for (int s = 0; s < stages; s += 2) {
 		step(s, lds, lds + T::kStage);
 		if (s + 1 < stages) step(s + 1, lds + T::kStage, lds);
@@ -180,6 +214,17 @@ __global__ __launch_bounds__(T::kThreads, 2) void gemm16_kernel(Gemm16Args a) {
 		for (int j = 0; j < J; ++j) {
 			const int n = n0 + wn + 32 * j + col;
 			if (n >= a.outer) continue;
+			if (a.parts) {
+				float* const o = a.parts + ((int64_t)blockIdx.y * a.outer + n) * a.inner;
+#pragma unroll
+				for (int i = 0; i < I; ++i)
+#pragma unroll
+					for (int x = 0; x < 16; ++x) {
+						const int m = mw + 32 * i + 8 * (x / 4) + x % 4;
+						if (m < a.inner) o[m] = acc[i][j][x];
+					}
+				continue;
+			}
 #pragma unroll
 			for (int i = 0; i < I; ++i)
 #pragma unroll

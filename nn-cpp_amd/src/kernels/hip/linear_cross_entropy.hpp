@@ -33,8 +33,10 @@ struct Gemm16Args {
 	// a gradient
 	const float* scale;  // device, or null
 	float factor;
-	float* sum;  // {outer, inner}: the parts so far
+	float* sum;  // {outer, inner}: what earlier pieces of the vocabulary add up to
 	int sum_in, sum_out, first;
+	float* parts;  // {n, outer, inner}: sums of runs of the depth, where the grid takes it in n runs of part_depth
+	int part_depth;
 };
 
 // Columns to a chunk of the statistics, by the outputs' size (the tile's choice).
@@ -42,6 +44,8 @@ int gemm16_chunk(int64_t inner, int64_t outer);
 hipError_t gemm16_scores(const Gemm16Args& a, int epilogue, int chunk, hipStream_t s);
 // A gradient: A's depth is its row axis; B's too where b_tr.
 hipError_t gemm16_out(const Gemm16Args& a, bool b_tr, hipStream_t s);
+// Floats of a.parts that such a product takes.
+size_t gemm16_parts_floats(int64_t inner, int64_t outer, int64_t depth);
 
 // rows x cols elements into rows of ldd (zeros behind cols).
 hipError_t pack16(const void* src, int64_t lds, void* dst, int64_t ldd, int64_t rows, int64_t cols, hipStream_t s);

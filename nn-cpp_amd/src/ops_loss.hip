@@ -37,7 +37,7 @@ struct Plan {
 	int64_t piece = 0, pieces = 1, ldz = 0, ldx = 0;  // ldx: D, or the packed row
 	int chunk = 0, chunks = 0;
 	int64_t part = 0;  // floats of the fp32 products' depth-cut partials
-	size_t z = 0, stats = 0, hit = 0, running = 0, loss = 0, lse = 0, weight = 0, factor = 0, sum = 0, bias = 0, px = 0, pw = 0, partials = 0, total = 0;
+	size_t z = 0, stats = 0, hit = 0, running = 0, loss = 0, lse = 0, weight = 0, factor = 0, sum = 0, bias = 0, px = 0, pw = 0, partials = 0, parts = 0, total = 0;
 };
 
 int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
@@ -74,6 +74,10 @@ Plan plan_of(const Head& h, Call call, bool pack_x, bool pack_w) {
 			p.hit = ws.add((size_t)rows * 4);
 		}
 		if (backward && p.pieces > 1) p.sum = ws.add((size_t)(rows * D) * 4);
+		size_t parts = 0;
+		for (const int64_t cols : {p.piece, V - (p.pieces - 1) * p.piece})
+			if (backward) parts = std::max({parts, gemm16_parts_floats(D, rows, cols), gemm16_parts_floats(D, cols, rows)});
+		p.parts = ws.add(parts * 4);
 		if (pack_x) p.px = ws.add((size_t)(rows * p.ldx) * 2);
 		if (pack_w) p.pw = ws.add((size_t)(V * p.ldx) * 2);
 	}
@@ -258,6 +262,7 @@ struct Run {
 				o.scale = factor;
 				o.factor = 1.0f;
 				o.ldo = D;
+				o.parts = ws.at<float>(p.parts);
 				if (e == hipSuccess && d.dx && rows) {
 					Gemm16Args a = o;  // dx = dz w
 					a.a = (const uint16_t*)w + from * ldw;
