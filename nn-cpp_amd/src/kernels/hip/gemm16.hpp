@@ -6,10 +6,14 @@
 //
 // What bounds it: the matrix cores, 32 cycles a 32 x 32 x 16 MFMA and SIMD. A workgroup's waves hold 128 x 64 (64 x 64) of the
 // tile each, so a depth of 16 takes 6 KB (4 KB) of operands from LDS for 256 (128) cycles of MFMA: three quarters of (as
-// much as) LDS delivers beside. Operands go from memory into LDS without passing through registers, one 64-deep stage
-// ahead of the one in use, one barrier a stage; an operand whose depth is not the contiguous axis is read by transposed LDS
-// reads and needs no transposed copy.
+// much as) LDS delivers beside. Operands go from memory into LDS without passing through registers, in stages of 64 depths,
+// one barrier a stage. A stage's two operands take LDS half of its MFMA time to fill (64 bytes a cycle and CU), so with two
+// whole stages of LDS a stage would arrive just when it is needed; the ring has five halves instead, A's half is under way
+// a stage longer, and only B's has to arrive between two barriers. An operand whose depth is not the contiguous axis is
+// read by transposed LDS reads and needs no transposed copy.
 #pragma once
+
+#include <type_traits>
 
 #include "linear_cross_entropy.hpp"
 #include "masked_attention_tile.hpp"
@@ -36,7 +40,9 @@ struct Tile {
 	static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;
 	static constexpr int kWaves = (BM / WM) * (BN / WN), kThreads = 64 * kWaves;
 	static constexpr int kA = BM * BK * 2, kB = BN * BK * 2, kStage = kA + kB;  // bytes
-	static constexpr int kLds = 2 * kStage > BM * BN * 2 ? 2 * kStage : BM * BN * 2;
+	static constexpr int kHalf = kA, kLoads = kHalf / 1024 / kWaves;  // an operand's part of a stage, a wave's loads for it
+	static constexpr int kLds = 5 * kHalf > BM * BN * 2 ? 5 * kHalf : BM * BN * 2;
+	static_assert(kA == kB, "the ring's places are alike");
 	static_assert(kA % (1024 * kWaves) == 0 && kB % (1024 * kWaves) == 0, "a stage splits evenly over the waves");
 	static_assert(kLds <= 160 * 1024, "LDS");
 };
@@ -64,16 +70,13 @@ struct Loader {
 			}
 		}
 	}
-	// Loads the stage and moves on; live: depths left (what is past them is zero).
+	// Loads the stage and moves on; live: depths left, none or less past the last stage (what is past them is zero).
 	__device__ __forceinline__ void load(char* tile, int live, int wave, int lane) {
 #pragma unroll
 		for (int j = 0; j < kSteps; ++j) {
 			const int w = (j * NW + wave) * 64 + lane;
-			const void* src = p[j];
-			if (live < BK) {
-				const int k = TR ? w / (R / 8) : ((w % 8) ^ attn::swizzle<128>(w / 8)) * 8;
-				if (k >= live) src = &attn::kZeroWord;
-			}
+			const int k = TR ? w / (R / 8) : ((w % 8) ^ attn::swizzle<128>(w / 8)) * 8;
+			const void* src = k < live ? (const void*)p[j] : (const void*)&attn::kZeroWord;
 			__builtin_amdgcn_global_load_lds((global_void*)src, (lds_void*)(tile + (j * NW + wave) * 1024), 16, 0, 0);
 			p[j] += step;
 		}
@@ -146,70 +149,111 @@ __global__ __launch_bounds__(T::kThreads, 2) void gemm16_kernel(Gemm16Args a) {
 	const Reader<BN, BTR> rb(wn, lane);
 	const int stages = (a.depth + BK - 1) / BK;
 	Frag<__bf16> fa[2][I], fb[2][J];
-	auto read = [&](int set, const char* at, int t) {
+	// Operands of depths 16 t .. of a stage whose halves are at `x` and `y`.
+	auto read = [&](int set, const char* x, const char* y, int t) {
 #pragma unroll
-		for (int i = 0; i < I; ++i) ra.read(fa[set][i], at, i, t);
+		for (int i = 0; i < I; ++i) ra.read(fa[set][i], x, i, t);
 #pragma unroll
-		for (int j = 0; j < J; ++j) rb.read(fb[set][j], at + T::kA, j, t);
+		for (int j = 0; j < J; ++j) rb.read(fb[set][j], y, j, t);
 	};
-	auto multiply = [&](int set) {
+	// The products of one operand set. A read of the next depths goes behind each, and of the loads that were issued before
+	// (kLoads where `loads`) one behind every other: a wave whose loads wait for their turn multiplies nothing meanwhile.
+	auto multiply = [&](int set, auto loads) {
 #pragma unroll
 		for (int i = 0; i < I; ++i)
 #pragma unroll
 			for (int j = 0; j < J; ++j) attn::mma(acc[i][j], fa[set][i], fb[set][j]);
-		// a read of the next depths behind each product of these
 		constexpr int kReads = I * (ATR ? 2 : 1) + J * (BTR ? 2 : 1);
 #pragma unroll
 		for (int x = 0; x < I * J; ++x) {
 			__builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
 			__builtin_amdgcn_sched_group_barrier(0x100, (kReads + I * J - 1) / (I * J), 0);
+			if (decltype(loads)::value && x % (I * J / T::kLoads) == I * J / T::kLoads - 1) __builtin_amdgcn_sched_group_barrier(0x010, 1, 0);
 		}
 		__builtin_amdgcn_sched_barrier(0);
 	};
-	// The stage at `at`, whose first operands are in registers. Before its last depths are multiplied every wave has read them,
-	// and the next stage (at `to`) has arrived: from there on the one after it may take this one's place, and its own
-	// first operands are read.
-	auto step = [&](int s, char* at, const char* to) {
+	// Stage s has its halves in places 2 s and 2 s + 1 of the ring.
+	auto place = [&](int x) { return lds + x % 5 * T::kHalf; };
+	// Stage s (s % 5 = S), whose first operands are in registers. Before its last depths are multiplied every wave has read
+	// them, and the next stage has arrived: from there on B of stage s + 2 and then, a step later, A of stage s + 3 may take its
+	// places, and the next one's first operands are read.
+	auto step = [&](int s, auto mod) {
+		constexpr int S = decltype(mod)::value;
+		read(1, place(2 * S), place(2 * S + 1), 1);
+		la.load(place(2 * S + 4), a.depth - (s + 2) * BK, wave, lane);
+		multiply(0, std::true_type{});
 #pragma unroll
-		for (int t = 0; t < BK / 16 - 1; ++t) {
-			read(~t & 1, at, t + 1);
-			multiply(t & 1);
+		for (int t = 1; t < BK / 16 - 1; ++t) {
+			read(~t & 1, place(2 * S), place(2 * S + 1), t + 1);
+			multiply(t & 1, std::false_type{});
 		}
-		if (s + 1 < stages) {
-			attn::wait_loads();
-			__builtin_amdgcn_s_barrier();
-			asm volatile("" ::: "memory");
-			if (s + 2 < stages) {
-				const int live = a.depth - (s + 2) * BK;
-				la.load(at, live, wave, lane);
-				lb.load(at + T::kA, live, wave, lane);
-			}
-			read(0, to, 0);
-		}
-		multiply(1);
-	};
-	if (stages > 0) {
-		la.load(lds, a.depth, wave, lane);
-		lb.load(lds + T::kA, a.depth, wave, lane);
-		if (stages > 1) {
-			la.load(lds + T::kStage, a.depth - BK, wave, lane);
-			lb.load(lds + T::kStage + T::kA, a.depth - BK, wave, lane);
-		}
-		attn::wait_loads();
+		asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(T::kLoads) : "memory");
 		__builtin_amdgcn_s_barrier();
 		asm volatile("" ::: "memory");
-		read(0, lds, 0);
+		read(0, place(2 * S + 2), place(2 * S + 3), 0);
+		lb.load(place(2 * S), a.depth - (s + 2) * BK, wave, lane);
+		multiply(1, std::true_type{});
+	};
+	la.load(place(0), a.depth, wave, lane);
+	lb.load(place(1), a.depth, wave, lane);
+	la.load(place(2), a.depth - BK, wave, lane);
+	lb.load(place(3), a.depth - BK, wave, lane);
+	asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * T::kLoads) : "memory");
+	__builtin_amdgcn_s_barrier();
+	asm volatile("" ::: "memory");
+	read(0, place(0), place(1), 0);
+	for (int s = 0; s < stages; s += 5) {
+		step(s, std::integral_constant<int, 0>{});
+		if (s + 1 < stages) step(s + 1, std::integral_constant<int, 1>{});
+		if (s + 2 < stages) step(s + 2, std::integral_constant<int, 2>{});
+		if (s + 3 < stages) step(s + 3, std::integral_constant<int, 3>{});
+		if (s + 4 < stages) step(s + 4, std::integral_constant<int, 4>{});
 	}
-	for (int s = 0; s < stages; s += 2) {
-		step(s, lds, lds + T::kStage);
-		if (s + 1 < stages) step(s + 1, lds + T::kStage, lds);
-	}
+	attn::wait_loads();
 	__syncthreads();  // LDS is the output tile's from here on
 
 	// register 4 g + x of block (i, j): inner m0 + wm + 32 i + 8 g + 4 half + x, outer n0 + wn + 32 j + col
 	const int mw = m0 + wm + 4 * half;
+	// The tile in 16 bits through LDS, 16-byte words permuted by row, for stores of whole rows.
+	auto store_rows = [&]() {
+		constexpr int W = BM / 8;  // words to a row
+		__bf16* const tile = (__bf16*)lds;
+#pragma unroll
+		for (int j = 0; j < J; ++j) {
+			const int r = wn + 32 * j + col;
+#pragma unroll
+			for (int i = 0; i < I; ++i)
+#pragma unroll
+				for (int g = 0; g < 4; ++g) {
+					union {
+						bf16x2 p[2];
+						uint64_t w;
+					} y;
+					y.p[0] = __builtin_convertvector(f32x2{acc[i][j][4 * g], acc[i][j][4 * g + 1]}, bf16x2);
+					y.p[1] = __builtin_convertvector(f32x2{acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]}, bf16x2);
+					const int m = wm + 32 * i + 8 * g;
+					*(uint64_t*)(tile + r * BM + (((m / 8) ^ (r % W)) * 8) + 4 * half) = y.w;
+				}
+		}
+		__syncthreads();
+		for (int w = threadIdx.x; w < BN * W; w += T::kThreads) {
+			const int r = w / W, c = w % W;
+			if (n0 + r < a.outer && m0 + c * 8 < a.ldo)
+				*(u32x4*)((__bf16*)a.out + (int64_t)(n0 + r) * a.ldo + m0 + c * 8) = *(const u32x4*)(tile + r * BM + ((c ^ (r % W)) * 8));
+		}
+	};
 	if constexpr (EPI == kGemm16Out) {
 		const float scale = a.scale ? *a.scale * a.factor : a.factor;
+		if (a.whole_words && !a.parts && !a.sum_in && !a.sum_out && a.first) {
+#pragma unroll
+			for (int i = 0; i < I; ++i)
+#pragma unroll
+				for (int j = 0; j < J; ++j)
+#pragma unroll
+					for (int x = 0; x < 16; ++x) acc[i][j][x] *= scale;
+			store_rows();
+			return;
+		}
 #pragma unroll
 		for (int j = 0; j < J; ++j) {
 			const int n = n0 + wn + 32 * j + col;
@@ -249,7 +293,6 @@ __global__ __launch_bounds__(T::kThreads, 2) void gemm16_kernel(Gemm16Args a) {
 	} else {
 		// a row's scores z = x w + b, in the lane: the whole softmax's statistics of this wave's WM columns, and what the
 		// tile stores
-		__bf16* const tile = (__bf16*)lds;
 		if (a.bias) {
 #pragma unroll
 			for (int i = 0; i < I; ++i)
@@ -311,33 +354,7 @@ __global__ __launch_bounds__(T::kThreads, 2) void gemm16_kernel(Gemm16Args a) {
 				if (on && half == 0 && m0 + wm < a.inner) ((f32x2*)a.stats)[(int64_t)n * a.chunks + chunk] = f32x2{top, sum};
 			}
 		}
-		if constexpr (EPI != kGemm16Stats) {
-			// the tile in 16 bits through LDS, 16-byte words permuted by row, for whole rows of stores
-			constexpr int W = BM / 8;  // words to a row
-#pragma unroll
-			for (int j = 0; j < J; ++j) {
-				const int r = wn + 32 * j + col;
-#pragma unroll
-				for (int i = 0; i < I; ++i)
-#pragma unroll
-					for (int g = 0; g < 4; ++g) {
-						union {
-							bf16x2 p[2];
-							uint64_t w;
-						} y;
-						y.p[0] = __builtin_convertvector(f32x2{acc[i][j][4 * g], acc[i][j][4 * g + 1]}, bf16x2);
-						y.p[1] = __builtin_convertvector(f32x2{acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]}, bf16x2);
-						const int m = wm + 32 * i + 8 * g;
-						*(uint64_t*)(tile + r * BM + (((m / 8) ^ (r % W)) * 8) + 4 * half) = y.w;
-					}
-			}
-			__syncthreads();
-			for (int w = threadIdx.x; w < BN * W; w += T::kThreads) {
-				const int r = w / W, c = w % W;
-				if (n0 + r < a.outer && m0 + c * 8 < a.ldo)
-					*(u32x4*)((__bf16*)a.out + (int64_t)(n0 + r) * a.ldo + m0 + c * 8) = *(const u32x4*)(tile + r * BM + ((c ^ (r % W)) * 8));
-			}
-		}
+		if constexpr (EPI != kGemm16Stats) store_rows();
 	}
 }
 

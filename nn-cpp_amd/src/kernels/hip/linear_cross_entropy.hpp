@@ -35,6 +35,7 @@ struct Gemm16Args {
 	float factor;
 	float* sum;  // {outer, inner}: what earlier pieces of the vocabulary add up to
 	int sum_in, sum_out, first;
+	int whole_words;  // out's rows start and end at multiples of 16 bytes (inner = ldo)
 	float* parts;  // {n, outer, inner}: sums of runs of the depth, where the grid takes it in n runs of part_depth
 	int part_depth;
 };

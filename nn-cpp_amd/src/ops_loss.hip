@@ -203,6 +203,8 @@ struct Run {
 		return a;
 	}
 
+	int whole(const void* out) const { return h.D % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0; }
+
 	// lse and each row's loss; with p.keep the scores stay in scratch.
 	int forward(float* lse, float* loss) {
 		if (h.rows == 0) return NNH_OK;
@@ -276,6 +278,7 @@ struct Run {
 					a.sum = ws.at<float>(p.sum);
 					a.sum_in = i > 0;
 					a.sum_out = i + 1 < p.pieces;
+					a.whole_words = whole(a.out);
 					e = gemm16_out(a, false, s);
 				}
 				if (e == hipSuccess && d.dw) {
@@ -288,6 +291,7 @@ struct Run {
 					a.depth = (int)rows;
 					a.out = (uint16_t*)d.dw + from * D;
 					a.first = d.dw_first;
+					a.whole_words = whole(a.out);
 					e = gemm16_out(a, true, s);
 				}
 				if (e == hipSuccess && d.db) e = ce_bias(z, p.ldz, rows, n, 1, factor, (uint16_t*)d.db + from, d.db_first != 0, ws.at<float>(p.bias), s);
