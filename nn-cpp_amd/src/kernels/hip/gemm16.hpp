@@ -71,12 +71,15 @@ struct Loader {
 		}
 	}
 	// Loads the stage and moves on; live: depths left, none or less past the last stage (what is past them is zero).
-	__device__ __forceinline__ void load(char* tile, int live, int wave, int lane) {
+	// on: with MASK, bit k of a word for each depth of the stage: whether it is to be loaded.
+	template <bool MASK = false>
+	__device__ __forceinline__ void load(char* tile, int live, int wave, int lane, uint64_t on = 0) {
 #pragma unroll
 		for (int j = 0; j < kSteps; ++j) {
 			const int w = (j * NW + wave) * 64 + lane;
 			const int k = TR ? w / (R / 8) : ((w % 8) ^ attn::swizzle<128>(w / 8)) * 8;
-			const void* src = k < live ? (const void*)p[j] : (const void*)&attn::kZeroWord;
+			const bool take = MASK ? (on >> k & 1) != 0 : k < live;
+			const void* src = take ? (const void*)p[j] : (const void*)&attn::kZeroWord;
 			__builtin_amdgcn_global_load_lds((global_void*)src, (lds_void*)(tile + (j * NW + wave) * 1024), 16, 0, 0);
 			p[j] += step;
 		}
@@ -174,13 +177,26 @@ __global__ __launch_bounds__(T::kThreads, 2) void gemm16_kernel(Gemm16Args a) {
 	};
 	// Stage s has its halves in places 2 s and 2 s + 1 of the ring.
 	auto place = [&](int x) { return lds + x % 5 * T::kHalf; };
+	// A's half of stage s; of the rows that count alone where a.live names them (a weight's gradient, kMask): dz is zero for the
+	// others, but x need not be finite there. Words past the last row's are zero, and the next stage's word is read a stage ahead.
+	constexpr bool kMask = EPI == kGemm16Out && BTR;
+	const uint64_t* const words = kMask ? a.live + from / BK : nullptr;
+	uint64_t word = kMask && a.depth > 0 ? words[0] : 0;
+	auto load_a = [&](int x, int s) {
+		if constexpr (kMask) {
+			la.template load<true>(place(x), 0, wave, lane, word);
+			word = s + 1 < stages ? words[s + 1] : 0;
+		} else {
+			la.load(place(x), a.depth - s * BK, wave, lane);
+		}
+	};
 	// Stage s (s % 5 = S), whose first operands are in registers. Before its last depths are multiplied every wave has read
 	// them, and the next stage has arrived: from there on B of stage s + 2 and then, a step later, A of stage s + 3 may take its
 	// places, and the next one's first operands are read.
 	auto step = [&](int s, auto mod) {
 		constexpr int S = decltype(mod)::value;
 		read(1, place(2 * S), place(2 * S + 1), 1);
-		la.load(place(2 * S + 4), a.depth - (s + 2) * BK, wave, lane);
+		load_a(2 * S + 4, s + 2);
 		multiply(0, std::true_type{});
 #pragma unroll
 		for (int t = 1; t < BK / 16 - 1; ++t) {
@@ -194,9 +210,9 @@ __global__ __launch_bounds__(T::kThreads, 2) void gemm16_kernel(Gemm16Args a) {
 		lb.load(place(2 * S), a.depth - (s + 2) * BK, wave, lane);
 		multiply(1, std::true_type{});
 	};
-	la.load(place(0), a.depth, wave, lane);
+	load_a(0, 0);
 	lb.load(place(1), a.depth, wave, lane);
-	la.load(place(2), a.depth - BK, wave, lane);
+	load_a(2, 1);
 	lb.load(place(3), a.depth - BK, wave, lane);
 	asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * T::kLoads) : "memory");
 	__builtin_amdgcn_s_barrier();

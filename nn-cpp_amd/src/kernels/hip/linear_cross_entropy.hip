@@ -111,9 +111,12 @@ __global__ __launch_bounds__(kThreads) void ce_rows32_kernel(const float* z, int
 
 template <int G>
 __global__ __launch_bounds__(kThreads) void ce_grad32_kernel(float* z, int64_t rows, int64_t cols, int64_t first, const int* targets,
-                                                             const float* lse, const float* weight, const float* scale) {
+                                                             const float* lse, const float* weight, const float* scale, const float* x,
+                                                             float* xs, int64_t D) {
 	const int64_t i = (int64_t)blockIdx.x * Group<G>::kRows + threadIdx.x / G;
 	if (i >= rows) return;
+	if (xs)
+		for (int64_t d = threadIdx.x % G; d < D; d += G) xs[i * D + d] = weight[i] == 0.0f ? 0.0f : x[i * D + d];
 	float* const row = z + i * cols;
 	const float base = lse[i] * kLog2e, w = weight[i], f = w * *scale;
 	const int64_t t = (int64_t)targets[i] - first;
@@ -154,16 +157,19 @@ __global__ __launch_bounds__(kThreads) void ce_grad16_kernel(__bf16* z, int64_t 
 
 // One workgroup: counts and sums in 64 bits, each thread's rows in order, then the threads' in a tree.
 __global__ __launch_bounds__(1024) void ce_reduce_kernel(const float* loss, const int* targets, int64_t rows, int64_t vocab, int reduction,
-                                                         const float* g, float* total, float* weight, float* factor) {
+                                                         const float* g, float* total, float* weight, uint64_t* live, float* factor) {
 	__shared__ double sums[1024];
 	__shared__ int counts[1024];
 	double sum = 0.0;
 	int count = 0;
-	for (int64_t i = threadIdx.x; i < rows; i += 1024) {
-		const bool on = targets[i] >= 0;
+	for (int64_t i = threadIdx.x; i < (rows + 63) / 64 * 64; i += 1024) {  // (a wave's 64 rows together)
+		const int t = i < rows ? targets[i] : -1;
+		const bool on = t >= 0, used = on && t < vocab;
 		count += on;
 		if (loss && on) sum += (double)loss[i];
-		if (weight) weight[i] = !on || targets[i] >= vocab ? 0.0f : reduction == 0 && g ? g[i] : 1.0f;
+		if (weight && i < rows) weight[i] = !used ? 0.0f : reduction == 0 && g ? g[i] : 1.0f;
+		const uint64_t word = __ballot(used);
+		if (live && (threadIdx.x & 63) == 0) live[i / 64] = word;
 	}
 	if (reduction == 0) {
 		if (factor && threadIdx.x == 0) *factor = 1.0f;
@@ -255,10 +261,10 @@ hipError_t ce_rows32(const float* z, int64_t rows, int64_t cols, int64_t first, 
 }
 
 hipError_t ce_grad32(float* z, int64_t rows, int64_t cols, int64_t first, const int* targets, const float* lse, const float* weight, const float* scale,
-                     hipStream_t s) {
+                     const float* x, float* xs, int64_t D, hipStream_t s) {
 	if (rows == 0) return hipSuccess;
-	if (cols <= 1024) ce_grad32_kernel<64><<<(unsigned)((rows + 3) / 4), kThreads, 0, s>>>(z, rows, cols, first, targets, lse, weight, scale);
-	else ce_grad32_kernel<256><<<(unsigned)rows, kThreads, 0, s>>>(z, rows, cols, first, targets, lse, weight, scale);
+	if (cols <= 1024) ce_grad32_kernel<64><<<(unsigned)((rows + 3) / 4), kThreads, 0, s>>>(z, rows, cols, first, targets, lse, weight, scale, x, xs, D);
+	else ce_grad32_kernel<256><<<(unsigned)rows, kThreads, 0, s>>>(z, rows, cols, first, targets, lse, weight, scale, x, xs, D);
 	return hipGetLastError();
 }
 
@@ -270,8 +276,8 @@ hipError_t ce_grad16(void* z, int64_t ldz, int64_t rows, int64_t vocab, const fl
 }
 
 hipError_t ce_reduce(const float* loss, const int* targets, int64_t rows, int64_t vocab, int reduction, const float* g, float* total, float* weight,
-                     float* factor, hipStream_t s) {
-	ce_reduce_kernel<<<1, 1024, 0, s>>>(loss, targets, rows, vocab, reduction, g, total, weight, factor);
+                     uint64_t* live, float* factor, hipStream_t s) {
+	ce_reduce_kernel<<<1, 1024, 0, s>>>(loss, targets, rows, vocab, reduction, g, total, weight, live, factor);
 	return hipGetLastError();
 }
 

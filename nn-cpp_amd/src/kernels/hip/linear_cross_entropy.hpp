@@ -36,6 +36,7 @@ struct Gemm16Args {
 	float* sum;  // {outer, inner}: what earlier pieces of the vocabulary add up to
 	int sum_in, sum_out, first;
 	int whole_words;  // out's rows start and end at multiples of 16 bytes (inner = ldo)
+	const uint64_t* live;  // a bit for each depth, 64 to a word, where A's rows without it are to be left out (null: none)
 	float* parts;  // {n, outer, inner}: sums of runs of the depth, where the grid takes it in n runs of part_depth
 	int part_depth;
 };
@@ -59,18 +60,18 @@ hipError_t ce_join(const float* stats, int chunks, const float* hit, const int* 
 // (maximum, sum, target's z) holds where `more`; the last piece writes lse and loss.
 hipError_t ce_rows32(const float* z, int64_t rows, int64_t cols, int64_t first, int64_t vocab, const int* targets, float* running,
                      bool more, bool last, float* lse, float* loss, hipStream_t s);
-// z {rows, cols} into dz in place, fp32.
+// z {rows, cols} into dz in place, fp32; and (xs not null) x {rows, D} into xs, zeros for the rows without a weight.
 hipError_t ce_grad32(float* z, int64_t rows, int64_t cols, int64_t first, const int* targets, const float* lse, const float* weight,
-                     const float* scale, hipStream_t s);
+                     const float* scale, const float* x, float* xs, int64_t D, hipStream_t s);
 // exp(z - the chunk's maximum) into dz in place, bf16, rows of ldz.
 hipError_t ce_grad16(void* z, int64_t ldz, int64_t rows, int64_t vocab, const float* stats, int chunks, int chunk, const int* targets,
                      const float* lse, const float* hit, const float* weight, hipStream_t s);
 // Per-row factors of dz and, of a mean or sum, the loss and the gradients' common factor. reduction: 0 none, 1 mean, 2 sum.
-//   weight[i]: 0 for a row without a target, else 1 (none: g[i])
+//   weight[i]: 0 for a row without a target, else 1 (none: g[i]); live: a bit for each row, whether it has one
 //   factor: 1 (none), g / count (mean; 0 without targets), g (sum); g null: 1
 //   total: the mean or sum of loss (null: not wanted; mean of nothing is NaN)
 hipError_t ce_reduce(const float* loss, const int* targets, int64_t rows, int64_t vocab, int reduction, const float* g, float* total,
-                     float* weight, float* factor, hipStream_t s);
+                     float* weight, uint64_t* live, float* factor, hipStream_t s);
 // db (+)= factor * column sums of dz {rows, cols}, rows of ld; type 0 fp32, 1 bf16.
 hipError_t ce_bias(const void* dz, int64_t ld, int64_t rows, int64_t cols, int type, const float* factor, void* db, bool first, float* partial,
                    hipStream_t s);

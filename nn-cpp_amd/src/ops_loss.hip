@@ -37,7 +37,7 @@ struct Plan {
 	int64_t piece = 0, pieces = 1, ldz = 0, ldx = 0;  // ldx: D, or the packed row
 	int chunk = 0, chunks = 0;
 	int64_t part = 0;  // floats of the fp32 products' depth-cut partials
-	size_t z = 0, stats = 0, hit = 0, running = 0, loss = 0, lse = 0, weight = 0, factor = 0, sum = 0, bias = 0, px = 0, pw = 0, partials = 0, parts = 0, total = 0;
+	size_t z = 0, stats = 0, hit = 0, running = 0, loss = 0, lse = 0, weight = 0, factor = 0, sum = 0, bias = 0, px = 0, pw = 0, partials = 0, parts = 0, live = 0, xs = 0, total = 0;
 };
 
 int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
@@ -85,6 +85,8 @@ Plan plan_of(const Head& h, Call call, bool pack_x, bool pack_w) {
 	if (call == kTrain) p.lse = ws.add((size_t)rows * 4);
 	if (backward) {
 		p.weight = ws.add((size_t)rows * 4);
+		p.live = ws.add((size_t)((rows + 63) / 64) * 8);
+		if (h.type == NNH_F32) p.xs = ws.add((size_t)(rows * D) * 4);
 		p.factor = ws.add(4);
 		p.bias = ws.add(std::max(ce_bias_partial_floats(rows, p.piece), ce_bias_partial_floats(rows, V - (p.pieces - 1) * p.piece)) * 4);
 	}
@@ -238,13 +240,13 @@ struct Run {
 			const int64_t from = i * p.piece, n = cols(i);
 			hipError_t e = hipSuccess;
 			if (h.type == NNH_F32) {
-				float* const z = ws.at<float>(p.z);
+				float *const z = ws.at<float>(p.z), *const xs = ws.at<float>(p.xs);
 				int rc = p.keep ? NNH_OK : scores32(i);
-				if (rc == NNH_OK) rc = hip_status(ce_grad32(z, rows, n, from, h.targets, lse, weight, factor, s), "linear cross entropy");
+				if (rc == NNH_OK) rc = hip_status(ce_grad32(z, rows, n, from, h.targets, lse, weight, factor, (const float*)h.x, d.dw && i == 0 ? xs : nullptr, D, s), "linear cross entropy");
 				if (rc == NNH_OK && d.dx && rows)
 					rc = product32(0, 0, h.rows, h.D, (size_t)n, z, (size_t)n, (const float*)h.w + from * D, h.D, (float*)d.dx, i > 0 || !d.dx_first, nullptr);
 				if (rc == NNH_OK && d.dw)
-					rc = product32(1, 0, (size_t)n, h.D, h.rows, z, (size_t)n, (const float*)h.x, h.D, (float*)d.dw + from * D, !d.dw_first, nullptr);
+					rc = product32(1, 0, (size_t)n, h.D, h.rows, z, (size_t)n, xs, h.D, (float*)d.dw + from * D, !d.dw_first, nullptr);
 				if (rc != NNH_OK) return rc;
 				if (d.db) e = ce_bias(z, n, rows, n, 0, nullptr, (float*)d.db + from, d.db_first != 0, ws.at<float>(p.bias), s);
 			} else {
@@ -291,6 +293,7 @@ struct Run {
 					a.depth = (int)rows;
 					a.out = (uint16_t*)d.dw + from * D;
 					a.first = d.dw_first;
+					a.live = ws.at<uint64_t>(p.live);
 					a.whole_words = whole(a.out);
 					e = gemm16_out(a, true, s);
 				}
@@ -345,7 +348,7 @@ int nnh_linear_cross_entropy_forward(int type, const void* x, size_t rows, size_
 	float* const each = reduction == NNH_REDUCE_NONE ? loss : ws.at<float>(p.loss);
 	if (rc == NNH_OK) rc = r.forward(lse, each);
 	if (rc == NNH_OK && reduction != NNH_REDUCE_NONE)
-		rc = hip_status(ce_reduce(each, targets, (int64_t)rows, (int64_t)V, reduction, nullptr, loss, nullptr, nullptr, s), "linear cross entropy");
+		rc = hip_status(ce_reduce(each, targets, (int64_t)rows, (int64_t)V, reduction, nullptr, loss, nullptr, nullptr, nullptr, s), "linear cross entropy");
 	return rc;
 }
 
@@ -371,7 +374,7 @@ int nnh_linear_cross_entropy_backward(int type, const float* g, const void* x, s
 	Run r{h, p, reduction, ws, s, nullptr, nullptr, 0, 0};
 	rc = r.begin();
 	if (rc == NNH_OK)
-		rc = hip_status(ce_reduce(nullptr, targets, (int64_t)rows, (int64_t)V, reduction, g, nullptr, ws.at<float>(p.weight), ws.at<float>(p.factor), s),
+		rc = hip_status(ce_reduce(nullptr, targets, (int64_t)rows, (int64_t)V, reduction, g, nullptr, ws.at<float>(p.weight), ws.at<uint64_t>(p.live), ws.at<float>(p.factor), s),
 		                "linear cross entropy");
 	return rc == NNH_OK ? r.backward(lse, d) : rc;
 }
@@ -402,7 +405,7 @@ int nnh_linear_cross_entropy_train(int type, const float* g, const void* x, size
 	if (rc == NNH_OK) rc = r.forward(lse, each);
 	if (rc == NNH_OK)
 		rc = hip_status(ce_reduce(each, targets, (int64_t)rows, (int64_t)V, reduction, g, reduction == NNH_REDUCE_NONE ? nullptr : loss,
-		                          ws.at<float>(p.weight), ws.at<float>(p.factor), s),
+		                          ws.at<float>(p.weight), ws.at<uint64_t>(p.live), ws.at<float>(p.factor), s),
 		                "linear cross entropy");
 	return rc == NNH_OK ? r.backward(lse, d) : rc;
 }
