@@ -93,6 +93,21 @@ private:
 	size_t size_ = 0;
 };
 
+// Whole numbers in HBM (int32): token targets, document numbers, lengths. Shares its storage like a Tensor; empty unless made.
+class IntTensor {
+public:
+	IntTensor() = default;
+	static IntTensor from_host(std::vector<size_t> shape, const int* data);
+	const std::vector<size_t>& shape() const { return shape_; }
+	size_t size() const { return size_; }
+	const int* data() const;  // device pointer, null when empty
+
+private:
+	std::shared_ptr<Block> storage_;
+	std::vector<size_t> shape_{0};
+	size_t size_ = 0;
+};
+
 // nn::matmul(a, b, trans_a, trans_b) (tensor.cpp:571-641): batched, broadcast, 2-D right operand folded.
 Tensor matmul(const Tensor& a, const Tensor& b, bool trans_a = false, bool trans_b = false);
 
@@ -210,6 +225,25 @@ Value embedding(const Value& weight, const Tensor& ids);
 Value embedding_add(const Value& weight, const std::vector<float>& ids, const std::vector<size_t>& ids_shape,
                     const Value& addend);
 Value embedding_add(const Value& weight, const Tensor& ids, const Value& addend);
+// Operators of language models, without a counterpart in the reference's op surface.
+// What masked_attention does with scores and which keys a query sees (nnh_attention_rule in nnh.h); what is empty is off.
+struct AttentionRule {
+	float scale = 0.0f;  // 0: 1 / sqrt(head width)
+	float cap = 0.0f;    // c = cap tanh(s / cap)
+	bool causal = false;
+	size_t window = 0;
+	Tensor slopes;       // {heads}: z = c - slope |distance|
+	IntTensor q_start, k_lens, prefix;  // {N}
+	IntTensor q_docs, k_docs;           // {N, Tq}, {N, Tk}; negative: no document
+};
+// Multi-head attention that keeps no probabilities: q {N, Tq, heads Dh}, k and v {N, Tk, kv_heads Dh}, Dh <= 128, kv_heads
+// dividing heads (each key head serves heads / kv_heads query heads).
+Value masked_attention(const Value& q, const Value& k, const Value& v, size_t heads, size_t kv_heads, const AttentionRule& rule);
+// The mean softmax cross entropy (a one-element Value) of the logits linear(x, weight, bias) over the rows that have a target,
+// without making the logits as a whole: x {..., D}, weight {V, D}, bias {V} (or a default Value: none), targets of x's leading
+// axes, negative for none.
+Value linear_cross_entropy(const Value& x, const Value& weight, const Value& bias, const IntTensor& targets);
+
 // positional.cpp:15-25: the fixed sinusoidal table {max_len, dim}, computed in double on the host and stored as fp32.
 Tensor sinusoidal_table(size_t max_len, size_t dim);
 

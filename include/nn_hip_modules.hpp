@@ -183,12 +183,15 @@ public:
 	// add(residual, forward(x)), the output projection's epilogue adding the residual (a transformer block's x +
 	// attn(ln1(x)))
 	Value forward_add(const Value& x, const Value& residual);
+	// the same with masked_attention in place of the attention op (self-attention; rule.causal is this module's)
+	Value forward_add(const Value& x, const Value& residual, const AttentionRule& rule);
 	std::vector<Value> parameters() const override;
 	std::vector<std::pair<std::string, Value>> named_parameters() const override;
 	void train(bool mode = true) override;
 
 private:
-	Value attend_impl(const Value& query, const Value& context, const Tensor& key_padding_mask, const Value* residual);
+	Value attend_impl(const Value& query, const Value& context, const Tensor& key_padding_mask, const Value* residual,
+	                  const AttentionRule* rule = nullptr);
 	size_t dim_, heads_;
 	bool causal_;
 	Linear q_, k_, v_, o_;
@@ -229,11 +232,13 @@ class TransformerBlock : public Module {
 public:
 	TransformerBlock(size_t dim, size_t heads, size_t mlp_ratio, float dropout, bool causal);
 	Value forward(const Value& x) override;
+	Value forward(const Value& x, const AttentionRule& rule);  // with masked_attention
 	std::vector<Value> parameters() const override;
 	std::vector<std::pair<std::string, Value>> named_parameters() const override;
 	void train(bool mode = true) override;
 
 private:
+	Value mlp_add(const Value& h);
 	LayerNorm ln1_;
 	MultiHeadAttention attn_;
 	LayerNorm ln2_;
@@ -249,16 +254,46 @@ class Transformer : public Module {
 public:
 	explicit Transformer(const TransformerConfig& config);
 	Value forward(const Value& ids) override;
+	// The mean cross entropy of forward(ids)'s logits against targets {N, T} (negative: none), which are never made as a whole
+	// (linear_cross_entropy).
+	Value loss(const Value& ids, const IntTensor& targets);
+	// The same with masked_attention under `rule` in every block: documents packed into a sequence, capped scores, a distance
+	// bias. Causality is the configuration's.
+	Value loss(const Value& ids, const IntTensor& targets, const AttentionRule& rule);
 	std::vector<Value> parameters() const override;
 	std::vector<std::pair<std::string, Value>> named_parameters() const override;
 	void train(bool mode = true) override;
 
 private:
+	Value hidden(const Value& ids, const AttentionRule* rule);
 	Embedding embed_;
 	PositionalEncoding pos_;
 	std::vector<std::unique_ptr<TransformerBlock>> blocks_;
 	LayerNorm ln_f_;
 	Linear head_;
+};
+
+// AdamW over parameters and their gradients on the device (nnh_adamw_step), one launch for 52 of them, the moments in 32 bits
+// or in 8. The reference's optimizer updates host tensors one by one (src/optim/adamw.cpp:15).
+struct AdamWOptions {
+	double lr = 1e-3, beta1 = 0.9, beta2 = 0.999, eps = 1e-8, weight_decay = 0.01;
+	int bits = 32;
+};
+
+class AdamW {
+public:
+	explicit AdamW(std::vector<Value> parameters, const AdamWOptions& options = AdamWOptions());
+	// One step; grad_scale (a one-element device tensor, or empty) multiplies every gradient.
+	void step(const Tensor& grad_scale = Tensor());
+	void zero_grad() const { nn::hip::zero_grad(parameters_); }
+	AdamWOptions& options() { return options_; }
+	size_t steps() const { return steps_; }
+
+private:
+	std::vector<Value> parameters_;
+	AdamWOptions options_;
+	std::vector<Tensor> m_, v_, m_scale_, v_scale_;  // (8 bits: the codes' and scales' bytes in fp32 storage)
+	size_t steps_ = 0;
 };
 
 }  // namespace hip

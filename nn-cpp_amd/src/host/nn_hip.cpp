@@ -142,6 +142,19 @@ std::vector<float> Tensor::to_host() const {
 	return v;
 }
 
+IntTensor IntTensor::from_host(std::vector<size_t> shape, const int* data) {
+	IntTensor t;
+	t.shape_ = std::move(shape);
+	t.size_ = numel(t.shape_);
+	if (t.size_ == 0) return t;
+	t.storage_ = std::make_shared<Block>(t.size_ * sizeof(int));
+	check_hip(hipMemcpyAsync(t.storage_->p, data, t.size_ * sizeof(int), hipMemcpyHostToDevice, g_stream), "copy in");
+	synchronize();  // data may be released on return
+	return t;
+}
+
+const int* IntTensor::data() const { return storage_ ? static_cast<const int*>(storage_->p) : nullptr; }
+
 float* Tensor::data() const { return storage_ ? static_cast<float*>(storage_->p) : nullptr; }
 
 Tensor Tensor::reshape(std::vector<size_t> new_shape) const {
@@ -892,6 +905,97 @@ Value embedding_add(const Value& weight, const Tensor& ids, const Value& addend)
 
 Value embedding(const Value& weight, const Tensor& ids) {
 	return embedding(weight, ids.to_host(), ids.shape());
+}
+
+namespace {
+
+// An option's device array: null when it is off, else of the given shape.
+const int* option(const IntTensor& t, std::vector<size_t> shape) {
+	if (t.size() == 0) return nullptr;
+	if (t.shape() != shape) throw TensorShapeError("nn::hip: masked_attention option shape");
+	return t.data();
+}
+
+}  // namespace
+
+Value masked_attention(const Value& q, const Value& k, const Value& v, size_t heads, size_t kv_heads, const AttentionRule& rule) {
+	const auto& qs = q.data().shape();
+	const auto& ks = k.data().shape();
+	if (qs.size() != 3 || ks.size() != 3 || v.data().shape() != ks || qs[0] != ks[0] || heads == 0 || kv_heads == 0 ||
+	    qs[2] % heads != 0 || ks[2] % kv_heads != 0 || qs[2] / heads != ks[2] / kv_heads)
+		throw TensorShapeError("nn::hip: masked_attention shapes");
+	const size_t N = qs[0], Tq = qs[1], Tk = ks[1], Dh = qs[2] / heads;
+	if (rule.slopes.size() != 0 && rule.slopes.shape() != std::vector<size_t>{heads})
+		throw TensorShapeError("nn::hip: masked_attention slopes shape");
+	const AttentionRule keep = rule;  // holds the arrays for the backward pass
+	const nnh_attention_rule r{rule.scale, rule.cap, rule.slopes.size() ? rule.slopes.data() : nullptr, rule.causal, rule.window,
+	                           option(rule.q_start, {N}), option(rule.k_lens, {N}), option(rule.prefix, {N}),
+	                           option(rule.q_docs, {N, Tq}), option(rule.k_docs, {N, Tk})};
+	const auto at = [=](float* p, bool query) {
+		const size_t width = query ? heads * Dh : kv_heads * Dh;
+		return nnh_head_tensor{p, (query ? Tq : Tk) * width, width, Dh};
+	};
+	Tensor out = Tensor::empty({N, Tq, heads * Dh}), lse = Tensor::empty({N, heads, Tq});
+	{
+		const nnh_head_tensor hq = at(q.data().data(), true), hk = at(k.data().data(), false), hv = at(v.data().data(), false),
+		                      ho = at(out.data(), true);
+		check(nnh_masked_attention_forward(NNH_F32, N, Tq, Tk, heads, kv_heads, Dh, &hq, &hk, &hv, &r, &ho, lse.data(), g_stream));
+	}
+	const Tensor kept = out;
+	return Value::node(std::move(out), {q, k, v}, [=](const Tensor& g) {
+		const Value* in[3] = {&q, &k, &v};
+		// one node as two operands: their gradients are made apart and added in turn
+		const bool shared = q.impl() == k.impl() || q.impl() == v.impl() || k.impl() == v.impl();
+		Tensor part[3];
+		nnh_head_tensor t[3];
+		bool first[3] = {true, true, true};
+		bool any = false;
+		for (int i = 0; i < 3; ++i) {
+			if (!in[i]->requires_grad()) continue;
+			any = true;
+			if (shared) part[i] = Tensor::empty(in[i]->data().shape());
+			t[i] = at(shared ? part[i].data() : grad_if(*in[i], first[i]), i == 0);
+		}
+		if (!any) return;
+		const auto given = [&](int i) { return in[i]->requires_grad() ? &t[i] : nullptr; };
+		const nnh_head_tensor hg = at(g.data(), true), hq = at(q.data().data(), true), hk = at(k.data().data(), false),
+		                      hv = at(v.data().data(), false), ho = at(kept.data(), true);
+		const nnh_attention_rule r{keep.scale, keep.cap, keep.slopes.size() ? keep.slopes.data() : nullptr, keep.causal, keep.window,
+		                           keep.q_start.data(), keep.k_lens.data(), keep.prefix.data(), keep.q_docs.data(), keep.k_docs.data()};
+		check(nnh_masked_attention_backward(NNH_F32, N, Tq, Tk, heads, kv_heads, Dh, &hg, &hq, &hk, &hv, &ho, lse.data(), &r, given(0),
+		                                    first[0], given(1), first[1], given(2), first[2], g_stream));
+		for (int i = 0; shared && i < 3; ++i) {
+			if (!in[i]->requires_grad()) continue;
+			bool fresh = false;
+			float* d = grad_if(*in[i], fresh);
+			check(nnh_add_to_grad(d, part[i].data(), part[i].size(), fresh, g_stream));
+		}
+	});
+}
+
+Value linear_cross_entropy(const Value& x, const Value& weight, const Value& bias, const IntTensor& targets) {
+	const auto& xs = x.data().shape();
+	const auto& ws = weight.data().shape();
+	if (xs.empty() || ws.size() != 2 || xs.back() != ws[1] || targets.shape() != std::vector<size_t>(xs.begin(), xs.end() - 1) ||
+	    (bias.impl() && bias.data().shape() != std::vector<size_t>{ws[0]}))
+		throw TensorShapeError("nn::hip: linear_cross_entropy shapes");
+	const size_t rows = targets.size(), D = ws[1], V = ws[0];
+	const float* b = bias.impl() ? bias.data().data() : nullptr;
+	Tensor loss = Tensor::empty({1}), lse = Tensor::empty({rows});
+	check(nnh_linear_cross_entropy_forward(NNH_F32, x.data().data(), rows, D, weight.data().data(), V, b, targets.data(),
+	                                       NNH_REDUCE_MEAN, loss.data(), lse.data(), g_stream));
+	std::vector<Value> parents{x, weight};
+	if (bias.impl()) parents.push_back(bias);
+	return Value::node(std::move(loss), std::move(parents), [=](const Tensor& g) {
+		bool fx = false, fw = false, fb = false;
+		float* dx = grad_if(x, fx);
+		float* dw = grad_if(weight, fw);
+		float* db = bias.impl() ? grad_if(bias, fb) : nullptr;
+		if (!dx && !dw && !db) return;
+		check(nnh_linear_cross_entropy_backward(NNH_F32, g.data(), x.data().data(), rows, D, weight.data().data(), V,
+		                                        bias.impl() ? bias.data().data() : nullptr, targets.data(), lse.data(),
+		                                        NNH_REDUCE_MEAN, dx, fx, dw, fw, db, fb, g_stream));
+	});
 }
 
 Tensor sinusoidal_table(size_t max_len, size_t dim) {

@@ -8,6 +8,7 @@
 #include <typeinfo>
 
 #include "nn_hip_modules.hpp"
+#include "nnh.h"
 
 namespace nn {
 namespace hip {
@@ -213,12 +214,16 @@ Value MultiHeadAttention::forward_add(const Value& x, const Value& residual) {
 	return attend_impl(x, x, Tensor({0}), &residual);
 }
 
+Value MultiHeadAttention::forward_add(const Value& x, const Value& residual, const AttentionRule& rule) {
+	return attend_impl(x, x, Tensor({0}), &residual, &rule);
+}
+
 Value MultiHeadAttention::attend(const Value& query, const Value& context, const Tensor& key_padding_mask) {
 	return attend_impl(query, context, key_padding_mask, nullptr);
 }
 
 Value MultiHeadAttention::attend_impl(const Value& query, const Value& context, const Tensor& key_padding_mask,
-                                      const Value* residual) {
+                                      const Value* residual, const AttentionRule* rule) {
 	const auto& qs = query.data().shape();
 	const auto& cs = context.data().shape();
 	if (qs.size() != 3 || cs.size() != 3 || qs[2] != dim_ || cs[2] != dim_ || qs[0] != cs[0])
@@ -234,7 +239,13 @@ Value MultiHeadAttention::attend_impl(const Value& query, const Value& context, 
 	if (query.impl() == context.impl()) {
 		const std::vector<Value> qkv = linear_many(query, {{q_.weight(), q_.bias()}, {k_.weight(), k_.bias()},
 		                                                   {v_.weight(), v_.bias()}});
-		a = attention(qkv[0], qkv[1], qkv[2], heads_, key_padding_mask, causal_);
+		if (rule) {
+			AttentionRule r = *rule;
+			r.causal = causal_;
+			a = masked_attention(qkv[0], qkv[1], qkv[2], heads_, heads_, r);
+		} else {
+			a = attention(qkv[0], qkv[1], qkv[2], heads_, key_padding_mask, causal_);
+		}
 	} else {
 		a = attention(q_.forward(query), k_.forward(context), v_.forward(context), heads_, key_padding_mask, causal_);
 	}
@@ -347,7 +358,14 @@ TransformerBlock::TransformerBlock(size_t dim, size_t heads, size_t mlp_ratio, f
 Value TransformerBlock::forward(const Value& x) {
 	// x + attn(ln1(x)) and h + drop(fc2(...)) with each add in the producing linear's epilogue (the same nodes and
 	// bits); an active dropout between fc2 and the add keeps the ops apart
-	const Value h = attn_.forward_add(ln1_.forward(x), x);
+	return mlp_add(attn_.forward_add(ln1_.forward(x), x));
+}
+
+Value TransformerBlock::forward(const Value& x, const AttentionRule& rule) {
+	return mlp_add(attn_.forward_add(ln1_.forward(x), x, rule));
+}
+
+Value TransformerBlock::mlp_add(const Value& h) {
 	const Value f = fc1_.forward_gelu(ln2_.forward(h));  // act_ is the GELU
 	return drop_.active() ? add(h, drop_.forward(fc2_.forward(f))) : fc2_.forward_add(f, h);
 }
@@ -380,12 +398,22 @@ Transformer::Transformer(const TransformerConfig& c)
 		blocks_.push_back(std::make_unique<TransformerBlock>(c.dim, c.heads, c.mlp_ratio, c.dropout, c.causal));
 }
 
-Value Transformer::forward(const Value& ids) {
+Value Transformer::forward(const Value& ids) { return head_.forward(hidden(ids, nullptr)); }
+
+Value Transformer::loss(const Value& ids, const IntTensor& targets) {
+	return linear_cross_entropy(hidden(ids, nullptr), head_.weight(), head_.bias(), targets);
+}
+
+Value Transformer::loss(const Value& ids, const IntTensor& targets, const AttentionRule& rule) {
+	return linear_cross_entropy(hidden(ids, &rule), head_.weight(), head_.bias(), targets);
+}
+
+Value Transformer::hidden(const Value& ids, const AttentionRule* rule) {
 	// pos(embed(ids)) with the positions added in the lookup's kernel for {N, T} ids (the same nodes and bits)
 	const auto& is = ids.data().shape();
 	Value h = is.size() == 2 ? embed_.forward_add(ids, pos_.rows(is[1])) : pos_.forward(embed_.forward(ids));
-	for (auto& b : blocks_) h = b->forward(h);
-	return head_.forward(ln_f_.forward(h));
+	for (auto& b : blocks_) h = rule ? b->forward(h, *rule) : b->forward(h);
+	return ln_f_.forward(h);
 }
 
 std::vector<Value> Transformer::parameters() const {
@@ -407,6 +435,44 @@ std::vector<std::pair<std::string, Value>> Transformer::named_parameters() const
 void Transformer::train(bool mode) {
 	for (auto& b : blocks_) b->train(mode);
 	training_ = mode;
+}
+
+AdamW::AdamW(std::vector<Value> parameters, const AdamWOptions& options) : parameters_(std::move(parameters)), options_(options) {
+	if (options.bits != 32 && options.bits != 8) throw std::invalid_argument("AdamW: moments are kept in 32 or 8 bits");
+	for (const Value& p : parameters_) {
+		const size_t n = p.data().size(), kept = options.bits == 32 ? n : (n + 3) / 4, scales = options.bits == 32 ? 0 : (n + 255) / 256;
+		m_.push_back(Tensor({kept}, 0.0f));
+		v_.push_back(Tensor({kept}, 0.0f));
+		m_scale_.push_back(Tensor({scales}, 0.0f));
+		v_scale_.push_back(Tensor({scales}, 0.0f));
+	}
+}
+
+void AdamW::step(const Tensor& grad_scale) {
+	if (grad_scale.size() > 1) throw TensorShapeError("nn::hip: AdamW's grad_scale has one element");
+	nnh_adamw o{};
+	o.p_type = o.g_type = NNH_F32;
+	o.bits = options_.bits;
+	o.lr = options_.lr;
+	o.beta1 = options_.beta1;
+	o.beta2 = options_.beta2;
+	o.eps = options_.eps;
+	o.weight_decay = options_.weight_decay;
+	o.step = steps_ + 1;
+	o.grad_scale = grad_scale.size() ? grad_scale.data() : nullptr;
+	std::vector<nnh_adamw_tensor> t;
+	for (size_t i = 0; i < parameters_.size(); ++i) {
+		const Value& p = parameters_[i];
+		if (p.data().size() == 0) continue;
+		if (p.grad().shape() != p.data().shape()) throw TensorShapeError("nn::hip: AdamW: a parameter without a gradient");
+		const auto bytes = [](const Tensor& x) { return reinterpret_cast<unsigned char*>(x.data()); };
+		t.push_back({p.data().data(), p.grad().data(), m_[i].data(), v_[i].data(), options_.bits == 8 ? bytes(m_scale_[i]) : nullptr,
+		             options_.bits == 8 ? bytes(v_scale_[i]) : nullptr, nullptr, p.data().size()});
+	}
+	const int rc = nnh_adamw_step(&o, t.data(), t.size(), current_stream());
+	if (rc == NNH_ERR_HIP) throw HipError(std::string("nn::hip: ") + nnh_last_error());
+	if (rc != NNH_OK) throw std::invalid_argument(std::string("nn::hip: ") + nnh_last_error());
+	++steps_;
 }
 
 }  // namespace hip
