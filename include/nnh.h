@@ -489,6 +489,7 @@ typedef struct nnh_attention_rule {
 /*
  * out = softmax(z over the keys seen) v, for H query heads over Hkv key heads (query head h reads key head h / (H / Hkv)), of
  * Dh <= 128 elements. lse {N, H, Tq} receives log(sum exp z). A query that sees no key gets zeros and an lse of -infinity.
+ * rest (of out's shape; null: not wanted; 16-bit types only) receives what out lost in being rounded, for the backward pass.
  * Keys past k_lens are never read; what a query does not see never reaches its result, infinities and NaN included.
  * For a training batch, q_start is null and k_lens the sequences' lengths; serving one token (or a few) against a cache,
  * q_start is what the cache held before them and k_lens that plus Tq. Up to 32 query rows take a form that divides the
@@ -496,14 +497,15 @@ typedef struct nnh_attention_rule {
  */
 int nnh_masked_attention_forward(int type, size_t N, size_t Tq, size_t Tk, size_t H, size_t Hkv, size_t Dh,
                                  const nnh_head_tensor* q, const nnh_head_tensor* k, const nnh_head_tensor* v,
-                                 const nnh_attention_rule* rule, const nnh_head_tensor* out, float* lse, void* stream);
+                                 const nnh_attention_rule* rule, const nnh_head_tensor* out, const nnh_head_tensor* rest,
+                                 float* lse, void* stream);
 
-/* Its backward rule, from the forward's out and lse: gradients of q, k and v (null: not wanted) given g, out's. *_first
+/* Its backward rule, from the forward's out, rest and lse (rest null: the gradients of q are off by out's rounding as well): gradients of q, k and v (null: not wanted) given g, out's. *_first
  * stores, otherwise the gradient is added to what is there. The gradients may lie beside each other in one buffer of
  * the same rows; they may not overlap. */
 int nnh_masked_attention_backward(int type, size_t N, size_t Tq, size_t Tk, size_t H, size_t Hkv, size_t Dh,
                                   const nnh_head_tensor* g, const nnh_head_tensor* q, const nnh_head_tensor* k,
-                                  const nnh_head_tensor* v, const nnh_head_tensor* out, const float* lse,
+                                  const nnh_head_tensor* v, const nnh_head_tensor* out, const nnh_head_tensor* rest, const float* lse,
                                   const nnh_attention_rule* rule, const nnh_head_tensor* dq, int dq_first,
                                   const nnh_head_tensor* dk, int dk_first, const nnh_head_tensor* dv, int dv_first,
                                   void* stream);

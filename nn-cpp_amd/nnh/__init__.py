@@ -125,8 +125,8 @@ _EXTRA_DECLS = {
     "nnh_gelu_backward": [_vp, _vp, _vp, _sz, _vp, C.c_int, _vp],
     "nnh_embedding_forward": [_vp, _sz, _sz, _vp, _sz, _vp, _vp],
     "nnh_embedding_backward": [_vp, _vp, _sz, _sz, _sz, _vp, C.c_int, _vp],
-    "nnh_masked_attention_forward": [C.c_int] + [_sz] * 6 + [_vp] * 7,
-    "nnh_masked_attention_backward": [C.c_int] + [_sz] * 6 + [_vp] * 8 + [C.c_int, _vp, C.c_int, _vp, C.c_int, _vp],
+    "nnh_masked_attention_forward": [C.c_int] + [_sz] * 6 + [_vp] * 8,
+    "nnh_masked_attention_backward": [C.c_int] + [_sz] * 6 + [_vp] * 9 + [C.c_int, _vp, C.c_int, _vp, C.c_int, _vp],
     "nnh_masked_attention_workspace_size": [_sz] * 6 + [C.c_int, C.c_int, _szp],
     "nnh_adamw_step": [_vp, _vp, _sz, _vp],
     "nnh_linear_cross_entropy_forward": [C.c_int, _vp, _sz, _sz, _vp, _sz, _vp, _vp, C.c_int, _vp, _vp, _vp],
@@ -689,9 +689,13 @@ def _attention_sizes(q, k, v):
     return N, Tq, k.shape[1], H, k.shape[2], Dh
 
 
-def masked_attention_forward(q, k, v, rule, out=None, lse=None, stream=None):
+def masked_attention_forward(q, k, v, rule, out=None, lse=None, stream=None, rest=True):
     """nnh_masked_attention_forward on {N, T, heads, Dh} tensors of fp32 or bf16 in place (any strides, the elements of a head
-    consecutive); returns (out, lse)."""
+    consecutive); returns (out, lse).
+
+    In bf16 the lse that is returned has an attribute `rest`, a tensor of out's shape with what out lost in being rounded:
+    masked_attention_backward reads it there (an lse without one, a copy for instance, leaves the gradients of q off by
+    out's rounding as well). rest: False where no gradients are wanted, or the tensor to use."""
     torch = _torch or _load_torch()
     N, Tq, Tk, H, Hkv, Dh = _attention_sizes(q, k, v)
     device = torch.cuda.current_device()
@@ -699,11 +703,14 @@ def masked_attention_forward(q, k, v, rule, out=None, lse=None, stream=None):
         out = torch.empty((N, Tq, H, Dh), dtype=q.dtype, device=q.device)
     if lse is None:
         lse = torch.empty((N, H, Tq), dtype=torch.float32, device=q.device)
+    if rest is True:
+        rest = torch.empty((N, Tq, H, Dh), dtype=q.dtype, device=q.device) if q.dtype == torch.bfloat16 else None
+    lse.rest = rest = None if rest is False else rest
     qs, ks = (N, Tq, H, Dh), (N, Tk, Hkv, Dh)
     t = [_heads(x, q, device, s, w) for x, s, w in ((q, qs, "q"), (k, ks, "k"), (v, ks, "v"), (out, qs, "out"))]
     r = rule._struct(N, Tq, Tk, H, device)
     check(lib().nnh_masked_attention_forward(_type(q), N, Tq, Tk, H, Hkv, Dh, C.byref(t[0]), C.byref(t[1]), C.byref(t[2]),
-                                             C.byref(r), C.byref(t[3]), _on(lse, device, torch.float32, (N, H, Tq), "lse"),
+                                             C.byref(r), C.byref(t[3]), rest if rest is None else C.byref(_heads(rest, q, device, qs, "rest")), _on(lse, device, torch.float32, (N, H, Tq), "lse"),
                                              _stream(stream)))
     return out, lse
 
@@ -720,11 +727,13 @@ def masked_attention_backward(g, q, k, v, out, lse, rule, dq=None, dq_first=True
         if t is None and not first:
             raise NnhError(ERR_INVALID, "a gradient to add to has to be given")
         grads.append(torch.empty(shape, dtype=q.dtype, device=q.device) if t is None else t)
+    rest = getattr(lse, "rest", None)
+    rest = rest if rest is None else C.byref(_heads(rest, q, device, qs, "rest"))
     named = ((g, qs, "g"), (q, qs, "q"), (k, ks, "k"), (v, ks, "v"), (out, qs, "out"), (grads[0], qs, "dq"),
              (grads[1], ks, "dk"), (grads[2], ks, "dv"))
     t = [C.byref(_heads(x, q, device, s, w)) for x, s, w in named]
     r = rule._struct(N, Tq, Tk, H, device)
-    check(lib().nnh_masked_attention_backward(_type(q), N, Tq, Tk, H, Hkv, Dh, *t[:5],
+    check(lib().nnh_masked_attention_backward(_type(q), N, Tq, Tk, H, Hkv, Dh, *t[:5], rest,
                                               _on(lse, device, torch.float32, (N, H, Tq), "lse"), C.byref(r), t[5],
                                               int(dq_first), t[6], int(dk_first), t[7], int(dv_first), _stream(stream)))
     return tuple(grads)

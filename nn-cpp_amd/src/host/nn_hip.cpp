@@ -939,7 +939,7 @@ Value masked_attention(const Value& q, const Value& k, const Value& v, size_t he
 	{
 		const nnh_head_tensor hq = at(q.data().data(), true), hk = at(k.data().data(), false), hv = at(v.data().data(), false),
 		                      ho = at(out.data(), true);
-		check(nnh_masked_attention_forward(NNH_F32, N, Tq, Tk, heads, kv_heads, Dh, &hq, &hk, &hv, &r, &ho, lse.data(), g_stream));
+		check(nnh_masked_attention_forward(NNH_F32, N, Tq, Tk, heads, kv_heads, Dh, &hq, &hk, &hv, &r, &ho, nullptr, lse.data(), g_stream));
 	}
 	const Tensor kept = out;
 	return Value::node(std::move(out), {q, k, v}, [=](const Tensor& g) {
@@ -962,7 +962,7 @@ Value masked_attention(const Value& q, const Value& k, const Value& v, size_t he
 		                      hv = at(v.data().data(), false), ho = at(kept.data(), true);
 		const nnh_attention_rule r{keep.scale, keep.cap, keep.slopes.size() ? keep.slopes.data() : nullptr, keep.causal, keep.window,
 		                           keep.q_start.data(), keep.k_lens.data(), keep.prefix.data(), keep.q_docs.data(), keep.k_docs.data()};
-		check(nnh_masked_attention_backward(NNH_F32, N, Tq, Tk, heads, kv_heads, Dh, &hg, &hq, &hk, &hv, &ho, lse.data(), &r, given(0),
+		check(nnh_masked_attention_backward(NNH_F32, N, Tq, Tk, heads, kv_heads, Dh, &hg, &hq, &hk, &hv, &ho, nullptr, lse.data(), &r, given(0),
 		                                    first[0], given(1), first[1], given(2), first[2], g_stream));
 		for (int i = 0; shared && i < 3; ++i) {
 			if (!in[i]->requires_grad()) continue;

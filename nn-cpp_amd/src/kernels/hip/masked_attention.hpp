@@ -32,6 +32,8 @@ struct MaskedAttentionArgs {
 	HeadStrides qs, ks, vs;
 	void* out;  // forward: written; backward: the forward's
 	HeadStrides os;
+	void* rest;  // in 16 bits, or null: what out lost in its rounding, itself in 16 bits
+	HeadStrides rs;
 	float* lse;  // {N, H, Tq}, natural logarithm
 	int N, Tq, Tk, H, Hkv, G, dh;  // G = H / Hkv query heads to a key head
 	float scale, cap;

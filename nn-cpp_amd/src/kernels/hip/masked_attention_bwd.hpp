@@ -77,8 +77,10 @@ __device__ __forceinline__ void weights(f32x16& s, f32x16& slope, const MaskedAt
 // dq: a workgroup's 128 queries of one head against the keys they see, as in the forward kernel: transposed scores, a query
 // a lane, dQ^T += K^T dS^T. The second pass is the forward's (values that are not finite in a partly seen tile).
 //
-// It starts from delta = g.out of the stored out, which in 16 bits is off by out's rounding. A row's p add up to 1, so its
-// sum of p (g.v - delta) is what delta was off by: the delta that is left for the other kernel has it added.
+// It starts from delta = g.out of the stored out and of what that lost in its rounding to 16 bits. Without the latter delta is
+// off by out's rounding, and with it a row's gradient by that times the keys' weighted mean: as much again as the rounding of dS
+// where scores are spread, three times that where a key or two have a row's weight. A row's p add up to 1, so its sum of
+// p (g.v - delta) is what delta was off by: the delta that is left for the other kernel has it added either way.
 template <typename T, int DH, bool VEC>
 __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void masked_attention_dq_kernel(MaskedAttentionArgs a) {
 	constexpr int RB = row_bytes<T, DH>(), KT = RB >= 512 ? 32 : 64, kTile = KT * RB;
@@ -117,6 +119,7 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 		const int64_t r = min(i, a.Tq - 1);
 		const T* qr = (const T*)a.q + n * a.qs.sample + r * a.qs.row + h * a.qs.head;
 		const T* gr = (const T*)a.g + n * a.gs.sample + r * a.gs.row + h * a.gs.head;
+		const T* rest = a.rest ? (const T*)a.rest + n * a.rs.sample + r * a.rs.row + h * a.rs.head : nullptr;
 		const T* orow = (const T*)a.out + n * a.os.sample + r * a.os.row + h * a.os.head;
 #pragma unroll
 		for (int t = 0; t < DH / 16; ++t) {
@@ -126,6 +129,11 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 			row_from<T, VEC>(o, orow, a.dh, half, t, live_row);
 #pragma unroll
 			for (int j = 0; j < 8; ++j) delta += to_float(g[t].e[j]) * to_float(o.e[j]);
+			if (sizeof(T) == 2 && rest) {
+				row_from<T, VEC>(o, rest, a.dh, half, t, live_row);
+#pragma unroll
+				for (int j = 0; j < 8; ++j) delta += to_float(g[t].e[j]) * to_float(o.e[j]);
+			}
 		}
 		delta = add_halves(delta);
 	}

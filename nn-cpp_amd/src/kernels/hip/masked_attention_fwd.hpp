@@ -172,9 +172,17 @@ __device__ __forceinline__ void take_keys(Rows<T, DH>& r, const MaskedAttentionA
 	}
 }
 
-// Stores a column: head row `o` takes the dh sums times f.
+// What a result loses in being rounded to T: out's rounding is half a step of 16 bits, but the backward pass needs g.out to more
+// than that (its difference from each g.v is what the gradients are made of where one key has most of a row's weight).
+template <typename T>
+__device__ __forceinline__ T rest_of(float x, T rounded) {
+	const float y = to_float(rounded);
+	return not_finite(y) ? (T)0.0f : (T)(x - y);
+}
+
+// Stores a column: head row `o` takes the dh sums times f, `rest` (16 bits only, or null) what they lose in their rounding.
 template <typename T, int DH, bool VEC>
-__device__ __forceinline__ void store_column(T* o, const f32x16* x, float f, int dh, int half) {
+__device__ __forceinline__ void store_column(T* o, T* rest, const f32x16* x, float f, int dh, int half) {
 #pragma unroll
 	for (int b = 0; b < DH / 32; ++b)
 #pragma unroll
@@ -196,6 +204,18 @@ __device__ __forceinline__ void store_column(T* o, const f32x16* x, float f, int
 #pragma unroll
 				for (int i = 0; i < 4; ++i)
 					if (d + i < dh) o[d + i] = y.e[i];
+			}
+			if constexpr (sizeof(T) == 2) {
+				if (!rest) continue;
+#pragma unroll
+				for (int i = 0; i < 4; ++i) y.e[i] = rest_of(x[b][4 * g + i] * f, y.e[i]);
+				if (VEC) {
+					if (d < dh) *(uint64_t*)(rest + d) = y.w8;
+				} else {
+#pragma unroll
+					for (int i = 0; i < 4; ++i)
+						if (d + i < dh) rest[d + i] = y.e[i];
+				}
 			}
 		}
 }
@@ -324,7 +344,8 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 	const float l = add_halves(r.l);
 	if (i < a.Tq) {
 		T* o = (T*)a.out + n * a.os.sample + (int64_t)i * a.os.row + h * a.os.head;
-		store_column<T, DH, VEC>(o, r.o, l == 0.0f ? 0.0f : 1.0f / l, a.dh, half);
+		T* rest = a.rest ? (T*)a.rest + n * a.rs.sample + (int64_t)i * a.rs.row + h * a.rs.head : nullptr;
+		store_column<T, DH, VEC>(o, rest, r.o, l == 0.0f ? 0.0f : 1.0f / l, a.dh, half);
 		if (half == 0) a.lse[((int64_t)n * a.H + h) * a.Tq + i] = l == 0.0f ? -kInf : r.m * kLn2 + logf(l);
 	}
 }
@@ -453,8 +474,12 @@ __global__ __launch_bounds__((64 * SplitShape<T, DH>::NW), 1) void masked_attent
 			float y = 0.0f;
 #pragma unroll
 			for (int w = 0; w < NW; ++w) y += f[w] * part[(w * 32 + x) * (DH + 4) + d];
-			if (a.splits == 1) o[d] = (T)(y * inv);
-			else to[2 + d] = y;
+			if (a.splits == 1) {
+				o[d] = (T)(y * inv);
+				if (sizeof(T) == 2 && a.rest) ((T*)a.rest)[n * a.rs.sample + (int64_t)ii * a.rs.row + hh * a.rs.head + d] = rest_of(y * inv, (T)(y * inv));
+			} else {
+				to[2 + d] = y;
+			}
 		}
 		if (lane == 0) {
 			if (a.splits == 1) {
@@ -493,7 +518,10 @@ __global__ __launch_bounds__(256) void masked_attention_join_kernel(MaskedAttent
 	const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
 	for (int x = 0; x < 2; ++x)
-		if (lane + 64 * x < a.dh) o[lane + 64 * x] = (T)(y[x] * inv);
+		if (lane + 64 * x < a.dh) {
+			o[lane + 64 * x] = (T)(y[x] * inv);
+			if (sizeof(T) == 2 && a.rest) ((T*)a.rest)[n * a.rs.sample + (int64_t)i * a.rs.row + h * a.rs.head + lane + 64 * x] = rest_of(y[x] * inv, (T)(y[x] * inv));
+		}
 	if (lane == 0) a.lse[row] = l == 0.0f ? -kInf : m * kLn2 + logf(l);
 }
 

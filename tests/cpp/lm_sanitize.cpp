@@ -37,7 +37,7 @@ void attention() {
 	nnh_attention_rule r{};
 	const auto fwd = [&](int type, size_t N, size_t Tq, size_t Tk, size_t H, size_t Hkv, size_t Dh, const nnh_head_tensor* a,
 	                     const nnh_head_tensor* b, const nnh_head_tensor* c, const nnh_head_tensor* out, float* l) {
-		return nnh_masked_attention_forward(type, N, Tq, Tk, H, Hkv, Dh, a, b, c, &r, out, l, nullptr);
+		return nnh_masked_attention_forward(type, N, Tq, Tk, H, Hkv, Dh, a, b, c, &r, out, nullptr, l, nullptr);
 	};
 	EXPECT(fwd(NNH_F32, 2, 8, 8, 4, 2, 16, &hq, &hk, &hv, &ho, lse.data()), HIP);
 	EXPECT(fwd(NNH_F32, 0, 8, 8, 4, 2, 16, nullptr, nullptr, nullptr, nullptr, nullptr), OK);
@@ -75,7 +75,15 @@ void attention() {
 	odd.data = reinterpret_cast<char*>(q.data()) + 2;
 	EXPECT(fwd(NNH_F32, 1, 4, 8, 4, 2, 16, &odd, &hk, &hv, &ho, lse.data()), INV);
 	EXPECT(fwd(NNH_BF16, 1, 4, 8, 4, 2, 16, &odd, &hk, &hv, &ho, lse.data()), HIP);
-	EXPECT(nnh_masked_attention_forward(NNH_F32, 2, 8, 8, 4, 2, 16, &hq, &hk, &hv, nullptr, &ho, lse.data(), nullptr), INV);
+	EXPECT(nnh_masked_attention_forward(NNH_F32, 2, 8, 8, 4, 2, 16, &hq, &hk, &hv, nullptr, &ho, nullptr, lse.data(), nullptr), INV);
+	EXPECT(nnh_masked_attention_forward(NNH_F32, 2, 8, 8, 4, 2, 16, &hq, &hk, &hv, &r, &ho, &hg, lse.data(), nullptr), INV);  // a rest of 32 bits
+	const auto rest = [&](nnh_head_tensor x) { return nnh_masked_attention_forward(NNH_BF16, 1, 8, 8, 4, 2, 16, &hq, &hk, &hv, &r, &ho, &x, lse.data(), nullptr); };
+	EXPECT(rest(hg), HIP);
+	EXPECT(rest(ho), ALIAS);
+	EXPECT(rest(hv), ALIAS);
+	EXPECT(rest({nullptr, 512, 64, 16}), INV);
+	EXPECT(rest({g.data(), 512, 64, 8}), ALIAS);
+	EXPECT(rest({lse.data(), 0, 0, 16}), ALIAS);
 	r.q_docs = docs.data();
 	EXPECT(fwd(NNH_F32, 2, 8, 8, 4, 2, 16, &hq, &hk, &hv, &ho, lse.data()), INV);
 	r.k_docs = docs.data();
@@ -94,7 +102,7 @@ void attention() {
 	EXPECT(fwd(NNH_F32, 2, 8, 8, 4, 2, 16, &hq, &hk, &hv, &ho, lse.data()), INV);
 	r.window = 0;
 	const auto bwd = [&](const nnh_head_tensor* a, const nnh_head_tensor* b, const nnh_head_tensor* c) {
-		return nnh_masked_attention_backward(NNH_F32, 2, 8, 8, 4, 2, 16, &hg, &hq, &hk, &hv, &ho, lse.data(), &r, a, 1, b, 1, c, 1, nullptr);
+		return nnh_masked_attention_backward(NNH_F32, 2, 8, 8, 4, 2, 16, &hg, &hq, &hk, &hv, &ho, nullptr, lse.data(), &r, a, 1, b, 1, c, 1, nullptr);
 	};
 	EXPECT(bwd(&hdq, &hdk, &hdv), HIP);
 	EXPECT(bwd(nullptr, nullptr, nullptr), OK);

@@ -232,3 +232,35 @@ def test_repeats_and_offsets_past_32_bits(gpu):
         assert_within(out, (want["out"][0][:, :n_q], want["out"][1][:, :n_q]), n_q)
         again, _ = nnh.masked_attention_forward(q[:, :n_q], strided, strided, rule)
         assert torch.equal(out, again)
+
+
+@pytest.mark.parametrize("n_q", [512, 12])
+@pytest.mark.parametrize("strided", [False, True])
+def test_rest_of_out(gpu, n_q, strided):
+    """Peaked rows of short documents, where out's rounding weighs most in the queries' gradients. With the rest two roundings
+    of half a step are left (dS and the result), of 2^-8 / sqrt(3) of the values' norm each at most: sqrt(2) 2^-8 / sqrt(3)
+    together. Both forms of the forward call (12 queries are split), rows that are not 16-byte aligned too."""
+    import nnh
+    gen = torch.Generator().manual_seed(n_q)
+    q, k, v, g = (torch.randn(1, n_q, 1, 64, generator=gen).bfloat16() for _ in range(4))
+    q *= 3
+    d = (torch.arange(n_q) // 16).int()[None]
+    o = dict(causal=True, cap=30.0, q_docs=d, k_docs=d)
+    want = masked_attention(q, k, v, g, **o)
+    rule = nnh.AttentionRule(causal=True, cap=30.0, q_docs=d.cuda(), k_docs=d.cuda())
+    q, k, v, g = (x.cuda() for x in (q, k, v, g))
+    rest = torch.full((1, n_q, 1, 65), 7.0).bfloat16().cuda()[..., :64] if strided else True
+    out, lse = nnh.masked_attention_forward(q, k, v, rule, rest=rest)
+    exact = want["out"][0]
+    lost = exact - out.double().cpu()
+    assert float((lse.rest.double().cpu() - lost).abs().max()) <= 2.0 ** -9 * float(exact.abs().max()) * 2.0 ** -2 + float(want["out"][1].max())
+    dq, dk, dv = nnh.masked_attention_backward(g, q, k, v, out, lse, rule)
+    for name, x in (("dq", dq), ("dk", dk), ("dv", dv)):
+        assert_within(x, want[name], name)
+        exact = want[name][0]
+        assert float((x.double().cpu() - exact).norm() / exact.norm()) <= (2.0 / 3.0) ** 0.5 * 2.0 ** -8
+    # a copy has none: the same out and lse, the bounds without it
+    copy = nnh.masked_attention_forward(q, k, v, rule, rest=False)
+    assert torch.equal(copy[0], out) and torch.equal(copy[1], lse) and copy[1].rest is None
+    for name, x in zip(("dq", "dk", "dv"), nnh.masked_attention_backward(g, q, k, v, *copy, rule)):
+        assert_within(x, want[name], name)
