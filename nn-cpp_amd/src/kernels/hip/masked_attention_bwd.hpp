@@ -21,32 +21,41 @@ constexpr int kBwdWaves = 4, kBwdRows = 32 * kBwdWaves;
 // Stores a column of a gradient, or adds it to what the row holds.
 template <typename T, int DH, bool VEC>
 __device__ __forceinline__ void store_gradient(T* o, const f32x16* x, float f, int dh, int half, bool first) {
+	if constexpr (VEC && sizeof(T) == 2) {  // (dh is a multiple of 8)
 #pragma unroll
-	for (int b = 0; b < DH / 32; ++b)
+		for (int b = 0; b < DH / 32; ++b)
 #pragma unroll
-		for (int g = 0; g < 4; ++g) {
-			const int d = 32 * b + 8 * g + 4 * half;
-			union {
-				T e[4];
-				uint64_t w8;
-				u32x4 w16;
-			} y;
-			if (VEC) {
-				if (d >= dh) continue;
-				if (!first) {
-					if constexpr (sizeof(T) == 2) y.w8 = *(const uint64_t*)(o + d);
-					else y.w16 = *(const u32x4*)(o + d);
+			for (int g = 0; g < 2; ++g) {
+				const int d = 32 * b + 16 * g + 8 * half;
+				Frag<T> y, old;
+				old.w = u32x4{0, 0, 0, 0};
+				if (!first) {  // (the swap of two halves undoes itself)
+					if (d < dh) old.w = *(const u32x4*)(o + d);
+					eight_of(old);
 				}
 #pragma unroll
-				for (int i = 0; i < 4; ++i) y.e[i] = (T)(first ? x[b][4 * g + i] * f : to_float(y.e[i]) + x[b][4 * g + i] * f);
-				if constexpr (sizeof(T) == 2) *(uint64_t*)(o + d) = y.w8;
-				else *(u32x4*)(o + d) = y.w16;
-			} else {
-#pragma unroll
-				for (int i = 0; i < 4; ++i)
-					if (d + i < dh) o[d + i] = (T)(first ? x[b][4 * g + i] * f : to_float(o[d + i]) + x[b][4 * g + i] * f);
+				for (int i = 0; i < 8; ++i) y.e[i] = (T)(first ? x[b][8 * g + i] * f : to_float(old.e[i]) + x[b][8 * g + i] * f);
+				eight_of(y);
+				if (d < dh) *(u32x4*)(o + d) = y.w;
 			}
-		}
+	} else {
+#pragma unroll
+		for (int b = 0; b < DH / 32; ++b)
+#pragma unroll
+			for (int g = 0; g < 4; ++g) {
+				const int d = 32 * b + 8 * g + 4 * half;
+				if constexpr (VEC) {
+					if (d >= dh) continue;
+					f32x4 y = f32x4{x[b][4 * g] * f, x[b][4 * g + 1] * f, x[b][4 * g + 2] * f, x[b][4 * g + 3] * f};
+					if (!first) y = *(const f32x4*)(o + d) + y;
+					*(f32x4*)(o + d) = y;
+				} else {
+#pragma unroll
+					for (int i = 0; i < 4; ++i)
+						if (d + i < dh) o[d + i] = (T)(first ? x[b][4 * g + i] * f : to_float(o[d + i]) + x[b][4 * g + i] * f);
+				}
+			}
+	}
 }
 
 // Turns a block of raw scores into p (before masking) and, where scores are capped, leaves 1 - (c / cap)^2 in slope.
@@ -129,11 +138,17 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 			row_from<T, VEC>(o, orow, a.dh, half, t, live_row);
 #pragma unroll
 			for (int j = 0; j < 8; ++j) delta += to_float(g[t].e[j]) * to_float(o.e[j]);
-			if (sizeof(T) == 2 && rest) {
+		}
+		if (sizeof(T) == 2 && rest) {
+			float more = 0.0f;
+#pragma unroll
+			for (int t = 0; t < DH / 16; ++t) {
+				Frag<T> o;
 				row_from<T, VEC>(o, rest, a.dh, half, t, live_row);
 #pragma unroll
-				for (int j = 0; j < 8; ++j) delta += to_float(g[t].e[j]) * to_float(o.e[j]);
+				for (int j = 0; j < 8; ++j) more += to_float(g[t].e[j]) * to_float(o.e[j]);
 			}
+			delta += more;
 		}
 		delta = add_halves(delta);
 	}

@@ -183,41 +183,42 @@ __device__ __forceinline__ T rest_of(float x, T rounded) {
 // Stores a column: head row `o` takes the dh sums times f, `rest` (16 bits only, or null) what they lose in their rounding.
 template <typename T, int DH, bool VEC>
 __device__ __forceinline__ void store_column(T* o, T* rest, const f32x16* x, float f, int dh, int half) {
+	if constexpr (VEC && sizeof(T) == 2) {  // (dh is a multiple of 8)
 #pragma unroll
-	for (int b = 0; b < DH / 32; ++b)
+		for (int b = 0; b < DH / 32; ++b)
 #pragma unroll
-		for (int g = 0; g < 4; ++g) {
-			const int d = 32 * b + 8 * g + 4 * half;
-			union {
-				T e[4];
-				uint64_t w8;
-				u32x4 w16;
-			} y;
+			for (int g = 0; g < 2; ++g) {
+				const int d = 32 * b + 16 * g + 8 * half;
+				Frag<T> y, z;
 #pragma unroll
-			for (int i = 0; i < 4; ++i) y.e[i] = (T)(x[b][4 * g + i] * f);
-			if (VEC) {
-				if (d < dh) {
-					if constexpr (sizeof(T) == 2) *(uint64_t*)(o + d) = y.w8;
-					else *(u32x4*)(o + d) = y.w16;
+				for (int i = 0; i < 8; ++i) {
+					y.e[i] = (T)(x[b][8 * g + i] * f);
+					z.e[i] = rest_of(x[b][8 * g + i] * f, y.e[i]);
 				}
-			} else {
-#pragma unroll
-				for (int i = 0; i < 4; ++i)
-					if (d + i < dh) o[d + i] = y.e[i];
+				eight_of(y);
+				eight_of(z);
+				if (d < dh) *(u32x4*)(o + d) = y.w;
+				if (rest && d < dh) *(u32x4*)(rest + d) = z.w;
 			}
-			if constexpr (sizeof(T) == 2) {
-				if (!rest) continue;
+	} else {
 #pragma unroll
-				for (int i = 0; i < 4; ++i) y.e[i] = rest_of(x[b][4 * g + i] * f, y.e[i]);
-				if (VEC) {
-					if (d < dh) *(uint64_t*)(rest + d) = y.w8;
+		for (int b = 0; b < DH / 32; ++b)
+#pragma unroll
+			for (int g = 0; g < 4; ++g) {
+				const int d = 32 * b + 8 * g + 4 * half;
+				if constexpr (VEC) {
+					if (d < dh) *(f32x4*)(o + d) = f32x4{x[b][4 * g] * f, x[b][4 * g + 1] * f, x[b][4 * g + 2] * f, x[b][4 * g + 3] * f};
 				} else {
 #pragma unroll
 					for (int i = 0; i < 4; ++i)
-						if (d + i < dh) rest[d + i] = y.e[i];
+						if (d + i < dh) {
+							const T y = (T)(x[b][4 * g + i] * f);
+							o[d + i] = y;
+							if (sizeof(T) == 2 && rest) rest[d + i] = rest_of(x[b][4 * g + i] * f, y);
+						}
 				}
 			}
-		}
+	}
 }
 
 constexpr int kWaves = 4, kQueries = 32 * kWaves;

@@ -250,6 +250,17 @@ __device__ __forceinline__ float add_halves(float x) {
 	return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// Rows of a block's column as they are stored in 16 bits: of the 16 elements 16 g .. 16 g + 15, of which a lane holds two runs of
+// four (registers 8 g .. 8 g + 7 of a block), the lower half takes the first eight and the upper half the others.
+__device__ __forceinline__ void eight_of(Frag<__bf16>& f) {
+#pragma unroll
+	for (int i = 0; i < 2; ++i) {
+		const auto r = __builtin_amdgcn_permlane32_swap(f.w[i], f.w[2 + i], false, false);
+		f.w[i] = r[0];
+		f.w[2 + i] = r[1];
+	}
+}
+
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // tanh(x). In 16 bits 1 - 2 / (1 + e^2x) with the hardware's reciprocal: off by about 1e-7 of 1, far below the operands'
