@@ -44,7 +44,7 @@ struct MaskedAttentionArgs {
 	// backward
 	const void* g;
 	HeadStrides gs;
-	float* delta;  // {N, H, Tq}: g.out per row
+	float *delta, *lse2;  // {N, H, Tq}: g.out per row, and lse in units of log 2
 	void *dq, *dk, *dv;
 	HeadStrides dqs, dks, dvs;
 	int dq_first, dk_first, dv_first;

@@ -4,7 +4,7 @@
 //   p = exp(z - lse),  dz = p (g.v - delta),  delta = g.out,  ds = dz (1 - (c / cap)^2)
 //   dq = scale ds k,   dk = scale ds^T q,     dv = p^T g
 //
-// Two kernels, each recomputing the scores of its own products: dq by query rows (which also leaves delta), then dk and dv
+// Two kernels, each recomputing the scores of its own products: dq by query rows (which also leaves delta and lse in units of log 2), then dk and dv
 // by key rows, where the queries of all heads that share the key head are added in their order. No gradient is added by
 // atomics, so the results repeat bit for bit; the price is seven products of a pair of rows where five would do.
 #pragma once
@@ -62,25 +62,23 @@ __device__ __forceinline__ void store_gradient(T* o, const f32x16* x, float f, i
 // far: the distance of register i's pair; lse2: its row's lse in units of log 2.
 template <typename T, typename Far, typename Lse>
 __device__ __forceinline__ void weights(f32x16& s, f32x16& slope, const MaskedAttentionArgs& a, float slope2, Far far, Lse lse2) {
+	float c = a.scale * kLog2e;
 	if (a.cap > 0.0f) {
-		const float in = a.scale / a.cap, out = a.cap * kLog2e;
+		const float in = a.scale / a.cap;
+		c = a.cap * kLog2e;
 #pragma unroll
 		for (int i = 0; i < 16; ++i) {
-			const float t = tanh_of<T>(s[i] * in);
-			slope[i] = 1.0f - t * t;
-			s[i] = t * out;
+			s[i] = tanh_of<T>(s[i] * in);
+			slope[i] = __builtin_fmaf(-s[i], s[i], 1.0f);
 		}
-	} else {
-		const float c = a.scale * kLog2e;
-#pragma unroll
-		for (int i = 0; i < 16; ++i) s[i] *= c;
 	}
 	if (a.slopes) {
 #pragma unroll
-		for (int i = 0; i < 16; ++i) s[i] -= slope2 * far(i);
+		for (int i = 0; i < 16; ++i) s[i] = __builtin_fmaf(s[i], c, -slope2 * far(i));
+		c = 1.0f;
 	}
 #pragma unroll
-	for (int i = 0; i < 16; ++i) s[i] = exp2_of(s[i] - lse2(i));
+	for (int i = 0; i < 16; ++i) s[i] = exp2_of(__builtin_fmaf(s[i], c, -lse2(i)));
 }
 
 // dq: a workgroup's 128 queries of one head against the keys they see, as in the forward kernel: transposed scores, a query
@@ -314,7 +312,10 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 	};
 	if (run(std::false_type{})) run(std::true_type{});
 	off = add_halves(off);
-	if (live_row && half == 0) a.delta[row] = delta + off;
+	if (live_row && half == 0) {
+		a.delta[row] = delta + off;
+		a.lse2[row] = lse2;
+	}
 	if (live_row && a.dq)
 		store_gradient<T, DH, VEC>((T*)a.dq + n * a.dqs.sample + (int64_t)i * a.dqs.row + h * a.dqs.head, d, a.scale, a.dh, half,
 		                           a.dq_first != 0);
@@ -436,7 +437,7 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 			load_tile<T, DH, QT, kBwdWaves, VEC>(ring + buf * 2 * kTile, (const T*)a.q + n * a.qs.sample + (int64_t)q0 * a.qs.row + h * a.qs.head, a.qs.row, a.Tq - q0, a.dh, wave, lane);
 			load_tile<T, DH, QT, kBwdWaves, VEC>(ring + (buf * 2 + 1) * kTile, (const T*)a.g + n * a.gs.sample + (int64_t)q0 * a.gs.row + h * a.gs.head, a.gs.row, a.Tq - q0, a.dh, wave, lane);
 			const int64_t r = min(q0 + lane, a.Tq - 1), row = ((int64_t)n * a.H + h) * a.Tq + r;
-			if (wave == 0) __builtin_amdgcn_global_load_lds((global_void*)(a.lse + row), (lds_void*)lse_of[buf], 4, 0, 0);
+			if (wave == 0) __builtin_amdgcn_global_load_lds((global_void*)(a.lse2 + row), (lds_void*)lse_of[buf], 4, 0, 0);
 			if (wave == 1) __builtin_amdgcn_global_load_lds((global_void*)(a.delta + row), (lds_void*)delta_of[buf], 4, 0, 0);
 			if (wave == 2 && a.q_docs) __builtin_amdgcn_global_load_lds((global_void*)(a.q_docs + (int64_t)n * a.Tq + r), (lds_void*)docs_of[buf], 4, 0, 0);
 		};
@@ -464,7 +465,7 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 			const int i0 = fresh(4 * half);  // the tile's row of register y: i0 + 8 (y / 4) + y % 4
 			weights<T>(s, slope, a, a.slopes ? a.slopes[h] * kLog2e : 0.0f,
 			           [&](int y) { const int z = pos0 + q0 + i0 + 8 * (y / 4) + y % 4 - j; return (float)(z < 0 ? -z : z); },
-			           [&](int y) { return lse[i0 + 8 * (y / 4) + y % 4] * kLog2e; });
+			           [&](int y) { return lse[i0 + 8 * (y / 4) + y % 4]; });
 			unsigned seen = 0xffff;
 			if (partial) {
 				seen = 0;

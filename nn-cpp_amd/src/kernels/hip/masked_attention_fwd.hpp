@@ -42,8 +42,8 @@ struct Rows {
 };
 
 // Takes the KT keys from k0 on, whose rows are in kt and vt, into the wave's columns. docs: the wave's own room for KT ints.
-template <typename T, int DH, int KT, bool SAFE>
-__device__ __forceinline__ void take_keys(Rows<T, DH>& r, const MaskedAttentionArgs& a, int n, const char* kt, const char* vt, int* docs, int k0, int lane) {
+template <typename T, int DH, int KT, bool SAFE, typename At>
+__device__ __forceinline__ void take_keys(Rows<T, DH>& r, const MaskedAttentionArgs& a, int n, At at, const char* kt, const char* vt, int* docs, int k0, int lane) {
 	constexpr int RB = row_bytes<T, DH>();
 	const int col = lane & 31, half = lane >> 5;
 	// whether some of the wave's queries see some of the tile, and whether all of them all of it
@@ -56,7 +56,6 @@ __device__ __forceinline__ void take_keys(Rows<T, DH>& r, const MaskedAttentionA
 	}
 	if (!__any(some)) return;
 	const bool partial = !__all(all);
-	const Reader<T, RB> at(fresh_lane());
 	const int j0 = fresh(k0 + 4 * half);  // the key of block x's register i: j0 + 32 x + 8 (i / 4) + i % 4
 
 	f32x16 s[KT / 32];
@@ -73,18 +72,14 @@ __device__ __forceinline__ void take_keys(Rows<T, DH>& r, const MaskedAttentionA
 			mma(s[x], k, r.q[t]);
 		}
 
+	float c = a.scale * kLog2e;  // of the scores as they are, in units of log 2: multiplied in the exponential's own step
 	if (a.cap > 0.0f) {
-		const float in = a.scale / a.cap, out = a.cap * kLog2e;
+		const float in = a.scale / a.cap;
+		c = a.cap * kLog2e;
 #pragma unroll
 		for (int x = 0; x < KT / 32; ++x)
 #pragma unroll
-			for (int i = 0; i < 16; ++i) s[x][i] = out * tanh_of<T>(s[x][i] * in);
-	} else {
-		const float c = a.scale * kLog2e;
-#pragma unroll
-		for (int x = 0; x < KT / 32; ++x)
-#pragma unroll
-			for (int i = 0; i < 16; ++i) s[x][i] *= c;
+			for (int i = 0; i < 16; ++i) s[x][i] = tanh_of<T>(s[x][i] * in);
 	}
 	if (a.slopes) {
 #pragma unroll
@@ -92,8 +87,9 @@ __device__ __forceinline__ void take_keys(Rows<T, DH>& r, const MaskedAttentionA
 #pragma unroll
 			for (int i = 0; i < 16; ++i) {
 				const int d = r.pos - (j0 + 32 * x + 8 * (i / 4) + i % 4);
-				s[x][i] -= r.slope2 * (float)(d < 0 ? -d : d);
+				s[x][i] = __builtin_fmaf(s[x][i], c, -r.slope2 * (float)(d < 0 ? -d : d));
 			}
+		c = 1.0f;
 	}
 	unsigned seen[KT / 32];  // bit i: the lane's query sees the key of register i
 	if (partial) {
@@ -121,8 +117,10 @@ __device__ __forceinline__ void take_keys(Rows<T, DH>& r, const MaskedAttentionA
 	for (int x = 0; x < KT / 32; ++x)
 #pragma unroll
 		for (int i = 0; i < 16; ++i) top = fmaxf(top, s[x][i]);
-	top = max_halves(top);
-	if (__any(top > r.m)) {  // seldom after a row's first tiles
+	top = max_halves(top) * c;
+	// The base that exponents are taken from follows the maximum only where that has passed it by 2^8: sums and products keep their
+	// relative precision at any base, and most tiles then rescale nothing (some of 32 rows have a new maximum in four tiles of ten).
+	if (__any(top > r.m + 8.0f)) {
 		const float m = fmaxf(r.m, top), f = m == -kInf ? 1.0f : exp2_of(r.m - m);
 		r.m = m;
 		r.l *= f;
@@ -136,7 +134,7 @@ __device__ __forceinline__ void take_keys(Rows<T, DH>& r, const MaskedAttentionA
 	for (int x = 0; x < KT / 32; ++x)
 #pragma unroll
 		for (int i = 0; i < 16; ++i) {
-			s[x][i] = exp2_of(s[x][i] - base);
+			s[x][i] = exp2_of(__builtin_fmaf(s[x][i], c, -base));
 			r.l += s[x][i];
 		}
 
@@ -297,6 +295,7 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 	}
 	const int nt = (max(hi, pre) + KT - 1) / KT;
 
+	std::conditional_t<sizeof(T) == 2 && VEC, Places<T, DH>, Reader<T, RB>> at(lane);
 	auto run = [&](auto safe) {
 		r.clear();
 		// the tiles that some query may see, 64 at a time
@@ -330,7 +329,7 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 			asm volatile("" ::: "memory");
 			const int then = next();
 			if (then >= 0) load(then, to);
-			take_keys<T, DH, KT, decltype(safe)::value>(r, a, n, from, from + kTile, docs[wave], cur * KT, lane);
+			take_keys<T, DH, KT, decltype(safe)::value>(r, a, n, at, from, from + kTile, docs[wave], cur * KT, lane);
 			cur = then;
 		};
 		if (cur >= 0) load(cur, lds);
@@ -431,7 +430,7 @@ __global__ __launch_bounds__((64 * SplitShape<T, DH>::NW), 1) void masked_attent
 				wait_loads();
 			}
 			const char* from = ring + stage * S::kStage;
-			take_keys<T, DH, KT, decltype(safe)::value>(r, a, n, from, from + S::kTile, docs[wave], x * KT, lane);
+			take_keys<T, DH, KT, decltype(safe)::value>(r, a, n, Reader<T, S::RB>(fresh_lane()), from, from + S::kTile, docs[wave], x * KT, lane);
 			// the stage is loaded over next: its reads are done
 			asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 			stage = (stage + 1) % ST;

@@ -205,6 +205,31 @@ struct Reader {
 	}
 };
 
+// The same places kept in registers, one to a read, for kernels with room for them: a tile's own place is then part of the
+// instruction, and no read costs an addition.
+template <typename T, int DH>
+struct Places {
+	static constexpr int RB = row_bytes<T, DH>();
+	int r[DH / 16], c[DH / 32][2];
+
+	__device__ __forceinline__ explicit Places(int lane) {
+		static_assert(sizeof(T) == 2, "16-bit types");
+		const Reader<T, RB> at(lane);
+#pragma unroll
+		for (int t = 0; t < DH / 16; ++t) r[t] = fresh(at.r ^ (32 * t));
+#pragma unroll
+		for (int b = 0; b < DH / 32; ++b) {
+			c[b][0] = fresh(at.c ^ (64 * b));
+			c[b][1] = fresh(at.c ^ (64 * b) ^ 32);
+		}
+	}
+	__device__ __forceinline__ void rows(Frag<T>& f, const char* at, int t) const { f.w = *(const u32x4*)(at + r[t]); }
+	__device__ __forceinline__ void columns(Frag<T>& f, const char* at, int block) const {
+		f.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + c[block][0]));
+		f.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 8 * RB + c[block][1]));
+	}
+};
+
 // One element of a tile.
 template <typename T, int DH>
 __device__ __forceinline__ float element_of(const char* tile, int row, int d) {

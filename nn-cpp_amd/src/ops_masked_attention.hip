@@ -143,7 +143,7 @@ bool beside(const Geom& g, const Operand& x, const Operand& y) {
 }
 
 struct Plan {
-	size_t q_ranges = 0, k_ranges = 0, partial = 0, delta = 0, total = 0;
+	size_t q_ranges = 0, k_ranges = 0, partial = 0, delta = 0, lse2 = 0, total = 0;
 	int splits = 0, parts = 1;
 };
 
@@ -157,6 +157,7 @@ Plan plan_of(const Geom& g, bool docs, bool backward) {
 	}
 	if (backward) {
 		p.delta = w.add(g.N * g.H * g.Tq * 4);
+		p.lse2 = w.add(g.N * g.H * g.Tq * 4);
 		p.parts = masked_attention_parts((int)g.N, (int)g.Tq, (int)g.Tk, (int)g.H, (int)g.Hkv);
 		if (p.parts > 1) p.partial = w.add((size_t)p.parts * 2 * g.N * g.Hkv * g.Tk * ((g.Dh + 3) / 4 * 4) * 4);
 	} else {
@@ -297,6 +298,7 @@ int nnh_masked_attention_backward(int type, size_t N, size_t Tq, size_t Tk, size
 	Scratch ws(s, p.total);
 	if (ws.status() != NNH_OK) return ws.status();
 	a.delta = ws.at<float>(p.delta);
+	a.lse2 = ws.at<float>(p.lse2);
 	a.parts = p.parts;
 	a.partial = ws.at<float>(p.partial);
 	rc = run_ranges(a, p, ws, s);
