@@ -26,11 +26,9 @@ using attn::f32x16;
 using attn::f32x2;
 using attn::f32x4;
 using attn::Frag;
-using attn::global_void;
 using attn::kInf;
 using attn::kLog2e;
 using attn::lds_s16x4;
-using attn::lds_void;
 using attn::u32x4;
 
 constexpr int BK = 64;
@@ -70,19 +68,15 @@ struct Loader {
 			}
 		}
 	}
-	// Loads the stage and moves on; live: depths left, none or less past the last stage (what is past them is zero).
+	// The stage's load j, after which it moves on; live: depths left, none or less past the last stage (what is past them is zero).
 	// on: with MASK, bit k of a word for each depth of the stage: whether it is to be loaded.
-	template <bool MASK = false>
+	template <int j, bool MASK = false>
 	__device__ __forceinline__ void load(char* tile, int live, int wave, int lane, uint64_t on = 0) {
-#pragma unroll
-		for (int j = 0; j < kSteps; ++j) {
-			const int w = (j * NW + wave) * 64 + lane;
-			const int k = TR ? w / (R / 8) : ((w % 8) ^ attn::swizzle<128>(w / 8)) * 8;
-			const bool take = MASK ? (on >> k & 1) != 0 : k < live;
-			const void* src = take ? (const void*)p[j] : (const void*)&attn::kZeroWord;
-			__builtin_amdgcn_global_load_lds((global_void*)src, (lds_void*)(tile + (j * NW + wave) * 1024), 16, 0, 0);
-			p[j] += step;
-		}
+		const int w = (j * NW + wave) * 64 + lane;
+		const int k = TR ? w / (R / 8) : ((w % 8) ^ attn::swizzle<128>(w / 8)) * 8;
+		const bool take = MASK ? (on >> k & 1) != 0 : k < live;
+		attn::load_words<j * NW * 1024>(take ? (const void*)p[j] : (const void*)&attn::kZeroWord, attn::lds_place(tile + wave * 1024));
+		p[j] += step;
 	}
 };
 
@@ -159,19 +153,19 @@ __global__ __launch_bounds__(T::kThreads, 2) void gemm16_kernel(Gemm16Args a) {
 #pragma unroll
 		for (int j = 0; j < J; ++j) rb.read(fb[set][j], y, j, t);
 	};
-	// The products of one operand set. A read of the next depths goes behind each, and of the loads that were issued before
-	// (kLoads where `loads`) one behind every other: a wave whose loads wait for their turn multiplies nothing meanwhile.
-	auto multiply = [&](int set, auto loads) {
-#pragma unroll
-		for (int i = 0; i < I; ++i)
-#pragma unroll
-			for (int j = 0; j < J; ++j) attn::mma(acc[i][j], fa[set][i], fb[set][j]);
+	// The products of one operand set. A read of the next depths goes behind each, and of a half stage's loads (load(0) ..
+	// load(kLoads - 1)) one behind every other: a wave whose loads wait for their turn multiplies nothing meanwhile.
+	auto multiply = [&](int set, auto load) {
 		constexpr int kReads = I * (ATR ? 2 : 1) + J * (BTR ? 2 : 1);
+		attn::each<I * J>([&](auto at) {
+			constexpr int x = decltype(at)::value, per = I * J / T::kLoads;
+			attn::mma(acc[x / J][x % J], fa[set][x / J], fb[set][x % J]);
+			if constexpr (x % per == per - 1) load(std::integral_constant<int, x / per>{});
+		});
 #pragma unroll
 		for (int x = 0; x < I * J; ++x) {
 			__builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
 			__builtin_amdgcn_sched_group_barrier(0x100, (kReads + I * J - 1) / (I * J), 0);
-			if (decltype(loads)::value && x % (I * J / T::kLoads) == I * J / T::kLoads - 1) __builtin_amdgcn_sched_group_barrier(0x010, 1, 0);
 		}
 		__builtin_amdgcn_sched_barrier(0);
 	};
@@ -182,38 +176,39 @@ __global__ __launch_bounds__(T::kThreads, 2) void gemm16_kernel(Gemm16Args a) {
 	constexpr bool kMask = EPI == kGemm16Out && BTR;
 	const uint64_t* const words = kMask ? a.live + from / BK : nullptr;
 	uint64_t word = kMask && a.depth > 0 ? words[0] : 0;
-	auto load_a = [&](int x, int s) {
+	auto load_a = [&](auto j, int x, int s) {
+		constexpr int J0 = decltype(j)::value;
 		if constexpr (kMask) {
-			la.template load<true>(place(x), 0, wave, lane, word);
-			word = s + 1 < stages ? words[s + 1] : 0;
+			la.template load<J0, true>(place(x), 0, wave, lane, word);
+			if (J0 == T::kLoads - 1) word = s + 1 < stages ? words[s + 1] : 0;
 		} else {
-			la.load(place(x), a.depth - s * BK, wave, lane);
+			la.template load<J0>(place(x), a.depth - s * BK, wave, lane);
 		}
 	};
+	auto load_b = [&](auto j, int x, int s) { lb.template load<decltype(j)::value>(place(x), a.depth - s * BK, wave, lane); };
 	// Stage s (s % 5 = S), whose first operands are in registers. Before its last depths are multiplied every wave has read
 	// them, and the next stage has arrived: from there on B of stage s + 2 and then, a step later, A of stage s + 3 may take its
 	// places, and the next one's first operands are read.
 	auto step = [&](int s, auto mod) {
 		constexpr int S = decltype(mod)::value;
 		read(1, place(2 * S), place(2 * S + 1), 1);
-		load_a(2 * S + 4, s + 2);
-		multiply(0, std::true_type{});
+		multiply(0, [&](auto j) { load_a(j, 2 * S + 4, s + 2); });
 #pragma unroll
 		for (int t = 1; t < BK / 16 - 1; ++t) {
 			read(~t & 1, place(2 * S), place(2 * S + 1), t + 1);
-			multiply(t & 1, std::false_type{});
+			multiply(t & 1, [](auto) {});
 		}
 		asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(T::kLoads) : "memory");
 		__builtin_amdgcn_s_barrier();
 		asm volatile("" ::: "memory");
 		read(0, place(2 * S + 2), place(2 * S + 3), 0);
-		lb.load(place(2 * S), a.depth - (s + 2) * BK, wave, lane);
-		multiply(1, std::true_type{});
+		multiply(1, [&](auto j) { load_b(j, 2 * S, s + 2); });
 	};
-	load_a(0, 0);
-	lb.load(place(1), a.depth, wave, lane);
-	load_a(2, 1);
-	lb.load(place(3), a.depth - BK, wave, lane);
+#pragma unroll
+	for (int s = 0; s < 2; ++s) {
+		attn::each<T::kLoads>([&](auto j) { load_a(j, 2 * s, s); });
+		attn::each<T::kLoads>([&](auto j) { load_b(j, 2 * s + 1, s); });
+	}
 	asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * T::kLoads) : "memory");
 	__builtin_amdgcn_s_barrier();
 	asm volatile("" ::: "memory");

@@ -91,11 +91,10 @@ __device__ __forceinline__ void weights(f32x16& s, f32x16& slope, const MaskedAt
 template <typename T, int DH, bool VEC>
 __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void masked_attention_dq_kernel(MaskedAttentionArgs a) {
 	constexpr int RB = row_bytes<T, DH>(), KT = RB >= 512 ? 32 : 64, kTile = KT * RB;
-	__shared__ __attribute__((aligned(1024))) char lds[4 * kTile];
-	__shared__ __attribute__((aligned(16))) int docs_of[kBwdWaves][KT];
+	__shared__ __attribute__((aligned(1024))) char lds[4 * kTile + 2 * 256 + kBwdWaves * 4];
+	char* const docs_at = lds + 4 * kTile;  // the two tiles'
 	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 	const int col = lane & 31, half = lane >> 5;
-	int* const docs = docs_of[wave];
 	const int tiles = (a.Tq + kBwdRows - 1) / kBwdRows, pairs = a.N * a.Hkv;
 	int tile, h, n;
 	{
@@ -176,6 +175,9 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 	const int nt = (max(hi, pre) + KT - 1) / KT;
 	f32x16 d[DH / 32];
 	float off;
+	arrived(q);
+	arrived(g);
+	arrived();
 
 	auto run = [&](auto safe) {
 		off = 0.0f;
@@ -185,6 +187,7 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 			for (int x = 0; x < 16; ++x) d[b][x] = 0.0f;
 		int base = -64;
 		uint64_t on = 0;
+		DocRange held{0, 0, 0}, ahead{0, 0, 0};  // the documents of tile base + lane, of the tile that next() named
 		auto next = [&]() -> int {
 			while (on == 0) {
 				base += 64;
@@ -192,30 +195,30 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 				const int x = base + lane, k0 = x * KT;
 				bool s = x < nt && ((k0 < hi && k0 + KT > lo) || k0 < pre);
 				if (s && a.k_docs) {
-					const DocRange r = a.k_ranges[(int64_t)n * kb + k0 / 64];
-					s = r.lo <= mine.hi && r.hi >= mine.lo;
+					held = a.k_ranges[(int64_t)n * kb + k0 / 64];
+					s = held.lo <= mine.hi && held.hi >= mine.lo;
 				}
 				on = __ballot(s);
 			}
 			const int x = __builtin_ctzll(on);
 			on &= on - 1;
+			if (a.k_docs) ahead = of_lane(held, x);
 			return base + x;
 		};
-		auto load = [&](int x, char* to) {
+		auto load = [&](int x, char* to, char* docs_to) {
+			if (a.k_docs && wave == 0) load_numbers(a.k_docs + (int64_t)n * a.Tk + min(x * KT + lane, a.Tk - 1), docs_to);
 			load_tile<T, DH, KT, kBwdWaves, VEC>(to, kbase + (int64_t)x * KT * a.ks.row, a.ks.row, live - x * KT, a.dh, wave, lane);
 			load_tile<T, DH, KT, kBwdWaves, VEC>(to + kTile, vbase + (int64_t)x * KT * a.vs.row, a.vs.row, live - x * KT, a.dh, wave, lane);
 		};
-		auto take = [&](const char* kt, const char* vt, int k0) {
+		auto take = [&](const char* kt, const char* vt, const int* docs, DocRange r, int k0) {
 			bool some = (k0 < see.hi && k0 + KT > see.lo) || k0 < see.pre;
 			bool all = (k0 >= see.lo && k0 + KT <= see.hi) || k0 + KT <= see.pre;
 			if (a.k_docs) {
-				const DocRange r = a.k_ranges[(int64_t)n * kb + k0 / 64];
 				some = some && see.doc >= r.lo && see.doc <= r.hi;
 				all = all && see.doc == r.lo && see.doc == r.hi && !r.none;
 			}
 			if (!__any(some)) return;
 			const bool partial = !__all(all);
-			if (partial && a.k_docs && lane < KT) docs[lane] = a.k_docs[(int64_t)n * a.Tk + min(k0 + lane, a.Tk - 1)];
 #pragma clang loop unroll(disable)
 			for (int x = 0; x < KT / 32; ++x) {
 				const Reader<T, RB> at(fresh_lane());
@@ -289,26 +292,29 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 			}
 		};
 		int cur = next();
-		auto step = [&](char* from, char* to) {
+		auto step = [&](auto buf) {
+			constexpr int B = decltype(buf)::value;
+			char* const from = lds + B * 2 * kTile;
 			wait_loads();
 			__builtin_amdgcn_s_barrier();
 			asm volatile("" ::: "memory");
+			const DocRange r = ahead;
 			const int then = next();
-			if (then >= 0) load(then, to);
-			take(from, from + kTile, cur * KT);
+			if (then >= 0) load(then, lds + (1 - B) * 2 * kTile, docs_at + (1 - B) * 256);
+			take(from, from + kTile, (const int*)(docs_at + B * 256), r, cur * KT);
 			cur = then;
 		};
-		if (cur >= 0) load(cur, lds);
+		if (cur >= 0) load(cur, lds, docs_at);
 		while (cur >= 0) {
-			step(lds, lds + 2 * kTile);
-			if (cur >= 0) step(lds + 2 * kTile, lds);
+			step(std::integral_constant<int, 0>{});
+			if (cur >= 0) step(std::integral_constant<int, 1>{});
 		}
 		bool bad = false;
 #pragma unroll
 		for (int b = 0; b < DH / 32; ++b)
 #pragma unroll
 			for (int x = 0; x < 16; ++x) bad |= not_finite(d[b][x]);
-		return __syncthreads_or(bad);
+		return any_wave<kBwdWaves>((int*)(docs_at + 2 * 256), wave, lane, bad);
 	};
 	if (run(std::false_type{})) run(std::true_type{});
 	off = add_halves(off);
@@ -330,11 +336,10 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 template <typename T, int DH, bool VEC>
 __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void masked_attention_dkv_kernel(MaskedAttentionArgs a) {
 	constexpr int RB = row_bytes<T, DH>(), QT = 32, kTile = QT * RB;
-	__shared__ __attribute__((aligned(1024))) char lds[kBwdRows * RB + 4 * kTile];
-	__shared__ __attribute__((aligned(16))) float lse_of[2][64], delta_of[2][64];
-	__shared__ __attribute__((aligned(16))) int docs_of[2][64];
+	__shared__ __attribute__((aligned(1024))) char lds[kBwdRows * RB + 4 * kTile + 2 * 3 * 256 + kBwdWaves * 4];
 	char* const vt = lds;
 	char* const ring = lds + kBwdRows * RB;
+	char* const rows = ring + 4 * kTile;  // per buffer 64 rows' lse, delta and documents
 	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 	const int col = lane & 31, half = lane >> 5;
 	const int pairs = a.N * a.Hkv;
@@ -402,6 +407,8 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 #pragma unroll
 		for (int t = 0; t < DH / 16; ++t) row_from<T, VEC>(kf[t], kr, a.dh, half, t, j < live);
 	}
+	arrived(kf);
+	arrived();
 	f32x16 dk[DH / 32], dv[DH / 32];
 
 	auto run = [&](auto safe) {
@@ -413,6 +420,7 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 		// workgroups of one key head read the same rows at about the same time.
 		int head = -1, base = -64;
 		uint64_t on = 0;
+		DocRange held{0, 0, 0}, ahead{0, 0, 0};  // the documents of tile base + lane, of the tile that next() named
 		auto next = [&]() -> int {
 			while (on == 0) {
 				base -= 64;
@@ -423,13 +431,14 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 				const int x = base + lane, q0 = x * QT;
 				bool s = x < nt && q0 + QT > lo && x % a.parts == part;
 				if (s && a.q_docs) {
-					const DocRange r = a.q_ranges[(int64_t)n * qb + q0 / 64];
-					s = r.lo <= mine.hi && r.hi >= mine.lo;
+					held = a.q_ranges[(int64_t)n * qb + q0 / 64];
+					s = held.lo <= mine.hi && held.hi >= mine.lo;
 				}
 				on = __ballot(s);
 			}
 			const int x = 63 - __builtin_clzll(on);
 			on &= ~((uint64_t)1 << x);
+			if (a.q_docs) ahead = of_lane(held, x);
 			return base + x;
 		};
 		auto load = [&](int x, int buf) {
@@ -437,14 +446,13 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 			load_tile<T, DH, QT, kBwdWaves, VEC>(ring + buf * 2 * kTile, (const T*)a.q + n * a.qs.sample + (int64_t)q0 * a.qs.row + h * a.qs.head, a.qs.row, a.Tq - q0, a.dh, wave, lane);
 			load_tile<T, DH, QT, kBwdWaves, VEC>(ring + (buf * 2 + 1) * kTile, (const T*)a.g + n * a.gs.sample + (int64_t)q0 * a.gs.row + h * a.gs.head, a.gs.row, a.Tq - q0, a.dh, wave, lane);
 			const int64_t r = min(q0 + lane, a.Tq - 1), row = ((int64_t)n * a.H + h) * a.Tq + r;
-			if (wave == 0) __builtin_amdgcn_global_load_lds((global_void*)(a.lse2 + row), (lds_void*)lse_of[buf], 4, 0, 0);
-			if (wave == 1) __builtin_amdgcn_global_load_lds((global_void*)(a.delta + row), (lds_void*)delta_of[buf], 4, 0, 0);
-			if (wave == 2 && a.q_docs) __builtin_amdgcn_global_load_lds((global_void*)(a.q_docs + (int64_t)n * a.Tq + r), (lds_void*)docs_of[buf], 4, 0, 0);
+			if (wave == 0) load_numbers(a.lse2 + row, rows + buf * 768);
+			if (wave == 1) load_numbers(a.delta + row, rows + buf * 768 + 256);
+			if (wave == 2 && a.q_docs) load_numbers(a.q_docs + (int64_t)n * a.Tq + r, rows + buf * 768 + 512);
 		};
-		auto take = [&](const char* qt, const char* gt, const float* lse, const float* delta, const int* docs, int q0, int h) {
+		auto take = [&](const char* qt, const char* gt, const float* lse, const float* delta, const int* docs, DocRange r, int q0, int h) {
 			bool some = q0 < see.hi && q0 + QT > see.lo, all = q0 >= see.lo && q0 + QT <= see.hi;
 			if (a.q_docs) {
-				const DocRange r = a.q_ranges[(int64_t)n * qb + q0 / 64];
 				some = some && see.doc >= r.lo && see.doc <= r.hi;
 				all = all && see.doc == r.lo && see.doc == r.hi && !r.none;
 			}
@@ -543,9 +551,10 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 			wait_loads();
 			__builtin_amdgcn_s_barrier();
 			asm volatile("" ::: "memory");
+			const DocRange r = ahead;
 			const int h = hk * a.G + head, then = next();
 			if (then >= 0) load(then, 1 - B);
-			take(ring + B * 2 * kTile, ring + (B * 2 + 1) * kTile, lse_of[B], delta_of[B], docs_of[B], cur * QT, h);
+			take(ring + B * 2 * kTile, ring + (B * 2 + 1) * kTile, (const float*)(rows + B * 768), (const float*)(rows + B * 768 + 256), (const int*)(rows + B * 768 + 512), r, cur * QT, h);
 			cur = then;
 		};
 		if (cur >= 0) load(cur, 0);
@@ -558,7 +567,7 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 		for (int b = 0; b < DH / 32; ++b)
 #pragma unroll
 			for (int x = 0; x < 16; ++x) bad |= not_finite(dk[b][x]) || not_finite(dv[b][x]);
-		return __syncthreads_or(bad);
+		return any_wave<kBwdWaves>((int*)(rows + 2 * 768), wave, lane, bad);
 	};
 	if (run(std::false_type{})) run(std::true_type{});
 	if (j >= a.Tk) return;

@@ -41,16 +41,15 @@ struct Rows {
 	}
 };
 
-// Takes the KT keys from k0 on, whose rows are in kt and vt, into the wave's columns. docs: the wave's own room for KT ints.
+// Takes the KT keys from k0 on, whose rows are in kt and vt and documents in docs and d, into the wave's columns.
 template <typename T, int DH, int KT, bool SAFE, typename At>
-__device__ __forceinline__ void take_keys(Rows<T, DH>& r, const MaskedAttentionArgs& a, int n, At at, const char* kt, const char* vt, int* docs, int k0, int lane) {
+__device__ __forceinline__ void take_keys(Rows<T, DH>& r, const MaskedAttentionArgs& a, At at, const char* kt, const char* vt, const int* docs, DocRange d, int k0, int lane) {
 	constexpr int RB = row_bytes<T, DH>();
 	const int col = lane & 31, half = lane >> 5;
 	// whether some of the wave's queries see some of the tile, and whether all of them all of it
 	bool some = (k0 < r.s.hi && k0 + KT > r.s.lo) || k0 < r.s.pre;
 	bool all = (k0 >= r.s.lo && k0 + KT <= r.s.hi) || k0 + KT <= r.s.pre;
 	if (a.k_docs) {
-		const DocRange d = a.k_ranges[(int64_t)n * ((a.Tk + 63) / 64) + k0 / 64];
 		some = some && r.s.doc >= d.lo && r.s.doc <= d.hi;
 		all = all && r.s.doc == d.lo && r.s.doc == d.hi && !d.none;
 	}
@@ -93,7 +92,6 @@ __device__ __forceinline__ void take_keys(Rows<T, DH>& r, const MaskedAttentionA
 	}
 	unsigned seen[KT / 32];  // bit i: the lane's query sees the key of register i
 	if (partial) {
-		if (a.k_docs && lane < KT) docs[lane] = a.k_docs[(int64_t)n * a.Tk + min(k0 + lane, a.Tk - 1)];
 #pragma unroll
 		for (int x = 0; x < KT / 32; ++x) {
 			seen[x] = 0;
@@ -102,9 +100,9 @@ __device__ __forceinline__ void take_keys(Rows<T, DH>& r, const MaskedAttentionA
 			if (a.k_docs) {
 #pragma unroll
 				for (int g = 0; g < 4; ++g) {
-					const i32x4 d = *(const i32x4*)(docs + 32 * x + 8 * g + 4 * half);
+					const i32x4 e = *(const i32x4*)(docs + 32 * x + 8 * g + 4 * half);
 #pragma unroll
-					for (int i = 0; i < 4; ++i) seen[x] &= d[i] == r.s.doc ? ~0u : ~(1u << (4 * g + i));
+					for (int i = 0; i < 4; ++i) seen[x] &= e[i] == r.s.doc ? ~0u : ~(1u << (4 * g + i));
 				}
 			}
 #pragma unroll
@@ -236,8 +234,8 @@ constexpr int keys_per_tile() {
 template <typename T, int DH, bool VEC>
 __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void masked_attention_forward_kernel(MaskedAttentionArgs a) {
 	constexpr int KT = keys_per_tile<T, DH>(), RB = row_bytes<T, DH>(), kTile = KT * RB;
-	__shared__ __attribute__((aligned(1024))) char lds[4 * kTile];
-	__shared__ __attribute__((aligned(16))) int docs[kWaves][KT];
+	__shared__ __attribute__((aligned(1024))) char lds[4 * kTile + 2 * 256 + kWaves * 4];
+	char* const docs = lds + 4 * kTile;  // the two tiles'
 	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 	const int col = lane & 31, half = lane >> 5;
 	// Heads of one key head stay on one XCD where the pairs divide evenly (its L2 then holds their keys); the queries that
@@ -294,13 +292,21 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 		}
 	}
 	const int nt = (max(hi, pre) + KT - 1) / KT;
+	arrived(r.q);
+	arrived();
 
-	std::conditional_t<sizeof(T) == 2 && VEC, Places<T, DH>, Reader<T, RB>> at(lane);
+	constexpr bool kPlaces = sizeof(T) == 2 && VEC;
+	const std::conditional_t<kPlaces, Places<T, DH>, int> places(lane);
+	auto at = [&] {
+		if constexpr (kPlaces) return places;
+		else return Reader<T, RB>(fresh_lane());
+	};
 	auto run = [&](auto safe) {
 		r.clear();
 		// the tiles that some query may see, 64 at a time
 		int base = -64;
 		uint64_t on = 0;
+		DocRange held{0, 0, 0}, ahead{0, 0, 0};  // the documents of tile base + lane, of the tile that next() named
 		auto next = [&]() -> int {
 			while (on == 0) {
 				base += 64;
@@ -308,36 +314,41 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 				const int x = base + lane, k0 = x * KT;
 				bool see = x < nt && ((k0 < hi && k0 + KT > lo) || k0 < pre);
 				if (see && a.k_docs) {
-					const DocRange d = a.k_ranges[(int64_t)n * ((a.Tk + 63) / 64) + k0 / 64];
-					see = d.lo <= mine.hi && d.hi >= mine.lo;
+					held = a.k_ranges[(int64_t)n * ((a.Tk + 63) / 64) + k0 / 64];
+					see = held.lo <= mine.hi && held.hi >= mine.lo;
 				}
 				on = __ballot(see);
 			}
 			const int x = __builtin_ctzll(on);
 			on &= on - 1;
+			if (a.k_docs) ahead = of_lane(held, x);
 			return base + x;
 		};
-		auto load = [&](int x, char* to) {
+		auto load = [&](int x, char* to, char* docs_to) {
+			if (a.k_docs && wave == 0) load_numbers(a.k_docs + (int64_t)n * a.Tk + min(x * KT + lane, a.Tk - 1), docs_to);
 			load_tile<T, DH, KT, kWaves, VEC>(to, kbase + (int64_t)x * KT * a.ks.row, a.ks.row, live - x * KT, a.dh, wave, lane);
 			load_tile<T, DH, KT, kWaves, VEC>(to + kTile, vbase + (int64_t)x * KT * a.vs.row, a.vs.row, live - x * KT, a.dh, wave, lane);
 		};
 		int cur = next();
 		// one tile from `from`, the next one on its way to `to`
-		auto step = [&](char* from, char* to) {
+		auto step = [&](auto buf) {
+			constexpr int B = decltype(buf)::value;
+			char* const from = lds + B * 2 * kTile;
 			wait_loads();
 			__builtin_amdgcn_s_barrier();  // this tile has arrived for all waves, and all are done with the last one
 			asm volatile("" ::: "memory");
+			const DocRange d = ahead;
 			const int then = next();
-			if (then >= 0) load(then, to);
-			take_keys<T, DH, KT, decltype(safe)::value>(r, a, n, at, from, from + kTile, docs[wave], cur * KT, lane);
+			if (then >= 0) load(then, lds + (1 - B) * 2 * kTile, docs + (1 - B) * 256);
+			take_keys<T, DH, KT, decltype(safe)::value>(r, a, at(), from, from + kTile, (const int*)(docs + B * 256), d, cur * KT, lane);
 			cur = then;
 		};
-		if (cur >= 0) load(cur, lds);
+		if (cur >= 0) load(cur, lds, docs);
 		while (cur >= 0) {
-			step(lds, lds + 2 * kTile);
-			if (cur >= 0) step(lds + 2 * kTile, lds);
+			step(std::integral_constant<int, 0>{});
+			if (cur >= 0) step(std::integral_constant<int, 1>{});
 		}
-		return __syncthreads_or(r.bad());
+		return any_wave<kWaves>((int*)(docs + 2 * 256), wave, lane, r.bad());
 	};
 	if (run(std::false_type{})) run(std::true_type{});
 
@@ -360,15 +371,14 @@ struct SplitShape {
 	static constexpr int kLoads = 2 * kTile / 1024;  // a wave's load instructions for a stage
 	static constexpr int kMerge = NW * 32 * (DH + 4) * 4;
 	static constexpr int kLds = NW * ST * kStage > kMerge ? NW * ST * kStage : kMerge;
-	static_assert(kLds <= 160 * 1024 && (ST - 1) * kLoads <= 63, "LDS, and loads that a wave may have outstanding");
+	static_assert(kLds + NW * ST * 256 + NW * 4 <= 160 * 1024 && (ST - 1) * kLoads <= 63, "LDS, and loads that a wave may have outstanding");
 };
 
 template <typename T, int DH, bool VEC>
 __global__ __launch_bounds__((64 * SplitShape<T, DH>::NW), 1) void masked_attention_split_kernel(MaskedAttentionArgs a) {
 	using S = SplitShape<T, DH>;
 	constexpr int KT = S::KT, NW = S::NW, ST = S::ST;
-	__shared__ __attribute__((aligned(1024))) char lds[S::kLds];
-	__shared__ __attribute__((aligned(16))) int docs[NW][KT];
+	__shared__ __attribute__((aligned(1024))) char lds[S::kLds + NW * ST * 256 + NW * 4];
 	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 	const int col = lane & 31, half = lane >> 5;
 	const int columns = a.Tq * a.G, pairs = a.N * a.Hkv;
@@ -405,11 +415,15 @@ __global__ __launch_bounds__((64 * SplitShape<T, DH>::NW), 1) void masked_attent
 	const int t0 = lo / KT, t1 = (hi + KT - 1) / KT, per = (max(t1 - t0, 0) + a.splits * NW - 1) / (a.splits * NW);
 	const int begin = min(t0 + (split * NW + wave) * per, t1), end = min(begin + per, t1);
 	char* const ring = lds + wave * ST * S::kStage;
+	char* const docs = lds + S::kLds + wave * ST * 256;
+	arrived(r.q);
+	arrived();
 
 	auto run = [&](auto safe) {
 		r.clear();
 		auto load = [&](int x, int stage) {
 			char* to = ring + stage * S::kStage;
+			if (a.k_docs) load_numbers(a.k_docs + (int64_t)n * a.Tk + min(x * KT + lane, a.Tk - 1), docs + stage * 256);
 			load_tile<T, DH, KT, 1, VEC>(to, kbase + (int64_t)x * KT * a.ks.row, a.ks.row, live - x * KT, a.dh, 0, lane);
 			load_tile<T, DH, KT, 1, VEC>(to + S::kTile, vbase + (int64_t)x * KT * a.vs.row, a.vs.row, live - x * KT, a.dh, 0, lane);
 		};
@@ -430,12 +444,14 @@ __global__ __launch_bounds__((64 * SplitShape<T, DH>::NW), 1) void masked_attent
 				wait_loads();
 			}
 			const char* from = ring + stage * S::kStage;
-			take_keys<T, DH, KT, decltype(safe)::value>(r, a, n, Reader<T, S::RB>(fresh_lane()), from, from + S::kTile, docs[wave], x * KT, lane);
+			DocRange d{0, 0, 0};
+			if (a.k_docs) d = a.k_ranges[(int64_t)n * ((a.Tk + 63) / 64) + x * KT / 64];
+			take_keys<T, DH, KT, decltype(safe)::value>(r, a, Reader<T, S::RB>(fresh_lane()), from, from + S::kTile, (const int*)(docs + stage * 256), d, x * KT, lane);
 			// the stage is loaded over next: its reads are done
 			asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 			stage = (stage + 1) % ST;
 		}
-		return __syncthreads_or(r.bad());
+		return any_wave<NW>((int*)(lds + S::kLds + NW * ST * 256), wave, lane, r.bad());
 	};
 	if (run(std::false_type{})) run(std::true_type{});
 

@@ -16,6 +16,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "masked_attention.hpp"
 
 namespace nnh {
@@ -29,9 +31,7 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) void lds_void;
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-typedef const __attribute__((address_space(1))) void global_void;
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kInf = __builtin_huge_valf();
@@ -114,36 +114,65 @@ __device__ __forceinline__ int fresh_lane() {
 	return x;
 }
 
+// Each lane's 16 (or 4) bytes at `src`, or at base + its offset, into LDS, 64 of them in a row from `to` (the wave's) on. Written
+// out, since the compiler's own form makes it wait for every such load that is on its way before the next transposed read of
+// any tile; the waits are the kernels' (wait_loads, and a barrier where waves share tiles). No vector
+// register receives anything, and nothing else in these kernels uses m0.
+// `AT` bytes behind a place that the wave's loads have in common: one scalar register for all of them.
+__device__ __forceinline__ unsigned lds_place(const char* to) {
+	return __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(const __attribute__((address_space(3))) char*)to);
+}
+template <int AT>
+__device__ __forceinline__ void load_words(const void* src, unsigned to) {
+	asm volatile("s_add_u32 m0, %0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(src), "i"(AT) : "scc");
+}
+template <int AT>
+__device__ __forceinline__ void load_words(const void* base, unsigned offset, unsigned to) {
+	asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base), "i"(AT) : "scc");
+}
+__device__ __forceinline__ void load_numbers(const void* src, char* to) {
+	asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(lds_place(to)), "v"(src));
+}
+
+// f(0) .. f(N - 1), the number a constant.
+template <int N, int I = 0, typename F>
+__device__ __forceinline__ void each(F f) {
+	if constexpr (I < N) {
+		f(std::integral_constant<int, I>{});
+		each<N, I + 1>(f);
+	}
+}
+
 // Loads a tile of R rows of `dh` elements from base + row * stride, NW waves sharing the work. Rows past the `live` (at least one)
 // first ones, which nothing sees, are the last live one again, or zeros. VEC: every row is 16-byte aligned, dh a whole number
 // of words and a tile's extent below 2^31 bytes (wide_row); then nothing passes through registers, and the caller waits
 // for the loads (wait_loads). A load instruction fills 64 words, whole rows of them from a row that is a multiple of their number
-// on: the permutation of a word is then the lane's own part XOR the instruction's.
+// on: the permutation of a word is then the lane's own part XOR the wave's XOR the instruction's.
 template <typename T, int DH, int R, int NW, bool VEC>
 __device__ __forceinline__ void load_tile(char* tile, const T* base, int64_t stride, int live, int dh, int wave, int lane) {
 	constexpr int RB = row_bytes<T, DH>(), W = RB / 16, E = 16 / (int)sizeof(T), kSteps = R * RB / 1024 / NW;
 	static_assert(kSteps * NW * 1024 == R * RB, "a tile splits evenly over the waves");
 	if constexpr (VEC) {
 		lane = fresh_lane();
-		const int r = lane / W, w = (lane % W) ^ swizzle<RB>(r);
-		const unsigned pitch = (unsigned)(stride * (int64_t)sizeof(T));
-		const unsigned at = r * pitch;
+		constexpr int kRows = 64 / W;  // of a load; load j of a wave has rows (j * NW + wave) * kRows ..
+		const int r = lane / W, w = (lane % W) ^ swizzle<RB>(r) ^ swizzle<RB>(wave * kRows);
+		const unsigned pitch = (unsigned)(stride * (int64_t)sizeof(T)), at = r * pitch;
+		const unsigned to = lds_place(tile + wave * 1024);
+		const char* const from = (const char*)(base + (int64_t)(wave * kRows) * stride);
 		if (live >= R && dh == DH) {
-#pragma unroll
-			for (int j = 0; j < kSteps; ++j) {
-				const int first = (j * NW + wave) * 64, row0 = first / W, c = w ^ swizzle<RB>(row0);
-				if (DH * (int)sizeof(T) == RB || c * E < DH)
-					__builtin_amdgcn_global_load_lds((global_void*)((const char*)(base + row0 * stride) + (at + c * 16)), (lds_void*)(tile + first * 16), 16, 0, 0);
-			}
+			each<kSteps>([&](auto step) {
+				constexpr int j = decltype(step)::value;
+				const int c = w ^ swizzle<RB>(j * NW * kRows);
+				if (DH * (int)sizeof(T) == RB || c * E < DH) load_words<j * NW * 1024>(from + j * NW * kRows * (int64_t)pitch, at + c * 16, to);
+			});
 		} else {
-#pragma unroll
-			for (int j = 0; j < kSteps; ++j) {
-				const int first = (j * NW + wave) * 64, row0 = first / W, c = w ^ swizzle<RB>(row0);
-				const void* src = (const char*)base + (min(row0 + r, live - 1) * pitch + c * 16);
+			each<kSteps>([&](auto step) {
+				constexpr int j = decltype(step)::value;
+				const int c = w ^ swizzle<RB>(j * NW * kRows);
+				const void* src = (const char*)base + (min((j * NW + wave) * kRows + r, live - 1) * pitch + c * 16);
 				if (c * E >= dh) src = &kZeroWord;  // depths past dh multiply zeros: finite ones
-				if (DH * (int)sizeof(T) == RB || c * E < DH)
-					__builtin_amdgcn_global_load_lds((global_void*)src, (lds_void*)(tile + first * 16), 16, 0, 0);
-			}
+				if (DH * (int)sizeof(T) == RB || c * E < DH) load_words<j * NW * 1024>(src, to);
+			});
 		}
 	} else {
 #pragma unroll
@@ -162,6 +191,34 @@ __device__ __forceinline__ void load_tile(char* tile, const T* base, int64_t str
 
 // Every load into LDS that the wave has issued has arrived.
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
+
+// Values loaded before a loop are here before it begins. Where the first use of one is in the loop, the compiler's wait for it is
+// there too, in every round, and waits for the tile that is on its way as well.
+template <int N>
+__device__ __forceinline__ void arrived(Frag<__bf16> (&f)[N]) {
+#pragma unroll
+	for (int t = 0; t < N; ++t) asm volatile("" : "+v"(f[t].w));
+}
+template <int N>
+__device__ __forceinline__ void arrived(Frag<float> (&f)[N]) {
+#pragma unroll
+	for (int t = 0; t < N; ++t) asm volatile("" : "+v"(f[t].w2[0]), "+v"(f[t].w2[1]));
+}
+__device__ __forceinline__ void arrived() { __builtin_amdgcn_s_waitcnt(0x0070); }  // vmcnt(0) lgkmcnt(0), known to the compiler
+
+// Whether any of the NW waves of a workgroup says so; flags: room for NW ints in the kernel's LDS.
+template <int NW>
+__device__ __forceinline__ bool any_wave(int* flags, int wave, int lane, bool x) {
+	const int mine = __any(x);
+	if (lane == 0) flags[wave] = mine;
+	__syncthreads();
+	int any = 0;
+#pragma unroll
+	for (int w = 0; w < NW; ++w) any |= flags[w];
+	any = __builtin_amdgcn_readfirstlane(any);
+	if (any) __syncthreads();  // the flags are written again
+	return any != 0;
+}
 
 // Where a lane reads its operands in a tile of RB-byte rows. The permutation XORs a row's low bits onto its words' numbers, so
 // with a lane's own part worked out once, every further step (depth, column block) is an XOR by a constant and every block of
@@ -307,6 +364,11 @@ __device__ __forceinline__ float tanh_of(float x) {
 		p = __builtin_fmaf(p, y, -1.0f / 3.0f);
 		return y < 0.3025f ? __builtin_fmaf(x * y, p, x) : 1.0f - 2.0f / (1.0f + e);
 	}
+}
+
+// Lane x's.
+__device__ __forceinline__ DocRange of_lane(const DocRange& r, int x) {
+	return {__builtin_amdgcn_readlane(r.lo, x), __builtin_amdgcn_readlane(r.hi, x), __builtin_amdgcn_readlane(r.none, x)};
 }
 
 // What one query sees of the keys: lo <= j < hi or j < pre, and its own document's. A query that is none (past the last
