@@ -187,7 +187,6 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 			for (int x = 0; x < 16; ++x) d[b][x] = 0.0f;
 		int base = -64;
 		uint64_t on = 0;
-		DocRange held{0, 0, 0}, ahead{0, 0, 0};  // the documents of tile base + lane, of the tile that next() named
 		auto next = [&]() -> int {
 			while (on == 0) {
 				base += 64;
@@ -195,14 +194,13 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 				const int x = base + lane, k0 = x * KT;
 				bool s = x < nt && ((k0 < hi && k0 + KT > lo) || k0 < pre);
 				if (s && a.k_docs) {
-					held = a.k_ranges[(int64_t)n * kb + k0 / 64];
-					s = held.lo <= mine.hi && held.hi >= mine.lo;
+					const DocRange r = a.k_ranges[(int64_t)n * kb + k0 / 64];
+					s = r.lo <= mine.hi && r.hi >= mine.lo;
 				}
 				on = __ballot(s);
 			}
 			const int x = __builtin_ctzll(on);
 			on &= on - 1;
-			if (a.k_docs) ahead = of_lane(held, x);
 			return base + x;
 		};
 		auto load = [&](int x, char* to, char* docs_to) {
@@ -225,14 +223,11 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 				f32x16 s, dp, slope;
 #pragma unroll
 				for (int j = 0; j < 16; ++j) s[j] = dp[j] = 0.0f;
-#pragma unroll
-				for (int t = 0; t < DH / 16; ++t) {
-					Frag<T> f;
-					at.rows(f, kt + 32 * x * RB, t);
-					mma(s, f, q[t]);
-					at.rows(f, vt + 32 * x * RB, t);
-					mma(dp, f, g[t]);
-				}
+				in_groups<Frag<T>, DH / 8, sizeof(T) == 2 ? 4 : 1>([&](int i, Frag<T>& f) { at.rows(f, (i % 2 ? vt : kt) + 32 * x * RB, i / 2); },
+				                                                  [&](int i, const Frag<T>& f) {
+					                                                  if (i % 2) mma(dp, f, g[i / 2]);
+					                                                  else mma(s, f, q[i / 2]);
+				                                                  });
 				const int j0 = fresh(k0 + 32 * x + 4 * half);
 				weights<T>(s, slope, a, slope2, [&](int j) { const int y = pos - (j0 + 8 * (j / 4) + j % 4); return (float)(y < 0 ? -y : y); },
 				           [&](int) { return lse2; });
@@ -263,18 +258,15 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 					for (int j = 0; j < 16; ++j) s[j] *= slope[j];
 				}
 				const bool clean = decltype(safe)::value && partial;
-#pragma unroll
-				for (int t = 0; t < 2; ++t) {
-					Frag<T> ds;
-					operand_of(ds, s, t);
-#pragma unroll
-					for (int b = 0; b < DH / 32; ++b) {
-						Frag<T> f;
-						at.columns(f, kt + (32 * x + 16 * t) * RB, b);
-						if (clean) only_finite(f);
-						mma(d[b], f, ds);
-					}
-				}
+				Frag<T> ds[2];
+				operand_of(ds[0], s, 0);
+				operand_of(ds[1], s, 1);
+				constexpr int B = DH / 32;
+				in_groups<Frag<T>, 2 * B, sizeof(T) == 2 ? 2 : 1>([&](int i, Frag<T>& f) { at.columns(f, kt + (32 * x + 16 * (i / B)) * RB, i % B); },
+				                                                 [&](int i, Frag<T>& f) {
+					                                                 if (clean) only_finite(f);
+					                                                 mma(d[i % B], f, ds[i / B]);
+				                                                 });
 				if (clean) {  // a key that is not finite makes the queries that see it NaN
 #pragma clang loop unroll(disable)
 					for (int j = 0; j < 32; ++j) {
@@ -298,7 +290,8 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 			wait_loads();
 			__builtin_amdgcn_s_barrier();
 			asm volatile("" ::: "memory");
-			const DocRange r = ahead;
+			DocRange r{0, 0, 0};
+			if (a.k_docs) r = range_at(a.k_ranges, (int64_t)n * kb + cur * KT / 64);
 			const int then = next();
 			if (then >= 0) load(then, lds + (1 - B) * 2 * kTile, docs_at + (1 - B) * 256);
 			take(from, from + kTile, (const int*)(docs_at + B * 256), r, cur * KT);
@@ -420,7 +413,6 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 		// workgroups of one key head read the same rows at about the same time.
 		int head = -1, base = -64;
 		uint64_t on = 0;
-		DocRange held{0, 0, 0}, ahead{0, 0, 0};  // the documents of tile base + lane, of the tile that next() named
 		auto next = [&]() -> int {
 			while (on == 0) {
 				base -= 64;
@@ -431,14 +423,13 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 				const int x = base + lane, q0 = x * QT;
 				bool s = x < nt && q0 + QT > lo && x % a.parts == part;
 				if (s && a.q_docs) {
-					held = a.q_ranges[(int64_t)n * qb + q0 / 64];
-					s = held.lo <= mine.hi && held.hi >= mine.lo;
+					const DocRange r = a.q_ranges[(int64_t)n * qb + q0 / 64];
+					s = r.lo <= mine.hi && r.hi >= mine.lo;
 				}
 				on = __ballot(s);
 			}
 			const int x = 63 - __builtin_clzll(on);
 			on &= ~((uint64_t)1 << x);
-			if (a.q_docs) ahead = of_lane(held, x);
 			return base + x;
 		};
 		auto load = [&](int x, int buf) {
@@ -463,12 +454,8 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 			f32x16 s, dp, slope;
 #pragma unroll
 			for (int y = 0; y < 16; ++y) s[y] = dp[y] = 0.0f;
-#pragma unroll
-			for (int t = 0; t < DH / 16; ++t) {
-				Frag<T> f;
-				at.rows(f, qt, t);
-				mma(s, f, kf[t]);
-			}
+			in_groups<Frag<T>, DH / 16, sizeof(T) == 2 ? 2 : 1>([&](int t, Frag<T>& f) { at.rows(f, qt, t); },
+			                                                   [&](int t, const Frag<T>& f) { mma(s, f, kf[t]); });
 			__builtin_amdgcn_sched_barrier(0);
 			const int i0 = fresh(4 * half);  // the tile's row of register y: i0 + 8 (y / 4) + y % 4
 			weights<T>(s, slope, a, a.slopes ? a.slopes[h] * kLog2e : 0.0f,
@@ -498,13 +485,10 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 				for (int y = 0; y < 16; ++y) s[y] *= slope[y];
 			}
 			__builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-			for (int t = 0; t < DH / 16; ++t) {
-				Frag<T> f, v;
-				at.rows(f, gt, t);
-				at.rows(v, vt + wave * 32 * RB, t);
-				mma(dp, f, v);
-			}
+			in_groups<FragPair<T>, DH / 16, 1>([&](int t, FragPair<T>& f) {
+				at.rows(f.a, gt, t);
+				at.rows(f.b, vt + wave * 32 * RB, t);
+			}, [&](int, const FragPair<T>& f) { mma(dp, f.a, f.b); });
 			__builtin_amdgcn_sched_barrier(0);
 #pragma unroll
 			for (int y = 0; y < 16; ++y) dp[y] = s[y] * (dp[y] - delta[i0 + 8 * (y / 4) + y % 4]);
@@ -513,21 +497,16 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 				for (int y = 0; y < 16; ++y) dp[y] = seen >> y & 1 ? dp[y] : 0.0f;
 			}
 			const bool clean = decltype(safe)::value && partial;
-#pragma unroll
-			for (int t = 0; t < 2; ++t) {
-				Frag<T> ds;
-				operand_of(ds, dp, t);
-#pragma unroll
-				for (int b = 0; b < DH / 32; ++b) {
-					Frag<T> f;
-					at.columns(f, gt + 16 * t * RB, b);
-					if (clean) only_finite(f);
-					mma(dv[b], f, p[t]);
-					at.columns(f, qt + 16 * t * RB, b);
-					if (clean) only_finite(f);
-					mma(dk[b], f, ds);
-				}
-			}
+			Frag<T> ds[2];
+			operand_of(ds[0], dp, 0);
+			operand_of(ds[1], dp, 1);
+			constexpr int kEach = DH / 16;  // products of 16 of the rows: dv and dk in turn
+			in_groups<Frag<T>, 2 * kEach, sizeof(T) == 2 ? 2 : 1>([&](int i, Frag<T>& f) { at.columns(f, (i % 2 ? qt : gt) + 16 * (i / kEach) * RB, i % kEach / 2); },
+			                                                     [&](int i, Frag<T>& f) {
+				                                                     if (clean) only_finite(f);
+				                                                     if (i % 2) mma(dk[i % kEach / 2], f, ds[i / kEach]);
+				                                                     else mma(dv[i % kEach / 2], f, p[i / kEach]);
+			                                                     });
 			if (clean) {  // rows that are not finite, to the keys that they see
 #pragma clang loop unroll(disable)
 				for (int i = 0; i < 32; ++i) {
@@ -551,7 +530,8 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 			wait_loads();
 			__builtin_amdgcn_s_barrier();
 			asm volatile("" ::: "memory");
-			const DocRange r = ahead;
+			DocRange r{0, 0, 0};
+			if (a.q_docs) r = range_at(a.q_ranges, (int64_t)n * qb + cur * QT / 64);
 			const int h = hk * a.G + head, then = next();
 			if (then >= 0) load(then, 1 - B);
 			take(ring + B * 2 * kTile, ring + (B * 2 + 1) * kTile, (const float*)(rows + B * 768), (const float*)(rows + B * 768 + 256), (const int*)(rows + B * 768 + 512), r, cur * QT, h);

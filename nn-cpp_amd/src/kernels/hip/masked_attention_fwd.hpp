@@ -62,14 +62,9 @@ __device__ __forceinline__ void take_keys(Rows<T, DH>& r, const MaskedAttentionA
 	for (int x = 0; x < KT / 32; ++x)
 #pragma unroll
 		for (int i = 0; i < 16; ++i) s[x][i] = 0.0f;
-#pragma unroll
-	for (int t = 0; t < DH / 16; ++t)
-#pragma unroll
-		for (int x = 0; x < KT / 32; ++x) {
-			Frag<T> k;
-			at.rows(k, kt + 32 * x * RB, t);
-			mma(s[x], k, r.q[t]);
-		}
+	constexpr int X = KT / 32, kGroup = sizeof(T) == 2 ? 2 * X : 1;
+	in_groups<Frag<T>, DH / 16 * X, kGroup>([&](int i, Frag<T>& k) { at.rows(k, kt + 32 * (i % X) * RB, i / X); },
+	                                        [&](int i, const Frag<T>& k) { mma(s[i % X], k, r.q[i / X]); });
 
 	float c = a.scale * kLog2e;  // of the scores as they are, in units of log 2: multiplied in the exponential's own step
 	if (a.cap > 0.0f) {
@@ -281,6 +276,7 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 			hi = min(hi, clamped(last + a.window, 0, live));
 		}
 	}
+	const int kb = (a.Tk + 63) / 64;
 	DocRange mine{0, 0, 0};
 	if (a.q_docs) {
 		const int nb = (a.Tq + 63) / 64, b0 = q0 / 64;
@@ -306,7 +302,6 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 		// the tiles that some query may see, 64 at a time
 		int base = -64;
 		uint64_t on = 0;
-		DocRange held{0, 0, 0}, ahead{0, 0, 0};  // the documents of tile base + lane, of the tile that next() named
 		auto next = [&]() -> int {
 			while (on == 0) {
 				base += 64;
@@ -314,14 +309,13 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 				const int x = base + lane, k0 = x * KT;
 				bool see = x < nt && ((k0 < hi && k0 + KT > lo) || k0 < pre);
 				if (see && a.k_docs) {
-					held = a.k_ranges[(int64_t)n * ((a.Tk + 63) / 64) + k0 / 64];
-					see = held.lo <= mine.hi && held.hi >= mine.lo;
+					const DocRange d = a.k_ranges[(int64_t)n * kb + k0 / 64];
+					see = d.lo <= mine.hi && d.hi >= mine.lo;
 				}
 				on = __ballot(see);
 			}
 			const int x = __builtin_ctzll(on);
 			on &= on - 1;
-			if (a.k_docs) ahead = of_lane(held, x);
 			return base + x;
 		};
 		auto load = [&](int x, char* to, char* docs_to) {
@@ -337,7 +331,8 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 			wait_loads();
 			__builtin_amdgcn_s_barrier();  // this tile has arrived for all waves, and all are done with the last one
 			asm volatile("" ::: "memory");
-			const DocRange d = ahead;
+			DocRange d{0, 0, 0};
+			if (a.k_docs) d = range_at(a.k_ranges, (int64_t)n * kb + cur * KT / 64);
 			const int then = next();
 			if (then >= 0) load(then, lds + (1 - B) * 2 * kTile, docs + (1 - B) * 256);
 			take_keys<T, DH, KT, decltype(safe)::value>(r, a, at(), from, from + kTile, (const int*)(docs + B * 256), d, cur * KT, lane);
@@ -445,7 +440,7 @@ __global__ __launch_bounds__((64 * SplitShape<T, DH>::NW), 1) void masked_attent
 			}
 			const char* from = ring + stage * S::kStage;
 			DocRange d{0, 0, 0};
-			if (a.k_docs) d = a.k_ranges[(int64_t)n * ((a.Tk + 63) / 64) + x * KT / 64];
+			if (a.k_docs) d = range_at(a.k_ranges, (int64_t)n * ((a.Tk + 63) / 64) + x * KT / 64);
 			take_keys<T, DH, KT, decltype(safe)::value>(r, a, Reader<T, S::RB>(fresh_lane()), from, from + S::kTile, (const int*)(docs + stage * 256), d, x * KT, lane);
 			// the stage is loaded over next: its reads are done
 			asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");

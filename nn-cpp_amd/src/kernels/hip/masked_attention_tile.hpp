@@ -143,6 +143,27 @@ __device__ __forceinline__ void each(F f) {
 	}
 }
 
+// N products in groups of G, the operands of the next group on their way from LDS while one multiplies: read(i, f), product(i, f).
+// Left to itself the compiler, short of registers elsewhere, reads each operand just before its product, which then waits for LDS
+// every time.
+template <typename F, int N, int G, typename Read, typename Product>
+__device__ __forceinline__ void in_groups(Read read, Product product) {
+	static_assert(N % G == 0, "whole groups");
+	F f[2][G];
+	each<G>([&](auto j) { read(decltype(j)::value, f[0][decltype(j)::value]); });
+	each<N / G>([&](auto group) {
+		constexpr int g = decltype(group)::value;
+		if constexpr (g + 1 < N / G) each<G>([&](auto j) { read((g + 1) * G + decltype(j)::value, f[(g + 1) % 2][decltype(j)::value]); });
+		each<G>([&](auto j) { product(g * G + decltype(j)::value, f[g % 2][decltype(j)::value]); });
+		__builtin_amdgcn_sched_barrier(0);
+	});
+}
+// Two operands of one product.
+template <typename T>
+struct FragPair {
+	Frag<T> a, b;
+};
+
 // Loads a tile of R rows of `dh` elements from base + row * stride, NW waves sharing the work. Rows past the `live` (at least one)
 // first ones, which nothing sees, are the last live one again, or zeros. VEC: every row is 16-byte aligned, dh a whole number
 // of words and a tile's extent below 2^31 bytes (wide_row); then nothing passes through registers, and the caller waits
@@ -366,9 +387,12 @@ __device__ __forceinline__ float tanh_of(float x) {
 	}
 }
 
-// Lane x's.
-__device__ __forceinline__ DocRange of_lane(const DocRange& r, int x) {
-	return {__builtin_amdgcn_readlane(r.lo, x), __builtin_amdgcn_readlane(r.hi, x), __builtin_amdgcn_readlane(r.none, x)};
+// A block's range as scalars: read through the constant cache, so that no wait for a vector load waits for tiles on their way too
+// (nothing writes the ranges while a kernel that reads them runs).
+__device__ __forceinline__ DocRange range_at(const DocRange* ranges, int64_t i) {
+	typedef const __attribute__((address_space(4))) int scalar_int;
+	const scalar_int* p = (const scalar_int*)(uintptr_t)(ranges + i);
+	return {p[0], p[1], p[2]};
 }
 
 // What one query sees of the keys: lo <= j < hi or j < pre, and its own document's. A query that is none (past the last
