@@ -111,9 +111,10 @@ __device__ __forceinline__ void take_keys(Rows<T, DH>& r, const MaskedAttentionA
 #pragma unroll
 		for (int i = 0; i < 16; ++i) top = fmaxf(top, s[x][i]);
 	top = max_halves(top) * c;
-	// The base that exponents are taken from follows the maximum only where that has passed it by 2^8: sums and products keep their
-	// relative precision at any base, and most tiles then rescale nothing (some of 32 rows have a new maximum in four tiles of ten).
-	if (__any(top > r.m + 8.0f)) {
+	// The base follows every new maximum (some of 32 rows have one in four tiles of ten): with one left behind by up to 2^8 no sum
+	// would lose precision, but a row's largest weight would no longer be 1, which 16 bits hold exactly, and where a key or two
+	// have a row's weight its rounding would be the result's (0.0021 for 0.0017 of the norm over a cache of 8192).
+	if (__any(top > r.m)) {
 		const float m = fmaxf(r.m, top), f = m == -kInf ? 1.0f : exp2_of(r.m - m);
 		r.m = m;
 		r.l *= f;
