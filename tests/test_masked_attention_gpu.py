@@ -264,3 +264,89 @@ def test_rest_of_out(gpu, n_q, strided):
     assert torch.equal(copy[0], out) and torch.equal(copy[1], lse) and copy[1].rest is None
     for name, x in zip(("dq", "dk", "dv"), nnh.masked_attention_backward(g, q, k, v, *copy, rule)):
         assert_within(x, want[name], name)
+
+
+@pytest.mark.parametrize("dtype,Tq", [("bf16", 200), ("f32", 130), ("bf16", 1)])
+def test_capture(gpu, dtype, Tq):
+    """Both passes captured once with a workspace of their own (documents' ranges, key tiles shared by workgroups, the split form) and
+    replayed on new inputs, with eager calls between; refused without one."""
+    import nnh
+    t, N, H, Hkv, D, Tk = T[dtype], 2, 4, 2, 64, max(Tq, 150)
+    code = nnh.BF16 if dtype == "bf16" else nnh.F32
+    assert code in (0, 1)
+    q, g = (draw(s, N, Tq, H, D, dtype=t).cuda() for s in (0, 1))
+    k, v = (draw(s, N, Tk, Hkv, D, dtype=t).cuda() for s in (2, 3))
+    docs = documents(N, Tk, 4).cuda()
+    starts = torch.full((N,), Tk - Tq).int().cuda()
+    rule = nnh.AttentionRule(causal=True, cap=20.0, q_start=starts, q_docs=docs[:, Tk - Tq:].contiguous(), k_docs=docs)
+    size = max(nnh.workspace_size("masked_attention", N, Tq, Tk, H, Hkv, D, 1, b) for b in (0, 1))
+    room = torch.empty(size, dtype=torch.uint8, device="cuda")
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+
+    def both():
+        out, lse = nnh.masked_attention_forward(q, k, v, rule)
+        return (out, lse) + nnh.masked_attention_backward(g, q, k, v, out, lse, rule)
+
+    nnh.set_workspace(room, side)
+    try:
+        with torch.cuda.graph(graph, stream=side):
+            got = both()
+        for seed in range(3):
+            for i, x in enumerate((q, k, v, g)):
+                x.copy_(draw(10 * seed + i, *x.shape, dtype=t))
+            want = both()
+            graph.replay()
+            torch.cuda.synchronize()
+            for x, y in zip(got, want):
+                assert torch.equal(x, y)
+    finally:
+        nnh.set_workspace(None, side)
+    other = torch.cuda.CUDAGraph()
+    with pytest.raises(nnh.NnhError, match="registered workspace"):
+        with torch.cuda.graph(other, stream=side):
+            both()
+
+
+def test_two_streams_at_once(gpu):
+    """Calls that need scratch on two streams with no order between them."""
+    import nnh
+    N, Tq, H, D = 1, 400, 2, 64
+    q, k, v, g = ([draw(4 * s + i, N, Tq, H, D, dtype=torch.bfloat16).cuda() for s in range(2)] for i in range(4))
+    docs = [documents(N, Tq, s).cuda() for s in range(2)]
+    rules = [nnh.AttentionRule(causal=True, q_docs=d, k_docs=d) for d in docs]
+
+    def both(s):
+        out, lse = nnh.masked_attention_forward(q[s], k[s], v[s], rules[s])
+        return (out, lse) + nnh.masked_attention_backward(g[s], q[s], k[s], v[s], out, lse, rules[s])
+
+    want = [both(s) for s in range(2)]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], [[], []]
+    for _ in range(4):
+        for s in range(2):
+            with torch.cuda.stream(streams[s]):
+                got[s].append(both(s))
+    torch.cuda.synchronize()
+    for s in range(2):
+        for one in got[s]:
+            for x, y in zip(one, want[s]):
+                assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("n_q", [1, 40])
+@pytest.mark.parametrize("far", ["rows", "samples"])
+def test_offsets_past_32_bits(gpu, n_q, far):
+    """Keys and values whose rows lie 2^22 elements apart (the last ones past 2^31 elements), or whose samples do 2^31."""
+    N, Tk, D = (1, 600, 64) if far == "rows" else (2, 70, 64)
+    strides = (0, 1 << 22, D, 1) if far == "rows" else ((1 << 31) + 64, D, D, 1)
+    q, k, v = draw(0, N, n_q, 1, D, dtype=torch.bfloat16), draw(1, N, Tk, 1, D, dtype=torch.bfloat16), draw(2, N, Tk, 1, D, dtype=torch.bfloat16)
+    room = [torch.empty((N - 1) * strides[0] + (Tk - 1) * strides[1] + D, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    kk, vv = (r.as_strided((N, Tk, 1, D), strides) for r in room)
+    kk.copy_(k)
+    vv.copy_(v)
+    g = draw(3, N, n_q, 1, D, dtype=torch.bfloat16)
+    want = masked_attention(q, k, v, g)
+    got = run(q, kk, vv, g)
+    for name, x in got.items():
+        assert_within(x, want[name], name)
