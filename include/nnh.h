@@ -500,7 +500,8 @@ int nnh_masked_attention_forward(int type, size_t N, size_t Tq, size_t Tk, size_
                                  const nnh_attention_rule* rule, const nnh_head_tensor* out, const nnh_head_tensor* rest,
                                  float* lse, void* stream);
 
-/* Its backward rule, from the forward's out, rest and lse (rest null: the gradients of q are off by out's rounding as well): gradients of q, k and v (null: not wanted) given g, out's. *_first
+/* Its backward rule, from the forward's out, rest and lse (rest null: the gradients of q are off by out's rounding as
+ * well): gradients of q, k and v (null: not wanted) given g, out's. *_first
  * stores, otherwise the gradient is added to what is there. The gradients may lie beside each other in one buffer of
  * the same rows; they may not overlap. */
 int nnh_masked_attention_backward(int type, size_t N, size_t Tq, size_t Tk, size_t H, size_t Hkv, size_t Dh,

@@ -11,6 +11,10 @@
 // whole stages of LDS a stage would arrive just when it is needed; the ring has five halves instead, A's half is under way
 // a stage longer, and only B's has to arrive between two barriers. An operand whose depth is not the contiguous axis is
 // read by transposed LDS reads and needs no transposed copy.
+//
+// 8192 rows, 4096 wide, 128000 words: the scores 6.8 ms (1260 TFLOP/s), the gradient of the rows 6.4 (1340), of the weight 8.1 (1060: its
+// operands are both read transposed, twice the LDS instructions), where a library product of 8192^3 reaches 1474. Power holds
+// the clock near 1.9 GHz meanwhile.
 #pragma once
 
 #include <type_traits>

@@ -7,6 +7,10 @@
 // Two kernels, each recomputing the scores of its own products: dq by query rows (which also leaves delta and lse in units of log 2), then dk and dv
 // by key rows, where the queries of all heads that share the key head are added in their order. No gradient is added by
 // atomics, so the results repeat bit for bit; the price is seven products of a pair of rows where five would do.
+//
+// Causal, 8192 tokens, 16 heads of 128 on 8 key heads, bf16: dq 490-500 us, dk and dv 755 + 28 us to add their parts (690 TFLOP/s
+// of the products made). As in the forward kernel the vector operations beside the products set the pace; dk and dv also read
+// 40 KB of LDS for 32 products, a quarter more than the products' time, since a wave has no registers left for V.
 #pragma once
 
 #include <type_traits>

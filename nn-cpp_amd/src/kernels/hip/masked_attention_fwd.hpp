@@ -4,6 +4,12 @@
 // One pass over the keys with the running maximum and sum of the softmax. Scores are computed transposed, S^T = K Q^T, so a
 // lane holds one query's column: its maximum, sum and rescaling are one number a lane, and P^T goes into O^T += V^T P^T from
 // the registers it was computed in (masked_attention_tile.hpp).
+//
+// Causal, 8192 tokens, 16 heads of 128 on 8 key heads, bf16: 330-360 us, 770-830 TFLOP/s of the pairs seen. The matrix units are
+// busy for 37% of that and the vector units (scale, exponential, maximum, sum, rounding: ten operations a score) for 57%; the
+// two overlap little, with two waves a SIMD. A wave of 64 queries would halve the reads of LDS, which take about as long as the
+// products, but leaves one wave a SIMD. Raising the priority of either phase's waves cost 10%.
+// Split form, 32 samples of up to 8192 keys, 8 key heads: 152-159 us for 624 MB, 4.0 TB/s, against 4.7 for a large copy.
 #pragma once
 
 #include <type_traits>
