@@ -128,7 +128,8 @@ __device__ __forceinline__ void load_words(const void* src, unsigned to) {
 }
 template <int AT>
 __device__ __forceinline__ void load_words(const void* base, unsigned offset, unsigned to) {
-	asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base), "i"(AT) : "scc");
+	// (a base that a vector instruction has just written, as one that reloads it does, may be read five wait states later)
+	asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base), "i"(AT) : "scc");
 }
 __device__ __forceinline__ void load_numbers(const void* src, char* to) {
 	asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(lds_place(to)), "v"(src));
