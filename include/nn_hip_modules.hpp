@@ -277,13 +277,14 @@ private:
 // or in 8. The reference's optimizer updates host tensors one by one (src/optim/adamw.cpp:15).
 struct AdamWOptions {
 	double lr = 1e-3, beta1 = 0.9, beta2 = 0.999, eps = 1e-8, weight_decay = 0.01;
-	int bits = 32;
+	int bits = 32;  // fixed with the moments: a step after a change of it is refused
 };
 
 class AdamW {
 public:
 	explicit AdamW(std::vector<Value> parameters, const AdamWOptions& options = AdamWOptions());
-	// One step; grad_scale (a one-element device tensor, or empty) multiplies every gradient.
+	// One step; grad_scale (a one-element device tensor, or empty) multiplies every gradient. A parameter keeps the number of
+	// elements that it had when the optimizer was made (TensorShapeError).
 	void step(const Tensor& grad_scale = Tensor());
 	void zero_grad() const { nn::hip::zero_grad(parameters_); }
 	AdamWOptions& options() { return options_; }
@@ -292,6 +293,8 @@ public:
 private:
 	std::vector<Value> parameters_;
 	AdamWOptions options_;
+	int bits_;                   // what the moments are kept in
+	std::vector<size_t> sizes_;  // elements that each parameter's moments are for
 	std::vector<Tensor> m_, v_, m_scale_, v_scale_;  // (8 bits: the codes' and scales' bytes in fp32 storage)
 	size_t steps_ = 0;
 };

@@ -437,10 +437,12 @@ void Transformer::train(bool mode) {
 	training_ = mode;
 }
 
-AdamW::AdamW(std::vector<Value> parameters, const AdamWOptions& options) : parameters_(std::move(parameters)), options_(options) {
+AdamW::AdamW(std::vector<Value> parameters, const AdamWOptions& options)
+    : parameters_(std::move(parameters)), options_(options), bits_(options.bits) {
 	if (options.bits != 32 && options.bits != 8) throw std::invalid_argument("AdamW: moments are kept in 32 or 8 bits");
 	for (const Value& p : parameters_) {
 		const size_t n = p.data().size(), kept = options.bits == 32 ? n : (n + 3) / 4, scales = options.bits == 32 ? 0 : (n + 255) / 256;
+		sizes_.push_back(n);
 		m_.push_back(Tensor({kept}, 0.0f));
 		v_.push_back(Tensor({kept}, 0.0f));
 		m_scale_.push_back(Tensor({scales}, 0.0f));
@@ -450,9 +452,10 @@ AdamW::AdamW(std::vector<Value> parameters, const AdamWOptions& options) : param
 
 void AdamW::step(const Tensor& grad_scale) {
 	if (grad_scale.size() > 1) throw TensorShapeError("nn::hip: AdamW's grad_scale has one element");
+	if (options_.bits != bits_) throw std::invalid_argument("nn::hip: AdamW's moments were made in other bits than its options now say");
 	nnh_adamw o{};
 	o.p_type = o.g_type = NNH_F32;
-	o.bits = options_.bits;
+	o.bits = bits_;
 	o.lr = options_.lr;
 	o.beta1 = options_.beta1;
 	o.beta2 = options_.beta2;
@@ -463,11 +466,12 @@ void AdamW::step(const Tensor& grad_scale) {
 	std::vector<nnh_adamw_tensor> t;
 	for (size_t i = 0; i < parameters_.size(); ++i) {
 		const Value& p = parameters_[i];
+		if (p.data().size() != sizes_[i]) throw TensorShapeError("nn::hip: AdamW: a parameter of another size than its moments");
 		if (p.data().size() == 0) continue;
 		if (p.grad().shape() != p.data().shape()) throw TensorShapeError("nn::hip: AdamW: a parameter without a gradient");
 		const auto bytes = [](const Tensor& x) { return reinterpret_cast<unsigned char*>(x.data()); };
-		t.push_back({p.data().data(), p.grad().data(), m_[i].data(), v_[i].data(), options_.bits == 8 ? bytes(m_scale_[i]) : nullptr,
-		             options_.bits == 8 ? bytes(v_scale_[i]) : nullptr, nullptr, p.data().size()});
+		t.push_back({p.data().data(), p.grad().data(), m_[i].data(), v_[i].data(), bits_ == 8 ? bytes(m_scale_[i]) : nullptr,
+		             bits_ == 8 ? bytes(v_scale_[i]) : nullptr, nullptr, p.data().size()});
 	}
 	const int rc = nnh_adamw_step(&o, t.data(), t.size(), current_stream());
 	if (rc == NNH_ERR_HIP) throw HipError(std::string("nn::hip: ") + nnh_last_error());
