@@ -830,58 +830,93 @@ class _AdamW(C.Structure):
 class AdamW:
     """AdamW over lists of parameters and their gradient buffers (contiguous, fp32 or bf16, one type each), both kept by the
     caller. The moments m and v are made here (zeros, kept in `bits` bits) or given: fp32 tensors, or uint8 codes with uint8
-    m_scale and v_scale of ceil(count / 64) elements. copies: bf16 tensors that the new parameters are also stored to."""
+    m_scale and v_scale of ceil(count / 64) elements. copies: bf16 tensors that the new parameters are also stored to.
+
+    The lists params, grads and copies may get other tensors, and their tensors other memory (.data, a new gradient buffer),
+    between steps: a step looks where they are, and refuses sizes that the moments are not for. The moments stay the tensors
+    they were made as; a saved state is copied into them."""
 
     def __init__(self, params, grads, m=None, v=None, m_scale=None, v_scale=None, copies=None, bits=32, lr=1e-3, beta1=0.9,
                  beta2=0.999, eps=1e-8, weight_decay=0.01, steps=0):
         torch = _torch or _load_torch()
-        device = torch.cuda.current_device()
-        self.params, self.grads, self.copies, n = list(params), list(grads), copies, len(params)
+        self.params, self.grads, n = list(params), list(grads), len(params)
+        self.copies = None if copies is None else list(copies)
         self.lr, self.beta1, self.beta2, self.eps, self.weight_decay = lr, beta1, beta2, eps, weight_decay
         self.steps = int(steps)
-        self.bits = bits if m is None else 8 if len(m) and m[0].dtype == torch.uint8 else 32
-        kept = torch.uint8 if self.bits == 8 else torch.float32
-        if (m is None) != (v is None) or (m is not None and self.bits == 8 and (m_scale is None or v_scale is None)):
+        self._bits = bits if m is None else 8 if len(m) and m[0].dtype == torch.uint8 else 32
+        kept = torch.uint8 if self._bits == 8 else torch.float32
+        if (m is None) != (v is None) or (m is not None and self._bits == 8 and (m_scale is None or v_scale is None)):
             raise NnhError(ERR_INVALID, "moments are given together, in 8 bits with their scales")
 
         def zeros(per, dtype):
-            return [torch.zeros((p.numel() + per - 1) // per, dtype=dtype, device=p.device) for p in self.params]
+            return tuple(torch.zeros((p.numel() + per - 1) // per, dtype=dtype, device=p.device) for p in self.params)
 
-        self.m, self.v = (zeros(1, kept), zeros(1, kept)) if m is None else (list(m), list(v))
-        self.m_scale = self.v_scale = [None] * n
-        if self.bits == 8:
-            self.m_scale, self.v_scale = (zeros(64, torch.uint8), zeros(64, torch.uint8)) if m is None else (list(m_scale), list(v_scale))
-        outs = [None] * n if copies is None else list(copies)
-        lists = (self.params, self.grads, self.m, self.v, self.m_scale, self.v_scale, outs)
+        self._m, self._v = (zeros(1, kept), zeros(1, kept)) if m is None else (tuple(m), tuple(v))
+        self._m_scale = self._v_scale = (None,) * n
+        if self._bits == 8:
+            self._m_scale, self._v_scale = (zeros(64, torch.uint8), zeros(64, torch.uint8)) if m is None else (tuple(m_scale), tuple(v_scale))
+        self._device = torch.cuda.current_device()
+        self._counts, self._types = [p.numel() for p in self.params], None
+        self._fill()
+
+    bits, m, v = property(lambda self: self._bits), property(lambda self: self._m), property(lambda self: self._v)
+    m_scale, v_scale = property(lambda self: self._m_scale), property(lambda self: self._v_scale)
+
+    def _where(self):
+        """Where the caller's tensors are (None: an entry is no tensor), 40 ns a tensor. Their memory of the last table is held
+        until the next one, so an address that is the same is the same memory."""
+        torch = _torch or _load_torch()
+        copies = () if self.copies is None else (t for t in self.copies if t is not None)
+        try:
+            return [*map(torch.Tensor.data_ptr, (*self.params, *self.grads, *copies))]
+        except TypeError:
+            return None
+
+    def _fill(self):
+        """The call's table of tensors, checked."""
+        torch = _torch or _load_torch()
+        n = len(self._counts)
+        outs = [None] * n if self.copies is None else self.copies
+        lists = (self.params, self.grads, self._m, self._v, self._m_scale, self._v_scale, outs)
         if any(len(x) != n for x in lists):
             raise ShapeError(ERR_SHAPE, "one tensor of each kind for every parameter")
-        self._tensors = (AdamWTensor * max(1, n))()
+        if any(t is None for t in (*self.params, *self.grads)):
+            raise NnhError(ERR_INVALID, "a parameter without a gradient")
+        if self._types is None:
+            self._types = (_type(self.params[0]), _type(self.grads[0])) if n else (F32, F32)
+        kept = torch.uint8 if self._bits == 8 else torch.float32
+        p_type, g_type = ((torch.float32, torch.bfloat16)[t] for t in self._types)
+        tensors = (AdamWTensor * max(1, n))()
         for i, row in enumerate(zip(*lists)):
-            count = row[0].numel()
+            count = self._counts[i]
             for t, what, dtype, size in zip(row, ("a parameter", "a gradient", "m", "v", "m_scale", "v_scale", "a copy"),
-                                            (self.params[0].dtype, self.grads[0].dtype, kept, kept, torch.uint8, torch.uint8, torch.bfloat16),
+                                            (p_type, g_type, kept, kept, torch.uint8, torch.uint8, torch.bfloat16),
                                             (count, count, count, count, (count + 63) // 64, (count + 63) // 64, count)):
                 if t is None:
                     continue
                 if t.numel() != size:
                     raise ShapeError(ERR_SHAPE, f"{what} has {t.numel()} elements, not {size}")
-                _on(t, device, dtype, tuple(t.shape), what)
-            self._tensors[i] = AdamWTensor(*(None if t is None else t.data_ptr() for t in row), count)
-        self._types = (_type(self.params[0]), _type(self.grads[0])) if n else (F32, F32)
-        self._n = n
+                _on(t, self._device, dtype, tuple(t.shape), what)
+            tensors[i] = AdamWTensor(*(None if t is None else t.data_ptr() for t in row), count)
+        self._tensors, self._known = tensors, self._where()
+        self._held = [t.detach() for t in (*self.params, *self.grads, *outs) if t is not None]
 
     def step(self, grad_scale=None, lr_device=None, step_device=None, stream=None):
         """One step; grad_scale and lr_device: one-element fp32 tensors, step_device: an int32 one that holds this step's number
         (for a captured step; self.steps counts calls either way)."""
         torch = _torch or _load_torch()
         device = torch.cuda.current_device()
+        if device != self._device:
+            raise NnhError(ERR_INVALID, "the moments are not on the current device")
+        if self._where() != self._known:
+            self._fill()
         for t, dtype, what in ((grad_scale, torch.float32, "grad_scale"), (lr_device, torch.float32, "lr_device"), (step_device, torch.int32, "step_device")):
             if t is not None and t.numel() != 1:
                 raise ShapeError(ERR_SHAPE, f"{what} must have one element")
             _on(t, device, dtype, None, what)
-        o = _AdamW(*self._types, self.bits, self.lr, self.beta1, self.beta2, self.eps, self.weight_decay, self.steps + 1,
+        o = _AdamW(*self._types, self._bits, self.lr, self.beta1, self.beta2, self.eps, self.weight_decay, self.steps + 1,
                    *(None if t is None else t.data_ptr() for t in (step_device, lr_device, grad_scale)))
-        check(lib().nnh_adamw_step(C.byref(o), self._tensors, self._n, _stream(stream)))
+        check(lib().nnh_adamw_step(C.byref(o), self._tensors, len(self._counts), _stream(stream)))
         self.steps += 1
 
 
