@@ -839,10 +839,12 @@ class AdamW:
     def __init__(self, params, grads, m=None, v=None, m_scale=None, v_scale=None, copies=None, bits=32, lr=1e-3, beta1=0.9,
                  beta2=0.999, eps=1e-8, weight_decay=0.01, steps=0):
         torch = _torch or _load_torch()
-        self.params, self.grads, n = list(params), list(grads), len(params)
+        self.params, self.grads = list(params), list(grads)
+        n = len(self.params)
         self.copies = None if copies is None else list(copies)
         self.lr, self.beta1, self.beta2, self.eps, self.weight_decay = lr, beta1, beta2, eps, weight_decay
         self.steps = int(steps)
+        m, v, m_scale, v_scale = (None if x is None else tuple(x) for x in (m, v, m_scale, v_scale))
         self._bits = bits if m is None else 8 if len(m) and m[0].dtype == torch.uint8 else 32
         kept = torch.uint8 if self._bits == 8 else torch.float32
         if (m is None) != (v is None) or (m is not None and self._bits == 8 and (m_scale is None or v_scale is None)):
@@ -851,10 +853,10 @@ class AdamW:
         def zeros(per, dtype):
             return tuple(torch.zeros((p.numel() + per - 1) // per, dtype=dtype, device=p.device) for p in self.params)
 
-        self._m, self._v = (zeros(1, kept), zeros(1, kept)) if m is None else (tuple(m), tuple(v))
+        self._m, self._v = (zeros(1, kept), zeros(1, kept)) if m is None else (m, v)
         self._m_scale = self._v_scale = (None,) * n
         if self._bits == 8:
-            self._m_scale, self._v_scale = (zeros(64, torch.uint8), zeros(64, torch.uint8)) if m is None else (tuple(m_scale), tuple(v_scale))
+            self._m_scale, self._v_scale = (zeros(64, torch.uint8), zeros(64, torch.uint8)) if m is None else (m_scale, v_scale)
         self._device = torch.cuda.current_device()
         self._counts, self._types = [p.numel() for p in self.params], None
         self._fill()

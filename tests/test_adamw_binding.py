@@ -120,3 +120,12 @@ def test_an_address_is_not_given_out_again_between_steps(calls):
     del held
     opt.step()
     assert all(r() is None for r in seen)  # and no longer
+
+
+def test_tensors_from_iterators(calls):
+    """model.parameters() and the like may be read once."""
+    p, g = [torch.zeros(5), torch.zeros(70)], [torch.ones(5), torch.ones(70)]
+    m, v = [torch.zeros(5), torch.zeros(70)], [torch.zeros(5), torch.zeros(70)]
+    opt = nnh.AdamW(iter(p), (x for x in g), m=iter(m), v=iter(v))
+    opt.step()
+    assert [(r["p"], r["g"], r["m"], r["v"]) for r in calls[-1][1]] == [tuple(t.data_ptr() for t in row) for row in zip(p, g, m, v)]
