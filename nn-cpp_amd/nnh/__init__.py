@@ -833,8 +833,8 @@ class AdamW:
     m_scale and v_scale of ceil(count / 64) elements. copies: bf16 tensors that the new parameters are also stored to.
 
     The lists params, grads and copies may get other tensors, and their tensors other memory (.data, a new gradient buffer),
-    between steps: a step looks where they are, and refuses sizes that the moments are not for. The moments stay the tensors
-    they were made as; a saved state is copied into them."""
+    between steps: a step looks where they are, and refuses sizes that the moments are not for. The moments stay in
+    the memory that they were made in; a saved state is copied into them."""
 
     def __init__(self, params, grads, m=None, v=None, m_scale=None, v_scale=None, copies=None, bits=32, lr=1e-3, beta1=0.9,
                  beta2=0.999, eps=1e-8, weight_decay=0.01, steps=0):
@@ -901,7 +901,7 @@ class AdamW:
                 _on(t, self._device, dtype, tuple(t.shape), what)
             tensors[i] = AdamWTensor(*(None if t is None else t.data_ptr() for t in row), count)
         self._tensors, self._known = tensors, self._where()
-        self._held = [t.detach() for t in (*self.params, *self.grads, *outs) if t is not None]
+        self._held = [t.detach() for x in lists for t in x if t is not None]
 
     def step(self, grad_scale=None, lr_device=None, step_device=None, stream=None):
         """One step; grad_scale and lr_device: one-element fp32 tensors, step_device: an int32 one that holds this step's number

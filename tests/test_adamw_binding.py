@@ -129,3 +129,16 @@ def test_tensors_from_iterators(calls):
     opt = nnh.AdamW(iter(p), (x for x in g), m=iter(m), v=iter(v))
     opt.step()
     assert [(r["p"], r["g"], r["m"], r["v"]) for r in calls[-1][1]] == [tuple(t.data_ptr() for t in row) for row in zip(p, g, m, v)]
+
+
+def test_the_moments_memory_is_held(calls):
+    """A step writes where the moments were made: that memory lives as long as the optimizer, whatever becomes of the tensors."""
+    opt, *_ = made(8)
+    opt.step()
+    row = dict(calls[-1][1][1])
+    for name in ("m", "v", "m_scale", "v_scale"):
+        t = getattr(opt, name)[1]
+        t.data = torch.zeros_like(t)
+        assert row[name] != t.data_ptr() and row[name] in [x.data_ptr() for x in opt._held]
+    opt.step()
+    assert calls[-1][1][1] == row
