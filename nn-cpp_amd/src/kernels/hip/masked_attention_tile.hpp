@@ -117,23 +117,27 @@ __device__ __forceinline__ int fresh_lane() {
 // Each lane's 16 (or 4) bytes at `src`, or at base + its offset, into LDS, 64 of them in a row from `to` (the wave's) on. Written
 // out, since the compiler's own form makes it wait for every such load that is on its way before the next transposed read of
 // any tile; the waits are the kernels' (wait_loads, and a barrier where waves share tiles). No vector
-// register receives anything, and nothing else in these kernels uses m0.
+// register receives anything. m0 has the place in LDS and is named as overwritten: the compiler gives it to no value of its own
+// (it is reserved, which the warning says), but its sequences that write m0 and read it again must not take one of these in between.
 // `AT` bytes behind a place that the wave's loads have in common: one scalar register for all of them.
 __device__ __forceinline__ unsigned lds_place(const char* to) {
 	return __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(const __attribute__((address_space(3))) char*)to);
 }
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 template <int AT>
 __device__ __forceinline__ void load_words(const void* src, unsigned to) {
-	asm volatile("s_add_u32 m0, %0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(src), "i"(AT) : "scc");
+	asm volatile("s_add_u32 m0, %0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(src), "i"(AT) : "m0", "scc");
 }
 template <int AT>
 __device__ __forceinline__ void load_words(const void* base, unsigned offset, unsigned to) {
 	// (a base that a vector instruction has just written, as one that reloads it does, may be read five wait states later)
-	asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base), "i"(AT) : "scc");
+	asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base), "i"(AT) : "m0", "scc");
 }
 __device__ __forceinline__ void load_numbers(const void* src, char* to) {
-	asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(lds_place(to)), "v"(src));
+	asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(lds_place(to)), "v"(src) : "m0");
 }
+#pragma clang diagnostic pop
 
 // f(0) .. f(N - 1), the number a constant.
 template <int N, int I = 0, typename F>
