@@ -482,7 +482,7 @@ typedef struct nnh_attention_rule {
 	const int* q_start; /* {N} */
 	const int* k_lens;  /* {N} */
 	const int* prefix;  /* {N} */
-	const int* q_docs;  /* {N, Tq}, together with k_docs */
+	const int* q_docs;  /* {N, Tq}, together with k_docs (either may be null where it has no elements) */
 	const int* k_docs;  /* {N, Tk} */
 } nnh_attention_rule;
 

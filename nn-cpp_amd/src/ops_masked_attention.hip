@@ -90,7 +90,8 @@ int check_rule(const Geom& g, const nnh_attention_rule* r, MaskedAttentionArgs& 
 	if (!(r->scale >= 0.0f) || !std::isfinite(r->scale) || !(r->cap >= 0.0f) || !std::isfinite(r->cap))
 		return fail(NNH_ERR_INVALID, "masked attention: scale and cap must be finite and not negative");
 	if (r->window > kMaxRows) return fail(NNH_ERR_INVALID, "masked attention: window out of range");
-	if (!r->q_docs != !r->k_docs) return fail(NNH_ERR_INVALID, "masked attention: documents need both the queries' and the keys'");
+	const bool pairs = g.N > 0 && g.Tq > 0 && g.Tk > 0;  // else there is nothing to keep apart, and an empty side's array may be null
+	if (pairs && !r->q_docs != !r->k_docs) return fail(NNH_ERR_INVALID, "masked attention: documents need both the queries' and the keys'");
 	a.scale = r->scale > 0.0f ? r->scale : 1.0f / std::sqrt((float)g.Dh);
 	a.cap = r->cap;
 	a.slopes = r->slopes;
@@ -99,8 +100,8 @@ int check_rule(const Geom& g, const nnh_attention_rule* r, MaskedAttentionArgs& 
 	a.q_start = r->q_start;
 	a.k_lens = r->k_lens;
 	a.prefix = r->prefix;
-	a.q_docs = r->q_docs;
-	a.k_docs = r->k_docs;
+	a.q_docs = pairs ? r->q_docs : nullptr;
+	a.k_docs = pairs ? r->k_docs : nullptr;
 	a.N = (int)g.N;
 	a.Tq = (int)g.Tq;
 	a.Tk = (int)g.Tk;
