@@ -49,6 +49,17 @@ inline bool count_ok(std::initializer_list<size_t> dims) {
 extern thread_local std::string g_last_error;
 int fail(int code, const std::string& msg);
 int hip_status(hipError_t e, const char* what);
+// The body of an entry point that makes lists: nothing is thrown across the C boundary. Without host memory, for a list or for a
+// message, the call fails with a message short enough to need none.
+template <class F>
+int guarded(F&& body) noexcept {
+	try {
+		return body();
+	} catch (...) {
+		g_last_error = "out of memory";
+		return NNH_ERR_INVALID;
+	}
+}
 bool ranges_overlap(const void* p0, uint64_t bytes0, const void* p1, uint64_t bytes1);
 // Overlap other than the same range twice (an op that goes element by element may write in place).
 inline bool partial_overlap(const void* p0, uint64_t bytes0, const void* p1, uint64_t bytes1) {

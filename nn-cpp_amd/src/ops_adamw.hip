@@ -3,7 +3,6 @@
 
 #include <algorithm>
 #include <cmath>
-#include <new>
 
 #include "abi_common.hpp"
 #include "kernels/hip/adamw.hpp"
@@ -93,11 +92,7 @@ int step(const nnh_adamw* o, const nnh_adamw_tensor* tensors, size_t n, void* st
 extern "C" {
 
 int nnh_adamw_step(const nnh_adamw* o, const nnh_adamw_tensor* tensors, size_t n, void* stream) {
-	try {
-		return step(o, tensors, n, stream);
-	} catch (const std::exception&) {  // no memory for the lists
-		return fail(NNH_ERR_INVALID, "adamw: out of host memory");
-	}
+	return guarded([&] { return step(o, tensors, n, stream); });
 }
 
 }  // extern "C"

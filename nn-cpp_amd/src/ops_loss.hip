@@ -320,94 +320,102 @@ int check_gradients(const Head& h, const Gradients& d, std::vector<Range>& outs)
 extern "C" {
 
 int nnh_linear_cross_entropy_workspace_size(int type, size_t rows, size_t D, size_t V, int call, int aligned, size_t* bytes) {
-	Head h{type, nullptr, nullptr, nullptr, nullptr, rows, D, V};
-	const int rc = check_head(h, NNH_REDUCE_NONE);
-	if (rc != NNH_OK) return rc;
-	if (call < kForward || call > kTrain) return fail(NNH_ERR_INVALID, "linear cross entropy: no such call");
-	const bool pack = type == NNH_BF16 && (D % 8 != 0 || !aligned);
-	return query_both_modes(bytes, [&](size_t* b) { return put_bytes(b, plan_of(h, (Call)call, pack, pack).total); });
+	return guarded([&] {
+		Head h{type, nullptr, nullptr, nullptr, nullptr, rows, D, V};
+		const int rc = check_head(h, NNH_REDUCE_NONE);
+		if (rc != NNH_OK) return rc;
+		if (call < kForward || call > kTrain) return fail(NNH_ERR_INVALID, "linear cross entropy: no such call");
+		const bool pack = type == NNH_BF16 && (D % 8 != 0 || !aligned);
+		return query_both_modes(bytes, [&](size_t* b) { return put_bytes(b, plan_of(h, (Call)call, pack, pack).total); });
+	});
 }
 
 int nnh_linear_cross_entropy_forward(int type, const void* x, size_t rows, size_t D, const void* w, size_t V, const void* bias,
                                      const int* targets, int reduction, float* loss, float* lse, void* stream) {
-	NumericsScope numerics_scope(stream);
-	const Head h{type, x, w, bias, targets, rows, D, V};
-	int rc = check_head(h, reduction);
-	if (rc == NNH_OK) rc = check_inputs(h);
-	if (rc != NNH_OK) return rc;
-	if ((!lse && rows) || (!loss && (rows || reduction != NNH_REDUCE_NONE))) return fail(NNH_ERR_INVALID, "linear cross entropy: null pointer");
-	rc = check_apart({{loss, (reduction == NNH_REDUCE_NONE ? rows : 1) * 4}, {lse, rows * 4}}, inputs_of(h));
-	if (rc != NNH_OK) return rc;
-	if (rows == 0 && reduction == NNH_REDUCE_NONE) return NNH_OK;
-	hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-	const Plan p = plan_of(h, kForward, packed(h, x), packed(h, w));
-	Scratch ws(s, p.total);
-	if (ws.status() != NNH_OK) return ws.status();
-	Run r{h, p, reduction, ws, s, nullptr, nullptr, 0, 0};
-	rc = r.begin();
-	float* const each = reduction == NNH_REDUCE_NONE ? loss : ws.at<float>(p.loss);
-	if (rc == NNH_OK) rc = r.forward(lse, each);
-	if (rc == NNH_OK && reduction != NNH_REDUCE_NONE)
-		rc = hip_status(ce_reduce(each, targets, (int64_t)rows, (int64_t)V, reduction, nullptr, loss, nullptr, nullptr, nullptr, s), "linear cross entropy");
-	return rc;
+	return guarded([&] {
+		NumericsScope numerics_scope(stream);
+		const Head h{type, x, w, bias, targets, rows, D, V};
+		int rc = check_head(h, reduction);
+		if (rc == NNH_OK) rc = check_inputs(h);
+		if (rc != NNH_OK) return rc;
+		if ((!lse && rows) || (!loss && (rows || reduction != NNH_REDUCE_NONE))) return fail(NNH_ERR_INVALID, "linear cross entropy: null pointer");
+		rc = check_apart({{loss, (reduction == NNH_REDUCE_NONE ? rows : 1) * 4}, {lse, rows * 4}}, inputs_of(h));
+		if (rc != NNH_OK) return rc;
+		if (rows == 0 && reduction == NNH_REDUCE_NONE) return NNH_OK;
+		hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+		const Plan p = plan_of(h, kForward, packed(h, x), packed(h, w));
+		Scratch ws(s, p.total);
+		if (ws.status() != NNH_OK) return ws.status();
+		Run r{h, p, reduction, ws, s, nullptr, nullptr, 0, 0};
+		rc = r.begin();
+		float* const each = reduction == NNH_REDUCE_NONE ? loss : ws.at<float>(p.loss);
+		if (rc == NNH_OK) rc = r.forward(lse, each);
+		if (rc == NNH_OK && reduction != NNH_REDUCE_NONE)
+			rc = hip_status(ce_reduce(each, targets, (int64_t)rows, (int64_t)V, reduction, nullptr, loss, nullptr, nullptr, nullptr, s), "linear cross entropy");
+		return rc;
+	});
 }
 
 int nnh_linear_cross_entropy_backward(int type, const float* g, const void* x, size_t rows, size_t D, const void* w, size_t V,
                                       const void* bias, const int* targets, const float* lse, int reduction, void* dx, int dx_first,
                                       void* dw, int dw_first, void* db, int db_first, void* stream) {
-	NumericsScope numerics_scope(stream);
-	const Head h{type, x, w, bias, targets, rows, D, V};
-	const Gradients d{g, dx, dx_first, dw, dw_first, db, db_first};
-	std::vector<Range> outs, ins = inputs_of(h);
-	int rc = check_head(h, reduction);
-	if (rc == NNH_OK) rc = check_inputs(h);
-	if (rc == NNH_OK && rows && !lse) rc = fail(NNH_ERR_INVALID, "linear cross entropy: null pointer");
-	if (rc == NNH_OK) rc = check_gradients(h, d, outs);
-	ins.push_back({lse, rows * 4});
-	ins.push_back({g, (reduction == NNH_REDUCE_NONE ? rows : 1) * 4});
-	if (rc == NNH_OK) rc = check_apart(outs, ins);
-	if (rc != NNH_OK || (!dx && !dw && !db)) return rc;
-	hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-	const Plan p = plan_of(h, kBackward, packed(h, x), packed(h, w));
-	Scratch ws(s, p.total);
-	if (ws.status() != NNH_OK) return ws.status();
-	Run r{h, p, reduction, ws, s, nullptr, nullptr, 0, 0};
-	rc = r.begin();
-	if (rc == NNH_OK)
-		rc = hip_status(ce_reduce(nullptr, targets, (int64_t)rows, (int64_t)V, reduction, g, nullptr, ws.at<float>(p.weight), ws.at<uint64_t>(p.live), ws.at<float>(p.factor), s),
-		                "linear cross entropy");
-	return rc == NNH_OK ? r.backward(lse, d) : rc;
+	return guarded([&] {
+		NumericsScope numerics_scope(stream);
+		const Head h{type, x, w, bias, targets, rows, D, V};
+		const Gradients d{g, dx, dx_first, dw, dw_first, db, db_first};
+		std::vector<Range> outs, ins = inputs_of(h);
+		int rc = check_head(h, reduction);
+		if (rc == NNH_OK) rc = check_inputs(h);
+		if (rc == NNH_OK && rows && !lse) rc = fail(NNH_ERR_INVALID, "linear cross entropy: null pointer");
+		if (rc == NNH_OK) rc = check_gradients(h, d, outs);
+		ins.push_back({lse, rows * 4});
+		ins.push_back({g, (reduction == NNH_REDUCE_NONE ? rows : 1) * 4});
+		if (rc == NNH_OK) rc = check_apart(outs, ins);
+		if (rc != NNH_OK || (!dx && !dw && !db)) return rc;
+		hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+		const Plan p = plan_of(h, kBackward, packed(h, x), packed(h, w));
+		Scratch ws(s, p.total);
+		if (ws.status() != NNH_OK) return ws.status();
+		Run r{h, p, reduction, ws, s, nullptr, nullptr, 0, 0};
+		rc = r.begin();
+		if (rc == NNH_OK)
+			rc = hip_status(ce_reduce(nullptr, targets, (int64_t)rows, (int64_t)V, reduction, g, nullptr, ws.at<float>(p.weight), ws.at<uint64_t>(p.live), ws.at<float>(p.factor), s),
+			                "linear cross entropy");
+		return rc == NNH_OK ? r.backward(lse, d) : rc;
+	});
 }
 
 int nnh_linear_cross_entropy_train(int type, const float* g, const void* x, size_t rows, size_t D, const void* w, size_t V,
                                    const void* bias, const int* targets, int reduction, float* loss, void* dx, int dx_first, void* dw,
                                    int dw_first, void* db, int db_first, void* stream) {
-	NumericsScope numerics_scope(stream);
-	const Head h{type, x, w, bias, targets, rows, D, V};
-	const Gradients d{g, dx, dx_first, dw, dw_first, db, db_first};
-	std::vector<Range> outs, ins = inputs_of(h);
-	int rc = check_head(h, reduction);
-	if (rc == NNH_OK) rc = check_inputs(h);
-	if (rc == NNH_OK && !loss && (rows || reduction != NNH_REDUCE_NONE)) rc = fail(NNH_ERR_INVALID, "linear cross entropy: null pointer");
-	if (rc == NNH_OK) rc = check_gradients(h, d, outs);
-	outs.push_back({loss, (reduction == NNH_REDUCE_NONE ? rows : 1) * 4});
-	ins.push_back({g, (reduction == NNH_REDUCE_NONE ? rows : 1) * 4});
-	if (rc == NNH_OK) rc = check_apart(outs, ins);
-	if (rc != NNH_OK) return rc;
-	hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-	const Plan p = plan_of(h, kTrain, packed(h, x), packed(h, w));
-	Scratch ws(s, p.total);
-	if (ws.status() != NNH_OK) return ws.status();
-	Run r{h, p, reduction, ws, s, nullptr, nullptr, 0, 0};
-	rc = r.begin();
-	float* const each = reduction == NNH_REDUCE_NONE ? loss : ws.at<float>(p.loss);
-	float* const lse = ws.at<float>(p.lse);
-	if (rc == NNH_OK) rc = r.forward(lse, each);
-	if (rc == NNH_OK)
-		rc = hip_status(ce_reduce(each, targets, (int64_t)rows, (int64_t)V, reduction, g, reduction == NNH_REDUCE_NONE ? nullptr : loss,
-		                          ws.at<float>(p.weight), ws.at<uint64_t>(p.live), ws.at<float>(p.factor), s),
-		                "linear cross entropy");
-	return rc == NNH_OK ? r.backward(lse, d) : rc;
+	return guarded([&] {
+		NumericsScope numerics_scope(stream);
+		const Head h{type, x, w, bias, targets, rows, D, V};
+		const Gradients d{g, dx, dx_first, dw, dw_first, db, db_first};
+		std::vector<Range> outs, ins = inputs_of(h);
+		int rc = check_head(h, reduction);
+		if (rc == NNH_OK) rc = check_inputs(h);
+		if (rc == NNH_OK && !loss && (rows || reduction != NNH_REDUCE_NONE)) rc = fail(NNH_ERR_INVALID, "linear cross entropy: null pointer");
+		if (rc == NNH_OK) rc = check_gradients(h, d, outs);
+		outs.push_back({loss, (reduction == NNH_REDUCE_NONE ? rows : 1) * 4});
+		ins.push_back({g, (reduction == NNH_REDUCE_NONE ? rows : 1) * 4});
+		if (rc == NNH_OK) rc = check_apart(outs, ins);
+		if (rc != NNH_OK) return rc;
+		hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+		const Plan p = plan_of(h, kTrain, packed(h, x), packed(h, w));
+		Scratch ws(s, p.total);
+		if (ws.status() != NNH_OK) return ws.status();
+		Run r{h, p, reduction, ws, s, nullptr, nullptr, 0, 0};
+		rc = r.begin();
+		float* const each = reduction == NNH_REDUCE_NONE ? loss : ws.at<float>(p.loss);
+		float* const lse = ws.at<float>(p.lse);
+		if (rc == NNH_OK) rc = r.forward(lse, each);
+		if (rc == NNH_OK)
+			rc = hip_status(ce_reduce(each, targets, (int64_t)rows, (int64_t)V, reduction, g, reduction == NNH_REDUCE_NONE ? nullptr : loss,
+			                          ws.at<float>(p.weight), ws.at<uint64_t>(p.live), ws.at<float>(p.factor), s),
+			                "linear cross entropy");
+		return rc == NNH_OK ? r.backward(lse, d) : rc;
+	});
 }
 
 }  // extern "C"

@@ -187,55 +187,59 @@ extern "C" {
 
 int nnh_masked_attention_workspace_size(size_t N, size_t Tq, size_t Tk, size_t H, size_t Hkv, size_t Dh, int documents,
                                         int backward, size_t* bytes) {
-	const Geom g{NNH_F32, N, Tq, Tk, H, Hkv, Dh};
-	const int rc = check_geometry(g);
-	return rc != NNH_OK ? rc : put_bytes(bytes, plan_of(g, documents != 0, backward != 0).total);
+	return guarded([&] {
+		const Geom g{NNH_F32, N, Tq, Tk, H, Hkv, Dh};
+		const int rc = check_geometry(g);
+		return rc != NNH_OK ? rc : put_bytes(bytes, plan_of(g, documents != 0, backward != 0).total);
+	});
 }
 
 int nnh_masked_attention_forward(int type, size_t N, size_t Tq, size_t Tk, size_t H, size_t Hkv, size_t Dh,
                                  const nnh_head_tensor* q, const nnh_head_tensor* k, const nnh_head_tensor* v,
                                  const nnh_attention_rule* rule, const nnh_head_tensor* out, const nnh_head_tensor* rest,
                                  float* lse, void* stream) {
-	const Geom g{type, N, Tq, Tk, H, Hkv, Dh};
-	MaskedAttentionArgs a{};
-	int rc = check_geometry(g);
-	if (rc == NNH_OK) rc = check_rule(g, rule, a);
-	Operand in[3] = {{q, Tq, H, "q"}, {k, Tk, Hkv, "k"}, {v, Tk, Hkv, "v"}}, o{out, Tq, H, "out"}, lost{rest, Tq, H, "rest"};
-	for (Operand& x : in)
-		if (rc == NNH_OK) rc = check_operand(g, x, false);
-	if (rc == NNH_OK) rc = check_operand(g, o, true);
-	if (rc == NNH_OK && rest) rc = check_rest(g, lost, true);
-	if (rc != NNH_OK) return rc;
-	if (N == 0 || Tq == 0) return NNH_OK;
-	if (!lse) return fail(NNH_ERR_INVALID, "masked attention: lse is null");
-	const Range stats{lse, (uint64_t)N * H * Tq * 4};
-	std::vector<Range> ins = rule_ranges(g, a);
-	for (const Operand& x : in) ins.push_back(range_of(g, x));
-	rc = check_apart({range_of(g, o), range_of(g, lost), stats}, ins);
-	if (rc == NNH_OK) rc = check_apart({stats}, {range_of(g, o), range_of(g, lost)});
-	if (rc == NNH_OK) rc = check_apart({range_of(g, o)}, {range_of(g, lost)});
-	if (rc != NNH_OK) return rc;
-	a.q = q->data;
-	a.k = Tk ? k->data : nullptr;
-	a.v = Tk ? v->data : nullptr;
-	a.out = out->data;
-	a.lse = lse;
-	a.qs = strides_of(q);
-	a.ks = strides_of(k);
-	a.vs = strides_of(v);
-	a.os = strides_of(out);
-	a.rest = rest ? rest->data : nullptr;
-	a.rs = strides_of(rest);
-	const bool vec = Dh * g.size() % 16 == 0 && wide(g, in[0]) && wide(g, in[1]) && wide(g, in[2]) && wide(g, o) && wide(g, lost);
-	const Plan p = plan_of(g, a.q_docs != nullptr, false);
-	hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-	Scratch ws(s, p.total);
-	if (ws.status() != NNH_OK) return ws.status();
-	rc = run_ranges(a, p, ws, s);
-	if (rc != NNH_OK) return rc;
-	a.splits = p.splits;
-	if (p.splits > 1) a.partial = ws.at<float>(p.partial);
-	return hip_status(p.splits ? masked_attention_split(a, type, vec, s) : masked_attention_forward(a, type, vec, s), "masked attention");
+	return guarded([&] {
+		const Geom g{type, N, Tq, Tk, H, Hkv, Dh};
+		MaskedAttentionArgs a{};
+		int rc = check_geometry(g);
+		if (rc == NNH_OK) rc = check_rule(g, rule, a);
+		Operand in[3] = {{q, Tq, H, "q"}, {k, Tk, Hkv, "k"}, {v, Tk, Hkv, "v"}}, o{out, Tq, H, "out"}, lost{rest, Tq, H, "rest"};
+		for (Operand& x : in)
+			if (rc == NNH_OK) rc = check_operand(g, x, false);
+		if (rc == NNH_OK) rc = check_operand(g, o, true);
+		if (rc == NNH_OK && rest) rc = check_rest(g, lost, true);
+		if (rc != NNH_OK) return rc;
+		if (N == 0 || Tq == 0) return NNH_OK;
+		if (!lse) return fail(NNH_ERR_INVALID, "masked attention: lse is null");
+		const Range stats{lse, (uint64_t)N * H * Tq * 4};
+		std::vector<Range> ins = rule_ranges(g, a);
+		for (const Operand& x : in) ins.push_back(range_of(g, x));
+		rc = check_apart({range_of(g, o), range_of(g, lost), stats}, ins);
+		if (rc == NNH_OK) rc = check_apart({stats}, {range_of(g, o), range_of(g, lost)});
+		if (rc == NNH_OK) rc = check_apart({range_of(g, o)}, {range_of(g, lost)});
+		if (rc != NNH_OK) return rc;
+		a.q = q->data;
+		a.k = Tk ? k->data : nullptr;
+		a.v = Tk ? v->data : nullptr;
+		a.out = out->data;
+		a.lse = lse;
+		a.qs = strides_of(q);
+		a.ks = strides_of(k);
+		a.vs = strides_of(v);
+		a.os = strides_of(out);
+		a.rest = rest ? rest->data : nullptr;
+		a.rs = strides_of(rest);
+		const bool vec = Dh * g.size() % 16 == 0 && wide(g, in[0]) && wide(g, in[1]) && wide(g, in[2]) && wide(g, o) && wide(g, lost);
+		const Plan p = plan_of(g, a.q_docs != nullptr, false);
+		hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+		Scratch ws(s, p.total);
+		if (ws.status() != NNH_OK) return ws.status();
+		rc = run_ranges(a, p, ws, s);
+		if (rc != NNH_OK) return rc;
+		a.splits = p.splits;
+		if (p.splits > 1) a.partial = ws.at<float>(p.partial);
+		return hip_status(p.splits ? masked_attention_split(a, type, vec, s) : masked_attention_forward(a, type, vec, s), "masked attention");
+	});
 }
 
 int nnh_masked_attention_backward(int type, size_t N, size_t Tq, size_t Tk, size_t H, size_t Hkv, size_t Dh,
@@ -244,67 +248,69 @@ int nnh_masked_attention_backward(int type, size_t N, size_t Tq, size_t Tk, size
                                   const nnh_attention_rule* rule, const nnh_head_tensor* dq, int dq_first,
                                   const nnh_head_tensor* dk, int dk_first, const nnh_head_tensor* dv, int dv_first,
                                   void* stream) {
-	const Geom g{type, N, Tq, Tk, H, Hkv, Dh};
-	MaskedAttentionArgs a{};
-	int rc = check_geometry(g);
-	if (rc == NNH_OK) rc = check_rule(g, rule, a);
-	if (rc != NNH_OK) return rc;
-	if (N == 0 || (!dq && !dk && !dv)) return NNH_OK;
-	Operand in[5] = {{g_, Tq, H, "g"}, {q, Tq, H, "q"}, {k, Tk, Hkv, "k"}, {v, Tk, Hkv, "v"}, {out, Tq, H, "out"}}, lost{rest, Tq, H, "rest"};
-	Operand grad[3] = {{dq, Tq, H, "dq"}, {dk, Tk, Hkv, "dk"}, {dv, Tk, Hkv, "dv"}};
-	for (Operand& x : in)
-		if (rc == NNH_OK) rc = check_operand(g, x, false);
-	if (rc == NNH_OK && rest) rc = check_rest(g, lost, false);
-	for (Operand& x : grad)
-		if (rc == NNH_OK && x.t) rc = check_operand(g, x, true);
-	if (rc != NNH_OK) return rc;
-	if (Tq && !lse) return fail(NNH_ERR_INVALID, "masked attention: lse is null");
-	std::vector<Range> ins = rule_ranges(g, a), outs;
-	for (const Operand& x : in) ins.push_back(range_of(g, x));
-	ins.push_back({lse, (uint64_t)N * H * Tq * 4});
-	ins.push_back(range_of(g, lost));
-	for (const Operand& x : grad) outs.push_back(range_of(g, x));
-	rc = check_apart(outs, ins);
-	if (rc != NNH_OK) return rc;
-	if (!beside(g, grad[0], grad[1]) || !beside(g, grad[0], grad[2]) || !beside(g, grad[1], grad[2]))
-		return fail(NNH_ERR_ALIAS, "masked attention: two gradients overlap");
-	auto data = [](const nnh_head_tensor* t) { return t ? t->data : nullptr; };
-	a.q = data(q);
-	a.k = data(k);
-	a.v = data(v);
-	a.g = data(g_);
-	a.out = data(out);
-	a.lse = const_cast<float*>(lse);
-	a.dq = data(dq);
-	a.dk = data(dk);
-	a.dv = data(dv);
-	a.qs = strides_of(q);
-	a.ks = strides_of(k);
-	a.vs = strides_of(v);
-	a.gs = strides_of(g_);
-	a.os = strides_of(out);
-	a.rest = data(rest);
-	a.rs = strides_of(rest);
-	a.dqs = strides_of(dq);
-	a.dks = strides_of(dk);
-	a.dvs = strides_of(dv);
-	a.dq_first = dq_first;
-	a.dk_first = dk_first;
-	a.dv_first = dv_first;
-	bool vec = Dh * g.size() % 16 == 0 && wide(g, lost);
-	for (const Operand& x : in) vec = vec && wide(g, x);
-	for (const Operand& x : grad) vec = vec && wide(g, x);
-	const Plan p = plan_of(g, a.q_docs != nullptr, true);
-	hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-	Scratch ws(s, p.total);
-	if (ws.status() != NNH_OK) return ws.status();
-	a.delta = ws.at<float>(p.delta);
-	a.lse2 = ws.at<float>(p.lse2);
-	a.parts = p.parts;
-	a.partial = ws.at<float>(p.partial);
-	rc = run_ranges(a, p, ws, s);
-	if (rc != NNH_OK) return rc;
-	return hip_status(masked_attention_backward(a, type, vec, s), "masked attention backward");
+	return guarded([&] {
+		const Geom g{type, N, Tq, Tk, H, Hkv, Dh};
+		MaskedAttentionArgs a{};
+		int rc = check_geometry(g);
+		if (rc == NNH_OK) rc = check_rule(g, rule, a);
+		if (rc != NNH_OK) return rc;
+		if (N == 0 || (!dq && !dk && !dv)) return NNH_OK;
+		Operand in[5] = {{g_, Tq, H, "g"}, {q, Tq, H, "q"}, {k, Tk, Hkv, "k"}, {v, Tk, Hkv, "v"}, {out, Tq, H, "out"}}, lost{rest, Tq, H, "rest"};
+		Operand grad[3] = {{dq, Tq, H, "dq"}, {dk, Tk, Hkv, "dk"}, {dv, Tk, Hkv, "dv"}};
+		for (Operand& x : in)
+			if (rc == NNH_OK) rc = check_operand(g, x, false);
+		if (rc == NNH_OK && rest) rc = check_rest(g, lost, false);
+		for (Operand& x : grad)
+			if (rc == NNH_OK && x.t) rc = check_operand(g, x, true);
+		if (rc != NNH_OK) return rc;
+		if (Tq && !lse) return fail(NNH_ERR_INVALID, "masked attention: lse is null");
+		std::vector<Range> ins = rule_ranges(g, a), outs;
+		for (const Operand& x : in) ins.push_back(range_of(g, x));
+		ins.push_back({lse, (uint64_t)N * H * Tq * 4});
+		ins.push_back(range_of(g, lost));
+		for (const Operand& x : grad) outs.push_back(range_of(g, x));
+		rc = check_apart(outs, ins);
+		if (rc != NNH_OK) return rc;
+		if (!beside(g, grad[0], grad[1]) || !beside(g, grad[0], grad[2]) || !beside(g, grad[1], grad[2]))
+			return fail(NNH_ERR_ALIAS, "masked attention: two gradients overlap");
+		auto data = [](const nnh_head_tensor* t) { return t ? t->data : nullptr; };
+		a.q = data(q);
+		a.k = data(k);
+		a.v = data(v);
+		a.g = data(g_);
+		a.out = data(out);
+		a.lse = const_cast<float*>(lse);
+		a.dq = data(dq);
+		a.dk = data(dk);
+		a.dv = data(dv);
+		a.qs = strides_of(q);
+		a.ks = strides_of(k);
+		a.vs = strides_of(v);
+		a.gs = strides_of(g_);
+		a.os = strides_of(out);
+		a.rest = data(rest);
+		a.rs = strides_of(rest);
+		a.dqs = strides_of(dq);
+		a.dks = strides_of(dk);
+		a.dvs = strides_of(dv);
+		a.dq_first = dq_first;
+		a.dk_first = dk_first;
+		a.dv_first = dv_first;
+		bool vec = Dh * g.size() % 16 == 0 && wide(g, lost);
+		for (const Operand& x : in) vec = vec && wide(g, x);
+		for (const Operand& x : grad) vec = vec && wide(g, x);
+		const Plan p = plan_of(g, a.q_docs != nullptr, true);
+		hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+		Scratch ws(s, p.total);
+		if (ws.status() != NNH_OK) return ws.status();
+		a.delta = ws.at<float>(p.delta);
+		a.lse2 = ws.at<float>(p.lse2);
+		a.parts = p.parts;
+		a.partial = ws.at<float>(p.partial);
+		rc = run_ranges(a, p, ws, s);
+		if (rc != NNH_OK) return rc;
+		return hip_status(masked_attention_backward(a, type, vec, s), "masked attention backward");
+	});
 }
 
 }  // extern "C"
