@@ -987,14 +987,27 @@ Value linear_cross_entropy(const Value& x, const Value& weight, const Value& bia
 	std::vector<Value> parents{x, weight};
 	if (bias.impl()) parents.push_back(bias);
 	return Value::node(std::move(loss), std::move(parents), [=](const Tensor& g) {
-		bool fx = false, fw = false, fb = false;
-		float* dx = grad_if(x, fx);
-		float* dw = grad_if(weight, fw);
-		float* db = bias.impl() ? grad_if(bias, fb) : nullptr;
-		if (!dx && !dw && !db) return;
+		const Value* in[3] = {&x, &weight, &bias};
+		// one node as two operands: their gradients are made apart and added in turn
+		const bool shared = x.impl() == weight.impl() || x.impl() == bias.impl();
+		Tensor part[3];
+		float* d[3] = {};
+		bool first[3] = {true, true, true};
+		for (int i = 0; i < 3; ++i) {
+			if (!in[i]->impl() || !in[i]->requires_grad()) continue;
+			if (shared) part[i] = Tensor::empty(in[i]->data().shape());
+			d[i] = shared ? part[i].data() : grad_if(*in[i], first[i]);
+		}
+		if (!d[0] && !d[1] && !d[2]) return;
 		check(nnh_linear_cross_entropy_backward(NNH_F32, g.data(), x.data().data(), rows, D, weight.data().data(), V,
 		                                        bias.impl() ? bias.data().data() : nullptr, targets.data(), lse.data(),
-		                                        NNH_REDUCE_MEAN, dx, fx, dw, fw, db, fb, g_stream));
+		                                        NNH_REDUCE_MEAN, d[0], first[0], d[1], first[1], d[2], first[2], g_stream));
+		for (int i = 0; shared && i < 3; ++i) {
+			if (!d[i]) continue;
+			bool fresh = false;
+			float* to = grad_if(*in[i], fresh);
+			check(nnh_add_to_grad(to, part[i].data(), part[i].size(), fresh, g_stream));
+		}
 	});
 }
 

@@ -63,4 +63,27 @@ int edges_adamw_changed(size_t n, int bits, int change, float* p, size_t* steps)
 	});
 }
 
+// linear_cross_entropy over nodes that are given twice: which 0 x is the weight too ({V, D}), 1 x of one row is the bias too (x {D}, bias
+// {V}, D = V), 2 all apart. add: the leaves' gradients hold ones before. loss {1}, and the gradients of x, weight and bias (of a node
+// given twice: the sum, in its first place).
+int edges_loss_shared(int which, int add, size_t V, size_t D, const float* x, const float* w, const float* b, const int* targets, float* loss,
+                      float* dx, float* dw, float* db) {
+	return guard([&] {
+		const size_t rows = which == 1 ? 1 : V;
+		const Value X = Value::leaf(Tensor::from_host(which == 1 ? std::vector<size_t>{D} : std::vector<size_t>{rows, D}, x), true);
+		const Value W = which == 0 ? X : Value::leaf(Tensor::from_host({V, D}, w), true);
+		const Value B = which == 1 ? X : Value::leaf(Tensor::from_host({V}, b), true);
+		const IntTensor y = IntTensor::from_host(which == 1 ? std::vector<size_t>{} : std::vector<size_t>{rows}, targets);
+		bool first = false;
+		if (add)
+			for (const Value* v : {&X, &W, &B}) v->grad_accum(first).fill_(1.0f);
+		Value l = linear_cross_entropy(X, W, B, y);
+		l.backward();
+		l.data().to_host(loss);
+		X.grad().to_host(dx);
+		if (which != 0) W.grad().to_host(dw);
+		if (which != 1) B.grad().to_host(db);
+	});
+}
+
 }  // extern "C"
