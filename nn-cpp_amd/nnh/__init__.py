@@ -705,13 +705,15 @@ def masked_attention_forward(q, k, v, rule, out=None, lse=None, stream=None, res
         lse = torch.empty((N, H, Tq), dtype=torch.float32, device=q.device)
     if rest is True:
         rest = torch.empty((N, Tq, H, Dh), dtype=q.dtype, device=q.device) if q.dtype == torch.bfloat16 else None
-    lse.rest = rest = None if rest is False else rest
+    elif rest is False:
+        rest = None
     qs, ks = (N, Tq, H, Dh), (N, Tk, Hkv, Dh)
     t = [_heads(x, q, device, s, w) for x, s, w in ((q, qs, "q"), (k, ks, "k"), (v, ks, "v"), (out, qs, "out"))]
     r = rule._struct(N, Tq, Tk, H, device)
     check(lib().nnh_masked_attention_forward(_type(q), N, Tq, Tk, H, Hkv, Dh, C.byref(t[0]), C.byref(t[1]), C.byref(t[2]),
                                              C.byref(r), C.byref(t[3]), rest if rest is None else C.byref(_heads(rest, q, device, qs, "rest")), _on(lse, device, torch.float32, (N, H, Tq), "lse"),
                                              _stream(stream)))
+    lse.rest = rest
     return out, lse
 
 
