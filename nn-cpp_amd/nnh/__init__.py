@@ -694,8 +694,8 @@ def masked_attention_forward(q, k, v, rule, out=None, lse=None, stream=None, res
     consecutive); returns (out, lse).
 
     In bf16 the lse that is returned has an attribute `rest`, a tensor of out's shape with what out lost in being rounded:
-    masked_attention_backward reads it there (an lse without one, a copy for instance, leaves the gradients of q off by
-    out's rounding as well). rest: False where no gradients are wanted, or the tensor to use."""
+    masked_attention_backward reads it there, or takes it as an argument beside a copy or a view of lse, which has none (without
+    it the gradients of q are off by out's rounding as well). rest: False where no gradients are wanted, or the tensor to use."""
     torch = _torch or _load_torch()
     N, Tq, Tk, H, Hkv, Dh = _attention_sizes(q, k, v)
     device = torch.cuda.current_device()
@@ -718,8 +718,9 @@ def masked_attention_forward(q, k, v, rule, out=None, lse=None, stream=None, res
 
 
 def masked_attention_backward(g, q, k, v, out, lse, rule, dq=None, dq_first=True, dk=None, dk_first=True, dv=None,
-                              dv_first=True, stream=None):
-    """nnh_masked_attention_backward; gradients that are not given are made (and returned with the others)."""
+                              dv_first=True, stream=None, rest=None):
+    """nnh_masked_attention_backward; gradients that are not given are made (and returned with the others). rest: the forward's
+    lse.rest, where lse is a copy or a view that does not have it (None: lse's own, if any), or False for none."""
     torch = _torch or _load_torch()
     N, Tq, Tk, H, Hkv, Dh = _attention_sizes(q, k, v)
     device = torch.cuda.current_device()
@@ -729,7 +730,7 @@ def masked_attention_backward(g, q, k, v, out, lse, rule, dq=None, dq_first=True
         if t is None and not first:
             raise NnhError(ERR_INVALID, "a gradient to add to has to be given")
         grads.append(torch.empty(shape, dtype=q.dtype, device=q.device) if t is None else t)
-    rest = getattr(lse, "rest", None)
+    rest = getattr(lse, "rest", None) if rest is None else None if rest is False else rest
     rest = rest if rest is None else C.byref(_heads(rest, q, device, qs, "rest"))
     named = ((g, qs, "g"), (q, qs, "q"), (k, ks, "k"), (v, ks, "v"), (out, qs, "out"), (grads[0], qs, "dq"),
              (grads[1], ks, "dk"), (grads[2], ks, "dv"))

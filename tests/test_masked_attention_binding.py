@@ -59,3 +59,16 @@ def test_a_refused_call_leaves_the_rest(library):
     library.refuse = False
     nnh.masked_attention_forward(q, k, v, nnh.AttentionRule(), out=out, lse=lse, rest=False)
     assert lse.rest is None
+
+
+def test_the_rest_beside_a_copy_of_lse(library):
+    """A copy, a view or a saved tensor has no attribute: the rest is then an argument of its own."""
+    q, k, v, g = inputs()
+    out, lse = nnh.masked_attention_forward(q, k, v, nnh.AttentionRule())
+    other = torch.zeros_like(out)
+    for given, rest, want in ((lse, None, lse.rest.data_ptr()), (lse.clone(), None, None), (lse.clone(), lse.rest, lse.rest.data_ptr()),
+                              (lse.view(-1).view(N, H, T), other, other.data_ptr()), (lse, other, other.data_ptr()), (lse, False, None)):
+        nnh.masked_attention_backward(g, q, k, v, out, given, nnh.AttentionRule(), rest=rest)
+        assert library.rest[-1] == want
+    with pytest.raises(nnh.ShapeError):
+        nnh.masked_attention_backward(g, q, k, v, out, lse, nnh.AttentionRule(), rest=other[:1])
