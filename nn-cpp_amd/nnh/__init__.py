@@ -703,8 +703,9 @@ def masked_attention_forward(q, k, v, rule, out=None, lse=None, stream=None, res
         out = torch.empty((N, Tq, H, Dh), dtype=q.dtype, device=q.device)
     if lse is None:
         lse = torch.empty((N, H, Tq), dtype=torch.float32, device=q.device)
+    made = None
     if rest is True:
-        rest = torch.empty((N, Tq, H, Dh), dtype=q.dtype, device=q.device) if q.dtype == torch.bfloat16 else None
+        rest = made = torch.empty((N, Tq, H, Dh), dtype=q.dtype, device=q.device) if q.dtype == torch.bfloat16 else None
     elif rest is False:
         rest = None
     qs, ks = (N, Tq, H, Dh), (N, Tk, Hkv, Dh)
@@ -713,6 +714,8 @@ def masked_attention_forward(q, k, v, rule, out=None, lse=None, stream=None, res
     check(lib().nnh_masked_attention_forward(_type(q), N, Tq, Tk, H, Hkv, Dh, C.byref(t[0]), C.byref(t[1]), C.byref(t[2]),
                                              C.byref(r), C.byref(t[3]), rest if rest is None else C.byref(_heads(rest, q, device, qs, "rest")), _on(lse, device, torch.float32, (N, H, Tq), "lse"),
                                              _stream(stream)))
+    if stream is not None and made is not None:  # the caller sees out and lse, and may not know of the third
+        made.record_stream(stream)
     lse.rest = rest
     return out, lse
 
@@ -731,14 +734,16 @@ def masked_attention_backward(g, q, k, v, out, lse, rule, dq=None, dq_first=True
             raise NnhError(ERR_INVALID, "a gradient to add to has to be given")
         grads.append(torch.empty(shape, dtype=q.dtype, device=q.device) if t is None else t)
     rest = getattr(lse, "rest", None) if rest is None else None if rest is False else rest
-    rest = rest if rest is None else C.byref(_heads(rest, q, device, qs, "rest"))
+    lost = rest if rest is None else C.byref(_heads(rest, q, device, qs, "rest"))
     named = ((g, qs, "g"), (q, qs, "q"), (k, ks, "k"), (v, ks, "v"), (out, qs, "out"), (grads[0], qs, "dq"),
              (grads[1], ks, "dk"), (grads[2], ks, "dv"))
     t = [C.byref(_heads(x, q, device, s, w)) for x, s, w in named]
     r = rule._struct(N, Tq, Tk, H, device)
-    check(lib().nnh_masked_attention_backward(_type(q), N, Tq, Tk, H, Hkv, Dh, *t[:5], rest,
+    check(lib().nnh_masked_attention_backward(_type(q), N, Tq, Tk, H, Hkv, Dh, *t[:5], lost,
                                               _on(lse, device, torch.float32, (N, H, Tq), "lse"), C.byref(r), t[5],
                                               int(dq_first), t[6], int(dk_first), t[7], int(dv_first), _stream(stream)))
+    if stream is not None and rest is not None:
+        rest.record_stream(stream)
     return tuple(grads)
 
 

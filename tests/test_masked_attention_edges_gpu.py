@@ -27,3 +27,29 @@ def test_documents_of_an_empty_side(gpu, dtype, N, Tq, Tk):
     grads = [torch.full_like(x, 7.0) for x in (q, k, v)]
     nnh.masked_attention_backward(g, q, k, v, out, lse, rule, *(y for x in grads for y in (x, False)))
     assert all(bool((x == 7.0).all()) for x in grads)
+
+
+@pytest.mark.parametrize("which", ["forward", "backward"])
+def test_the_rest_is_kept_for_another_stream(gpu, which):
+    """A call on a stream given to it: what the call has made and lse carries is not given to others while that stream may use it."""
+    import nnh
+    q, k, v = (torch.randn(1, 300, 2, 64, device="cuda").bfloat16() for _ in range(3))
+    side = torch.cuda.Stream()
+    rule = nnh.AttentionRule()
+    if which == "backward":
+        out, lse = nnh.masked_attention_forward(q, k, v, rule)
+    torch.cuda.synchronize()
+    nnh.bench_delay(100000, side)
+    if which == "backward":
+        grads = nnh.masked_attention_backward(q, q, k, v, out, lse, rule, stream=side)
+    else:
+        out, lse = nnh.masked_attention_forward(q, k, v, rule, stream=side)
+        grads = ()
+    for x in (q, k, v, out, lse) + grads:
+        x.record_stream(side)  # the caller's own
+    at, like = lse.rest.data_ptr(), torch.empty_like(lse.rest, device="cpu")
+    del lse
+    others = [torch.empty(like.shape, dtype=like.dtype, device="cuda") for _ in range(4)]
+    busy = not side.query()
+    torch.cuda.synchronize()
+    assert busy and at not in [x.data_ptr() for x in others]
