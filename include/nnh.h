@@ -451,7 +451,8 @@ int nnh_embedding_backward(const float* g, const int* rows, size_t count, size_t
  * nnh_attention_forward above) and no bits of its to keep: results are those of the formulas in fp32 (or better, where
  * said), repeat bit for bit, and never depend on atomics. Operands are fp32 or bf16 (nnh types below); sums and statistics
  * are fp32 in both. Captured into a graph, a call that needs scratch takes the buffer registered for its stream
- * (nnh_set_workspace) and is refused with NNH_ERR_WORKSPACE without one; graphs that may run at once need one each.
+ * (nnh_set_workspace) and is refused with NNH_ERR_WORKSPACE without one; graphs that may run at once need one each. A registered
+ * buffer must begin at a multiple of 16 bytes for these operators (NNH_ERR_WORKSPACE).
  */
 #define NNH_F32 0
 #define NNH_BF16 1
