@@ -61,6 +61,12 @@ int guarded(F&& body) noexcept {
 	}
 }
 bool ranges_overlap(const void* p0, uint64_t bytes0, const void* p1, uint64_t bytes1);
+// Whether one of some arrays of 32-bit elements (null ones aside) does not begin at a multiple of 4 bytes.
+inline bool off_words(std::initializer_list<const void*> arrays) {
+	for (const void* p : arrays)
+		if (reinterpret_cast<uintptr_t>(p) % 4 != 0) return true;
+	return false;
+}
 // Overlap other than the same range twice (an op that goes element by element may write in place).
 inline bool partial_overlap(const void* p0, uint64_t bytes0, const void* p1, uint64_t bytes1) {
 	return !(p0 == p1 && bytes0 == bytes1) && ranges_overlap(p0, bytes0, p1, bytes1);

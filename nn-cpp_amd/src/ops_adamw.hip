@@ -40,6 +40,7 @@ int step(const nnh_adamw* o, const nnh_adamw_tensor* tensors, size_t n, void* st
 	    !std::isfinite(o->weight_decay))
 		return fail(NNH_ERR_INVALID, "adamw: the betas must be in [0, 1), eps not negative, lr and weight_decay finite");
 	if (!o->step_device && o->step == 0) return fail(NNH_ERR_INVALID, "adamw: steps count from 1");
+	if (off_words({o->step_device, o->lr_device, o->grad_scale})) return fail(NNH_ERR_INVALID, "adamw: a pointer is not aligned to its elements");
 	const uint64_t ps = o->p_type == NNH_F32 ? 4 : 2, gs = o->g_type == NNH_F32 ? 4 : 2, ss = o->bits == 32 ? 4 : 1;
 	std::vector<AdamWTensor> t;
 	std::vector<Range> ranges;

@@ -107,10 +107,11 @@ int check_head(const Head& h, int reduction) {
 	return NNH_OK;
 }
 
-int check_inputs(const Head& h) {
+int check_inputs(const Head& h, std::initializer_list<const void*> words) {
 	if (!h.w || (h.rows > 0 && (!h.x || !h.targets))) return fail(NNH_ERR_INVALID, "linear cross entropy: null pointer");
 	for (const void* p : {h.x, h.w, h.bias})
 		if (reinterpret_cast<uintptr_t>(p) % h.size() != 0) return fail(NNH_ERR_INVALID, "linear cross entropy: a pointer is not aligned to its elements");
+	if (off_words({h.targets}) || off_words(words)) return fail(NNH_ERR_INVALID, "linear cross entropy: a pointer is not aligned to its elements");
 	return NNH_OK;
 }
 
@@ -336,7 +337,7 @@ int nnh_linear_cross_entropy_forward(int type, const void* x, size_t rows, size_
 		NumericsScope numerics_scope(stream);
 		const Head h{type, x, w, bias, targets, rows, D, V};
 		int rc = check_head(h, reduction);
-		if (rc == NNH_OK) rc = check_inputs(h);
+		if (rc == NNH_OK) rc = check_inputs(h, {loss, lse});
 		if (rc != NNH_OK) return rc;
 		if ((!lse && rows) || (!loss && (rows || reduction != NNH_REDUCE_NONE))) return fail(NNH_ERR_INVALID, "linear cross entropy: null pointer");
 		rc = check_apart({{loss, (reduction == NNH_REDUCE_NONE ? rows : 1) * 4}, {lse, rows * 4}}, inputs_of(h));
@@ -365,7 +366,7 @@ int nnh_linear_cross_entropy_backward(int type, const float* g, const void* x, s
 		const Gradients d{g, dx, dx_first, dw, dw_first, db, db_first};
 		std::vector<Range> outs, ins = inputs_of(h);
 		int rc = check_head(h, reduction);
-		if (rc == NNH_OK) rc = check_inputs(h);
+		if (rc == NNH_OK) rc = check_inputs(h, {g, lse});
 		if (rc == NNH_OK && rows && !lse) rc = fail(NNH_ERR_INVALID, "linear cross entropy: null pointer");
 		if (rc == NNH_OK) rc = check_gradients(h, d, outs);
 		ins.push_back({lse, rows * 4});
@@ -394,7 +395,7 @@ int nnh_linear_cross_entropy_train(int type, const float* g, const void* x, size
 		const Gradients d{g, dx, dx_first, dw, dw_first, db, db_first};
 		std::vector<Range> outs, ins = inputs_of(h);
 		int rc = check_head(h, reduction);
-		if (rc == NNH_OK) rc = check_inputs(h);
+		if (rc == NNH_OK) rc = check_inputs(h, {g, loss});
 		if (rc == NNH_OK && !loss && (rows || reduction != NNH_REDUCE_NONE)) rc = fail(NNH_ERR_INVALID, "linear cross entropy: null pointer");
 		if (rc == NNH_OK) rc = check_gradients(h, d, outs);
 		outs.push_back({loss, (reduction == NNH_REDUCE_NONE ? rows : 1) * 4});

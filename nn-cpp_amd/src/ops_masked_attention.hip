@@ -92,6 +92,8 @@ int check_rule(const Geom& g, const nnh_attention_rule* r, MaskedAttentionArgs& 
 	if (r->window > kMaxRows) return fail(NNH_ERR_INVALID, "masked attention: window out of range");
 	const bool pairs = g.N > 0 && g.Tq > 0 && g.Tk > 0;  // else there is nothing to keep apart, and an empty side's array may be null
 	if (pairs && !r->q_docs != !r->k_docs) return fail(NNH_ERR_INVALID, "masked attention: documents need both the queries' and the keys'");
+	if (off_words({r->slopes, r->q_start, r->k_lens, r->prefix, r->q_docs, r->k_docs}))
+		return fail(NNH_ERR_INVALID, "masked attention: an array of the rule is not aligned to its elements");
 	a.scale = r->scale > 0.0f ? r->scale : 1.0f / std::sqrt((float)g.Dh);
 	a.cap = r->cap;
 	a.slopes = r->slopes;
@@ -211,6 +213,7 @@ int nnh_masked_attention_forward(int type, size_t N, size_t Tq, size_t Tk, size_
 		if (rc != NNH_OK) return rc;
 		if (N == 0 || Tq == 0) return NNH_OK;
 		if (!lse) return fail(NNH_ERR_INVALID, "masked attention: lse is null");
+		if (off_words({lse})) return fail(NNH_ERR_INVALID, "masked attention: lse is not aligned to its elements");
 		const Range stats{lse, (uint64_t)N * H * Tq * 4};
 		std::vector<Range> ins = rule_ranges(g, a);
 		for (const Operand& x : in) ins.push_back(range_of(g, x));
@@ -264,6 +267,7 @@ int nnh_masked_attention_backward(int type, size_t N, size_t Tq, size_t Tk, size
 			if (rc == NNH_OK && x.t) rc = check_operand(g, x, true);
 		if (rc != NNH_OK) return rc;
 		if (Tq && !lse) return fail(NNH_ERR_INVALID, "masked attention: lse is null");
+		if (off_words({lse})) return fail(NNH_ERR_INVALID, "masked attention: lse is not aligned to its elements");
 		std::vector<Range> ins = rule_ranges(g, a), outs;
 		for (const Operand& x : in) ins.push_back(range_of(g, x));
 		ins.push_back({lse, (uint64_t)N * H * Tq * 4});

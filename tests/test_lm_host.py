@@ -6,7 +6,7 @@ import pytest
 from test_sanitize import _check, _run, built  # noqa: F401
 
 
-@pytest.mark.parametrize("program,says", [("lm_empty_sanitize", "empty sides: "), ("lm_nomem", "without memory: ")])
+@pytest.mark.parametrize("program,says", [("lm_empty_sanitize", "empty sides: "), ("lm_nomem", "without memory: "), ("lm_align_sanitize", "alignment: ")])
 def test_program(built, program, says):  # noqa: F811
     r = _run(os.path.join(built, program))
     if r.returncode == 77:
