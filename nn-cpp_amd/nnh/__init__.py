@@ -867,6 +867,13 @@ class AdamW:
             self._m_scale, self._v_scale = (zeros(64, torch.uint8), zeros(64, torch.uint8)) if m is None else (m_scale, v_scale)
         self._device = torch.cuda.current_device()
         self._counts, self._types = [p.numel() for p in self.params], None
+        if any(len(x) != n for x in (self._m, self._v, self._m_scale, self._v_scale)):
+            raise ShapeError(ERR_SHAPE, "one tensor of each kind for every parameter")
+        blocks = [(count + 63) // 64 for count in self._counts]
+        self._moments = tuple(zip(self._places(self._m, "m", kept, self._counts), self._places(self._v, "v", kept, self._counts),
+                                  self._places(self._m_scale, "m_scale", torch.uint8, blocks),
+                                  self._places(self._v_scale, "v_scale", torch.uint8, blocks)))
+        self._kept = [t.detach() for t in self._m + self._v + self._m_scale + self._v_scale if t is not None]
         self._fill()
 
     bits, m, v = property(lambda self: self._bits), property(lambda self: self._m), property(lambda self: self._v)
@@ -882,34 +889,34 @@ class AdamW:
         except TypeError:
             return None
 
+    def _places(self, tensors, what, dtype, counts):
+        """The tensors' addresses, their sizes, types and places checked."""
+        for t, count in zip(tensors, counts):
+            if t is None:
+                continue
+            if t.numel() != count:
+                raise ShapeError(ERR_SHAPE, f"{what} has {t.numel()} elements, not {count}")
+            if t.dtype != dtype or t.get_device() != self._device or not t.is_contiguous():
+                _on(t, self._device, dtype, tuple(t.shape), what)
+        return [None if t is None else t.data_ptr() for t in tensors]
+
     def _fill(self):
-        """The call's table of tensors, checked."""
+        """The call's table of tensors."""
         torch = _torch or _load_torch()
         n = len(self._counts)
-        outs = [None] * n if self.copies is None else self.copies
-        lists = (self.params, self.grads, self._m, self._v, self._m_scale, self._v_scale, outs)
-        if any(len(x) != n for x in lists):
+        copies = [None] * n if self.copies is None else self.copies
+        if any(len(x) != n for x in (self.params, self.grads, copies)):
             raise ShapeError(ERR_SHAPE, "one tensor of each kind for every parameter")
         if any(t is None for t in (*self.params, *self.grads)):
             raise NnhError(ERR_INVALID, "a parameter without a gradient")
         if self._types is None:
             self._types = (_type(self.params[0]), _type(self.grads[0])) if n else (F32, F32)
-        kept = torch.uint8 if self._bits == 8 else torch.float32
         p_type, g_type = ((torch.float32, torch.bfloat16)[t] for t in self._types)
-        tensors = (AdamWTensor * max(1, n))()
-        for i, row in enumerate(zip(*lists)):
-            count = self._counts[i]
-            for t, what, dtype, size in zip(row, ("a parameter", "a gradient", "m", "v", "m_scale", "v_scale", "a copy"),
-                                            (p_type, g_type, kept, kept, torch.uint8, torch.uint8, torch.bfloat16),
-                                            (count, count, count, count, (count + 63) // 64, (count + 63) // 64, count)):
-                if t is None:
-                    continue
-                if t.numel() != size:
-                    raise ShapeError(ERR_SHAPE, f"{what} has {t.numel()} elements, not {size}")
-                _on(t, self._device, dtype, tuple(t.shape), what)
-            tensors[i] = AdamWTensor(*(None if t is None else t.data_ptr() for t in row), count)
+        rows = zip(self._places(self.params, "a parameter", p_type, self._counts), self._places(self.grads, "a gradient", g_type, self._counts),
+                   self._moments, self._places(copies, "a copy", torch.bfloat16, self._counts), self._counts)
+        tensors = (AdamWTensor * max(1, n))(*(AdamWTensor(p, g, *moments, copy, count) for p, g, moments, copy, count in rows))
         self._tensors, self._known = tensors, self._where()
-        self._held = [t.detach() for x in lists for t in x if t is not None]
+        self._held = [t.detach() for t in (*self.params, *self.grads, *copies) if t is not None]
 
     def step(self, grad_scale=None, lr_device=None, step_device=None, stream=None):
         """One step; grad_scale and lr_device: one-element fp32 tensors, step_device: an int32 one that holds this step's number

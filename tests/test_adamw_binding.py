@@ -139,6 +139,6 @@ def test_the_moments_memory_is_held(calls):
     for name in ("m", "v", "m_scale", "v_scale"):
         t = getattr(opt, name)[1]
         t.data = torch.zeros_like(t)
-        assert row[name] != t.data_ptr() and row[name] in [x.data_ptr() for x in opt._held]
+        assert row[name] != t.data_ptr() and row[name] in [x.data_ptr() for x in opt._kept]
     opt.step()
     assert calls[-1][1][1] == row
