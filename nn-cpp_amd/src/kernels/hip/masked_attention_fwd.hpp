@@ -364,11 +364,12 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void mask
 }
 
 // The split form, for few query rows: the G heads of a key head and the Tq queries together are the columns (32 to a
-// workgroup), and the keys are divided over the grid and over a workgroup's waves, each with a ring of tiles of its own.
+// workgroup), and the keys are divided over the grid and over a workgroup's waves, each with a ring of tiles of its own: of four
+// where LDS holds them, two for rows of 256 bytes, and one, with no load ahead of its use, for fp32 heads of more than 64.
 template <typename T, int DH>
 struct SplitShape {
 	static constexpr int KT = 32, RB = row_bytes<T, DH>(), kTile = KT * RB, kStage = 2 * kTile;
-	static constexpr int NW = kStage * 4 <= 128 * 1024 ? 4 : 2;
+	static constexpr int NW = 4;
 	static constexpr int ST = kStage * NW * 4 <= 128 * 1024 ? 4 : kStage * NW * 2 <= 128 * 1024 ? 2 : 1;
 	static constexpr int kLoads = 2 * kTile / 1024;  // a wave's load instructions for a stage
 	static constexpr int kMerge = NW * 32 * (DH + 4) * 4;
