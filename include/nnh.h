@@ -559,7 +559,8 @@ int nnh_adamw_step(const nnh_adamw* options, const nnh_adamw_tensor* tensors, si
  * Softmax cross entropy of a linear head: z = x w^T + bias, lse = log sum exp z over the vocabulary, loss = lse - z[target],
  * for x {rows, D}, w {V, D}, bias {V} or NULL (all of one type, contiguous) and targets {rows} (int32, device memory). A
  * negative target means none: loss 0, no gradient, not counted by the mean. A target of V or more gives a NaN loss and no
- * gradient. The scores are made in pieces of the vocabulary and not kept; loss {rows} or {1} and lse {rows} are fp32.
+ * gradient. The scores are made in pieces of the vocabulary and not kept (the one call below keeps them); loss {rows} or {1}
+ * and lse {rows} are fp32.
  * bf16 rows of a length that is no multiple of 8, or not 16-byte aligned, are first copied to scratch.
  */
 int nnh_linear_cross_entropy_forward(int type, const void* x, size_t rows, size_t D, const void* w, size_t V, const void* bias,
@@ -571,8 +572,11 @@ int nnh_linear_cross_entropy_backward(int type, const float* g, const void* x, s
                                       const void* bias, const int* targets, const float* lse, int reduction, void* dx, int dx_first,
                                       void* dw, int dw_first, void* db, int db_first, void* stream);
 
-/* Both in one call, for a g known beforehand: the scores are made once where rows * V elements take at most 4 GiB, which
- * they then do in scratch for the length of the call. */
+/* Both in one call, for a g known beforehand: the scores are made once where rows * V elements take at most 4 GiB of scratch. In
+ * bf16 it keeps them rounded, so that a probability in the scores' gradient (rounded to bf16 in either call, an operand of its
+ * products) has two roundings here and one in the backward call or past 4 GiB. The library's own scratch keeps its size until the
+ * process ends; a registered buffer that does not hold the scores is refused, and the forward and the backward call, which take
+ * pieces of 1 GiB (of 256 words where rows are so many that these take more), need less. */
 int nnh_linear_cross_entropy_train(int type, const float* g, const void* x, size_t rows, size_t D, const void* w, size_t V,
                                    const void* bias, const int* targets, int reduction, float* loss, void* dx, int dx_first, void* dw,
                                    int dw_first, void* db, int db_first, void* stream);

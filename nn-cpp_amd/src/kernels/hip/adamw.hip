@@ -14,7 +14,7 @@
 // An infinite or NaN moment becomes e4m3's NaN and leaves its block's scale to the others.
 //
 // Measured: 8-bit moments of 16-bit gradients and 32-bit parameters with a bf16 copy, 6.5 GB a step, 1548 us (4.2 TB/s; a
-// large copy reaches 4.7). A step of 0.1 million parameters is one launch, 8 us with its call.
+// large copy reaches 4.7). A step of 0.1 million parameters is one launch of 7 us, 11 us a step from Python.
 #include "adamw.hpp"
 
 #include <cmath>

@@ -4,6 +4,14 @@
 // product's kernel), the backward makes a piece again, turns it into its gradient in scratch and takes the piece's part of dx
 // and all of its dw and db from that, four products in all. The two in one call (train) make the scores once where all of
 // them fit kKeep bytes of scratch, three products: bf16 keeps exp(z - its chunk's maximum), fp32 the scores.
+//
+// bf16's dz is rounded to bf16, the products' operand type (their sums and the common factor are fp32); train rounds what it keeps
+// too, so that a probability in dz has two roundings there where backward gives it one. The target's element is made from its own
+// score, not from what was kept: near a probability of 1 its difference from 1 is all of it. Against 64 bits the gradients of 4096 rows
+// and 50257 words are off by 0.0017 of their norm, as fp32 products rounded once are.
+//
+// Scratch: a piece takes kPiece bytes, or 256 words' scores where these are more (from 2^20 rows on in fp32, 2^21 in bf16: rows are
+// not cut); fp32 gradients add a copy of x, bf16 ones of several pieces a sum of dx.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
