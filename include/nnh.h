@@ -584,6 +584,45 @@ int nnh_linear_cross_entropy_train(int type, const float* g, const void* x, size
 /* Scratch of a call: 0 forward, 1 backward, 2 train; aligned: whether bf16 x and w are 16-byte aligned. */
 int nnh_linear_cross_entropy_workspace_size(int type, size_t rows, size_t D, size_t V, int call, int aligned, size_t* bytes);
 
+/*
+ * Serving: keys and values of many sequences in pages of one pool, a step over new tokens of some of them.
+ *
+ * Where tokens are kept: token j of sequence n is in slot j % page_size of page table[n * width + j / page_size], and element
+ * (page, slot, head h, d) of the keys is k[page * page + slot * slot + h * head + d], of the values the same place of v. Strides are in
+ * elements and any are taken; pages whose rows begin at multiples of 16 bytes and are as long are faster. Keys and values may lie side
+ * by side in one buffer. A page number that is negative or not below `pages` is no page: what would be there is not stored, and not seen.
+ */
+typedef struct nnh_paged_cache {
+	void *k, *v;
+	size_t page, slot, head;
+	size_t pages, page_size;
+	const int* table; /* {N, width}, device memory */
+	size_t width;
+} nnh_paged_cache;
+
+/*
+ * Stores the new tokens of N sequences: rows starts[n] .. starts[n + 1] - 1 of k and v {rows, Hkv, Dh} (`sample` is not used) are the
+ * last of the lens[n] tokens that sequence n has with them. starts {N + 1}, rising, and lens {N} are int32 in device memory. Rows behind
+ * starts[N], and tokens past the table or in no page, are stored nowhere. Two rows of one call must not have one place (which of them
+ * is then kept is not defined).
+ */
+int nnh_paged_append(int type, size_t N, size_t rows, size_t Hkv, size_t Dh, const nnh_head_tensor* k, const nnh_head_tensor* v,
+                     const int* starts, const int* lens, const nnh_paged_cache* cache, void* stream);
+
+/*
+ * Attention of the new tokens of N sequences over their pages: row starts[n] + i of q {rows, H, Dh} is at position k_lens[n] -
+ * (starts[n + 1] - starts[n]) + i of sequence n and sees its k_lens[n] tokens as the rule says (nnh_attention_rule, whose k_lens is
+ * needed here; q_start and documents are refused). Dh <= 128. out {rows, H, Dh} and lse {rows, H} (log(sum exp z)) are stored for those
+ * rows, zeros and -infinity where a row sees nothing; rows behind starts[N] are left as they are. most: at least the rows of any one
+ * sequence (of one with more, only the first `most` are done).
+ * A sequence of at most 64 rows times H / Hkv has its keys divided over the GPU, the others too where they are few.
+ * Scratch: nnh_paged_attention_workspace_size (keys: width * page_size).
+ */
+int nnh_paged_attention(int type, size_t N, size_t rows, size_t most, size_t H, size_t Hkv, size_t Dh, const nnh_head_tensor* q,
+                        const nnh_paged_cache* cache, const int* starts, const nnh_attention_rule* rule, const nnh_head_tensor* out,
+                        float* lse, void* stream);
+int nnh_paged_attention_workspace_size(size_t N, size_t rows, size_t most, size_t keys, size_t H, size_t Hkv, size_t Dh, size_t* bytes);
+
 #ifdef __cplusplus
 }
 #endif

@@ -135,6 +135,9 @@ _EXTRA_DECLS = {
     "nnh_linear_cross_entropy_train": [C.c_int, _vp, _vp, _sz, _sz, _vp, _sz, _vp, _vp, C.c_int, _vp, _vp, C.c_int, _vp,
                                        C.c_int, _vp, C.c_int, _vp],
     "nnh_linear_cross_entropy_workspace_size": [C.c_int, _sz, _sz, _sz, C.c_int, C.c_int, _szp],
+    "nnh_paged_append": [C.c_int] + [_sz] * 4 + [_vp] * 6,
+    "nnh_paged_attention": [C.c_int] + [_sz] * 6 + [_vp] * 7,
+    "nnh_paged_attention_workspace_size": [_sz] * 7 + [_szp],
     "nnh_set_stream_numerics": [_vp, C.c_int],
     "nnh_get_stream_numerics": [_vp],
 }
@@ -935,6 +938,80 @@ class AdamW:
                    *(None if t is None else t.data_ptr() for t in (step_device, lr_device, grad_scale)))
         check(lib().nnh_adamw_step(C.byref(o), self._tensors, len(self._counts), _stream(stream)))
         self.steps += 1
+
+
+class _Cache(C.Structure):
+    _fields_ = [("k", _vp), ("v", _vp), ("page", _sz), ("slot", _sz), ("head", _sz), ("pages", _sz), ("page_size", _sz), ("table", _vp),
+                ("width", _sz)]
+
+
+class PagedCache:
+    """Keys and values of many sequences in pages (nnh_paged_cache in nnh.h): k and v {pages, page_size, Hkv, Dh} of one type and
+    the same strides (the elements of a head consecutive), table {N, width} int32: the pages of each sequence in order, a negative number
+    for none. All three are the caller's and may be given other tensors between calls."""
+
+    def __init__(self, k, v, table):
+        self.k, self.v, self.table = k, v, table
+
+    def _struct(self, device):
+        torch = _torch or _load_torch()
+        k, v, table = self.k, self.v, self.table
+        if k.dim() != 4 or k.shape != v.shape or table.dim() != 2:
+            raise ShapeError(ERR_SHAPE, "k and v are {pages, page_size, Hkv, Dh}, the table {N, width}")
+        if k.dtype != v.dtype or k.stride() != v.stride() or (k.stride(3) != 1 and k.shape[3] > 1):
+            raise NnhError(ERR_INVALID, "k and v must have one type and the same strides, the elements of a head consecutive")
+        page, slot, head, _ = k.stride()
+        return _Cache(_on(k, device, what="k"), _on(v, device, what="v"), page, slot, head, k.shape[0], k.shape[1],
+                      _on(table, device, torch.int32, tuple(table.shape), "table"), table.shape[1])
+
+
+def _packed(t, cache, device, shape, what):
+    """Rows {rows, heads, Dh} of the cache's type in place."""
+    if t.dtype != cache.k.dtype:
+        raise NnhError(ERR_INVALID, f"{what} must be {cache.k.dtype}, not {t.dtype}")
+    if tuple(t.shape) != shape:
+        raise ShapeError(ERR_SHAPE, f"{what} must be {shape}, not {tuple(t.shape)}")
+    r, h, d = t.stride()
+    if d != 1 and shape[2] > 1:
+        raise NnhError(ERR_INVALID, f"{what}: the elements of a head must be consecutive")
+    return C.byref(HeadTensor(_on(t, device, what=what), 0, r, h))
+
+
+def paged_append(cache, k, v, starts, lens, stream=None):
+    """nnh_paged_append: rows starts[n] .. starts[n + 1] - 1 of k and v {rows, Hkv, Dh} become the last of sequence n's lens[n] tokens;
+    starts {N + 1} and lens {N} are int32."""
+    torch = _torch or _load_torch()
+    device = torch.cuda.current_device()
+    N, (_, _, Hkv, Dh) = cache.table.shape[0], cache.k.shape
+    if k.dim() != 3:
+        raise ShapeError(ERR_SHAPE, "k and v are {rows, Hkv, Dh}")
+    c, shape = cache._struct(device), (k.shape[0], Hkv, Dh)
+    check(lib().nnh_paged_append(_type(cache.k), N, k.shape[0], Hkv, Dh, _packed(k, cache, device, shape, "k"),
+                                 _packed(v, cache, device, shape, "v"), _on(starts, device, torch.int32, (N + 1,), "starts"),
+                                 _on(lens, device, torch.int32, (N,), "lens"), C.byref(c), _stream(stream)))
+
+
+def paged_attention(q, cache, starts, most, rule, out=None, lse=None, stream=None):
+    """nnh_paged_attention on packed rows q {rows, H, Dh} (starts {N + 1} int32 on the device, no sequence having more than `most` of
+    them); the rule's k_lens {N} are the tokens that each sequence has in the cache, the new ones included. Returns (out {rows, H, Dh},
+    lse {rows, H} in fp32); rows behind the last sequence are left as they are in tensors that are given, and are not set in others."""
+    torch = _torch or _load_torch()
+    device = torch.cuda.current_device()
+    N, (_, page_size, Hkv, Dh) = cache.table.shape[0], cache.k.shape
+    if q.dim() != 3:
+        raise ShapeError(ERR_SHAPE, "q is {rows, H, Dh}")
+    rows, H, _ = q.shape
+    if most < 0:
+        raise NnhError(ERR_INVALID, "most must not be negative")
+    if out is None:
+        out = torch.empty((rows, H, Dh), dtype=q.dtype, device=q.device)
+    if lse is None:
+        lse = torch.empty((rows, H), dtype=torch.float32, device=q.device)
+    c, r, shape = cache._struct(device), rule._struct(N, rows, cache.table.shape[1] * page_size, H, device), (rows, H, Dh)
+    check(lib().nnh_paged_attention(_type(cache.k), N, rows, most, H, Hkv, Dh, _packed(q, cache, device, shape, "q"), C.byref(c),
+                                    _on(starts, device, torch.int32, (N + 1,), "starts"), C.byref(r), _packed(out, cache, device, shape, "out"),
+                                    _on(lse, device, torch.float32, (rows, H), "lse"), _stream(stream)))
+    return out, lse
 
 
 _bench_lib = None
