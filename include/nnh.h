@@ -623,6 +623,40 @@ int nnh_paged_attention(int type, size_t N, size_t rows, size_t most, size_t H, 
                         float* lse, void* stream);
 int nnh_paged_attention_workspace_size(size_t N, size_t rows, size_t most, size_t keys, size_t H, size_t Hkv, size_t Dh, size_t* bytes);
 
+/*
+ * Rows in 8-bit integers: scale[r] = max |x[r]| / 127 in 32 bits and codes[r, d] the whole number nearest to x[r, d] / scale[r], ties to
+ * even (0 in a row of zeros). A row with an infinity or NaN has a scale of NaN and codes of 0. x {rows, D} has a pitch of ldx elements,
+ * codes one of ldc bytes; where it has room, codes are followed by zeros up to a multiple of 16.
+ */
+int nnh_quantize_rows(int type, const void* x, size_t rows, size_t D, size_t ldx, signed char* codes, size_t ldc, float* scale, void* stream);
+
+/*
+ * y = x W^T + bias for weights kept in 8 bits, W[v, d] = w[v * ldw + d] w_scale[v] (nnh_quantize_rows makes them): x's rows are quantised as
+ * above, products are summed in 32-bit integers, and each sum is multiplied by its row's and its column's scale and added to the bias.
+ * x {rows, D} and y {rows, V} (pitches ldx, ldy) and bias {V} or NULL are of one type. The weight's rows begin at multiples of 16 bytes;
+ * all V * ldw bytes are readable, and what lies behind a row's D codes does not matter. D <= 131071.
+ * Scratch: nnh_linear_int8_workspace_size.
+ */
+int nnh_linear_int8(int type, const void* x, size_t rows, size_t D, size_t ldx, const signed char* w, size_t ldw, const float* w_scale, size_t V,
+                    const void* bias, void* y, size_t ldy, void* stream);
+int nnh_linear_int8_workspace_size(size_t rows, size_t D, size_t V, size_t* bytes);
+
+/*
+ * A token of each row of logits {rows, V} (pitch ld): with the row's logits in descending order, equal ones by their index, and weights
+ * w = exp((z - max) / temperature),
+ *   min_p:  those with w >= min_p are kept, the largest always (off: 0)
+ *   top_k:  the first top_k of them (off: 0 or less)
+ *   top_p:  the shortest beginning of these whose weights sum to top_p of theirs or more, one at least (off: 1 or more)
+ * and the token is the first of what is kept whose sum of weights, its own with those ahead of it, is more than u times the sum of all.
+ * A temperature that is not above 0 takes the first of the largest logits. logprob (or NULL) is the logarithm of the token's share of
+ * what is kept, 0 without a temperature. NaN counts as -infinity, which is never taken: a row of nothing else has token -1 and logprob
+ * -infinity; among +infinities the weights are 1, all others 0. u is in [0, 1); temperature, top_k, top_p and min_p {rows} may be NULL (1
+ * and off). NaN in one of the last two turns it off. Sums are of whole numbers and exact: a weight is rounded to 2^-bits, bits 62 less
+ * the vocabulary's (45 for 128000 tokens, 51 at most).
+ */
+int nnh_sample(int type, const void* logits, size_t rows, size_t V, size_t ld, const float* u, const float* temperature, const int* top_k,
+               const float* top_p, const float* min_p, int* tokens, float* logprob, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -138,6 +138,10 @@ _EXTRA_DECLS = {
     "nnh_paged_append": [C.c_int] + [_sz] * 4 + [_vp] * 6,
     "nnh_paged_attention": [C.c_int] + [_sz] * 6 + [_vp] * 7,
     "nnh_paged_attention_workspace_size": [_sz] * 7 + [_szp],
+    "nnh_quantize_rows": [C.c_int, _vp, _sz, _sz, _sz, _vp, _sz, _vp, _vp],
+    "nnh_linear_int8": [C.c_int, _vp, _sz, _sz, _sz, _vp, _sz, _vp, _sz, _vp, _vp, _sz, _vp],
+    "nnh_linear_int8_workspace_size": [_sz] * 3 + [_szp],
+    "nnh_sample": [C.c_int, _vp, _sz, _sz, _sz] + [_vp] * 8,
     "nnh_set_stream_numerics": [_vp, C.c_int],
     "nnh_get_stream_numerics": [_vp],
 }
@@ -1012,6 +1016,82 @@ def paged_attention(q, cache, starts, most, rule, out=None, lse=None, stream=Non
                                     _on(starts, device, torch.int32, (N + 1,), "starts"), C.byref(r), _packed(out, cache, device, shape, "out"),
                                     _on(lse, device, torch.float32, (rows, H), "lse"), _stream(stream)))
     return out, lse
+
+
+def _matrix(t, device, dtype, shape, what):
+    """(address, pitch) of a matrix whose rows' elements are consecutive."""
+    if t.dim() != 2 or (shape is not None and tuple(t.shape) != shape):
+        raise ShapeError(ERR_SHAPE, f"{what} must be {shape or 'a matrix'}, not {tuple(t.shape)}")
+    rows, cols = t.shape
+    if t.stride(1) != 1 and cols > 1:
+        raise NnhError(ERR_INVALID, f"{what}: the elements of a row must be consecutive")
+    return _on(t, device, dtype, None, what), t.stride(0) if rows > 1 else max(cols, t.stride(0))
+
+
+def quantize_rows(x, codes=None, scale=None, stream=None):
+    """nnh_quantize_rows on x {rows, D} (fp32 or bf16); returns (codes {rows, D} int8, scale {rows} fp32). Codes that are made here have rows
+    that begin at multiples of 16 bytes, as linear_int8 needs its weight's."""
+    torch = _torch or _load_torch()
+    device = torch.cuda.current_device()
+    px, ldx = _matrix(x, device, None, None, "x")
+    rows, D = x.shape
+    if codes is None:
+        codes = torch.empty((rows, -(-D // 16) * 16), dtype=torch.int8, device=x.device)[:, :D]
+    if scale is None:
+        scale = torch.empty(rows, dtype=torch.float32, device=x.device)
+    pc, ldc = _matrix(codes, device, torch.int8, (rows, D), "codes")
+    check(lib().nnh_quantize_rows(_type(x), px, rows, D, ldx, pc, ldc, _on(scale, device, torch.float32, (rows,), "scale"), _stream(stream)))
+    return codes, scale
+
+
+def linear_int8(x, w, w_scale, bias=None, out=None, stream=None):
+    """nnh_linear_int8: x {..., D} (fp32 or bf16; a matrix may have a pitch, others are contiguous) times the transpose of the weight that w
+    {V, D} int8 (rows that begin at multiples of 16 bytes) and w_scale {V} stand for, plus bias {V}; returns {..., V} of x's type."""
+    torch = _torch or _load_torch()
+    device = torch.cuda.current_device()
+    if x.dim() < 1 or w.dim() != 2 or x.shape[-1] != w.shape[1]:
+        raise ShapeError(ERR_SHAPE, "x is {..., D} and w {V, D}")
+    V, D = w.shape
+    lead = tuple(x.shape[:-1])
+    if x.dim() != 2:
+        _on(x, device, None, lead + (D,), "x")
+        x = x.view(-1, D) if D else x.new_empty((_count(lead), 0))
+    if out is None:
+        out = torch.empty(lead + (V,), dtype=x.dtype, device=x.device)
+    if len(lead) != 1:
+        _on(out, device, x.dtype, lead + (V,), "out")
+    y = out if len(lead) == 1 else out.view(_count(lead), V)
+    rows = x.shape[0]
+    px, ldx = _matrix(x, device, None, None, "x")
+    pw, ldw = _matrix(w, device, torch.int8, None, "w")
+    py, ldy = _matrix(y, device, x.dtype, (rows, V), "out")
+    check(lib().nnh_linear_int8(_type(x), px, rows, D, ldx, pw, ldw, _on(w_scale, device, torch.float32, (V,), "w_scale"), V,
+                                _on(bias, device, x.dtype, (V,), "bias"), py, ldy, _stream(stream)))
+    return out
+
+
+def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, tokens=None, logprob=None, stream=None):
+    """nnh_sample: a token of each row of logits {rows, V} (fp32 or bf16) by random numbers u {rows} in [0, 1); temperature, top_p and min_p
+    {rows} in fp32, top_k {rows} in int32. Returns (tokens {rows} int32, logprob {rows} fp32)."""
+    torch = _torch or _load_torch()
+    device, f32 = torch.cuda.current_device(), torch.float32
+    p, ld = _matrix(logits, device, None, None, "logits")
+    rows, V = logits.shape
+    if tokens is None:
+        tokens = torch.empty(rows, dtype=torch.int32, device=logits.device)
+    if logprob is None:
+        logprob = torch.empty(rows, dtype=f32, device=logits.device)
+    given = [_on(t, device, dtype, (rows,), what) for t, dtype, what in ((u, f32, "u"), (temperature, f32, "temperature"), (top_k, torch.int32, "top_k"), (top_p, f32, "top_p"),
+                                                                         (min_p, f32, "min_p"), (tokens, torch.int32, "tokens"), (logprob, f32, "logprob"))]
+    check(lib().nnh_sample(_type(logits), p, rows, V, ld, *given, _stream(stream)))
+    return tokens, logprob
+
+
+def _count(shape):
+    n = 1
+    for d in shape:
+        n *= d
+    return n
 
 
 _bench_lib = None

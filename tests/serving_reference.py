@@ -2,6 +2,7 @@
 CPU, and random batches to run them on."""
 import math
 
+import numpy as np
 import torch
 
 from lm_reference import U32, masked_attention, unit
@@ -127,31 +128,30 @@ def linear_int8(x, w, w_scale, bias=None):
 
 def sample_row(z, u, temperature=1.0, top_k=None, top_p=None, min_p=None):
     """(token, log-probability) of one row of logits; ties in the order of the index."""
-    z = [float(x) for x in z.double()]
-    z = [-math.inf if math.isnan(x) else x for x in z]
-    top = max(z) if z else -math.inf
+    z = z.double().numpy()
+    z = np.where(np.isnan(z), -math.inf, z)
+    top = z.max()
     if top == -math.inf:
         return -1, -math.inf
-    order = sorted(range(len(z)), key=lambda i: (-z[i], i))
+    order = np.argsort(-z, kind="stable")
     if not temperature > 0:
-        return order[0], 0.0
-    far = [(0.0 if z[i] == top else math.inf) if top == math.inf else (top - z[i]) / temperature for i in order]
-    w = [math.exp(-d) for d in far]
+        return int(order[0]), 0.0
+    z = z[order]
+    if top == math.inf:
+        far = np.where(z == top, 0.0, math.inf)
+    else:
+        far = (top - z) / temperature
+    w = np.exp(-far)
     keep = len(w)
     if min_p is not None and min_p > 0:
-        keep = max(1, sum(x >= min_p for x in w))
+        keep = max(1, int((w >= min_p).sum()))
     if top_k is not None and top_k > 0:
         keep = min(keep, top_k)
+    total = w[:keep].cumsum()
     if top_p is not None and top_p < 1:
-        total, before, n = math.fsum(w[:keep]), 0.0, 0
-        while n < keep and (n == 0 or before < top_p * total):
-            before, n = before + w[n], n + 1
-        keep = n
-    total, sofar = math.fsum(w[:keep]), 0.0
-    for n in range(keep):
-        sofar += w[n]
-        if sofar > u * total:
-            break
+        keep = max(1, int((total - w[:keep] < top_p * total[-1]).sum()))
+    total = total[:keep]
+    n = min(int((total <= u * total[-1]).sum()), keep - 1)
     while w[n] == 0.0:
         n -= 1
-    return order[n], -far[n] - math.log(total)
+    return int(order[n]), float(-far[n] - math.log(total[-1]))
