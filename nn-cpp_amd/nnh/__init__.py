@@ -142,6 +142,7 @@ _EXTRA_DECLS = {
     "nnh_linear_int8": [C.c_int, _vp, _sz, _sz, _sz, _vp, _sz, _vp, _sz, _vp, _vp, _sz, _vp],
     "nnh_linear_int8_workspace_size": [_sz] * 3 + [_szp],
     "nnh_sample": [C.c_int, _vp, _sz, _sz, _sz] + [_vp] * 8,
+    "nnh_sample_workspace_size": [C.c_int, _sz, _sz, _szp],
     "nnh_set_stream_numerics": [_vp, C.c_int],
     "nnh_get_stream_numerics": [_vp],
 }

@@ -19,7 +19,12 @@ struct SampleArgs {
 	const float *top_p, *min_p;
 	int* tokens;
 	float* logprob;
+	int slices;     // workgroups that share a row's first passes, or 0
+	void* scratch;  // theirs
 };
+
+// Scratch of a call, and its slices.
+size_t sample_scratch(int64_t rows, int64_t V, int type, int& slices);
 
 hipError_t sample(const SampleArgs& a, int type, hipStream_t s);
 

@@ -5,6 +5,7 @@
 
 #include "abi_common.hpp"
 #include "kernels/hip/sample.hpp"
+#include "scratch.hpp"
 #include "nnh.h"
 
 using namespace nnh;
@@ -43,8 +44,21 @@ int nnh_sample(int type, const void* logits, size_t rows, size_t V, size_t ld, c
 		if (logprob && ranges_overlap(tokens, rows * 4, logprob, rows * 4)) return refuse(NNH_ERR_ALIAS, "the two outputs overlap");
 		int bits = 62;
 		while (((uint64_t)1 << (62 - bits)) < V) --bits;
-		const SampleArgs a{logits, (int64_t)ld, (int64_t)rows, (int)V, std::min(bits, 51), u, temperature, top_k, top_p, min_p, tokens, logprob};
-		return hip_status(sample(a, type, reinterpret_cast<hipStream_t>(stream)), "sample");
+		SampleArgs a{logits, (int64_t)ld, (int64_t)rows, (int)V, std::min(bits, 51), u, temperature, top_k, top_p, min_p, tokens, logprob, 0, nullptr};
+		hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+		Scratch ws(s, sample_scratch((int64_t)rows, (int64_t)V, type, a.slices));
+		if (ws.status() != NNH_OK) return ws.status();
+		a.scratch = ws.at<void>(0);
+		return hip_status(sample(a, type, s), "sample");
+	});
+}
+
+int nnh_sample_workspace_size(int type, size_t rows, size_t V, size_t* bytes) {
+	return guarded([&] {
+		if (type != NNH_F32 && type != NNH_BF16) return refuse(NNH_ERR_INVALID, "no such element type");
+		if (rows > kMaxRows || V > kMaxVocabulary) return refuse(NNH_ERR_INVALID, "size out of range");
+		int slices = 0;
+		return put_bytes(bytes, sample_scratch((int64_t)rows, (int64_t)V, type, slices));
 	});
 }
 

@@ -139,6 +139,19 @@ def test_pitch_and_alignment(gpu, dtype, V):
         check(z, uniform(2, 6), got=run(room[:, :V], uniform(2, 6), **o), **o)
 
 
+@pytest.mark.parametrize("wide", [3.0, 0.05, 1e-3, 300.0])
+@pytest.mark.parametrize("name", ["none", "kp", "all"])
+def test_values_that_are_counted(gpu, wide, name):
+    """16-bit logits of few values and of magnitudes below 2^-8 and above 2^8, whose weights are found in another way."""
+    z = draw(8, 6, 30000, dtype=torch.bfloat16, scale=wide)
+    z[1] = z[1].round()
+    z[2, ::3] = -z[2, ::3].abs()
+    z[3, 5::7] = 0.0
+    z[4, ::2] = -math.inf
+    t = torch.tensor([1.0, 0.5, 1.0, wide, 1.0, 100.0]) * max(1.0, wide / 3)
+    check(z, uniform(9, 6), temperature=t, **options(name, 6))
+
+
 def test_frequencies(gpu):
     """Every token comes up for the share of u that is its own."""
     V, n = 6, 1 << 12
@@ -151,20 +164,34 @@ def test_frequencies(gpu):
     assert (logprob.cpu().double() - torch.log(p)[tokens.cpu().long()]).abs().max() < 1e-6
 
 
-def test_captured_and_on_two_streams(gpu):
+@pytest.mark.parametrize("rows,V", [(20, 40000), (3, 500), (300, 9000)])
+def test_captured_and_on_two_streams(gpu, rows, V):
+    """Large vocabularies need scratch: captured with exactly the size asked for, refused without."""
     import nnh
-    z = [draw(i, 20, 40000, dtype=torch.bfloat16).cuda() for i in range(2)]
-    u, k = uniform(1, 20).cuda(), torch.full((20,), 2000, dtype=torch.int32, device="cuda")
+    z = [draw(i, rows, V, dtype=torch.bfloat16).cuda() for i in range(2)]
+    u, k = uniform(1, rows).cuda(), torch.full((rows,), min(V, 2000), dtype=torch.int32, device="cuda")
+    size = nnh.workspace_size("sample", nnh.BF16, rows, V)
+    assert (size > 0) == (V > 8192)
+    room = torch.full((size + 4096,), 7, dtype=torch.uint8, device="cuda")
     side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
     torch.cuda.synchronize()
-    with torch.cuda.graph(graph, stream=side):
-        got = nnh.sample(z[0], u, top_k=k)
-    for seed in range(3):
-        z[0].copy_(draw(10 + seed, 20, 40000, dtype=torch.bfloat16))
-        want = nnh.sample(z[0], u, top_k=k)
-        graph.replay()
-        torch.cuda.synchronize()
-        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    if size:
+        with pytest.raises(nnh.NnhError, match="workspace"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=side):
+                nnh.sample(z[0], u, top_k=k)
+        nnh.set_workspace(room[:size], side)
+    try:
+        with torch.cuda.graph(graph, stream=side):
+            got = nnh.sample(z[0], u, top_k=k)
+        for seed in range(3):
+            z[0].copy_(draw(10 + seed, rows, V, dtype=torch.bfloat16))
+            want = nnh.sample(z[0], u, top_k=k)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+        assert bool((room[size:] == 7).all())
+    finally:
+        nnh.set_workspace(None, side)
     want = [nnh.sample(x, u, top_k=k) for x in z]
     streams = [torch.cuda.Stream() for _ in range(2)]
     torch.cuda.synchronize()
@@ -172,6 +199,18 @@ def test_captured_and_on_two_streams(gpu):
         outs = [nnh.sample(x, u, top_k=k, stream=s) for x, s in zip(z, streams)]
         torch.cuda.synchronize()
         assert all(torch.equal(a[0], b[0]) and torch.equal(a[1], b[1]) for a, b in zip(outs, want))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,V", [(130, 20001), (300, 20001), (1100, 8200)])
+def test_more_rows(gpu, dtype, rows, V):
+    """Rows that share the GPU in slices, two to a row, rows of one workgroup each, more of them than are done at a time."""
+    z = draw(4, rows, V, dtype=T[dtype], scale=3.0)
+    t = uniform(5, rows, 0.2, 1.2)
+    t[3] = 0
+    z[5] = -math.inf
+    check(z, uniform(6, rows), temperature=t)
+    check(z, uniform(7, rows), temperature=t, **options("all", rows))
 
 
 def test_rows_past_32_bits(gpu):
