@@ -20,13 +20,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs p) {
 	const int lane = threadIdx.x & 63;
 	const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
 	if (row >= p.s.rows) return;
-	// the sequence that has the row, by its bounds in order
-	int lo = 0, hi = p.s.N;
-	while (lo < hi) {
-		const int mid = (lo + hi) / 2;
-		if (p.s.starts[mid + 1] <= row) lo = mid + 1;
-		else hi = mid;
-	}
+	const int lo = sequence_with(p.s, row, lane);
 	if (lo == p.s.N || row < p.s.starts[lo]) return;
 	const int64_t at = (int64_t)p.s.lens[lo] - p.s.starts[lo + 1] + row;
 	if (at < 0 || at >= (int64_t)p.t.width * p.t.size.d) return;
@@ -59,18 +53,26 @@ hipError_t append_of(const PagedAppendArgs& p, bool vec, hipStream_t s) {
 
 }  // namespace
 
-// Columns: a sequence of at most 64 takes the split form, whose waves share the keys, not the columns. The parts are as many as
-// bring 512 workgroups together, with 256 keys to each at least; the rows that a form has are not known here, so they are taken
-// to be the most that may be.
-PagedPlan paged_attention_plan(int N, int rows, int most, int keys, int H, int Hkv) {
-	constexpr int kFew = 64;
-	PagedPlan p{kFew, 0, 0};
+// Columns: a sequence of at most 64 takes the split form, whose waves share the keys, not the columns. The keys are divided so that
+// three workgroups a CU come together, two in the other form, or up to four times as many (rounds_of), 256 keys to each at least; where
+// the rows alone bring enough, or a sequence has fewer than 512 keys, they are not. (768 for 512 wanted: mixed lengths around 3000, 12 heads of
+// 80, 98 -> 89 us; 1024: 86, but 128 sequences of 1000 keys 89 -> 106.) A sequence has one group at least, and one part of each group.
+PagedPlan paged_attention_plan(int64_t N, int64_t rows, int64_t most, int64_t keys, int H, int Hkv, int Dh) {
+	constexpr int kFew = 64, kSplitWanted = 768, kWideWanted = 512;
+	PagedPlan p{kFew, {false, 5, 5, 0, 0, 0, nullptr}, {true, 7, 6, 0, 0, 0, nullptr}, 0, 0};
 	if (N == 0 || rows == 0 || most == 0) return p;
-	const int64_t G = H / Hkv, columns = (int64_t)most * G;
-	const auto parts = [&](int64_t groups) { return (int)std::max<int64_t>(1, std::min<int64_t>((512 + groups - 1) / groups, keys / 256)); };
-	if (columns <= kFew || N > 1) p.splits = parts((std::min<int64_t>(columns, kFew) + 31) / 32 * N * Hkv);
-	if (columns > kFew) p.wide_splits = parts(((int64_t)rows * G + 127) / 128 * Hkv);
-	if (!p.splits) p.few = 0;
+	const int64_t G = H / Hkv, columns = std::min(most, rows) * G;
+	const auto divide = [&](Form& f, int64_t groups, bool enough, int wanted, size_t& floats) {
+		if (!enough && keys >= 512) f.target = (wanted + Hkv - 1) / Hkv;
+		const int64_t tiles = groups * ((keys + 31) / 32);
+		f.pairs = (int)(groups + (f.target ? std::min<int64_t>(f.target * rounds_of(tiles, f.target), tiles / (kLeastKeys / 32) + 1) : 0));
+		f.room = (int)std::min<int64_t>(1 << f.width, columns);
+		floats = f.target ? (size_t)Hkv * f.pairs * f.room * (Dh + 2) : 0;
+	};
+	const bool split = columns <= kFew || N > 1;
+	if (split) divide(p.split, std::min(2 * N, N + rows * G / 32), N * Hkv >= 8 * kSplitWanted, kSplitWanted, p.split_floats);
+	else p.few = 0;
+	if (columns > kFew) divide(p.wide, N + rows * G / 128, rows * G / 128 * Hkv >= kWideWanted, kWideWanted, p.wide_floats);
 	return p;
 }
 

@@ -22,6 +22,15 @@ struct PackedRows {
 	int N, rows;
 };
 
+// The sequence that has a row (N: none), by a wave that looks at 64 bounds at a time.
+__device__ __forceinline__ int sequence_with(const PackedRows& s, int64_t row, int lane) {
+	for (int n0 = 0; n0 < s.N; n0 += 64) {
+		const uint64_t behind = __ballot(n0 + lane < s.N && s.starts[n0 + lane + 1] <= row);
+		if (behind != ~0ull) return n0 + __builtin_ctzll(~behind);
+	}
+	return s.N;
+}
+
 struct PagedAppendArgs {
 	const void *k, *v;
 	HeadStrides ks, vs;  // (sample: unused)
@@ -31,22 +40,41 @@ struct PagedAppendArgs {
 	int Hkv, dh;
 };
 
-struct PagedAttentionArgs {
-	MaskedAttentionArgs a;  // q, k and v (the pages), out, the rule; Tk: the most tokens that a sequence may have
-	PageTable t;
-	PackedRows s;
-	int most;         // rows of a sequence, at most
-	int few;          // sequences of so many columns (rows times the heads of a key head) or fewer take the split form
-	int splits, wide_splits;  // parts that the keys of a sequence are divided into: in the split form, in the other one
-	float* lse;       // {rows, H}
-	float* partial;   // {parts, rows, H}: maximum, sum and dh sums of p v each
+// One of the two forms: columns in groups of 2^width, keys in tiles of 2^shift.
+struct Form {
+	bool wide;
+	int width, shift;
+	int target;      // pairs of a group and a part of the keys that are wanted, to a key head; 0: the keys are not divided
+	int pairs;       // and at most so many there will be; 0: the form has no sequence to take
+	int room;        // columns of a group, at most
+	float* partial;  // {Hkv, pairs, room}: maximum, sum and dh sums of p v each
 };
 
-// How a call is divided, from what the host knows of it.
-struct PagedPlan {
-	int few, splits, wide_splits;  // splits or wide_splits 0: that form has no sequence to take
+struct PagedAttentionArgs {
+	MaskedAttentionArgs a;  // q, k and v (the pages), out, the rule
+	PageTable t;
+	PackedRows s;
+	int most;          // rows of a sequence, at most
+	int few;           // sequences of so many columns (rows times the heads of a key head) or fewer take the split form
+	Form split, wide;
+	float* lse;        // {rows, H}
 };
-PagedPlan paged_attention_plan(int N, int rows, int most, int keys, int H, int Hkv);
+
+// A pair's fixed cost is that of some ten tiles of the split form, and more pairs share the work more evenly: up to four rounds over
+// the GPU, where each pair has 48 tiles.
+__host__ __device__ inline int rounds_of(int64_t tiles, int target) {
+	const int64_t rounds = tiles / ((int64_t)target * 48);
+	return rounds < 1 ? 1 : rounds > 4 ? 4 : (int)rounds;
+}
+constexpr int kLeastKeys = 256;  // of a part
+
+// How a call is divided, from what the host knows of it, and the floats of the forms' `partial`.
+struct PagedPlan {
+	int few;
+	Form split, wide;
+	size_t split_floats, wide_floats;
+};
+PagedPlan paged_attention_plan(int64_t N, int64_t rows, int64_t most, int64_t keys, int H, int Hkv, int Dh);
 
 hipError_t paged_append(const PagedAppendArgs& p, int type, bool vec, hipStream_t s);
 hipError_t paged_attention(const PagedAttentionArgs& p, int type, bool vec, hipStream_t s);

@@ -32,28 +32,95 @@ __device__ __forceinline__ Sequence sequence_of(const PackedRows& s, const PageT
 	return q;
 }
 
-// Keys that the rows of a sequence from position `first` to `last` may see: tiles of KT keys, numbered in one go over those of the
-// prefix and those of the causal or window range.
-template <int KT>
+// Keys that the rows of a sequence from position `first` to `last` may see: tiles of 2^shift keys, numbered in one go over those of
+// the prefix and those of the causal or window range.
 struct Tiles {
-	int lo, hi, pre;    // keys lo .. hi - 1 and those below pre
 	int prefix, skip, count;  // tiles of the prefix; tiles left out behind them; tiles in all
-	__device__ __forceinline__ Tiles(const MaskedAttentionArgs& a, int n, int64_t first, int64_t last, int live) {
-		lo = 0;
-		hi = live;
-		pre = a.prefix ? clamped(a.prefix[n], 0, live) : 0;
+	__device__ __forceinline__ Tiles(const MaskedAttentionArgs& a, int n, int64_t first, int64_t last, int live, int shift) {
+		int lo = 0, hi = live;
+		const int pre = a.prefix ? clamped(a.prefix[n], 0, live) : 0, up = (1 << shift) - 1;
 		if (a.causal) hi = clamped(last + 1, 0, live);
 		if (a.window) {
 			lo = clamped(first - a.window + 1, 0, live);
 			hi = min(hi, clamped(last + a.window, 0, live));
 		}
-		prefix = (pre + KT - 1) / KT;
-		const int from = max(lo / KT, prefix), to = max((hi + KT - 1) / KT, from);
+		prefix = (pre + up) >> shift;
+		const int from = max(lo >> shift, prefix), to = max((hi + up) >> shift, from);
 		skip = from - prefix;
 		count = prefix + to - from;
 	}
 	__device__ __forceinline__ int at(int t) const { return t < prefix ? t : t + skip; }
 };
+
+// How the sequences that a form takes are divided: a sequence's columns in groups (of 2^width), the keys that its rows see in parts of
+// `chunk` tiles, as many as bring about `target` pairs of the two together over all sequences, whatever their lengths. A grid of
+// a few more workgroups than there are pairs has them in order; a workgroup finds its own, a wave looking at 64 sequences at a time.
+struct Share {
+	int groups, tiles;
+	Sequence s;
+};
+__device__ __forceinline__ Share share_of(const PagedAttentionArgs& p, const Form& f, int n) {
+	const Sequence s = sequence_of(p.s, p.t, n);
+	const int count = min(s.count, p.most), columns = count * p.a.G;
+	if (columns == 0 || (columns > p.few) != f.wide) return {0, 0, s};
+	return {(columns + (1 << f.width) - 1) >> f.width, Tiles(p.a, n, s.pos0, (int64_t)s.pos0 + count - 1, s.live, f.shift).count, s};
+}
+__device__ __forceinline__ int parts_of(const Share& x, int chunk) { return max(1, (int)(((int64_t)x.tiles + chunk / 2) / chunk)); }
+__device__ __forceinline__ int chunk_of(const PagedAttentionArgs& p, const Form& f) {
+	if (f.target == 0) return 1 << 30;
+	int64_t work = 0;
+	for (int n = threadIdx.x & 63; n < p.s.N; n += 64) {
+		const Share x = share_of(p, f, n);
+		work += (int64_t)x.groups * x.tiles;
+	}
+#pragma unroll
+	for (int d = 32; d; d >>= 1) work += __shfl_xor(work, d);
+	const int64_t target = f.target * (int64_t)rounds_of(work, f.target);
+	return max(kLeastKeys >> f.shift, (int)((work + target - 1) / target));
+}
+// Pair `index` of a group and a part, or sequence `of`'s first one; n < 0: there are not so many.
+struct Turn {
+	int n, group, part, parts;
+	int64_t first;
+	Sequence s;
+};
+__device__ __forceinline__ Turn turn_of(const PagedAttentionArgs& p, const Form& f, int index, int of) {
+	const int lane = threadIdx.x & 63, chunk = chunk_of(p, f);
+	int64_t ahead = 0;
+	for (int n0 = 0; n0 < p.s.N; n0 += 64) {
+		const int n = n0 + lane;
+		const Share x = n < p.s.N ? share_of(p, f, n) : Share{0, 0, {0, 0, 0, 0}};
+		const int parts = parts_of(x, chunk);
+		const int64_t own = (int64_t)x.groups * parts;
+		int64_t up = own;
+#pragma unroll
+		for (int d = 1; d < 64; d *= 2) {
+			const int64_t o = __shfl_up(up, d);
+			if (lane >= d) up += o;
+		}
+		const int64_t first = ahead + up - own;
+		const uint64_t hit = __ballot(of >= 0 ? n == of : index >= first && index < first + own);
+		if (hit) {
+			const int at = __builtin_ctzll(hit);
+			Turn t;
+			t.n = n0 + at;
+			t.first = __shfl(first, at);
+			t.parts = __builtin_amdgcn_readfirstlane(__shfl(parts, at));
+			const int in = __builtin_amdgcn_readfirstlane((int)(index - t.first));  // (sequence `of`'s: not used)
+			t.group = in / t.parts;
+			t.part = in % t.parts;
+			const auto own_of = [&](int v) { return __builtin_amdgcn_readfirstlane(__shfl(v, at)); };
+			t.s = {own_of(x.s.first), own_of(x.s.count), own_of(x.s.pos0), own_of(x.s.live)};
+			return t;
+		}
+		ahead += __shfl(up, 63);
+	}
+	return {-1, 0, 0, 1, 0, {0, 0, 0, 0}};
+}
+// Where a column of a pair leaves its maximum, sum and dh sums.
+__device__ __forceinline__ float* partial_of(const PagedAttentionArgs& p, const Form& f, int hk, int index, int column) {
+	return f.partial + (((int64_t)hk * f.pairs + index) * f.room + column) * (p.a.dh + 2);
+}
 
 // A tile's rows: lane l's is row l % KT.
 struct Places64 {
@@ -138,8 +205,8 @@ __device__ __forceinline__ void begin_column(Rows<T, DH>& r, const PagedAttentio
 	r.slope2 = a.slopes ? a.slopes[h] * kLog2e : 0.0f;
 }
 
-// A workgroup's 128 columns of one sequence and key head against the keys they see, or one part of `wide_splits` of these; the
-// tiles are read by all four waves. Values that are not finite in masked places: as in masked_attention_forward_kernel.
+// A workgroup's 128 columns of one sequence and key head against a part of the keys they see (mostly all); the tiles are read by all
+// four waves. Values that are not finite in masked places: as in masked_attention_forward_kernel.
 template <typename T, int DH, bool VEC>
 __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void paged_attention_kernel(PagedAttentionArgs p) {
 	constexpr int KT = keys_per_tile<T, DH>(), RB = row_bytes<T, DH>(), kTile = KT * RB;
@@ -148,32 +215,16 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void page
 	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 	int* const marks = (int*)(pages + 2 * 256 + wave * 2 * 256);  // the wave's own, of two tiles
 	const int col = lane & 31, half = lane >> 5;
-	// Tiles of one key head stay on one XCD where the pairs divide evenly (its L2 then holds the keys); those that see most come first.
-	const int pairs = p.s.N * p.a.Hkv, splits = p.wide_splits;
-	int tile, part, hk, n;
-	{
-		const unsigned block = blockIdx.x;
-		unsigned pair, rest;
-		if (pairs % 8 == 0) {
-			const unsigned per = pairs / 8, in = block / 8;
-			pair = block % 8 * per + in % per;
-			rest = in / per;
-		} else {
-			pair = block % pairs;
-			rest = block / pairs;
-		}
-		n = pair / p.a.Hkv;
-		hk = pair % p.a.Hkv;
-		part = rest % splits;
-		tile = rest / splits;
-	}
-	const Sequence s = sequence_of(p.s, p.t, n);
+	// (workgroups of one key head side by side on one XCD, where the heads are eight or divide by it: its L2 then holds the keys)
+	const int hk = blockIdx.x % p.a.Hkv, index = blockIdx.x / p.a.Hkv;
+	const Turn turn = turn_of(p, p.wide, index, -1);
+	const int n = turn.n;
+	if (n < 0) return;
+	const Sequence s = turn.s;
 	MaskedAttentionArgs a = p.a;
 	a.Tq = min(s.count, p.most);
-	const int columns = a.Tq * a.G, tiles = (columns + kQueries - 1) / kQueries;
-	if (columns <= p.few || tile >= tiles) return;
-	tile = tiles - 1 - tile;
-	const int c0 = tile * kQueries, c = c0 + wave * 32 + col;
+	// the columns that see most come first
+	const int columns = a.Tq * a.G, c0 = ((columns - 1) / kQueries - turn.group) * kQueries, c = c0 + wave * 32 + col;
 	const int i = c < columns ? c / a.G : a.Tq, h = hk * a.G + c % a.G;
 	const T* const kbase = (const T*)a.k + hk * p.t.head;
 	const T* const vbase = (const T*)a.v + hk * p.t.head;
@@ -185,8 +236,15 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void page
 #pragma unroll
 		for (int t = 0; t < DH / 16; ++t) row_from<T, VEC>(r.q[t], row, a.dh, half, t, i < a.Tq);
 	}
-	const Tiles<KT> seen(a, n, (int64_t)s.pos0 + c0 / a.G, (int64_t)s.pos0 + (min(c0 + kQueries, columns) - 1) / a.G, s.live);
-	const int begin = (int)((int64_t)seen.count * part / splits), end = (int)((int64_t)seen.count * (part + 1) / splits);
+	const Tiles seen(a, n, (int64_t)s.pos0 + c0 / a.G, (int64_t)s.pos0 + (min(c0 + kQueries, columns) - 1) / a.G, s.live, KT == 64 ? 6 : 5);
+	const int begin = (int)((int64_t)seen.count * turn.part / turn.parts), end = (int)((int64_t)seen.count * (turn.part + 1) / turn.parts);
+	// the page numbers of the first two tiles, on their way beside q
+	const auto first_numbers = [&] {
+		if (wave != 0 || begin >= end) return;
+		load_pages<KT>(p.t, n, seen.at(begin), s.live, lane, pages);
+		if (begin + 1 < end) load_pages<KT>(p.t, n, seen.at(begin + 1), s.live, lane, pages + 256);
+	};
+	first_numbers();
 	arrived(r.q);
 	arrived();
 
@@ -221,10 +279,7 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void page
 			take_keys<T, DH, KT, decltype(safe)::value>(r, a, at(), from, from + kTile, marks + B * 64, DocRange{0, 0, 1}, seen.at(t) * KT, lane);
 		};
 		if (begin < end) {
-			if (wave == 0) {
-				load_pages<KT>(p.t, n, seen.at(begin), s.live, lane, pages);
-				if (begin + 1 < end) load_pages<KT>(p.t, n, seen.at(begin + 1), s.live, lane, pages + 256);
-			}
+			if (decltype(safe)::value) first_numbers();
 			wait_loads();
 			__syncthreads();
 			load(begin, std::integral_constant<int, 0>{});
@@ -240,12 +295,12 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void page
 	const float l = add_halves(r.l);
 	if (i >= a.Tq) return;
 	const int64_t row = s.first + i;
-	if (splits == 1) {
+	if (turn.parts == 1) {
 		T* o = (T*)a.out + row * a.os.row + h * a.os.head;
 		store_column<T, DH, VEC>(o, (T*)nullptr, r.o, l == 0.0f ? 0.0f : 1.0f / l, a.dh, half);
 		if (half == 0) p.lse[row * a.H + h] = l == 0.0f ? -kInf : r.m * kLn2 + logf(l);
 	} else {
-		float* const to = p.partial + (((int64_t)part * p.s.rows + row) * a.H + h) * (a.dh + 2);
+		float* const to = partial_of(p, p.wide, hk, index, c - c0);
 #pragma unroll
 		for (int b = 0; b < DH / 32; ++b)
 #pragma unroll
@@ -262,29 +317,37 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void page
 
 // The split form, for sequences of few columns: 32 to a workgroup, the keys divided over the grid and over a workgroup's waves,
 // each with a ring of tiles and of page numbers of its own.
-template <typename T, int DH>
-struct PagedSplitShape : SplitShape<T, DH> {
-	using S = SplitShape<T, DH>;
-	static constexpr int kPages = 2 * S::ST * 256, kMarks = S::ST * 128;  // of a wave
-	static constexpr int kAll = S::kLds + S::NW * (kPages + kMarks) + S::NW * 4;
-	static_assert(kAll <= 160 * 1024 && (S::ST - 1) * (S::kLoads + 1) <= 63, "LDS, and loads that a wave may have outstanding");
+// Two waves and few tiles on their way, so that four workgroups share a CU (two where a row is 512 bytes or more) and some stream while
+// others begin or end: a workgroup's bounds, page numbers and first tiles are trips to memory one after another, 6 us of its time.
+// Four waves where all pairs run at once and are short.
+template <typename T, int DH, int NW_>
+struct PagedSplitShape {
+	static constexpr int KT = 32, RB = row_bytes<T, DH>(), kTile = KT * RB, kStage = 2 * kTile;
+	static constexpr int NW = NW_;
+	static constexpr int ST = RB <= 128 ? 2 : 1;
+	static constexpr int kLoads = 2 * kTile / 1024;  // a wave's load instructions for a stage
+	static constexpr int kMerge = NW * 32 * (DH + 4) * 4;
+	static constexpr int kLds = NW * ST * kStage > kMerge ? NW * ST * kStage : kMerge;
+	static constexpr int kPages = 2 * ST * 256, kMarks = ST * 128;  // of a wave
+	static constexpr int kAll = kLds + NW * (kPages + kMarks) + NW * 4;
+	static_assert(kAll <= (RB >= 512 ? 40 : 20) * NW * 1024 && (ST - 1) * (kLoads + 1) <= 63, "LDS of two workgroups a CU, and loads that a wave may have outstanding");
 };
 
-template <typename T, int DH, bool VEC>
-__global__ __launch_bounds__((64 * SplitShape<T, DH>::NW), 1) void paged_attention_split_kernel(PagedAttentionArgs p) {
-	using S = PagedSplitShape<T, DH>;
-	constexpr int KT = S::KT, NW = S::NW, ST = S::ST;
+template <typename T, int DH, bool VEC, int NW>
+__global__ __launch_bounds__(64 * NW, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void paged_attention_split_kernel(PagedAttentionArgs p) {
+	using S = PagedSplitShape<T, DH, NW>;
+	constexpr int KT = S::KT, ST = S::ST;
 	__shared__ __attribute__((aligned(1024))) char lds[S::kAll];
 	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 	const int col = lane & 31, half = lane >> 5;
-	const int pairs = p.s.N * p.a.Hkv;
-	const int split = blockIdx.x % p.splits, pair = blockIdx.x / p.splits % pairs, group = blockIdx.x / p.splits / pairs;
-	const int n = pair / p.a.Hkv, hk = pair % p.a.Hkv;
-	const Sequence s = sequence_of(p.s, p.t, n);
+	const int hk = blockIdx.x % p.a.Hkv, index = blockIdx.x / p.a.Hkv;
+	const Turn turn = turn_of(p, p.split, index, -1);
+	const int n = turn.n;
+	if (n < 0) return;
+	const Sequence s = turn.s;
 	MaskedAttentionArgs a = p.a;
 	a.Tq = min(s.count, p.most);
-	const int columns = a.Tq * a.G, c = group * 32 + col;
-	if (columns > p.few || group * 32 >= columns) return;
+	const int columns = a.Tq * a.G, c = turn.group * 32 + col;
 	const bool on_col = c < columns;
 	const int i = on_col ? c / a.G : a.Tq, h = hk * a.G + (on_col ? c % a.G : 0);
 	const T* const kbase = (const T*)a.k + hk * p.t.head;
@@ -297,31 +360,34 @@ __global__ __launch_bounds__((64 * SplitShape<T, DH>::NW), 1) void paged_attenti
 #pragma unroll
 		for (int t = 0; t < DH / 16; ++t) row_from<T, VEC>(r.q[t], row, a.dh, half, t, on_col);
 	}
-	// the keys that some row of the sequence may see, divided into splits * NW runs of whole tiles
-	const Tiles<KT> seen(a, n, s.pos0, (int64_t)s.pos0 + a.Tq - 1, s.live);
-	const int per = (seen.count + p.splits * NW - 1) / (p.splits * NW);
-	const int begin = min((split * NW + wave) * per, seen.count), end = min(begin + per, seen.count);
+	// the part's keys, divided over the waves in whole tiles
+	const Tiles seen(a, n, s.pos0, (int64_t)s.pos0 + a.Tq - 1, s.live, 5);
+	const int begin = (int)((int64_t)seen.count * (turn.part * NW + wave) / (turn.parts * NW)), end = (int)((int64_t)seen.count * (turn.part * NW + wave + 1) / (turn.parts * NW));
 	char* const ring = lds + wave * ST * S::kStage;
 	char* const pages = lds + S::kLds + wave * S::kPages;
 	int* const marks = (int*)(lds + S::kLds + NW * S::kPages + wave * S::kMarks);
+	// (numbers past the run's end are some tile's of the sequence: loaded for the count of loads alone)
+	const auto numbers = [&](int t) { load_pages<KT>(p.t, n, seen.at(min(t, seen.count - 1)), s.live, lane, pages + t % (2 * ST) * 256); };
+	// those of the first tiles, on their way beside q
+	const auto first_numbers = [&] {
+		if (begin < end)
+			for (int x = 0; x < ST; ++x) numbers(begin + x);
+	};
+	first_numbers();
 	arrived(r.q);
 	arrived();
 
 	auto run = [&](auto safe) {
 		r.clear();
 		unsigned bad = 0;  // bit: the stage's tile has rows without a page
-		// (numbers past the run's end are some tile's of the sequence: loaded for the count of loads alone)
-		auto numbers = [&](int t) { load_pages<KT>(p.t, n, seen.at(min(t, seen.count - 1)), s.live, lane, pages + t % (2 * ST) * 256); };
 		auto load = [&](int t, int stage) {
 			const Places64 x = places_of<KT>(p.t, seen.at(t), s.live, lane, pages + t % (2 * ST) * 256);
 			bad = (bad & ~(1u << stage)) | (mark_bad<KT>(x, marks + stage * KT, lane) ? 1u << stage : 0u);
 			char* to = ring + stage * S::kStage;
 			load_rows<T, DH, KT, 1, VEC>(to, to + S::kTile, kbase, vbase, x.at, a.dh, 0, lane);
 		};
-		if (begin < end) {
-			for (int x = 0; x < ST; ++x) numbers(begin + x);
-			wait_loads();
-		}
+		if (decltype(safe)::value) first_numbers();
+		wait_loads();
 #pragma unroll
 		for (int x = 0; x < ST - 1; ++x)
 			if (begin + x < end) {
@@ -366,8 +432,8 @@ __global__ __launch_bounds__((64 * SplitShape<T, DH>::NW), 1) void paged_attenti
 		}
 	}
 	__syncthreads();
-	for (int x = wave; x < 32 && group * 32 + x < columns; x += NW) {
-		const int cc = group * 32 + x, ii = cc / a.G, hh = hk * a.G + cc % a.G;
+	for (int x = wave; x < 32 && turn.group * 32 + x < columns; x += NW) {
+		const int cc = turn.group * 32 + x, ii = cc / a.G, hh = hk * a.G + cc % a.G;
 		float m = -kInf, l = 0.0f, f[NW];
 #pragma unroll
 		for (int w = 0; w < NW; ++w) m = fmaxf(m, part[(w * 32 + x) * (DH + 4) + DH]);
@@ -378,18 +444,18 @@ __global__ __launch_bounds__((64 * SplitShape<T, DH>::NW), 1) void paged_attenti
 			l += f[w] * part[(w * 32 + x) * (DH + 4) + DH + 1];
 		}
 		const int64_t row = s.first + ii;
-		float* const to = p.partial + (((int64_t)split * p.s.rows + row) * a.H + hh) * (a.dh + 2);
+		float* const to = partial_of(p, p.split, hk, index, x);
 		T* const o = (T*)a.out + row * a.os.row + hh * a.os.head;
 		const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 		for (int d = lane; d < a.dh; d += 64) {
 			float y = 0.0f;
 #pragma unroll
 			for (int w = 0; w < NW; ++w) y += f[w] * part[(w * 32 + x) * (DH + 4) + d];
-			if (p.splits == 1) o[d] = (T)(y * inv);
+			if (turn.parts == 1) o[d] = (T)(y * inv);
 			else to[2 + d] = y;
 		}
 		if (lane == 0) {
-			if (p.splits == 1) {
+			if (turn.parts == 1) {
 				p.lse[row * a.H + hh] = l == 0.0f ? -kInf : m * kLn2 + logf(l);
 			} else {
 				to[0] = m;
@@ -406,33 +472,50 @@ __global__ __launch_bounds__(256) void paged_attention_join_kernel(PagedAttentio
 	const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
 	if (at >= (int64_t)p.s.rows * p.a.H) return;
 	const int row = (int)(at / p.a.H), h = (int)(at % p.a.H);
-	// the sequence that has the row, by its bounds in order
-	int lo = 0, hi = p.s.N;
-	while (lo < hi) {
-		const int mid = (lo + hi) / 2;
-		if (p.s.starts[mid + 1] <= row) lo = mid + 1;
-		else hi = mid;
-	}
+	const int lo = sequence_with(p.s, row, lane);
 	if (lo == p.s.N) return;
 	const Sequence s = sequence_of(p.s, p.t, lo);
 	const int count = min(s.count, p.most);
 	if (row < s.first || row >= s.first + count) return;
-	const int splits = count * p.a.G <= p.few ? p.splits : p.wide_splits;
+	const Form& form = count * p.a.G > p.few ? p.wide : p.split;
+	const Turn turn = turn_of(p, form, 0, lo);
+	const int splits = turn.parts;
 	if (splits == 1) return;
-	const int64_t step = (int64_t)p.s.rows * p.a.H * (p.a.dh + 2);
-	const float* const from = p.partial + at * (p.a.dh + 2);
+	const int hk = h / p.a.G, column = (row - s.first) * p.a.G + h % p.a.G, groups = (count * p.a.G + (1 << form.width) - 1) >> form.width;
+	const int group = form.wide ? groups - 1 - (column >> form.width) : column >> form.width;
+	if (turn.first + (int64_t)groups * splits > form.pairs) return;  // (bounds of rows that overlap: more pairs than there is room for)
+	const int64_t step = (int64_t)(p.a.dh + 2) * form.room;
+	const float* const from = partial_of(p, form, hk, (int)turn.first + group * splits, column & ((1 << form.width) - 1));
 	float m = -kInf;
 	for (int x = lane; x < splits; x += 64) m = fmaxf(m, from[x * step]);
 	for (int x = 32; x; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
 	const float base = m == -kInf ? 0.0f : m;
+	// each lane a part's factor, then all parts' sums in their order, several loads on their way
 	float l = 0.0f, y[2] = {0.0f, 0.0f};
-	for (int x = 0; x < splits; ++x) {
-		const float* q = from + x * step;
-		const float f = exp2_of(q[0] - base);
-		l += f * q[1];
+	for (int x0 = 0; x0 < splits; x0 += 64) {
+		const bool on = x0 + lane < splits;
+		const float mine = on ? exp2_of(from[(x0 + lane) * step] - base) : 0.0f, own = on ? mine * from[(x0 + lane) * step + 1] : 0.0f;
+		const int some = min(64, splits - x0);
+		const auto add = [&](int x, float a, float b) {
+			const float f = __shfl(mine, x);
+			l += __shfl(own, x);
+			y[0] += f * a;
+			y[1] += f * b;
+		};
+		const float* const at = from + x0 * step + 2;
+		const int d0 = min(lane, p.a.dh - 1), d1 = min(lane + 64, p.a.dh - 1);
+		int x = 0;
+		for (; x + 8 <= some; x += 8) {
+			float a[8], b[8];
 #pragma unroll
-		for (int d = 0; d < 2; ++d)
-			if (lane + 64 * d < p.a.dh) y[d] += f * q[2 + lane + 64 * d];
+			for (int i = 0; i < 8; ++i) {
+				a[i] = at[(x + i) * step + d0];
+				b[i] = at[(x + i) * step + d1];
+			}
+#pragma unroll
+			for (int i = 0; i < 8; ++i) add(x + i, a[i], b[i]);
+		}
+		for (; x < some; ++x) add(x, at[x * step + d0], at[x * step + d1]);
 	}
 	T* const o = (T*)p.a.out + row * p.a.os.row + h * p.a.os.head;
 	const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -443,19 +526,21 @@ __global__ __launch_bounds__(256) void paged_attention_join_kernel(PagedAttentio
 }
 
 template <typename T, int DH, bool VEC>
-hipError_t launch_paged(const PagedAttentionArgs& p, hipStream_t s) {
-	const int64_t pairs = (int64_t)p.s.N * p.a.Hkv, most = (int64_t)p.most * p.a.G;  // (checked to be an int)
+hipError_t launch_paged(const PagedAttentionArgs& given, hipStream_t s) {
+	PagedAttentionArgs p = given;
+	p.wide.shift = keys_per_tile<T, DH>() == 64 ? 6 : 5;
 	hipError_t e = hipSuccess;
-	if (p.wide_splits) {
-		paged_attention_kernel<T, DH, VEC><<<(unsigned)(pairs * ((most + kQueries - 1) / kQueries) * p.wide_splits), 256, 0, s>>>(p);
+	if (p.wide.pairs) {
+		paged_attention_kernel<T, DH, VEC><<<(unsigned)((int64_t)p.wide.pairs * p.a.Hkv), 256, 0, s>>>(p);
 		e = hipGetLastError();
 	}
-	if (e == hipSuccess && p.splits) {
-		const int64_t groups = ((most < p.few ? most : p.few) + 31) / 32;
-		paged_attention_split_kernel<T, DH, VEC><<<(unsigned)(pairs * groups * p.splits), 64 * SplitShape<T, DH>::NW, 0, s>>>(p);
+	if (e == hipSuccess && p.split.pairs) {
+		const int64_t blocks = (int64_t)p.split.pairs * p.a.Hkv;
+		if (!p.split.target && blocks <= 1024) paged_attention_split_kernel<T, DH, VEC, 4><<<(unsigned)blocks, 256, 0, s>>>(p);
+		else paged_attention_split_kernel<T, DH, VEC, 2><<<(unsigned)blocks, 128, 0, s>>>(p);
 		e = hipGetLastError();
 	}
-	if (e == hipSuccess && (p.wide_splits > 1 || p.splits > 1)) {
+	if (e == hipSuccess && (p.wide.target || p.split.target)) {
 		paged_attention_join_kernel<T><<<(unsigned)(((int64_t)p.s.rows * p.a.H + 3) / 4), 256, 0, s>>>(p);
 		e = hipGetLastError();
 	}

@@ -139,17 +139,22 @@ HeadStrides strides_of(const nnh_head_tensor* t) { return {0, (int64_t)t->row, (
 int check_blocks(size_t N, size_t rows, size_t most, size_t H, size_t Hkv) {
 	uint64_t x = 0;
 	if (H > kMost || Hkv > kMost || H == 0 || Hkv == 0 || H % Hkv != 0) return refuse(NNH_ERR_SHAPE, "the key heads must divide the query heads, heads must not be empty");
-	// (most rows of a sequence have 128 columns or more to a workgroup, in 512 parts at most where there are few of them)
-	if (most > kMost || !count_ok({most, H / Hkv}, x) || x > kMost || !count_ok({rows, H}, x) || x > 4 * kMaxBlocks ||
-	    !count_ok({N, Hkv, (most * (H / Hkv) + 127) / 128 + 2}, x) || x > kMaxBlocks / 512)
+	// (workgroups: a group of 32 columns or more each, two to a sequence more at most, and the 512 that the keys are divided for)
+	if (most > kMost || !count_ok({rows, H}, x) || x > 4 * kMaxBlocks || !count_ok({2 * N + 1024, Hkv}, x) || x > kMaxBlocks / 2)
 		return refuse(NNH_ERR_INVALID, "size out of range");
 	return NNH_OK;
 }
 
-size_t partial_bytes(const PagedPlan& p, size_t rows, size_t H, size_t Dh) {
-	const int parts = std::max(p.splits, p.wide_splits);
-	return parts > 1 ? (size_t)parts * rows * H * (Dh + 2) * 4 : 0;
-}
+struct Room {
+	PagedPlan plan;
+	size_t split = 0, wide = 0, total = 0;
+	Room(size_t N, size_t rows, size_t most, size_t keys, size_t H, size_t Hkv, size_t Dh) : plan(paged_attention_plan(N, rows, most, keys, (int)H, (int)Hkv, (int)Dh)) {
+		WorkspacePlan w;
+		split = w.add(plan.split_floats * 4);
+		wide = w.add(plan.wide_floats * 4);
+		total = w.total;
+	}
+};
 
 }  // namespace
 
@@ -194,7 +199,7 @@ int nnh_paged_attention_workspace_size(size_t N, size_t rows, size_t most, size_
 		const int rc = check_blocks(N, rows, most, H, Hkv);
 		if (rc != NNH_OK) return rc;
 		if (keys > kMost || N >= kMost || rows > kMost || Dh > 128) return refuse(NNH_ERR_INVALID, "size out of range");
-		return put_bytes(bytes, partial_bytes(paged_attention_plan((int)N, (int)rows, (int)most, (int)keys, (int)H, (int)Hkv), rows, H, Dh));
+		return put_bytes(bytes, Room(N, rows, most, keys, H, Hkv, Dh).total);
 	});
 }
 
@@ -233,7 +238,6 @@ int nnh_paged_attention(int type, size_t N, size_t rows, size_t most, size_t H, 
 		a.qs = strides_of(q);
 		a.os = strides_of(out);
 		a.N = (int)N;
-		a.Tk = (int)c.keys();
 		a.H = (int)H;
 		a.Hkv = (int)Hkv;
 		a.G = (int)(H / Hkv);
@@ -248,14 +252,15 @@ int nnh_paged_attention(int type, size_t N, size_t rows, size_t most, size_t H, 
 		p.s = {starts, rule->k_lens, (int)N, (int)rows};
 		p.most = (int)std::min(most, rows);
 		p.lse = lse;
-		const PagedPlan plan = paged_attention_plan((int)N, (int)rows, (int)most, (int)c.keys(), (int)H, (int)Hkv);
-		p.few = plan.few;
-		p.splits = plan.splits;
-		p.wide_splits = plan.wide_splits;
+		const Room room(N, rows, most, c.any_page() ? c.keys() : 0, H, Hkv, Dh);
+		p.few = room.plan.few;
+		p.split = room.plan.split;
+		p.wide = room.plan.wide;
 		hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-		Scratch ws(s, partial_bytes(plan, rows, H, Dh));
+		Scratch ws(s, room.total);
 		if (ws.status() != NNH_OK) return ws.status();
-		p.partial = ws.at<float>(0);
+		p.split.partial = ws.at<float>(room.split);
+		p.wide.partial = ws.at<float>(room.wide);
 		return hip_status(paged_attention(p, type, wide(c) && wide(c, q) && wide(c, out), s), "paged attention");
 	});
 }
