@@ -47,7 +47,14 @@ static hipError_t tile_of_type(const LinearInt8Args& given, hipStream_t s) {
 
 template <int I, int J, int NW, typename T>
 static hipError_t few_launch(const LinearInt8Args& a, hipStream_t s) {
-	linear_int8_few_kernel<I, J, NW, T><<<(unsigned)((a.V + 16 * I - 1) / (16 * I)), 64 * NW, 0, s>>>(a);
+	const unsigned blocks = (unsigned)((a.V + 16 * I - 1) / (16 * I));
+	if constexpr (J == 1) {
+		if (a.whole) {
+			linear_int8_few_kernel<I, J, NW, T, true><<<blocks, 64 * NW, 0, s>>>(a);
+			return hipGetLastError();
+		}
+	}
+	linear_int8_few_kernel<I, J, NW, T, false><<<blocks, 64 * NW, 0, s>>>(a);
 	return hipGetLastError();
 }
 template <int J, typename T>
@@ -68,6 +75,7 @@ static hipError_t few(const LinearInt8Args& a, hipStream_t s) {
 }  // namespace i8
 
 bool linear_int8_few(int64_t rows) { return rows <= i8::kFewRows; }
+bool linear_int8_whole(int64_t rows, int64_t D) { return rows <= 16 && rows * i8::whole_pitch(D) <= i8::kWhole; }
 
 size_t linear_int8_parts(int64_t rows, int64_t D, int64_t V) {
 	if (linear_int8_few(rows)) return 0;

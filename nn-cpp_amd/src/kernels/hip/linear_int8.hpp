@@ -29,12 +29,18 @@ struct LinearInt8Args {
 	void* y;
 	int64_t ldy;
 	int whole_words;  // y's rows can be stored in 16-byte words
+	// the few rows' own form: rows to quantise (null where they have no elements), in the place of x and x_scale
+	int whole;
+	const void* rows_in;
+	int64_t ld_in;
+	int wide_in;      // they can be read in 16-byte words
 	int* parts;       // {parts, rows, V}: sums of runs of the depth, or null
 	int part_units;   // a run's depth, in units of 2 codes
 };
 
-// Whether a product takes the form for few rows.
+// Whether a product takes the form for few rows, and whether that quantises them itself (whole).
 bool linear_int8_few(int64_t rows);
+bool linear_int8_whole(int64_t rows, int64_t D);
 // Elements of LinearInt8Args::parts.
 size_t linear_int8_parts(int64_t rows, int64_t D, int64_t V);
 

@@ -3,11 +3,12 @@
 // y[row][col] = sum over depth of W[col][depth] X[row][depth]. Both operands have their depth contiguous, and 32 of their codes are
 // the 32 bytes that 16 depths of a bf16 product take: tiles, ring, loads and reads of LDS are gemm16.hpp's, in units of two codes, and
 // an MFMA of 32 x 32 x 32 does twice the depth in the same time. The bounds are the same too, with twice the operations: 8192 rows,
-// 4096 deep, 16384 columns.
+// 4096 deep, 16384 columns take 490 to 520 us (2110 to 2240 TOP/s; the library's product of such codes 2126).
 #pragma once
 
 #include "gemm16.hpp"
 #include "linear_int8.hpp"
+#include "quantize.hpp"
 
 namespace nnh {
 namespace i8 {
@@ -209,12 +210,44 @@ __global__ __launch_bounds__(256) void linear_int8_join_kernel(LinearInt8Args a,
 }
 
 // Few rows (at most 64): bound by the weights' bytes. A workgroup takes 16 I columns, its NW waves the depth in NW runs, each weight
-// code going from memory into the registers of the one MFMA (16 x 16 x 64) block that uses it, eight loads at a time on their way;
-// whole numbers are added through LDS, so the order does not matter. The rows' codes come from L2, J blocks of 16.
-template <int I, int J, int NW, typename T>
+// code going from memory into the registers of the one MFMA (16 x 16 x 64) block that uses it, the loads of U steps on their way while
+// U others are multiplied; whole numbers are added through LDS, so the order does not matter. The rows' codes come from L2, J blocks of
+// 16. WHOLE: of fewer codes still (kWhole bytes), which every workgroup makes for itself in LDS: one launch in the place of two (1 row, 4096
+// deep, 4096 columns: 7.9 us; by a launch of quantize_rows and this one 4.2 + 6.2, and one launch more on the host).
+constexpr int kWhole = 16 * 1024;
+__host__ __device__ inline int64_t whole_pitch(int64_t D) { return (D + 63) / 64 * 64 + 16; }  // (16 rows in 16 places of the banks)
+
+template <int NW, typename T, bool VEC>
+__device__ __forceinline__ void quantize_into(const LinearInt8Args& a, int8_t* codes, float* scales, float* tops) {
+	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, pitch = (int)whole_pitch(a.D);
+	int team = NW;  // waves to a row
+	while (team > 1 && NW / team < a.rows) team /= 2;
+	const int t = wave % team * 64 + lane;
+	for (int r0 = 0; r0 < a.rows; r0 += NW / team) {
+		const int r = r0 + wave / team;
+		const bool on = r < a.rows;
+		const T* const x = (const T*)a.rows_in + (int64_t)(on ? r : 0) * a.ld_in;
+		float top = q8::share_top<T, VEC>(x, a.D, t * 8, team * 512);
+#pragma unroll
+		for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+		__syncthreads();
+		if (lane == 0) tops[wave] = top;
+		__syncthreads();
+		for (int w = 0; w < team; ++w) top = fmaxf(top, tops[wave / team * team + w]);
+		const q8::Scale scale(top);
+		if (!on) continue;
+		if (t == 0) scales[r] = scale.value;
+		for (int at = t * 8; at < pitch - 16; at += team * 512) *(uint64_t*)(codes + r * pitch + at) = q8::eight_codes<T, VEC>(x, a.D, at, scale);
+	}
+	__syncthreads();
+}
+
+template <int I, int J, int NW, typename T, bool WHOLE>
 __global__ __launch_bounds__(64 * NW) void linear_int8_few_kernel(LinearInt8Args a) {
-	constexpr int U = I * J > 4 ? 4 : 8;
+	constexpr int U = I * J > 4 ? 2 : 4;
 	__shared__ int sums[NW][J * 16][I * 16 + 1];
+	__shared__ __attribute__((aligned(16))) int8_t codes[WHOLE ? kWhole : 16];
+	__shared__ float scales[16], tops[NW];
 	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 	const int r = lane & 15, q = lane >> 4, m0 = blockIdx.x * 16 * I;
 	const int steps = (a.D + 63) / 64, per = (steps + NW - 1) / NW, begin = min(wave * per, steps), end = min(begin + per, steps);
@@ -223,30 +256,64 @@ __global__ __launch_bounds__(64 * NW) void linear_int8_few_kernel(LinearInt8Args
 	const int8_t* x[J];
 #pragma unroll
 	for (int i = 0; i < I; ++i) w[i] = a.w + (int64_t)min(m0 + 16 * i + r, a.V - 1) * a.ldw;
-#pragma unroll
-	for (int j = 0; j < J; ++j) x[j] = a.x + (int64_t)min(16 * j + r, a.rows - 1) * a.ldx;
-	i32x4 acc[I][J];
-#pragma unroll
-	for (int i = 0; i < I; ++i)
-#pragma unroll
-		for (int j = 0; j < J; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
-	for (int s = begin; s < end; s += U) {
-		i32x4 fa[U][I], fb[U][J];
+	i32x4 fa[2][U][I], fb[2][U][J], acc[I][J];
+	const auto load_w = [&](int set, int s) {
 #pragma unroll
 		for (int u = 0; u < U; ++u) {
-			// a step past the run's end multiplies the last one's weights with zeros
-			const int k = min(s + u, end - 1) * 64 + 16 * q, at = k < limit ? k : 0;  // (x is zero past the limit)
+			// a step past the run's end multiplies the last one's weights with zeros; the rows' codes are zero past the limit
+			const int k = min(s + u, end - 1) * 64 + 16 * q, at = k < limit ? k : 0;
 #pragma unroll
-			for (int i = 0; i < I; ++i) fa[u][i] = *(const i32x4*)(w[i] + at);
-#pragma unroll
-			for (int j = 0; j < J; ++j) fb[u][j] = s + u < end ? *(const i32x4*)(x[j] + k) : i32x4{0, 0, 0, 0};
+			for (int i = 0; i < I; ++i) fa[set][u][i] = *(const i32x4*)(w[i] + at);
 		}
+	};
+	const auto load_x = [&](int set, int s) {
+#pragma unroll
+		for (int u = 0; u < U; ++u) {
+			const int k = min(s + u, end - 1) * 64 + 16 * q;
+#pragma unroll
+			for (int j = 0; j < J; ++j) fb[set][u][j] = s + u < end ? *(const i32x4*)(x[j] + k) : i32x4{0, 0, 0, 0};
+		}
+	};
+	const auto multiply = [&](int set) {
 #pragma unroll
 		for (int u = 0; u < U; ++u)
 #pragma unroll
 			for (int i = 0; i < I; ++i)
 #pragma unroll
-				for (int j = 0; j < J; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fa[u][i], fb[u][j], acc[i][j], 0, 0, 0);
+				for (int j = 0; j < J; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fa[set][u][i], fb[set][u][j], acc[i][j], 0, 0, 0);
+	};
+#pragma unroll
+	for (int i = 0; i < I; ++i)
+#pragma unroll
+		for (int j = 0; j < J; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
+	if (begin < end) {  // (the first weights are on their way while the rows are quantised)
+		load_w(0, begin);
+		load_w(1, begin + U);
+	}
+	if constexpr (WHOLE) {
+		if (a.wide_in) quantize_into<NW, T, true>(a, codes, scales, tops);
+		else quantize_into<NW, T, false>(a, codes, scales, tops);
+	}
+#pragma unroll
+	for (int j = 0; j < J; ++j) {
+		const int row = min(16 * j + r, a.rows - 1);
+		x[j] = WHOLE ? codes + row * (int)whole_pitch(a.D) : a.x + (int64_t)row * a.ldx;
+	}
+	if (begin < end) {
+		load_x(0, begin);
+		load_x(1, begin + U);
+		for (int s = begin; s < end; s += 2 * U) {
+			multiply(0);
+			if (s + 2 * U < end) {
+				load_w(0, s + 2 * U);
+				load_x(0, s + 2 * U);
+			}
+			if (s + U < end) multiply(1);
+			if (s + 3 * U < end) {
+				load_w(1, s + 3 * U);
+				load_x(1, s + 3 * U);
+			}
+		}
 	}
 	// register e of block (i, j): column 16 i + 4 q + e, row 16 j + r
 #pragma unroll
@@ -262,7 +329,7 @@ __global__ __launch_bounds__(64 * NW) void linear_int8_few_kernel(LinearInt8Args
 		int sum = 0;
 #pragma unroll
 		for (int n = 0; n < NW; ++n) sum += sums[n][row][c];
-		((T*)a.y)[row * a.ldy + col] = (T)scaled(sum, a.x_scale[row], a.w_scale[col], bias_at<T>(a, col));
+		((T*)a.y)[row * a.ldy + col] = (T)scaled(sum, WHOLE ? scales[row] : a.x_scale[row], a.w_scale[col], bias_at<T>(a, col));
 	}
 }
 

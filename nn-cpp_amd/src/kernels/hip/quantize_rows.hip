@@ -1,55 +1,15 @@
-// quantize_rows.hip - rows to 8-bit codes with a scale each (linear_int8.hpp).
+// quantize_rows.hip - rows to 8-bit codes with a scale each (quantize.hpp).
 //
-// scale = max |x| / 127 rounded to 32 bits, code = the whole number nearest to x / scale, ties to even. The nearest is found by a
-// product with the scale's reciprocal, which may be off by one in the last place, and put right by the rest x - code scale: a fused
-// multiply-add gives it exactly where it decides, near half a scale (both have 24 bits, and the rest's bits lie above half the scale's
-// last place). Rows of such a small scale that its reciprocal is not a number to work with divide in 64 bits.
-//
-// Bound by memory: a row is read once for its maximum and again, from the caches, for its codes.
-#include <cmath>
-
-#include "linear_int8.hpp"
+// Bound by memory: a row of up to 8192 elements is read once, into registers, a longer one once more, from the caches, for its codes.
+// 8192 rows of 4096 take 40 us (100 MB, 2.5 TB/s); 32 of them 5 us, a launch and two trips to memory.
+#include "quantize.hpp"
 
 namespace nnh {
 
 namespace {
 
-template <typename T>
-__device__ __forceinline__ float float_of(T x) { return (float)x; }
-
-struct alignas(16) Word {
-	unsigned x[4];
-};
-
-// Eight consecutive elements; those past D are zero.
-template <typename T, bool VEC>
-__device__ __forceinline__ void eight(float (&y)[8], const T* row, int at, int D) {
-	if constexpr (VEC) {
-		union {
-			Word w[8 * sizeof(T) / 16];
-			T e[8];
-		} u;
-#pragma unroll
-		for (int i = 0; i < (int)(8 * sizeof(T) / 16); ++i) u.w[i] = ((const Word*)(row + at))[i];
-#pragma unroll
-		for (int i = 0; i < 8; ++i) y[i] = float_of(u.e[i]);
-	} else {
-#pragma unroll
-		for (int i = 0; i < 8; ++i) y[i] = at + i < D ? float_of(row[at + i]) : 0.0f;
-	}
-}
-
-__device__ __forceinline__ int code_of(float x, float scale, float inv) {
-	float n = rintf(x * inv);
-	const float d = __builtin_fmaf(-n, scale, x), h = 0.5f * scale;
-	const bool odd = ((int)n & 1) != 0;
-	if (d > h || (d == h && odd)) n += 1.0f;
-	if (d < -h || (d == -h && odd)) n -= 1.0f;
-	return (int)n;
-}
-
-// TPR threads to a row: a wave for short rows, a workgroup for others.
-template <typename T, bool VEC, int TPR>
+// TPR threads to a row: a wave for short rows, a workgroup for others. A thread holds 8 HOLD elements (0: it reads them again).
+template <typename T, bool VEC, int TPR, int HOLD>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(QuantizeArgs a) {
 	constexpr int kRows = 256 / TPR;
 	__shared__ float part[4];
@@ -57,18 +17,20 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(QuantizeArgs a) {
 	const int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / TPR;
 	const bool on = row < a.rows;
 	const T* const x = (const T*)a.x + (on ? row : 0) * a.ldx;
-	float top = 0.0f;
-	bool fine = true;
-	float v[8];
-	for (int at = t * 8; at < a.D; at += TPR * 8) {
-		eight<T, VEC>(v, x, at, a.D);
+	float v[HOLD ? HOLD : 1][8], top = 0.0f;
+	if constexpr (HOLD > 0) {
 #pragma unroll
-		for (int i = 0; i < 8; ++i) {
-			top = fmaxf(top, fabsf(v[i]));  // (leaves NaN out)
-			fine = fine && !(__float_as_uint(v[i]) << 1 >= 0xff000000u);
+		for (int k = 0; k < HOLD; ++k) {
+			const int at = (k * TPR + t) * 8;
+#pragma unroll
+			for (int i = 0; i < 8; ++i) v[k][i] = 0.0f;
+			if (at < a.D) q8::eight<T, VEC>(v[k], x, at, a.D);
 		}
+#pragma unroll
+		for (int k = 0; k < HOLD; ++k) top = fmaxf(top, q8::top_of(v[k]));
+	} else {
+		top = q8::share_top<T, VEC>(x, a.D, t * 8, TPR * 8);
 	}
-	if (!fine) top = __builtin_huge_valf();
 #pragma unroll
 	for (int s = 32; s; s >>= 1) top = fmaxf(top, __shfl_xor(top, s));
 	if (TPR > 64) {
@@ -77,43 +39,34 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(QuantizeArgs a) {
 		top = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
 	}
 	if (!on) return;
-	fine = top < __builtin_huge_valf();
-	const float scale = fine ? top / 127.0f : __builtin_nanf("");
-	if (t == 0) a.scale[row] = scale;
+	const q8::Scale scale(top);
+	if (t == 0) a.scale[row] = scale.value;
 	int8_t* const c = a.codes + row * a.ldc;
-	const bool none = !fine || scale == 0.0f, small = scale < 0x1p-100f;
-	const float inv = 1.0f / scale;
-	for (int at = t * 8; at < a.pad; at += TPR * 8) {
-		int code[8];
-		if (at < a.D) {
-			eight<T, VEC>(v, x, at, a.D);
-#pragma unroll
-			for (int i = 0; i < 8; ++i) {
-				// (a scale below the least normal number may be rounded down by more than its share: codes stay within 127)
-				if (small && !none) code[i] = (int)fmin(fmax(rint((double)v[i] / (double)scale), -127.0), 127.0);
-				else code[i] = none ? 0 : code_of(v[i], scale, inv);
-			}
-		} else {
-#pragma unroll
-			for (int i = 0; i < 8; ++i) code[i] = 0;
-		}
+	const auto store = [&](int at, uint64_t w) {
 		if constexpr (VEC) {
-			uint64_t w = 0;
-#pragma unroll
-			for (int i = 0; i < 8; ++i) w |= (uint64_t)(code[i] & 255) << (8 * i);
 			*(uint64_t*)(c + at) = w;
 		} else {
 #pragma unroll
 			for (int i = 0; i < 8; ++i)
-				if (at + i < a.pad) c[at + i] = (int8_t)code[i];
+				if (at + i < a.pad) c[at + i] = (int8_t)(w >> (8 * i));
 		}
+	};
+	if constexpr (HOLD > 0) {
+#pragma unroll
+		for (int k = 0; k < HOLD; ++k) {
+			const int at = (k * TPR + t) * 8;
+			if (at < a.pad) store(at, q8::codes_of(v[k], scale));
+		}
+	} else {
+		for (int at = t * 8; at < a.pad; at += TPR * 8) store(at, q8::eight_codes<T, VEC>(x, a.D, at, scale));
 	}
 }
 
 template <typename T, bool VEC>
 hipError_t launch(const QuantizeArgs& a, hipStream_t s) {
-	if (a.D <= 1024) quantize_rows_kernel<T, VEC, 64><<<(unsigned)((a.rows + 3) / 4), 256, 0, s>>>(a);
-	else quantize_rows_kernel<T, VEC, 256><<<(unsigned)a.rows, 256, 0, s>>>(a);
+	if (a.pad <= 1024) quantize_rows_kernel<T, VEC, 64, 2><<<(unsigned)((a.rows + 3) / 4), 256, 0, s>>>(a);
+	else if (a.pad <= 8192) quantize_rows_kernel<T, VEC, 256, 4><<<(unsigned)a.rows, 256, 0, s>>>(a);
+	else quantize_rows_kernel<T, VEC, 256, 0><<<(unsigned)a.rows, 256, 0, s>>>(a);
 	return hipGetLastError();
 }
 

@@ -37,7 +37,7 @@ struct Plan {
 };
 Plan plan_of(uint64_t rows, uint64_t D, uint64_t V) {
 	Plan p;
-	if (rows == 0 || V == 0) return p;
+	if (rows == 0 || V == 0 || linear_int8_whole((int64_t)rows, (int64_t)D)) return p;
 	WorkspacePlan w;
 	p.pitch = up(D, 64);
 	p.codes = w.add(rows * p.pitch);
@@ -104,19 +104,26 @@ int nnh_linear_int8(int type, const void* x, size_t rows, size_t D, size_t ldx, 
 		hipStream_t s = reinterpret_cast<hipStream_t>(stream);
 		Scratch ws(s, p.total);
 		if (ws.status() != NNH_OK) return ws.status();
-		const QuantizeArgs q{x, (int64_t)ldx, (int64_t)rows, (int)D, ws.at<int8_t>(p.codes), (int64_t)p.pitch, (int)p.pitch, ws.at<float>(p.scale)};
-		rc = hip_status(quantize_rows(q, type, s), "linear in 8 bits");
-		if (rc != NNH_OK) return rc;
 		LinearInt8Args a{};
+		if (linear_int8_whole((int64_t)rows, (int64_t)D)) {
+			a.whole = 1;
+			a.rows_in = x;
+			a.ld_in = (int64_t)ldx;
+			a.wide_in = !off(x, 16) && ldx * size % 16 == 0 && D % 8 == 0;
+		} else {
+			const QuantizeArgs q{x, (int64_t)ldx, (int64_t)rows, (int)D, ws.at<int8_t>(p.codes), (int64_t)p.pitch, (int)p.pitch, ws.at<float>(p.scale)};
+			rc = hip_status(quantize_rows(q, type, s), "linear in 8 bits");
+			if (rc != NNH_OK) return rc;
+			a.x = q.codes;
+			a.x_scale = q.scale;
+		}
 		a.w = reinterpret_cast<const int8_t*>(w);
-		a.x = q.codes;
 		a.ldw = (int64_t)ldw;
 		a.ldx = (int64_t)p.pitch;
 		a.rows = (int)rows;
 		a.D = (int)D;
 		a.V = (int)V;
 		a.w_scale = w_scale;
-		a.x_scale = q.scale;
 		a.bias = bias;
 		a.y = y;
 		a.ldy = (int64_t)ldy;

@@ -29,7 +29,7 @@ def check(dtype, rows, D, V, bias=True, seed=0):
 
 
 SHAPES = [(1, 1, 1), (1, 16, 16), (1, 4096, 100), (3, 100, 33), (16, 64, 64), (17, 1000, 257), (32, 48, 130), (33, 65, 17), (64, 2047, 129), (65, 64, 64), (100, 1000, 257),
-          (130, 33, 130), (257, 129, 300), (65, 5000, 64), (300, 4096, 520), (2, 8192, 8200), (20, 300, 16400), (70, 131, 1)]
+          (130, 33, 130), (257, 129, 300), (65, 5000, 64), (300, 4096, 520), (2, 8192, 8200), (20, 300, 16400), (70, 131, 1), (2, 4000, 300), (4, 4080, 33), (4, 4081, 33), (16, 960, 16384), (5, 1000, 8200), (1, 16300, 20), (3, 5, 16385)]
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
@@ -164,20 +164,24 @@ def test_quantised_weight(gpu):
     assert bool(((y - want).abs() <= bound * (1 + 1e-5)).all())
 
 
-@pytest.mark.parametrize("rows,D,V", [(4, 300, 200), (100, 4096, 300)])
+@pytest.mark.parametrize("rows,D,V", [(4, 300, 200), (20, 300, 200), (100, 4096, 300)])
 def test_captured_and_on_two_streams(gpu, rows, D, V):
+    """Where the rows' codes need scratch: captured with exactly the size asked for, refused without."""
     import nnh
     w, s = weight(1, V, D)
     w, s = w.cuda()[:, :D], s.cuda()
     x = [draw(i, rows, D, dtype=torch.bfloat16).cuda() for i in range(2)]
     size = nnh.workspace_size("linear_int8", rows, D, V)
+    assert (size > 0) == (rows > 4)
     room = torch.full((size + 4096,), 7, dtype=torch.uint8, device="cuda")
     side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
     torch.cuda.synchronize()
-    with pytest.raises(nnh.NnhError, match="workspace"):
-        with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=side):
-            nnh.linear_int8(x[0], w, s)
-    nnh.set_workspace(room[:size], side)
+    if size:
+        with pytest.raises(nnh.NnhError, match="workspace"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=side):
+                nnh.linear_int8(x[0], w, s)
+    if size:
+        nnh.set_workspace(room[:size], side)
     try:
         with torch.cuda.graph(graph, stream=side):
             y = nnh.linear_int8(x[0], w, s)
