@@ -97,10 +97,13 @@ private:
 class IntTensor {
 public:
 	IntTensor() = default;
+	static IntTensor empty(std::vector<size_t> shape);  // uninitialised
 	static IntTensor from_host(std::vector<size_t> shape, const int* data);
+	std::vector<int> to_host() const;
 	const std::vector<size_t>& shape() const { return shape_; }
 	size_t size() const { return size_; }
 	const int* data() const;  // device pointer, null when empty
+	int* data();
 
 private:
 	std::shared_ptr<Block> storage_;
@@ -243,6 +246,46 @@ Value masked_attention(const Value& q, const Value& k, const Value& v, size_t he
 // without making the logits as a whole: x {..., D}, weight {V, D}, bias {V} (or a default Value: none), targets of x's leading
 // axes, negative for none.
 Value linear_cross_entropy(const Value& x, const Value& weight, const Value& bias, const IntTensor& targets);
+
+// Serving: none of these records a graph.
+// Columns begin and on of a two-dimensional tensor's rows (the keys in the result of a joint projection).
+struct Columns {
+	Tensor rows;
+	size_t begin;
+	Columns(Tensor rows, size_t begin = 0) : rows(std::move(rows)), begin(begin) {}
+};
+// Keys and values of many sequences in pages of one pool (nnh_paged_cache in nnh.h), uninitialised.
+struct PagedCache {
+	PagedCache(size_t pages, size_t page_size, size_t kv_heads, size_t head_width);
+	Tensor k, v;  // {pages, page_size, kv_heads, head_width}
+};
+// The new tokens of N sequences, packed into rows in turn, and where these sequences' tokens are kept.
+struct PagedStep {
+	IntTensor table;   // {N, width}: the pages of each sequence
+	IntTensor starts;  // {N + 1}: sequence n's new tokens are rows starts[n] .. starts[n + 1] - 1
+	IntTensor lens;    // {N}: its tokens, the new ones among them
+	size_t most = 1;   // at least the new tokens of any one sequence
+};
+// The new tokens' keys and values into their places: kv_heads head_width columns of each row.
+void paged_append(PagedCache& cache, const Columns& k, const Columns& v, const PagedStep& step);
+// Attention of the new tokens over their sequences' pages: heads head_width columns of q's rows, {rows, heads head_width} back. Of the
+// rule's lengths and documents only prefix is taken, what a sequence holds is the step's.
+Tensor paged_attention(const Columns& q, const PagedCache& cache, size_t heads, const PagedStep& step, const AttentionRule& rule);
+// A linear's weights {out, in} in 8 bits with a scale to each row (nnh_quantize_rows); of several weights, their rows in turn.
+struct QuantizedWeight {
+	size_t out = 0, in = 0, pitch = 0;  // a row's codes begin at row * pitch bytes
+	Tensor codes, scale;                // (the codes' bytes in fp32 storage)
+};
+QuantizedWeight quantize(const std::vector<Tensor>& weights);
+// x W^T + bias of rows quantised on the way (nnh_linear_int8): x {..., in}, bias {out} or empty.
+Tensor linear_int8(const Tensor& x, const QuantizedWeight& weight, const Tensor& bias);
+// How a token is chosen (nnh_sample in nnh.h), an entry to each row; what is empty is off.
+struct SampleRule {
+	Tensor temperature, top_p, min_p;  // {rows}
+	IntTensor top_k;                   // {rows}
+};
+// A token {rows} of each row of logits {rows, V} by u {rows}, uniform in [0, 1); logprob (optional) receives {rows}.
+IntTensor sample(const Tensor& logits, const Tensor& u, const SampleRule& rule = SampleRule(), Tensor* logprob = nullptr);
 
 // positional.cpp:15-25: the fixed sinusoidal table {max_len, dim}, computed in double on the host and stored as fp32.
 Tensor sinusoidal_table(size_t max_len, size_t dim);

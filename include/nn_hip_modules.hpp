@@ -84,6 +84,19 @@ private:
 	Value weight_, bias_;
 };
 
+// Linears with their weights in 8 bits (quantize, linear_int8), those of several layers side by side in its result, as the weights and
+// biases are when it is made. It has no gradient: an input that asks for one is refused (std::invalid_argument).
+class QuantizedLinear : public Module {
+public:
+	explicit QuantizedLinear(const std::vector<Linear>& layers);
+	Value forward(const Value& input) override;
+	const QuantizedWeight& weight() const { return weight_; }
+
+private:
+	QuantizedWeight weight_;
+	Tensor bias_;
+};
+
 // conv2d.cpp: square kernels; W {out, in, k, k} uniform in +-1/sqrt(in k k), b zeros. A following ReLU folds into
 // conv2d_relu.
 class Conv2d : public Module {
@@ -152,6 +165,7 @@ public:
 	Value forward_add(const Value& ids, const Value& addend);
 	std::vector<Value> parameters() const override;
 	std::vector<std::pair<std::string, Value>> named_parameters() const override;
+	const Value& weight() const { return weight_; }
 
 private:
 	Value weight_;
@@ -165,6 +179,8 @@ public:
 	Value forward(const Value& input) override;
 	// the addend forward adds to a {N, T, dim} input: the table's first T rows (the same node forward builds)
 	Value rows(size_t T);
+	// its rows of these positions (whole numbers below max_len), {positions, dim}
+	Value at(const std::vector<float>& positions);
 	std::vector<Value> parameters() const override;
 	std::vector<std::pair<std::string, Value>> named_parameters() const override;
 
@@ -190,6 +206,7 @@ public:
 	void train(bool mode = true) override;
 
 private:
+	friend class Decoder;
 	Value attend_impl(const Value& query, const Value& context, const Tensor& key_padding_mask, const Value* residual,
 	                  const AttentionRule* rule = nullptr);
 	size_t dim_, heads_;
@@ -238,6 +255,7 @@ public:
 	void train(bool mode = true) override;
 
 private:
+	friend class Decoder;
 	Value mlp_add(const Value& h);
 	LayerNorm ln1_;
 	MultiHeadAttention attn_;
@@ -265,12 +283,66 @@ public:
 	void train(bool mode = true) override;
 
 private:
+	friend class Decoder;
+	TransformerConfig config_;
 	Value hidden(const Value& ids, const AttentionRule* rule);
 	Embedding embed_;
 	PositionalEncoding pos_;
 	std::vector<std::unique_ptr<TransformerBlock>> blocks_;
 	LayerNorm ln_f_;
 	Linear head_;
+};
+
+// Generation from a causal Transformer, for many sequences at a time: their keys and values are kept in pages (paged_append), and a step
+// takes new tokens of any of them, whole prompts beside single tokens, through the model in one batch (paged_attention). It has no
+// counterpart in the reference, whose model runs over all of a sequence for every token. The parameters are the model's own, in its
+// eval mode; with int8 the linears' weights are 8-bit copies, made here.
+struct DecoderOptions {
+	size_t sequences = 1;   // that can be held at a time
+	size_t page_size = 64;  // tokens to a page
+	size_t pages = 0;       // to a layer; 0: enough for max_len tokens of every sequence
+	bool int8 = false;
+};
+
+class Decoder {
+public:
+	struct Turn {
+		size_t sequence;
+		std::vector<int> tokens;
+	};
+	explicit Decoder(const Transformer& model, const DecoderOptions& options = DecoderOptions());
+	// The new tokens of some sequences (one turn to a sequence, one token at least); the logits {turns, vocab_size} after each one's
+	// last. A call that the pages, max_len or the vocabulary do not allow is refused before anything is stored (std::invalid_argument).
+	Tensor step(const std::vector<Turn>& turns);
+	// `count` tokens to each prompt (two or more turns are served together), chosen by `rule` (of as many rows as prompts) with
+	// numbers from manual_seed's "sample" stream. The last one is not stored.
+	std::vector<std::vector<int>> generate(const std::vector<Turn>& prompts, size_t count, const SampleRule& rule = SampleRule());
+	void drop(size_t sequence);  // forgets its tokens; the pages are free again
+	size_t length(size_t sequence) const { return held_.at(sequence).length; }
+	size_t free_pages() const { return free_.size(); }
+
+private:
+	struct Layer {
+		LayerNorm ln1, ln2;
+		Linear q, k, v, o, fc1, fc2;
+		std::unique_ptr<QuantizedLinear> qkv8, o8, fc1_8, fc2_8;
+		PagedCache cache;
+	};
+	struct Held {
+		size_t length = 0;
+		std::vector<int> pages;
+	};
+	TransformerConfig config_;
+	size_t page_size_;
+	Embedding embed_;
+	PositionalEncoding pos_;
+	std::vector<Layer> layers_;
+	LayerNorm ln_f_;
+	Linear head_;
+	std::unique_ptr<QuantizedLinear> head8_;
+	std::vector<Held> held_;
+	std::vector<int> free_;
+	std::mt19937 gen_;
 };
 
 // AdamW over parameters and their gradients on the device (nnh_adamw_step), one launch for 52 of them, the moments in 32 bits

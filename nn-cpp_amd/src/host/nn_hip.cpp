@@ -153,6 +153,22 @@ IntTensor IntTensor::from_host(std::vector<size_t> shape, const int* data) {
 	return t;
 }
 
+IntTensor IntTensor::empty(std::vector<size_t> shape) {
+	IntTensor t;
+	t.shape_ = std::move(shape);
+	t.size_ = numel(t.shape_);
+	if (t.size_ != 0) t.storage_ = std::make_shared<Block>(t.size_ * sizeof(int));
+	return t;
+}
+
+std::vector<int> IntTensor::to_host() const {
+	std::vector<int> out(size_);
+	if (size_ != 0) check_hip(hipMemcpyAsync(out.data(), data(), size_ * sizeof(int), hipMemcpyDeviceToHost, g_stream), "copy out");
+	synchronize();
+	return out;
+}
+
+int* IntTensor::data() { return storage_ ? static_cast<int*>(storage_->p) : nullptr; }
 const int* IntTensor::data() const { return storage_ ? static_cast<const int*>(storage_->p) : nullptr; }
 
 float* Tensor::data() const { return storage_ ? static_cast<float*>(storage_->p) : nullptr; }
@@ -1009,6 +1025,108 @@ Value linear_cross_entropy(const Value& x, const Value& weight, const Value& bia
 			check(nnh_add_to_grad(to, part[i].data(), part[i].size(), fresh, g_stream));
 		}
 	});
+}
+
+PagedCache::PagedCache(size_t pages, size_t page_size, size_t kv_heads, size_t head_width)
+	: k(Tensor::empty({pages, page_size, kv_heads, head_width})), v(Tensor::empty({pages, page_size, kv_heads, head_width})) {}
+
+namespace {
+
+nnh_paged_cache paged(const PagedCache& cache, const PagedStep& step) {
+	const auto& s = cache.k.shape();
+	const auto& t = step.table.shape();
+	if (s.size() != 4 || cache.v.shape() != s || t.size() != 2 || step.lens.shape() != std::vector<size_t>{t[0]} ||
+	    step.starts.shape() != std::vector<size_t>{t[0] + 1})
+		throw TensorShapeError("nn::hip: paged cache shapes");
+	return nnh_paged_cache{cache.k.data(), cache.v.data(), s[1] * s[2] * s[3], s[2] * s[3], s[3], s[0], s[1], step.table.data(), t[1]};
+}
+
+nnh_head_tensor heads_of(const Columns& c, size_t heads, size_t width) {
+	const auto& s = c.rows.shape();
+	if (s.size() != 2 || c.begin > s[1] || heads * width > s[1] - c.begin) throw TensorShapeError("nn::hip: columns of packed rows");
+	return nnh_head_tensor{c.rows.data() + c.begin, s[0] * s[1], s[1], width};
+}
+
+}  // namespace
+
+void paged_append(PagedCache& cache, const Columns& k, const Columns& v, const PagedStep& step) {
+	const nnh_paged_cache c = paged(cache, step);
+	const size_t heads = cache.k.shape()[2], width = cache.k.shape()[3];
+	const nnh_head_tensor hk = heads_of(k, heads, width), hv = heads_of(v, heads, width);
+	if (k.rows.shape()[0] != v.rows.shape()[0]) throw TensorShapeError("nn::hip: paged_append rows");
+	check(nnh_paged_append(NNH_F32, step.lens.size(), k.rows.shape()[0], heads, width, &hk, &hv, step.starts.data(), step.lens.data(), &c, g_stream));
+}
+
+Tensor paged_attention(const Columns& q, const PagedCache& cache, size_t heads, const PagedStep& step, const AttentionRule& rule) {
+	const nnh_paged_cache c = paged(cache, step);
+	const size_t N = step.lens.size(), kv_heads = cache.k.shape()[2], width = cache.k.shape()[3];
+	const nnh_head_tensor hq = heads_of(q, heads, width);
+	const size_t rows = q.rows.shape()[0];
+	if (rule.slopes.size() != 0 && rule.slopes.shape() != std::vector<size_t>{heads})
+		throw TensorShapeError("nn::hip: paged_attention slopes shape");
+	if (rule.q_start.size() != 0 || rule.k_lens.size() != 0 || rule.q_docs.size() != 0 || rule.k_docs.size() != 0)
+		throw std::invalid_argument("nn::hip: paged_attention takes a step's lengths, no starts, lengths or documents of a rule");
+	const nnh_attention_rule r{rule.scale, rule.cap, rule.slopes.size() ? rule.slopes.data() : nullptr, rule.causal, rule.window,
+	                           nullptr, step.lens.data(), option(rule.prefix, {N}), nullptr, nullptr};
+	Tensor out = Tensor::empty({rows, heads * width}), lse = Tensor::empty({rows, heads});
+	const nnh_head_tensor ho{out.data(), rows * heads * width, heads * width, width};
+	check(nnh_paged_attention(NNH_F32, N, rows, step.most, heads, kv_heads, width, &hq, &c, step.starts.data(), &r, &ho, lse.data(), g_stream));
+	return out;
+}
+
+QuantizedWeight quantize(const std::vector<Tensor>& weights) {
+	QuantizedWeight w;
+	for (const Tensor& t : weights) {
+		if (t.ndim() != 2 || (w.out != 0 && t.shape()[1] != w.in)) throw TensorShapeError("nn::hip: quantize takes weights {out, in} of one depth");
+		w.in = t.shape()[1];
+		w.out += t.shape()[0];
+	}
+	w.pitch = (w.in + 15) / 16 * 16;
+	w.codes = Tensor::empty({w.out * w.pitch / sizeof(float)});
+	w.scale = Tensor::empty({w.out});
+	size_t at = 0;
+	for (const Tensor& t : weights) {
+		check(nnh_quantize_rows(NNH_F32, t.data(), t.shape()[0], w.in, w.in, reinterpret_cast<signed char*>(w.codes.data()) + at * w.pitch,
+		                        w.pitch, w.scale.data() + at, g_stream));
+		at += t.shape()[0];
+	}
+	return w;
+}
+
+Tensor linear_int8(const Tensor& x, const QuantizedWeight& weight, const Tensor& bias) {
+	if (x.ndim() == 0 || x.shape().back() != weight.in || (bias.size() != 0 && bias.shape() != std::vector<size_t>{weight.out}))
+		throw TensorShapeError("nn::hip: linear_int8 shapes");
+	std::vector<size_t> shape = x.shape();
+	shape.back() = 1;
+	const size_t rows = numel(shape);
+	shape.back() = weight.out;
+	Tensor y = Tensor::empty(shape);
+	check(nnh_linear_int8(NNH_F32, x.data(), rows, weight.in, weight.in, reinterpret_cast<const signed char*>(weight.codes.data()), weight.pitch,
+	                      weight.scale.data(), weight.out, bias.size() ? bias.data() : nullptr, y.data(), weight.out, g_stream));
+	return y;
+}
+
+namespace {
+
+template <typename T>
+auto entry(const T& t, size_t rows) -> decltype(t.data()) {
+	if (t.size() == 0) return nullptr;
+	if (t.shape() != std::vector<size_t>{rows}) throw TensorShapeError("nn::hip: sample takes an entry to each row");
+	return t.data();
+}
+
+}  // namespace
+
+IntTensor sample(const Tensor& logits, const Tensor& u, const SampleRule& rule, Tensor* logprob) {
+	const auto& s = logits.shape();
+	if (s.size() != 2 || u.shape() != std::vector<size_t>{s[0]}) throw TensorShapeError("nn::hip: sample takes logits {rows, V} and u {rows}");
+	const size_t rows = s[0];
+	IntTensor tokens = IntTensor::empty({rows});
+	Tensor share = logprob ? Tensor::empty({rows}) : Tensor();
+	check(nnh_sample(NNH_F32, logits.data(), rows, s[1], s[1], u.data(), entry(rule.temperature, rows), entry(rule.top_k, rows),
+	                 entry(rule.top_p, rows), entry(rule.min_p, rows), tokens.data(), logprob ? share.data() : nullptr, g_stream));
+	if (logprob) *logprob = share;
+	return tokens;
 }
 
 Tensor sinusoidal_table(size_t max_len, size_t dim) {

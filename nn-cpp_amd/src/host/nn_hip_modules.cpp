@@ -1,5 +1,6 @@
 // nn_hip_modules.cpp - nn-cpp's module layer over device-resident Values (include/nn_hip_modules.hpp), and the
 // library-wide seeding its initial values come from (include/nn/random.hpp, src/random.cpp; src/tensor.cpp:504-522).
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 #include <map>
@@ -195,12 +196,32 @@ Value PositionalEncoding::rows(size_t T) {
 	if (T > max_len_) throw TensorShapeError("nn::hip: PositionalEncoding takes {N, T <= max_len, dim}");
 	return slice(pe_, 0, 0, T);
 }
+Value PositionalEncoding::at(const std::vector<float>& positions) { return embedding(pe_, positions, {positions.size()}); }
 std::vector<Value> PositionalEncoding::parameters() const {
 	return learned_ ? std::vector<Value>{pe_} : std::vector<Value>{};
 }
 std::vector<std::pair<std::string, Value>> PositionalEncoding::named_parameters() const {
 	return learned_ ? std::vector<std::pair<std::string, Value>>{{"pe", pe_}}
 	                : std::vector<std::pair<std::string, Value>>{};
+}
+
+QuantizedLinear::QuantizedLinear(const std::vector<Linear>& layers) {
+	std::vector<Tensor> weights;
+	std::vector<float> bias;
+	for (const Linear& l : layers) {
+		weights.push_back(l.weight().data());
+		const std::vector<float> b = l.bias().data().to_host();
+		bias.insert(bias.end(), b.begin(), b.end());
+	}
+	weight_ = quantize(weights);
+	bias_ = Tensor::from_host({bias.size()}, bias.data());
+	synchronize();  // bias is released on return
+}
+
+Value QuantizedLinear::forward(const Value& input) {
+	if (NoGradGuard::grad_enabled() && input.requires_grad())
+		throw std::invalid_argument("nn::hip: QuantizedLinear has no gradient");
+	return Value::leaf(linear_int8(input.data(), weight_, bias_));
 }
 
 MultiHeadAttention::MultiHeadAttention(size_t dim, size_t heads, bool causal, float dropout)
@@ -393,7 +414,7 @@ void TransformerBlock::train(bool mode) {
 }
 
 Transformer::Transformer(const TransformerConfig& c)
-	: embed_(checked_vocab(c), c.dim), pos_(c.max_len, c.dim, c.learned_positions), ln_f_(c.dim), head_(c.dim, c.vocab_size) {
+	: config_(c), embed_(checked_vocab(c), c.dim), pos_(c.max_len, c.dim, c.learned_positions), ln_f_(c.dim), head_(c.dim, c.vocab_size) {
 	for (size_t i = 0; i < c.layers; ++i)
 		blocks_.push_back(std::make_unique<TransformerBlock>(c.dim, c.heads, c.mlp_ratio, c.dropout, c.causal));
 }
@@ -435,6 +456,128 @@ std::vector<std::pair<std::string, Value>> Transformer::named_parameters() const
 void Transformer::train(bool mode) {
 	for (auto& b : blocks_) b->train(mode);
 	training_ = mode;
+}
+
+namespace {
+constexpr size_t kIds = (size_t)1 << 24;  // whole numbers that embedding's ids, being floats, can be
+}
+
+Decoder::Decoder(const Transformer& model, const DecoderOptions& options)
+	: config_(model.config_),
+	  page_size_(options.page_size),
+	  embed_(model.embed_),
+	  pos_(model.pos_),
+	  ln_f_(model.ln_f_),
+	  head_(model.head_),
+	  held_(options.sequences),
+	  gen_(derive_generator("sample")) {
+	if (!config_.causal) throw std::invalid_argument("nn::hip::Decoder: the model must be causal");
+	if (options.sequences == 0 || page_size_ == 0) throw std::invalid_argument("nn::hip::Decoder: sizes must be non-zero");
+	if (config_.dim / config_.heads > 128) throw std::invalid_argument("nn::hip::Decoder: heads of at most 128");
+	if (config_.vocab_size > kIds || config_.max_len > kIds) throw std::invalid_argument("nn::hip::Decoder: at most 2^24 tokens and positions");
+	const size_t each = (config_.max_len - 1) / page_size_ + 1;
+	if (!options.pages && options.sequences > (size_t)INT32_MAX / each) throw std::invalid_argument("nn::hip::Decoder: too many pages");
+	const size_t pages = options.pages ? options.pages : options.sequences * each;
+	if (pages > (size_t)INT32_MAX) throw std::invalid_argument("nn::hip::Decoder: too many pages");
+	for (size_t p = pages; p-- > 0;) free_.push_back(static_cast<int>(p));
+	const auto eight = [&](const std::vector<Linear>& l) { return options.int8 ? std::make_unique<QuantizedLinear>(l) : nullptr; };
+	for (const auto& b : model.blocks_) {
+		const MultiHeadAttention& a = b->attn_;
+		layers_.push_back(Layer{b->ln1_, b->ln2_, a.q_, a.k_, a.v_, a.o_, b->fc1_, b->fc2_, eight({a.q_, a.k_, a.v_}), eight({a.o_}),
+		                        eight({b->fc1_}), eight({b->fc2_}), PagedCache(pages, page_size_, config_.heads, config_.dim / config_.heads)});
+	}
+	head8_ = eight({head_});
+}
+
+Tensor Decoder::step(const std::vector<Turn>& turns) {
+	const size_t N = turns.size();
+	size_t need = 0, rows = 0, width = 1, most = 1;
+	std::vector<bool> seen(held_.size(), false);
+	for (const Turn& t : turns) {
+		if (t.sequence >= held_.size() || seen[t.sequence]) throw std::invalid_argument("nn::hip::Decoder: a turn to each sequence, below DecoderOptions' number");
+		seen[t.sequence] = true;
+		const Held& h = held_[t.sequence];
+		if (t.tokens.empty() || t.tokens.size() > config_.max_len - h.length)
+			throw std::invalid_argument("nn::hip::Decoder: a turn has a token at least, a sequence max_len at most");
+		for (int id : t.tokens)
+			if (id < 0 || static_cast<size_t>(id) >= config_.vocab_size) throw std::invalid_argument("nn::hip::Decoder: token out of the vocabulary");
+		const size_t pages = (h.length + t.tokens.size() - 1) / page_size_ + 1;
+		need += pages - std::min(pages, h.pages.size());
+		width = std::max(width, pages);
+		most = std::max(most, t.tokens.size());
+		rows += t.tokens.size();
+	}
+	if (need > free_.size()) throw std::invalid_argument("nn::hip::Decoder: no pages left");
+	if (rows > kIds) throw std::invalid_argument("nn::hip::Decoder: at most 2^24 tokens to a step");
+	if (N == 0) return Tensor::empty({0, config_.vocab_size});
+	std::vector<int> table(N * width, -1), starts{0}, lens;
+	std::vector<float> ids, positions, last;
+	for (size_t n = 0; n < N; ++n) {
+		const Turn& t = turns[n];
+		Held& h = held_[t.sequence];
+		const size_t length = h.length + t.tokens.size();
+		while (h.pages.size() * page_size_ < length) {
+			h.pages.push_back(free_.back());
+			free_.pop_back();
+		}
+		std::copy(h.pages.begin(), h.pages.begin() + std::min(width, h.pages.size()), table.begin() + n * width);
+		for (size_t i = 0; i < t.tokens.size(); ++i) {
+			ids.push_back(static_cast<float>(t.tokens[i]));
+			positions.push_back(static_cast<float>(h.length + i));
+		}
+		starts.push_back(static_cast<int>(ids.size()));
+		lens.push_back(static_cast<int>(length));
+		last.push_back(static_cast<float>(ids.size() - 1));
+	}
+	PagedStep step{IntTensor::from_host({N, width}, table.data()), IntTensor::from_host({N + 1}, starts.data()), IntTensor::from_host({N}, lens.data()), most};
+	AttentionRule rule;
+	rule.causal = true;
+	NoGradGuard guard;
+	Value x = embedding_add(embed_.weight(), ids, {rows}, pos_.at(positions));
+	for (Layer& l : layers_) {
+		const Value h = l.ln1.forward(x);
+		Tensor a;
+		if (l.qkv8) {
+			const Tensor qkv = l.qkv8->forward(h).data();
+			paged_append(l.cache, {qkv, config_.dim}, {qkv, 2 * config_.dim}, step);
+			a = paged_attention(qkv, l.cache, config_.heads, step, rule);
+		} else {
+			const std::vector<Value> qkv = linear_many(h, {{l.q.weight(), l.q.bias()}, {l.k.weight(), l.k.bias()}, {l.v.weight(), l.v.bias()}});
+			paged_append(l.cache, qkv[1].data(), qkv[2].data(), step);
+			a = paged_attention(qkv[0].data(), l.cache, config_.heads, step, rule);
+		}
+		const Value att = Value::leaf(std::move(a));
+		x = l.o8 ? add(x, l.o8->forward(att)) : l.o.forward_add(att, x);
+		const Value m = l.ln2.forward(x);
+		x = l.fc2_8 ? add(x, l.fc2_8->forward(gelu(l.fc1_8->forward(m)))) : l.fc2.forward_add(l.fc1.forward_gelu(m), x);
+	}
+	const Value h = ln_f_.forward(rows == N ? x : embedding(x, last, {N}));
+	Tensor logits = (head8_ ? head8_->forward(h) : head_.forward(h)).data();
+	for (const Turn& t : turns) held_[t.sequence].length += t.tokens.size();
+	return logits;
+}
+
+std::vector<std::vector<int>> Decoder::generate(const std::vector<Turn>& prompts, size_t count, const SampleRule& rule) {
+	std::vector<std::vector<int>> out(prompts.size());
+	std::vector<Turn> turns = prompts;
+	for (size_t i = 0; i < count && !turns.empty(); ++i) {
+		const Tensor logits = step(turns);
+		std::vector<float> u(turns.size());
+		for (float& x : u) x = static_cast<float>(gen_() >> 8) * (1.0f / 16777216.0f);  // the top 24 bits
+		const std::vector<int> tokens = sample(logits, Tensor::from_host({u.size()}, u.data()), rule).to_host();
+		for (size_t n = 0; n < turns.size(); ++n) {
+			if (tokens[n] < 0) throw std::runtime_error("nn::hip::Decoder: logits without a number");
+			out[n].push_back(tokens[n]);
+			turns[n].tokens = {tokens[n]};
+		}
+	}
+	return out;
+}
+
+void Decoder::drop(size_t sequence) {
+	Held& h = held_.at(sequence);
+	free_.insert(free_.end(), h.pages.rbegin(), h.pages.rend());
+	h = Held();
 }
 
 AdamW::AdamW(std::vector<Value> parameters, const AdamWOptions& options)
