@@ -10,8 +10,6 @@ namespace i8 {
 using Large = g16::Tile<256, 256, 128, 64>;
 using Small = g16::Tile<128, 128, 64, 64>;
 
-constexpr int64_t kFewRows = 64;
-
 template <class S>
 static int64_t tiles(int64_t V, int64_t rows) { return ((V + S::BM - 1) / S::BM) * ((rows + S::BN - 1) / S::BN); }
 
@@ -59,10 +57,17 @@ static hipError_t few_launch(const LinearInt8Args& a, hipStream_t s) {
 }
 template <int J, typename T>
 static hipError_t few_of(const LinearInt8Args& a, hipStream_t s) {
-	// 32 columns to a workgroup where that still makes 512 of them (the rows' codes are then read half as often), else 16; the depth
-	// over as many waves as bring 2048 together
-	if (a.V >= 32 * 512) return few_launch<2, J, 4, T>(a, s);
-	if (a.V >= 16 * 512) return few_launch<1, J, 4, T>(a, s);
+	if constexpr (J == 1) {
+		// 32 columns to a workgroup where that still makes 512 of them (the rows' codes are then read half as often), else 16; the depth
+		// over as many waves as bring 2048 together
+		if (a.V >= 32 * 512) return few_launch<2, J, 4, T>(a, s);
+		if (a.V >= 16 * 512) return few_launch<1, J, 4, T>(a, s);
+	} else {
+		// the rows' codes are as many bytes as those of 32 or 64 columns: the fewest columns that make one round of the 256 CUs, 64 at most
+		// (32 rows, 4096 deep, 10240 columns: 64 to a workgroup 27 us, 32 31; 64 rows: 32 and 39; 8192 columns: 26 and 22 us, 32 and 26)
+		if (a.V > 32 * 256) return few_launch<4, J, 4, T>(a, s);
+		if (a.V > 16 * 256) return few_launch<2, J, 8, T>(a, s);
+	}
 	return few_launch<1, J, 8, T>(a, s);
 }
 template <typename T>
@@ -74,18 +79,19 @@ static hipError_t few(const LinearInt8Args& a, hipStream_t s) {
 
 }  // namespace i8
 
-bool linear_int8_few(int64_t rows) { return rows <= i8::kFewRows; }
+// (64 rows, 4096 deep: 16384 columns 35 us here and 41 in tiles, 24576 55 and 46)
+bool linear_int8_few(int64_t rows, int64_t V) { return rows <= 32 || (rows <= 64 && V <= 64 * 256); }
 bool linear_int8_whole(int64_t rows, int64_t D) { return rows <= 16 && rows * i8::whole_pitch(D) <= i8::kWhole; }
 
 size_t linear_int8_parts(int64_t rows, int64_t D, int64_t V) {
-	if (linear_int8_few(rows)) return 0;
+	if (linear_int8_few(rows, V)) return 0;
 	const i8::Cut c = i8::cut_of(rows, D, V);
 	return c.parts > 1 ? (size_t)(c.parts * rows * V) : 0;
 }
 
 hipError_t linear_int8(const LinearInt8Args& a, int type, hipStream_t s) {
 	if (a.rows == 0 || a.V == 0) return hipSuccess;
-	if (linear_int8_few(a.rows)) return type == kF32 ? i8::few<float>(a, s) : i8::few<__bf16>(a, s);
+	if (linear_int8_few(a.rows, a.V)) return type == kF32 ? i8::few<float>(a, s) : i8::few<__bf16>(a, s);
 	return type == kF32 ? i8::tile_of_type<float>(a, s) : i8::tile_of_type<__bf16>(a, s);
 }
 

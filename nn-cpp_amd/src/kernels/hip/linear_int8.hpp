@@ -39,7 +39,7 @@ struct LinearInt8Args {
 };
 
 // Whether a product takes the form for few rows, and whether that quantises them itself (whole).
-bool linear_int8_few(int64_t rows);
+bool linear_int8_few(int64_t rows, int64_t V);
 bool linear_int8_whole(int64_t rows, int64_t D);
 // Elements of LinearInt8Args::parts.
 size_t linear_int8_parts(int64_t rows, int64_t D, int64_t V);

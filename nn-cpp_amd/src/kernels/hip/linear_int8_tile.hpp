@@ -209,7 +209,7 @@ __global__ __launch_bounds__(256) void linear_int8_join_kernel(LinearInt8Args a,
 	((T*)a.y)[row * a.ldy + col] = (T)scaled(sum, a.x_scale[row], a.w_scale[col], bias_at<T>(a, col));
 }
 
-// Few rows (at most 64): bound by the weights' bytes. A workgroup takes 16 I columns, its NW waves the depth in NW runs, each weight
+// Few rows (at most 32, 64 where the columns are few): bound by the weights' bytes. A workgroup takes 16 I columns, its NW waves the depth in NW runs, each weight
 // code going from memory into the registers of the one MFMA (16 x 16 x 64) block that uses it, the loads of U steps on their way while
 // U others are multiplied; whole numbers are added through LDS, so the order does not matter. The rows' codes come from L2, J blocks of
 // 16. WHOLE: of fewer codes still (kWhole bytes), which every workgroup makes for itself in LDS: one launch in the place of two (1 row, 4096
@@ -218,7 +218,7 @@ constexpr int kWhole = 16 * 1024;
 __host__ __device__ inline int64_t whole_pitch(int64_t D) { return (D + 63) / 64 * 64 + 16; }  // (16 rows in 16 places of the banks)
 
 template <int NW, typename T, bool VEC>
-__device__ __forceinline__ void quantize_into(const LinearInt8Args& a, int8_t* codes, float* scales, float* tops) {
+__device__ __forceinline__ void quantize_into(const LinearInt8Args& a, int8_t* codes, float* scales, unsigned* tops) {
 	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, pitch = (int)whole_pitch(a.D);
 	int team = NW;  // waves to a row
 	while (team > 1 && NW / team < a.rows) team /= 2;
@@ -227,13 +227,13 @@ __device__ __forceinline__ void quantize_into(const LinearInt8Args& a, int8_t* c
 		const int r = r0 + wave / team;
 		const bool on = r < a.rows;
 		const T* const x = (const T*)a.rows_in + (int64_t)(on ? r : 0) * a.ld_in;
-		float top = q8::share_top<T, VEC>(x, a.D, t * 8, team * 512);
+		unsigned top = q8::share_top<T, VEC>(x, a.D, t * 8, team * 512);
 #pragma unroll
-		for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+		for (int d = 32; d; d >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, d));
 		__syncthreads();
 		if (lane == 0) tops[wave] = top;
 		__syncthreads();
-		for (int w = 0; w < team; ++w) top = fmaxf(top, tops[wave / team * team + w]);
+		for (int w = 0; w < team; ++w) top = max(top, tops[wave / team * team + w]);
 		const q8::Scale scale(top);
 		if (!on) continue;
 		if (t == 0) scales[r] = scale.value;
@@ -247,7 +247,8 @@ __global__ __launch_bounds__(64 * NW) void linear_int8_few_kernel(LinearInt8Args
 	constexpr int U = I * J > 4 ? 2 : 4;
 	__shared__ int sums[NW][J * 16][I * 16 + 1];
 	__shared__ __attribute__((aligned(16))) int8_t codes[WHOLE ? kWhole : 16];
-	__shared__ float scales[16], tops[NW];
+	__shared__ float scales[16];
+	__shared__ unsigned tops[NW];
 	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 	const int r = lane & 15, q = lane >> 4, m0 = blockIdx.x * 16 * I;
 	const int steps = (a.D + 63) / 64, per = (steps + NW - 1) / NW, begin = min(wave * per, steps), end = min(begin + per, steps);

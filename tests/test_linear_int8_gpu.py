@@ -29,7 +29,8 @@ def check(dtype, rows, D, V, bias=True, seed=0):
 
 
 SHAPES = [(1, 1, 1), (1, 16, 16), (1, 4096, 100), (3, 100, 33), (16, 64, 64), (17, 1000, 257), (32, 48, 130), (33, 65, 17), (64, 2047, 129), (65, 64, 64), (100, 1000, 257),
-          (130, 33, 130), (257, 129, 300), (65, 5000, 64), (300, 4096, 520), (2, 8192, 8200), (20, 300, 16400), (70, 131, 1), (2, 4000, 300), (4, 4080, 33), (4, 4081, 33), (16, 960, 16384), (5, 1000, 8200), (1, 16300, 20), (3, 5, 16385)]
+          (130, 33, 130), (257, 129, 300), (65, 5000, 64), (300, 4096, 520), (2, 8192, 8200), (20, 300, 16400), (70, 131, 1), (2, 4000, 300), (4, 4080, 33), (4, 4081, 33), (16, 960, 16384), (5, 1000, 8200), (1, 16300, 20), (3, 5, 16385),
+          (24, 130, 5000), (40, 200, 5000), (50, 130, 9000), (64, 65, 16384), (64, 65, 16385), (32, 40, 40000)]
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
