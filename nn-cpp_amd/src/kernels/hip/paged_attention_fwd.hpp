@@ -467,11 +467,11 @@ __global__ __launch_bounds__(64 * NW, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void 
 
 // Joins the parts, one wave to a row and head, in their order.
 template <typename T>
-__global__ __launch_bounds__(256) void paged_attention_join_kernel(PagedAttentionArgs p) {
+__global__ __launch_bounds__(256) void paged_attention_join_kernel(PagedAttentionArgs p, int per) {
 	const int lane = threadIdx.x & 63;
 	const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-	if (at >= (int64_t)p.s.rows * p.a.H) return;
-	const int row = (int)(at / p.a.H), h = (int)(at % p.a.H);
+	const int shares = (p.a.H + per - 1) / per, row = (int)(at / shares), h0 = (int)(at % shares) * per;
+	if (row >= p.s.rows) return;
 	const int lo = sequence_with(p.s, row, lane);
 	if (lo == p.s.N) return;
 	const Sequence s = sequence_of(p.s, p.t, lo);
@@ -481,48 +481,50 @@ __global__ __launch_bounds__(256) void paged_attention_join_kernel(PagedAttentio
 	const Turn turn = turn_of(p, form, 0, lo);
 	const int splits = turn.parts;
 	if (splits == 1) return;
-	const int hk = h / p.a.G, column = (row - s.first) * p.a.G + h % p.a.G, groups = (count * p.a.G + (1 << form.width) - 1) >> form.width;
-	const int group = form.wide ? groups - 1 - (column >> form.width) : column >> form.width;
-	if (turn.first + (int64_t)groups * splits > form.pairs) return;  // (bounds of rows that overlap: more pairs than there is room for)
-	const int64_t step = (int64_t)(p.a.dh + 2) * form.room;
-	const float* const from = partial_of(p, form, hk, (int)turn.first + group * splits, column & ((1 << form.width) - 1));
-	float m = -kInf;
-	for (int x = lane; x < splits; x += 64) m = fmaxf(m, from[x * step]);
-	for (int x = 32; x; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
-	const float base = m == -kInf ? 0.0f : m;
-	// each lane a part's factor, then all parts' sums in their order, several loads on their way
-	float l = 0.0f, y[2] = {0.0f, 0.0f};
-	for (int x0 = 0; x0 < splits; x0 += 64) {
-		const bool on = x0 + lane < splits;
-		const float mine = on ? exp2_of(from[(x0 + lane) * step] - base) : 0.0f, own = on ? mine * from[(x0 + lane) * step + 1] : 0.0f;
-		const int some = min(64, splits - x0);
-		const auto add = [&](int x, float a, float b) {
-			const float f = __shfl(mine, x);
-			l += __shfl(own, x);
-			y[0] += f * a;
-			y[1] += f * b;
-		};
-		const float* const at = from + x0 * step + 2;
-		const int d0 = min(lane, p.a.dh - 1), d1 = min(lane + 64, p.a.dh - 1);
-		int x = 0;
-		for (; x + 8 <= some; x += 8) {
-			float a[8], b[8];
+	const int groups = (count * p.a.G + (1 << form.width) - 1) >> form.width;
+	for (int h = h0; h < min(h0 + per, p.a.H); ++h) {
+		const int hk = h / p.a.G, column = (row - s.first) * p.a.G + h % p.a.G;
+		const int group = form.wide ? groups - 1 - (column >> form.width) : column >> form.width;
+		if (turn.first + (int64_t)groups * splits > form.pairs) continue;  // (bounds of rows that overlap: more pairs than there is room for)
+		const int64_t step = (int64_t)(p.a.dh + 2) * form.room;
+		const float* const from = partial_of(p, form, hk, (int)turn.first + group * splits, column & ((1 << form.width) - 1));
+		float m = -kInf;
+		for (int x = lane; x < splits; x += 64) m = fmaxf(m, from[x * step]);
+		for (int x = 32; x; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
+		const float base = m == -kInf ? 0.0f : m;
+		// each lane a part's factor, then all parts' sums in their order, several loads on their way
+		float l = 0.0f, y[2] = {0.0f, 0.0f};
+		for (int x0 = 0; x0 < splits; x0 += 64) {
+			const bool on = x0 + lane < splits;
+			const float mine = on ? exp2_of(from[(x0 + lane) * step] - base) : 0.0f, own = on ? mine * from[(x0 + lane) * step + 1] : 0.0f;
+			const int some = min(64, splits - x0);
+			const auto add = [&](int x, float a, float b) {
+				const float f = __shfl(mine, x);
+				l += __shfl(own, x);
+				y[0] += f * a;
+				y[1] += f * b;
+			};
+			const float* const at = from + x0 * step + 2;
+			const int d0 = min(lane, p.a.dh - 1), d1 = min(lane + 64, p.a.dh - 1);
+			for (int x = 0; x < some; x += 8) {
+				float a[8], b[8];
 #pragma unroll
-			for (int i = 0; i < 8; ++i) {
-				a[i] = at[(x + i) * step + d0];
-				b[i] = at[(x + i) * step + d1];
+				for (int i = 0; i < 8; ++i) {  // (past the last part: that one's again, not added)
+					a[i] = at[min(x + i, some - 1) * step + d0];
+					b[i] = at[min(x + i, some - 1) * step + d1];
+				}
+#pragma unroll
+				for (int i = 0; i < 8; ++i)
+					if (x + i < some) add(x + i, a[i], b[i]);
 			}
-#pragma unroll
-			for (int i = 0; i < 8; ++i) add(x + i, a[i], b[i]);
 		}
-		for (; x < some; ++x) add(x, at[x * step + d0], at[x * step + d1]);
+		T* const o = (T*)p.a.out + row * p.a.os.row + h * p.a.os.head;
+		const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+	#pragma unroll
+		for (int d = 0; d < 2; ++d)
+			if (lane + 64 * d < p.a.dh) o[lane + 64 * d] = (T)(y[d] * inv);
+		if (lane == 0) p.lse[(int64_t)row * p.a.H + h] = l == 0.0f ? -kInf : m * kLn2 + logf(l);
 	}
-	T* const o = (T*)p.a.out + row * p.a.os.row + h * p.a.os.head;
-	const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-#pragma unroll
-	for (int d = 0; d < 2; ++d)
-		if (lane + 64 * d < p.a.dh) o[lane + 64 * d] = (T)(y[d] * inv);
-	if (lane == 0) p.lse[at] = l == 0.0f ? -kInf : m * kLn2 + logf(l);
 }
 
 template <typename T, int DH, bool VEC>
@@ -541,7 +543,10 @@ hipError_t launch_paged(const PagedAttentionArgs& given, hipStream_t s) {
 		e = hipGetLastError();
 	}
 	if (e == hipSuccess && (p.wide.target || p.split.target)) {
-		paged_attention_join_kernel<T><<<(unsigned)(((int64_t)p.s.rows * p.a.H + 3) / 4), 256, 0, s>>>(p);
+		// what the heads of a row share takes a wave as long as a head does: several heads to a wave where that still makes 4096 of them
+		const int per = (int)std::max<int64_t>(1, std::min<int64_t>(p.a.H, (int64_t)p.s.rows * p.a.H / 4096));
+		const int64_t waves = (int64_t)p.s.rows * ((p.a.H + per - 1) / per);
+		paged_attention_join_kernel<T><<<(unsigned)((waves + 3) / 4), 256, 0, s>>>(p, per);
 		e = hipGetLastError();
 	}
 	return e;
