@@ -387,13 +387,13 @@ __device__ __forceinline__ float all_top(float best, float* wave_top) {
 // The first pass, over all there is: a word's elements side by side, each step of the one filling the waits of the others. What is no
 // number is further away than any weight (the least of the two is the number), as are those below the least weight.
 struct Notes {
-	Lds<unsigned> at;  // the wave's own: indexes of its elements within kNear steps
+	Lds<u64> at;  // the wave's own: keys of its elements within kNear steps
 	int count;         // may pass kNearWave; lane 0's, which is the last to leave, counts
-	__device__ __forceinline__ void add(bool near, int index) {
+	__device__ __forceinline__ void add(bool near, float z, int index) {
 		const uint64_t on = __ballot(near);
 		if (!on) return;
 		const int to = count + __builtin_amdgcn_mbcnt_hi((unsigned)(on >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)on, 0));
-		if (near && to < kNearWave) at[to] = index;
+		if (near && to < kNearWave) at[to] = key_of(z, index);
 		count += __builtin_popcountll(on);
 	}
 };
@@ -417,7 +417,7 @@ __device__ __forceinline__ double add_first(const R& row, const Weights& w, Lds<
 		for (int i = 0; i < R::E; ++i) {
 			if (k[i] < kWindow) add_to(sum + (unsigned)k[i] / kBin, NUMBER ? (u64)1 : Weights::number(y[i]));
 			else if (!NUMBER) tail += y[i] - 0x1p52;
-			if constexpr (NOTE) notes.add(k[i] < kNear, at + i);
+			if constexpr (NOTE) notes.add(k[i] < kNear, R::element(u, i), at + i);
 		}
 	});
 	return tail;
@@ -450,7 +450,7 @@ __device__ __forceinline__ double count_first(const R& row, const Weights& w, bo
 			const float z = R::element(u, i);
 			if (place < kValues / 2) add_to(counts + (place | (raw >> 15) * (kValues / 2)), 1u);
 			else if (z >= w.bottom) weigh(z, 1);
-			notes.add(z >= near, at + i);
+			notes.add(z >= near, z, at + i);
 		}
 	});
 	__syncthreads();
@@ -538,14 +538,14 @@ __device__ __forceinline__ void add_tail(double tail, u64* to) {
 }
 
 // Large vocabularies: the two passes that see all of a row, the maximum and the first window's bins, are taken by workgroups of their
-// own, several to a row where there are few. Whole numbers are added up in memory, and where the elements near the largest are is noted,
+// own, several to a row where there are few. Whole numbers are added up in memory, and the elements near the largest are noted,
 // so that the workgroup that then answers the questions for the row seldom reads it again (one alone reads 10 bytes a cycle).
 struct Slices {
 	int count;        // to a row; 0: none
 	int64_t row0;     // the first row
 	float* top;       // {rows, count}
 	u64* sum;         // {rows, kSliceBins + 2}: the first window's bins, what lies behind it, and how many elements are noted
-	unsigned* noted;  // {rows, kNearRow}
+	u64* noted;       // {rows, kNearRow}: keys
 };
 
 template <typename T>
@@ -579,7 +579,7 @@ template <typename T>
 __global__ __launch_bounds__(kSliceThreads) void sample_bins_kernel(SampleArgs a, Slices x) {
 	__shared__ u64 sum[kSliceBins + 1];
 	__shared__ double table[kFine];
-	__shared__ unsigned notes[kSliceWaves * kNearWave];
+	__shared__ u64 notes[kSliceWaves * kNearWave];
 	__shared__ unsigned counts[sizeof(T) == 2 ? kValues : 1];
 	const int64_t n = blockIdx.y;
 	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -624,20 +624,27 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a, Slices slices)
 	Noted<NT> noted{lds_of((const u64*)s.near), 0};
 	bool near = false;  // what is within kNear steps is noted
 
+	const Asked q(a, n);
+	float best;
+	u64 bins[SLICED ? BINS / NT : 1], tail_sum = 0, count = 0;
+	if constexpr (SLICED) {  // (what the slices have left is on its way while the table is made)
+		static_assert(BINS == kSliceBins, "the slices' bins");
+#pragma unroll
+		for (int i = 0; i < BINS / NT; ++i) bins[i] = sliced[i * NT + threadIdx.x];
+		tail_sum = sliced[BINS];
+		count = sliced[BINS + 1];
+	}
 	fill_table<NT>(s.table, a.bits);
 	if (threadIdx.x == 0) s.low = ~0ull;
-	float best;
 	if constexpr (SLICED) {
-		static_assert(BINS == kSliceBins, "the slices' bins");
+#pragma unroll
+		for (int i = 0; i < BINS / NT; ++i) s.sum[i * NT + threadIdx.x] = bins[i];
+		if (threadIdx.x == 0) s.tail = tail_sum;
 		best = top_of(slices, blockIdx.x);
-		const u64 count = sliced[kSliceBins + 1];
 		near = count <= kNearRow;
 		if (near) {
 			noted.count = (int)count;
-			for (int i = threadIdx.x; i < noted.count; i += NT) {
-				const unsigned at = slices.noted[(int64_t)blockIdx.x * kNearRow + i];
-				s.near[i] = key_of((float)((const T*)a.logits)[n * a.ld + at], (int)at);
-			}
+			for (int i = threadIdx.x; i < noted.count; i += NT) s.near[i] = slices.noted[(int64_t)blockIdx.x * kNearRow + i];
 		}
 		__syncthreads();
 	} else {
@@ -650,7 +657,6 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a, Slices slices)
 		}
 		return;
 	}
-	const Asked q(a, n);
 	if (!(q.temperature > 0.0f)) {  // the first of the largest
 		row.each(best, best, [&](float, int i) { atomicMin(&s.low, (u64)i); });
 		__syncthreads();
@@ -693,10 +699,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a, Slices slices)
 			for (;;) {
 				if (fill) {
 					// the window's bins, and with the first one the weights behind it
-					if (SLICED && filled < 0) {
-						for (int i = threadIdx.x; i < BINS; i += NT) s.sum[i] = sliced[i];
-						if (threadIdx.x == 0) s.tail = sliced[BINS];
-					} else {
+					if (!SLICED || filled >= 0) {  // (else they are there)
 						for (int i = threadIdx.x; i < BINS; i += NT) s.sum[i] = 0;
 						if (threadIdx.x == 0) s.tail = 0;
 						__syncthreads();
@@ -814,7 +817,7 @@ hipError_t launch(const SampleArgs& a, hipStream_t s) {
 	}
 	const int64_t at_once = std::min(a.rows, kSliceRows);
 	x.sum = (u64*)a.scratch;
-	x.noted = (unsigned*)(x.sum + at_once * (kSliceBins + 2));
+	x.noted = x.sum + at_once * (kSliceBins + 2);
 	x.top = (float*)(x.noted + at_once * kNearRow);
 	for (; x.row0 < a.rows; x.row0 += at_once) {
 		const unsigned rows = (unsigned)std::min(at_once, a.rows - x.row0);
@@ -829,7 +832,7 @@ hipError_t launch(const SampleArgs& a, hipStream_t s) {
 
 size_t sample_scratch(int64_t rows, int64_t V, int type, int& slices) {
 	slices = slices_of(rows, V, type == kF32 ? 4 : 2);
-	return slices ? (size_t)std::min(rows, kSliceRows) * ((kSliceBins + 2) * sizeof(u64) + (kNearRow + slices) * 4) : 0;
+	return slices ? (size_t)std::min(rows, kSliceRows) * ((kSliceBins + 2 + kNearRow) * sizeof(u64) + slices * 4) : 0;
 }
 
 hipError_t sample(const SampleArgs& a, int type, hipStream_t s) {
