@@ -9,15 +9,21 @@
 // not depend on an order, and the products with u and top_p are taken exactly too (128 bits): what rounds is each w alone, by half of
 // 2^-bits beside the largest weight of 1, and a choice differs from that of exact weights only where a sum is nearer than that to its border.
 //
-// A workgroup takes a row. A pass finds the maximum, one sums weights (with top-k: counts) by bins
-// of a share of a factor of two, in the order wanted: a window of 16 factors of two, in which the element nearly always is, the rest in
-// registers. Then the element asked for is in a known bin, whose elements go into a list in LDS and are ordered by comparing each with
-// each. With top-k the list takes all elements up to the k-th where they are few, and the later questions are answered there. A bin with
-// more than the list holds is divided further by the order's own key (32 bits of the logit, then the index).
+// One pass over a row finds the maximum, one sums weights (with top-k: counts) by bins of a share of a factor of two, in the order wanted:
+// a window of 32 factors of two, in which the element nearly always is, the rest in registers. Then the element asked for is in a known
+// bin, whose elements go into a list in LDS and are ordered by comparing each with each. With top-k the list takes all elements up to
+// the k-th where they are few, and the later questions are answered there. A bin with more than the list holds is divided further by the
+// order's own key (32 bits of the logit, then the index).
+//
+// A vocabulary of up to 8192 is a workgroup's alone, in one launch. Of larger ones a workgroup would read 10 bytes a cycle, so the two passes
+// have launches of their own, several workgroups to a row (Slices), which also note the elements within 10 factors of two of the largest: a
+// third launch, a workgroup to a row, answers from the bins and the notes, and reads the row again where the element lies deeper or the notes
+// are more than it holds (13 us a question, 256 rows of 128000 in bf16; without notes every question cost that).
 // The exponential: 2^-d = 2^-n 2^-(k/1024) 2^-r from a table of 1024 and the power series to r^3 (|r| <= 3.4e-4: off by 2^-50 of it).
 //
-// Bound by vector instructions (a pass of sums has about 25 an element, most of them in 64 bits, at the rate of 32) once the row has
-// been read: logits that cannot count (below the least weight, or of no bin asked for) are left by two comparisons.
+// The second pass is bound by vector instructions (fp32: about 25 an element, most of them in 64 bits, at the rate of 32; 16-bit values are
+// counted instead, and weighed once each), the third launch by latency (13 to 17 us: loads, scan, list and order one after another).
+// Measured: 1 x 50257 3 + 6 + 13 us, 64 x 32000 5.5 + 12 + 14.5, 256 x 128000 in bf16 (with top-p and min-p) 13.5 + 34 + 46.
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
@@ -33,7 +39,9 @@ typedef unsigned long long u64;
 
 constexpr double kLog2e = 1.4426950408889634074, kLn2 = 0.6931471805599453094;
 constexpr int kFine = 1 << 10;       // steps to a factor of two, entries of the table
-constexpr int kWindow = 16 * kFine;  // steps that the bins cover
+// Steps that the bins cover. (256 rows of 128000 in bf16, logits of standard deviation 3 drawn from whole: 83 us, with half of it 142, as one
+// row of a hundred goes past it; deviation 0.75: 123 and 93, as a bin is then more than the list holds.)
+constexpr int kWindow = 32 * kFine;
 // (large vocabularies: see Slices)
 constexpr int kSliceThreads = 512, kSliceBins = 2048, kSliceWaves = kSliceThreads / 64;
 constexpr int64_t kSliceRows = 512;  // rows at a time
@@ -725,7 +733,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a, Slices slices)
 					window = 0;
 					base = 0;
 				} else if (x - base > s.sum[BINS]) {
-					if (window == 3) {  // fewer than top_k have a weight (2^-52 is the least)
+					if (window == 64 * kFine / kWindow - 1) {  // fewer than top_k have a weight (2^-52 is the least)
 						found = false;
 						break;
 					}
