@@ -315,10 +315,11 @@ public:
 	// last. A call that the pages, max_len or the vocabulary do not allow is refused before anything is stored (std::invalid_argument).
 	Tensor step(const std::vector<Turn>& turns);
 	// `count` tokens to each prompt (two or more turns are served together), chosen by `rule` (of as many rows as prompts) with
-	// numbers from manual_seed's "sample" stream. The last one is not stored.
+	// numbers from manual_seed's "sample" stream. The last one is not stored. Refused as step is, before anything is stored, where all of
+	// it does not fit.
 	std::vector<std::vector<int>> generate(const std::vector<Turn>& prompts, size_t count, const SampleRule& rule = SampleRule());
 	void drop(size_t sequence);  // forgets its tokens; the pages are free again
-	size_t length(size_t sequence) const { return held_.at(sequence).length; }
+	size_t length(size_t sequence) const { return held_[checked(sequence)].length; }
 	size_t free_pages() const { return free_.size(); }
 
 private:
@@ -328,6 +329,8 @@ private:
 		std::unique_ptr<QuantizedLinear> qkv8, o8, fc1_8, fc2_8;
 		PagedCache cache;
 	};
+	size_t checked(size_t sequence) const;
+	void check(const std::vector<Turn>& turns, size_t more) const;  // that these turns fit, and `more` tokens to each after them
 	struct Held {
 		size_t length = 0;
 		std::vector<int> pages;

@@ -626,7 +626,7 @@ int nnh_paged_attention_workspace_size(size_t N, size_t rows, size_t most, size_
 /*
  * Rows in 8-bit integers: scale[r] = max |x[r]| / 127 in 32 bits and codes[r, d] the whole number nearest to x[r, d] / scale[r], ties to
  * even (0 in a row of zeros). A row with an infinity or NaN has a scale of NaN and codes of 0. x {rows, D} has a pitch of ldx elements,
- * codes one of ldc bytes; where it has room, codes are followed by zeros up to a multiple of 16.
+ * codes one of ldc bytes; nothing is stored behind a row's D codes.
  */
 int nnh_quantize_rows(int type, const void* x, size_t rows, size_t D, size_t ldx, signed char* codes, size_t ldc, float* scale, void* stream);
 

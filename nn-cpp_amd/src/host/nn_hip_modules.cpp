@@ -489,26 +489,40 @@ Decoder::Decoder(const Transformer& model, const DecoderOptions& options)
 	head8_ = eight({head_});
 }
 
-Tensor Decoder::step(const std::vector<Turn>& turns) {
-	const size_t N = turns.size();
-	size_t need = 0, rows = 0, width = 1, most = 1;
+size_t Decoder::checked(size_t sequence) const {
+	if (sequence >= held_.size()) throw std::invalid_argument("nn::hip::Decoder: no such sequence");
+	return sequence;
+}
+
+void Decoder::check(const std::vector<Turn>& turns, size_t more) const {
+	size_t need = 0, rows = 0;
 	std::vector<bool> seen(held_.size(), false);
 	for (const Turn& t : turns) {
-		if (t.sequence >= held_.size() || seen[t.sequence]) throw std::invalid_argument("nn::hip::Decoder: a turn to each sequence, below DecoderOptions' number");
+		const Held& h = held_[checked(t.sequence)];
+		if (seen[t.sequence]) throw std::invalid_argument("nn::hip::Decoder: one turn to a sequence");
 		seen[t.sequence] = true;
-		const Held& h = held_[t.sequence];
-		if (t.tokens.empty() || t.tokens.size() > config_.max_len - h.length)
+		const size_t room = config_.max_len - h.length;
+		if (t.tokens.empty() || t.tokens.size() > room || more > room - t.tokens.size())
 			throw std::invalid_argument("nn::hip::Decoder: a turn has a token at least, a sequence max_len at most");
 		for (int id : t.tokens)
 			if (id < 0 || static_cast<size_t>(id) >= config_.vocab_size) throw std::invalid_argument("nn::hip::Decoder: token out of the vocabulary");
-		const size_t pages = (h.length + t.tokens.size() - 1) / page_size_ + 1;
+		const size_t pages = (h.length + t.tokens.size() + more - 1) / page_size_ + 1;
 		need += pages - std::min(pages, h.pages.size());
-		width = std::max(width, pages);
-		most = std::max(most, t.tokens.size());
 		rows += t.tokens.size();
 	}
 	if (need > free_.size()) throw std::invalid_argument("nn::hip::Decoder: no pages left");
 	if (rows > kIds) throw std::invalid_argument("nn::hip::Decoder: at most 2^24 tokens to a step");
+}
+
+Tensor Decoder::step(const std::vector<Turn>& turns) {
+	check(turns, 0);
+	const size_t N = turns.size();
+	size_t rows = 0, width = 1, most = 1;
+	for (const Turn& t : turns) {
+		width = std::max(width, (held_[t.sequence].length + t.tokens.size() - 1) / page_size_ + 1);
+		most = std::max(most, t.tokens.size());
+		rows += t.tokens.size();
+	}
 	if (N == 0) return Tensor::empty({0, config_.vocab_size});
 	std::vector<int> table(N * width, -1), starts{0}, lens;
 	std::vector<float> ids, positions, last;
@@ -558,6 +572,11 @@ Tensor Decoder::step(const std::vector<Turn>& turns) {
 }
 
 std::vector<std::vector<int>> Decoder::generate(const std::vector<Turn>& prompts, size_t count, const SampleRule& rule) {
+	const std::vector<size_t> rows{prompts.size()};
+	for (const Tensor* t : {&rule.temperature, &rule.top_p, &rule.min_p})
+		if (t->size() != 0 && t->shape() != rows) throw TensorShapeError("nn::hip::Decoder: a rule has an entry to each prompt");
+	if (rule.top_k.size() != 0 && rule.top_k.shape() != rows) throw TensorShapeError("nn::hip::Decoder: a rule has an entry to each prompt");
+	if (count > 0) check(prompts, count - 1);
 	std::vector<std::vector<int>> out(prompts.size());
 	std::vector<Turn> turns = prompts;
 	for (size_t i = 0; i < count && !turns.empty(); ++i) {
@@ -575,7 +594,7 @@ std::vector<std::vector<int>> Decoder::generate(const std::vector<Turn>& prompts
 }
 
 void Decoder::drop(size_t sequence) {
-	Held& h = held_.at(sequence);
+	Held& h = held_[checked(sequence)];
 	free_.insert(free_.end(), h.pages.rbegin(), h.pages.rend());
 	h = Held();
 }

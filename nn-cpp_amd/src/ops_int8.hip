@@ -67,10 +67,10 @@ int nnh_quantize_rows(int type, const void* x, size_t rows, size_t D, size_t ldx
 		if (rc == NNH_OK) rc = check_matrix(codes, rows, D, ldc, 1, "codes");
 		if (rc != NNH_OK || rows == 0) return rc;
 		if (!scale || off(scale, 4)) return refuse(NNH_ERR_INVALID, "the scales are null or not aligned to their elements");
-		const uint64_t pad = up(D, 16) <= ldc ? up(D, 16) : D, xb = extent(rows, D, ldx, size_of(type)), cb = extent(rows, pad, ldc, 1);
+		const uint64_t xb = extent(rows, D, ldx, size_of(type)), cb = extent(rows, D, ldc, 1);
 		if (ranges_overlap(x, xb, codes, cb) || ranges_overlap(x, xb, scale, rows * 4) || ranges_overlap(codes, cb, scale, rows * 4))
 			return refuse(NNH_ERR_ALIAS, "an output overlaps the input or the other output");
-		const QuantizeArgs a{x, (int64_t)ldx, (int64_t)rows, (int)D, reinterpret_cast<int8_t*>(codes), (int64_t)ldc, (int)pad, scale};
+		const QuantizeArgs a{x, (int64_t)ldx, (int64_t)rows, (int)D, reinterpret_cast<int8_t*>(codes), (int64_t)ldc, (int)D, scale};
 		return hip_status(quantize_rows(a, type, reinterpret_cast<hipStream_t>(stream)), "quantize rows");
 	});
 }

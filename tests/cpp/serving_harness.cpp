@@ -182,6 +182,11 @@ int serving_refused(int which) {
 			rule.top_p = Tensor({3}, 0.5f);
 			sample(x, Tensor({4}, 0.5f), rule);
 		}
+		if (which == 20) decoder.generate({{0, {1, 2}}}, 40);  // 41 tokens
+		if (which == 21) decoder.generate({{0, {1}}, {1, {1}}}, 17, SampleRule{Tensor({1}, 1.0f), Tensor(), Tensor(), IntTensor()});
+		if (which == 22) decoder.generate({{0, {1}}, {1, {1}}}, 34);  // three pages each
+		if (which == 23) decoder.drop(2);
+		if (which == 24) decoder.length(2);
 		if (which == 19) linear_int8(Tensor({4, 8}, 0.0f), quantize({Tensor({3, 8}, 1.0f)}), Tensor({2}, 0.0f));
 	});
 }
