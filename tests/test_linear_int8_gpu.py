@@ -41,6 +41,19 @@ def test_shapes(gpu, dtype, shape, bias):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("D,V", [(1000, 300), (200, 9000), (130, 17000)])
+def test_rows_by_themselves(gpu, dtype, D, V):
+    """A row's result does not depend on what it is computed with: whole, few rows' and tiles' forms give the same bits."""
+    import nnh
+    x = (draw(1, 200, D, dtype=T[dtype]) * torch.exp(draw(2, 200, 1)).to(T[dtype])).cuda()
+    w, s = weight(3, V, D)
+    w, s, b = w.cuda()[:, :D], s.cuda(), draw(4, V, dtype=T[dtype]).cuda()
+    all_rows = nnh.linear_int8(x, w, s, b)
+    for rows in (1, 7, 16, 17, 32, 40, 64, 65):
+        assert torch.equal(nnh.linear_int8(x[100:100 + rows], w, s, b), all_rows[100:100 + rows]), rows
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("V", [16384, 16383])
 def test_large_tiles(gpu, dtype, V):
     """256 x 256 tiles, with a last one seen in part, and several stages of depth."""
