@@ -648,8 +648,8 @@ def _on(t, device, dtype=None, shape=None, what="tensor"):
     if dtype is not None and t.dtype != dtype:
         raise NnhError(ERR_INVALID, f"{what} must be {dtype}, not {t.dtype}")
     if shape is not None:
-        if tuple(t.shape) != shape:
-            raise ShapeError(ERR_SHAPE, f"{what} must be {shape}, not {tuple(t.shape)}")
+        if t.shape != shape:
+            raise ShapeError(ERR_SHAPE, f"{what} must be {tuple(shape)}, not {tuple(t.shape)}")
         if not t.is_contiguous():
             raise NnhError(ERR_INVALID, f"{what} must be contiguous")
     return t.data_ptr()
@@ -959,27 +959,31 @@ class PagedCache:
         self.k, self.v, self.table = k, v, table
 
     def _struct(self, device):
+        """(the struct, the pages' type, N, Hkv, Dh, keys to a sequence)"""
         torch = _torch or _load_torch()
         k, v, table = self.k, self.v, self.table
-        if k.dim() != 4 or k.shape != v.shape or table.dim() != 2:
+        shape, strides, bounds, dtype = k.shape, k.stride(), table.shape, k.dtype
+        if len(shape) != 4 or v.shape != shape or len(bounds) != 2:
             raise ShapeError(ERR_SHAPE, "k and v are {pages, page_size, Hkv, Dh}, the table {N, width}")
-        if k.dtype != v.dtype or k.stride() != v.stride() or (k.stride(3) != 1 and k.shape[3] > 1):
+        pages, size, heads, Dh = shape
+        if v.dtype != dtype or v.stride() != strides or (strides[3] != 1 and Dh > 1):
             raise NnhError(ERR_INVALID, "k and v must have one type and the same strides, the elements of a head consecutive")
-        page, slot, head, _ = k.stride()
-        return _Cache(_on(k, device, what="k"), _on(v, device, what="v"), page, slot, head, k.shape[0], k.shape[1],
-                      _on(table, device, torch.int32, tuple(table.shape), "table"), table.shape[1])
+        N, width = bounds
+        c = _Cache(_on(k, device, None, None, "k"), _on(v, device, None, None, "v"), strides[0], strides[1], strides[2], pages, size,
+                   _on(table, device, torch.int32, bounds, "table"), width)
+        return c, dtype, N, heads, Dh, width * size
 
 
-def _packed(t, cache, device, shape, what):
+def _packed(t, dtype, device, shape, what):
     """Rows {rows, heads, Dh} of the cache's type in place."""
-    if t.dtype != cache.k.dtype:
-        raise NnhError(ERR_INVALID, f"{what} must be {cache.k.dtype}, not {t.dtype}")
-    if tuple(t.shape) != shape:
+    if t.dtype != dtype:
+        raise NnhError(ERR_INVALID, f"{what} must be {dtype}, not {t.dtype}")
+    if t.shape != shape:
         raise ShapeError(ERR_SHAPE, f"{what} must be {shape}, not {tuple(t.shape)}")
     r, h, d = t.stride()
     if d != 1 and shape[2] > 1:
         raise NnhError(ERR_INVALID, f"{what}: the elements of a head must be consecutive")
-    return C.byref(HeadTensor(_on(t, device, what=what), 0, r, h))
+    return C.byref(HeadTensor(_on(t, device, None, None, what), 0, r, h))
 
 
 def paged_append(cache, k, v, starts, lens, stream=None):
@@ -987,13 +991,14 @@ def paged_append(cache, k, v, starts, lens, stream=None):
     starts {N + 1} and lens {N} are int32."""
     torch = _torch or _load_torch()
     device = torch.cuda.current_device()
-    N, (_, _, Hkv, Dh) = cache.table.shape[0], cache.k.shape
     if k.dim() != 3:
         raise ShapeError(ERR_SHAPE, "k and v are {rows, Hkv, Dh}")
-    c, shape = cache._struct(device), (k.shape[0], Hkv, Dh)
-    check(lib().nnh_paged_append(_type(cache.k), N, k.shape[0], Hkv, Dh, _packed(k, cache, device, shape, "k"),
-                                 _packed(v, cache, device, shape, "v"), _on(starts, device, torch.int32, (N + 1,), "starts"),
-                                 _on(lens, device, torch.int32, (N,), "lens"), C.byref(c), _stream(stream)))
+    c, dtype, N, Hkv, Dh, _ = cache._struct(device)
+    rows, i32 = k.shape[0], torch.int32
+    shape = (rows, Hkv, Dh)
+    check(lib().nnh_paged_append(_type(cache.k), N, rows, Hkv, Dh, _packed(k, dtype, device, shape, "k"),
+                                 _packed(v, dtype, device, shape, "v"), _on(starts, device, i32, (N + 1,), "starts"),
+                                 _on(lens, device, i32, (N,), "lens"), C.byref(c), _stream(stream)))
 
 
 def paged_attention(q, cache, starts, most, rule, out=None, lse=None, stream=None):
@@ -1002,31 +1007,32 @@ def paged_attention(q, cache, starts, most, rule, out=None, lse=None, stream=Non
     lse {rows, H} in fp32); rows behind the last sequence are left as they are in tensors that are given, and are not set in others."""
     torch = _torch or _load_torch()
     device = torch.cuda.current_device()
-    N, (_, page_size, Hkv, Dh) = cache.table.shape[0], cache.k.shape
     if q.dim() != 3:
         raise ShapeError(ERR_SHAPE, "q is {rows, H, Dh}")
     rows, H, _ = q.shape
     if most < 0:
         raise NnhError(ERR_INVALID, "most must not be negative")
+    c, dtype, N, Hkv, Dh, keys = cache._struct(device)
     if out is None:
         out = torch.empty((rows, H, Dh), dtype=q.dtype, device=q.device)
     if lse is None:
         lse = torch.empty((rows, H), dtype=torch.float32, device=q.device)
-    c, r, shape = cache._struct(device), rule._struct(N, rows, cache.table.shape[1] * page_size, H, device), (rows, H, Dh)
-    check(lib().nnh_paged_attention(_type(cache.k), N, rows, most, H, Hkv, Dh, _packed(q, cache, device, shape, "q"), C.byref(c),
-                                    _on(starts, device, torch.int32, (N + 1,), "starts"), C.byref(r), _packed(out, cache, device, shape, "out"),
+    r, shape = rule._struct(N, rows, keys, H, device), (rows, H, Dh)
+    check(lib().nnh_paged_attention(_type(cache.k), N, rows, most, H, Hkv, Dh, _packed(q, dtype, device, shape, "q"), C.byref(c),
+                                    _on(starts, device, torch.int32, (N + 1,), "starts"), C.byref(r), _packed(out, dtype, device, shape, "out"),
                                     _on(lse, device, torch.float32, (rows, H), "lse"), _stream(stream)))
     return out, lse
 
 
 def _matrix(t, device, dtype, shape, what):
     """(address, pitch) of a matrix whose rows' elements are consecutive."""
-    if t.dim() != 2 or (shape is not None and tuple(t.shape) != shape):
-        raise ShapeError(ERR_SHAPE, f"{what} must be {shape or 'a matrix'}, not {tuple(t.shape)}")
-    rows, cols = t.shape
-    if t.stride(1) != 1 and cols > 1:
+    given = t.shape
+    if len(given) != 2 or (shape is not None and given != shape):
+        raise ShapeError(ERR_SHAPE, f"{what} must be {shape or 'a matrix'}, not {tuple(given)}")
+    (rows, cols), (pitch, step) = given, t.stride()
+    if step != 1 and cols > 1:
         raise NnhError(ERR_INVALID, f"{what}: the elements of a row must be consecutive")
-    return _on(t, device, dtype, None, what), t.stride(0) if rows > 1 else max(cols, t.stride(0))
+    return _on(t, device, dtype, None, what), pitch if rows > 1 else max(cols, pitch)
 
 
 def quantize_rows(x, codes=None, scale=None, stream=None):
@@ -1050,11 +1056,12 @@ def linear_int8(x, w, w_scale, bias=None, out=None, stream=None):
     {V, D} int8 (rows that begin at multiples of 16 bytes) and w_scale {V} stand for, plus bias {V}; returns {..., V} of x's type."""
     torch = _torch or _load_torch()
     device = torch.cuda.current_device()
-    if x.dim() < 1 or w.dim() != 2 or x.shape[-1] != w.shape[1]:
+    given, bounds = tuple(x.shape), w.shape
+    if not given or len(bounds) != 2 or given[-1] != bounds[1]:
         raise ShapeError(ERR_SHAPE, "x is {..., D} and w {V, D}")
-    V, D = w.shape
-    lead = tuple(x.shape[:-1])
-    if x.dim() != 2:
+    V, D = bounds
+    lead = given[:-1]
+    if len(lead) != 1:
         _on(x, device, None, lead + (D,), "x")
         x = x.view(-1, D) if D else x.new_empty((_count(lead), 0))
     if out is None:
