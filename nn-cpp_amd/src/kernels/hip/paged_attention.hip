@@ -55,24 +55,26 @@ hipError_t append_of(const PagedAppendArgs& p, bool vec, hipStream_t s) {
 
 // Columns: a sequence of at most 64 takes the split form, whose waves share the keys, not the columns. The keys are divided so that
 // three workgroups a CU come together, two in the other form, or up to four times as many (rounds_of), 256 keys to each at least; where
-// the rows alone bring enough, or a sequence has fewer than 512 keys, they are not. (768 for 512 wanted: mixed lengths around 3000, 12 heads of
+// the rows alone bring enough, or a sequence has room for fewer than 1024 keys (512 in the wide form), they are not: a second launch, and
+// parts to memory and back, take longer than four tiles to a wave. (One token, 8 key heads: 500 keys undivided 13 us in bf16 of 128 and 18 in
+// fp32 of 64, divided 24 and 30; 1000: 18 and 29, but 60 for 46 in fp32 of 128; 1900: 28 and 52.) (768 for 512 wanted: mixed lengths around 3000, 12 heads of
 // 80, 98 -> 89 us; 1024: 86, but 128 sequences of 1000 keys 89 -> 106.) A sequence has one group at least, and one part of each group.
 PagedPlan paged_attention_plan(int64_t N, int64_t rows, int64_t most, int64_t keys, int H, int Hkv, int Dh) {
 	constexpr int kFew = 64, kSplitWanted = 768, kWideWanted = 512;
 	PagedPlan p{kFew, {false, 5, 5, 0, 0, 0, nullptr}, {true, 7, 6, 0, 0, 0, nullptr}, 0, 0};
 	if (N == 0 || rows == 0 || most == 0) return p;
 	const int64_t G = H / Hkv, columns = std::min(most, rows) * G;
-	const auto divide = [&](Form& f, int64_t groups, bool enough, int wanted, size_t& floats) {
-		if (!enough && keys >= 512) f.target = (wanted + Hkv - 1) / Hkv;
+	const auto divide = [&](Form& f, int64_t groups, bool enough, int64_t from, int wanted, size_t& floats) {
+		if (!enough && keys >= from) f.target = (wanted + Hkv - 1) / Hkv;
 		const int64_t tiles = groups * ((keys + 31) / 32);
 		f.pairs = (int)(groups + (f.target ? std::min<int64_t>(f.target * rounds_of(tiles, f.target), tiles / (kLeastKeys / 32) + 1) : 0));
 		f.room = (int)std::min<int64_t>(1 << f.width, columns);
 		floats = f.target ? (size_t)Hkv * f.pairs * f.room * (Dh + 2) : 0;
 	};
 	const bool split = columns <= kFew || N > 1;
-	if (split) divide(p.split, std::min(2 * N, N + rows * G / 32), N * Hkv >= 8 * kSplitWanted, kSplitWanted, p.split_floats);
+	if (split) divide(p.split, std::min(2 * N, N + rows * G / 32), N * Hkv >= 8 * kSplitWanted, 1024, kSplitWanted, p.split_floats);
 	else p.few = 0;
-	if (columns > kFew) divide(p.wide, N + rows * G / 128, rows * G / 128 * Hkv >= kWideWanted, kWideWanted, p.wide_floats);
+	if (columns > kFew) divide(p.wide, N + rows * G / 128, rows * G / 128 * Hkv >= kWideWanted, 512, kWideWanted, p.wide_floats);
 	return p;
 }
 

@@ -320,7 +320,8 @@ __global__ __launch_bounds__(256, (row_bytes<T, DH>() >= 512 ? 1 : 2)) void page
 // each with a ring of tiles and of page numbers of its own.
 // Two waves and few tiles on their way, so that four workgroups share a CU (two where a row is 512 bytes or more) and some stream while
 // others begin or end: a workgroup's bounds, page numbers and first tiles are trips to memory one after another, 6 us of its time.
-// Four waves where all pairs run at once and are short.
+// Four waves where all pairs run at once and are short, eight where a CU has one alone (one token over 500 keys, 8 key heads of 128 in bf16:
+// 13 us, four 16; of 300 keys 12.6 and 13.4).
 // Bound by memory: a token of each of 64 sequences of up to 8192, 32 on 8 heads of 128, in bf16: 268 us, 4.9 TB/s.
 template <typename T, int DH, int NW_>
 struct PagedSplitShape {
@@ -541,7 +542,9 @@ hipError_t launch_paged(const PagedAttentionArgs& given, hipStream_t s) {
 	}
 	if (e == hipSuccess && p.split.pairs) {
 		const int64_t blocks = (int64_t)p.split.pairs * p.a.Hkv;
-		if (!p.split.target && blocks <= 1024) paged_attention_split_kernel<T, DH, VEC, 4><<<(unsigned)blocks, 256, 0, s>>>(p);
+		constexpr int kMost = row_bytes<T, DH>() <= 256 ? 8 : 4;  // waves that fit a CU's LDS
+		if (!p.split.target && blocks <= 256) paged_attention_split_kernel<T, DH, VEC, kMost><<<(unsigned)blocks, 64 * kMost, 0, s>>>(p);
+		else if (!p.split.target && blocks <= 1024) paged_attention_split_kernel<T, DH, VEC, 4><<<(unsigned)blocks, 256, 0, s>>>(p);
 		else paged_attention_split_kernel<T, DH, VEC, 2><<<(unsigned)blocks, 128, 0, s>>>(p);
 		e = hipGetLastError();
 	}
