@@ -615,7 +615,7 @@ int nnh_paged_append(int type, size_t N, size_t rows, size_t Hkv, size_t Dh, con
  * needed here; q_start and documents are refused). Dh <= 128. out {rows, H, Dh} and lse {rows, H} (log(sum exp z)) are stored for those
  * rows, zeros and -infinity where a row sees nothing; rows behind starts[N] are left as they are. most: at least the rows of any one
  * sequence (of one with more, only the first `most` are done).
- * A sequence of at most 64 rows times H / Hkv has its keys divided over the GPU, the others too where they are few.
+ * Where rows are few and the tables have room for many keys (1024; 512 for chunks), the keys are divided over the GPU.
  * Scratch: nnh_paged_attention_workspace_size (keys: width * page_size).
  */
 int nnh_paged_attention(int type, size_t N, size_t rows, size_t most, size_t H, size_t Hkv, size_t Dh, const nnh_head_tensor* q,
