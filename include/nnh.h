@@ -652,8 +652,8 @@ int nnh_linear_int8_workspace_size(size_t rows, size_t D, size_t V, size_t* byte
  * what is kept, 0 without a temperature. NaN counts as -infinity, which is never taken: a row of nothing else has token -1 and logprob
  * -infinity; among +infinities the weights are 1, all others 0. u is in [0, 1); temperature, top_k, top_p and min_p {rows} may be NULL (1
  * and off). NaN in one of the last two turns it off. Sums are of whole numbers and exact: a weight is rounded to 2^-bits, bits 62 less
- * the vocabulary's (45 for 128000 tokens, 51 at most). Vocabularies of more than 8192 take scratch, with any number of rows:
- * nnh_sample_workspace_size.
+ * the vocabulary's (45 for 128000 tokens, 51 at most), from an exponential that is off by less than 2^-49 of the largest
+ * weight. Vocabularies of more than 8192 take scratch, with any number of rows: nnh_sample_workspace_size.
  */
 int nnh_sample(int type, const void* logits, size_t rows, size_t V, size_t ld, const float* u, const float* temperature, const int* top_k,
                const float* top_p, const float* min_p, int* tokens, float* logprob, void* stream);

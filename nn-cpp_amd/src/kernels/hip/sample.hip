@@ -6,8 +6,9 @@
 // element has before < X <= before + own, with `before` the sum (or the number) of the elements ahead of it; nothing is sorted.
 //
 // Weights are whole numbers: w 2^bits rounded to the nearest, bits 45 for a vocabulary of 128000. Their sums are exact, so they do
-// not depend on an order, and the products with u and top_p are taken exactly too (128 bits): what rounds is each w alone, by half of
-// 2^-bits beside the largest weight of 1, and a choice differs from that of exact weights only where a sum is nearer than that to its border.
+// not depend on an order, and the products with u and top_p are taken exactly too (128 bits): what is off is each w alone, by half of
+// 2^-bits and the exponential's 2^-49 beside the largest weight of 1, and a choice differs from that of exact weights only where a sum is nearer
+// to its border than these add up to.
 //
 // One pass over a row finds the maximum, one sums weights (with top-k: counts) by bins of a share of a factor of two, in the order wanted:
 // a window of 32 factors of two, in which the element nearly always is, the rest in registers. Then the element asked for is in a known
@@ -19,7 +20,9 @@
 // have launches of their own, several workgroups to a row (Slices), which also note the elements within 10 factors of two of the largest: a
 // third launch, a workgroup to a row, answers from the bins and the notes, and reads the row again where the element lies deeper or the notes
 // are more than it holds (13 us a question, 256 rows of 128000 in bf16; without notes every question cost that).
-// The exponential: 2^-d = 2^-n 2^-(k/1024) 2^-r from a table of 1024 and the power series to r^3 (|r| <= 3.4e-4: off by 2^-50 of it).
+// The exponential: 2^-d = 2^-n 2^-(k/1024) 2^-r from a table of 1024 and the power series to r^3 (|r| ln 2 <= 3.4e-4: off by 2^-50.7 of it).
+// With the roundings of the table (2^-52), the series and the product (2^-53 each) and of d (four of 2^-53, as much of d e^-d, 0.37 at most)
+// it is off by 2^-49.6 of the largest weight: more than half of 2^-bits for vocabularies of up to 8192.
 //
 // The second pass is bound by vector instructions (fp32: about 25 an element, most of them in 64 bits, at the rate of 32; 16-bit values are
 // counted instead, and weighed once each), the third launch by latency (13 to 17 us: loads, scan, list and order one after another).
