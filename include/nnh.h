@@ -616,7 +616,7 @@ int nnh_paged_append(int type, size_t N, size_t rows, size_t Hkv, size_t Dh, con
  * rows, zeros and -infinity where a row sees nothing; rows behind starts[N] are left as they are. most: at least the rows of any one
  * sequence (of one with more, only the first `most` are done).
  * Where rows are few and the tables have room for many keys (1024; 512 for chunks), the keys are divided over the GPU.
- * Scratch: nnh_paged_attention_workspace_size (keys: width * page_size).
+ * Scratch: nnh_paged_attention_workspace_size (keys: width * page_size); none where keys are not divided, so fewer rows may take more.
  */
 int nnh_paged_attention(int type, size_t N, size_t rows, size_t most, size_t H, size_t Hkv, size_t Dh, const nnh_head_tensor* q,
                         const nnh_paged_cache* cache, const int* starts, const nnh_attention_rule* rule, const nnh_head_tensor* out,
@@ -635,7 +635,7 @@ int nnh_quantize_rows(int type, const void* x, size_t rows, size_t D, size_t ldx
  * above, products are summed in 32-bit integers, and each sum is multiplied by its row's and its column's scale and added to the bias.
  * x {rows, D} and y {rows, V} (pitches ldx, ldy) and bias {V} or NULL are of one type. The weight's rows begin at multiples of 16 bytes;
  * all V * ldw bytes are readable, and what lies behind a row's D codes does not matter. D <= 131071.
- * Scratch: nnh_linear_int8_workspace_size.
+ * Scratch: nnh_linear_int8_workspace_size; fewer rows may take more, as the depth is then divided.
  */
 int nnh_linear_int8(int type, const void* x, size_t rows, size_t D, size_t ldx, const signed char* w, size_t ldw, const float* w_scale, size_t V,
                     const void* bias, void* y, size_t ldy, void* stream);

@@ -42,3 +42,10 @@ def test_sampling_takes_scratch_by_the_vocabulary(rows):
         assert nnh.workspace_size("sample", code, rows, 8192) == 0
         assert nnh.workspace_size("sample", code, rows, 8193) > 0
         assert nnh.workspace_size("sample", code, rows, 8193) <= nnh.workspace_size("sample", code, 512, 8193)
+
+
+def test_fewer_rows_may_take_more():
+    """A workspace for several shapes is sized by asking for each: the largest batch's is not the largest."""
+    few, many = (nnh.workspace_size("linear_int8", rows, 4096, 4096) for rows in (1024, 4096))
+    assert few > 2 * many > 0
+    assert paged(767, 767, 1, 8192, 32, 8, 128) > paged(768, 768, 1, 8192, 32, 8, 128)
