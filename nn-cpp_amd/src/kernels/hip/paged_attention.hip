@@ -57,7 +57,8 @@ hipError_t append_of(const PagedAppendArgs& p, bool vec, hipStream_t s) {
 // three workgroups a CU come together, two in the other form, or up to four times as many (rounds_of), 256 keys to each at least; where
 // the rows alone bring enough, or a sequence has room for fewer than 1024 keys (512 in the wide form), they are not: a second launch, and
 // parts to memory and back, take longer than four tiles to a wave. (One token, 8 key heads: 500 keys undivided 13 us in bf16 of 128 and 18 in
-// fp32 of 64, divided 24 and 30; 1000: 18 and 29, but 60 for 46 in fp32 of 128; 1900: 28 and 52.) (768 for 512 wanted: mixed lengths around 3000, 12 heads of
+// fp32 of 64, divided 24 and 30; 1000: 18 and 29, but 60 for 46 in fp32 of 128; 1900: 28 and 52. Room is not length: 500 keys under a
+// table of 1024 places are divided.) (768 for 512 wanted: mixed lengths around 3000, 12 heads of
 // 80, 98 -> 89 us; 1024: 86, but 128 sequences of 1000 keys 89 -> 106.) A sequence has one group at least, and one part of each group.
 PagedPlan paged_attention_plan(int64_t N, int64_t rows, int64_t most, int64_t keys, int H, int Hkv, int Dh) {
 	constexpr int kFew = 64, kSplitWanted = 768, kWideWanted = 512;
